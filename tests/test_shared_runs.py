@@ -1,0 +1,128 @@
+"""Which leading pages the requests of a batch share, against a look at every pair of rows; no GPU."""
+from __future__ import annotations
+
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from tokenizer_amd.kernels.shared_prefix import SharedPrefixes, find_shared_runs
+
+
+def _table(rows, width=None):
+    width = width or max([1] + [len(r) for r in rows])
+    return np.array([list(r) + [-1] * (width - len(r)) for r in rows], dtype=np.int32).reshape(len(rows), width)
+
+
+def _checked(rows, positions, page_size, min_keys, width=None):
+    table = _table(rows, width)
+    order, runs, own = find_shared_runs(table, positions, page_size, min_keys)
+    assert sorted(order) == list(range(len(rows)))
+    place = {r: i for i, r in enumerate(order)}
+    covered = {r: 0 for r in range(len(rows))}
+    for run in runs:
+        at = sorted(place[r] for r in run.rows)
+        assert len(at) >= 2 and at == list(range(at[0], at[0] + len(at))) and [order[i] for i in at] == run.rows
+        assert run.key_end - run.key_begin >= min_keys and run.key_begin % page_size == 0 and run.key_end % page_size == 0
+        first = run.rows[0]
+        for r in run.rows:
+            assert covered[r] == run.key_begin                 # a row's runs follow each other from its first key on
+            covered[r] = run.key_end
+            assert run.key_end <= positions[r] + 1
+            assert rows[r][:run.key_end // page_size] == rows[first][:run.key_end // page_size]
+    assert [covered[r] for r in range(len(rows))] == own.tolist()
+    return order, runs, own
+
+
+def test_nothing_shared():
+    _, runs, own = _checked([[0, 1], [2, 3], [4]], [31, 20, 3], 16, 16)
+    assert runs == [] and own.tolist() == [0, 0, 0]
+
+
+def test_no_rows_and_rows_without_keys():
+    order, runs, own = find_shared_runs(np.zeros((0, 3), np.int32), np.zeros(0, np.int64), 16, 16)
+    assert (order, runs, own.tolist()) == ([], [], [])
+    _, runs, own = _checked([[3, 4], [3, 4], [3, 4]], [-1, -1, 14], 16, 16)
+    assert runs == [] and own.tolist() == [0, 0, 0]
+
+
+def test_all_share_and_the_last_page_is_not_full():
+    _, runs, own = _checked([[5, 6, 7], [5, 6, 8], [5, 6, 7]], [40, 33, 46], 16, 16)
+    assert [(sorted(r.rows), r.key_begin, r.key_end) for r in runs] == [([0, 1, 2], 0, 32)] and own.tolist() == [32, 32, 32]
+
+
+def test_rows_that_are_all_alike_up_to_the_width():
+    _, runs, own = _checked([[5, 6], [5, 6]], [31, 31], 16, 16)
+    assert [(r.key_begin, r.key_end) for r in runs] == [(0, 32)] and own.tolist() == [32, 32]
+
+
+def test_branches():
+    rows = [[1, 2, 3, 10], [1, 2, 3, 11], [1, 2, 4, 12], [9, 2, 3, 13], [1, 2, 4, 14]]
+    _, runs, own = _checked(rows, [63] * 5, 16, 16)
+    found = {(tuple(sorted(r.rows)), r.key_begin, r.key_end) for r in runs}
+    assert found == {((0, 1, 2, 4), 0, 32), ((0, 1), 32, 48), ((2, 4), 32, 48)}
+    assert own.tolist() == [48, 48, 48, 0, 48]
+
+
+def test_a_short_run_goes_to_the_runs_behind_it():
+    rows = [[1, 2, 3, 4, 20], [1, 2, 3, 4, 21], [1, 30, 31, 32, 33]]
+    _, runs, own = _checked(rows, [70, 70, 70], 16, 32)
+    assert [(sorted(r.rows), r.key_begin, r.key_end) for r in runs] == [([0, 1], 0, 64)] and own.tolist() == [64, 64, 0]
+
+
+def test_a_page_that_is_not_there_ends_what_is_shared():
+    _, runs, own = _checked([[1, -1, 3], [1, -1, 3]], [47, 47], 16, 16)
+    assert [(r.key_begin, r.key_end) for r in runs] == [(0, 16)] and own.tolist() == [16, 16]
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_any_batch(seed):
+    rng = random.Random(seed)
+    pool, rows = list(range(10 ** 4)), []
+    rng.shuffle(pool)
+    for _ in range(rng.randint(1, 25)):
+        table = list(rng.choice(rows))[:rng.randint(0, 30)] if rows and rng.random() < 0.7 else []
+        table += [pool.pop() for _ in range(rng.randint(1, 12))]
+        rows.append(table)
+    page = rng.choice([16, 32])
+    positions = [rng.randint((len(t) - 1) * page, len(t) * page - 1) for t in rows]
+    min_keys = rng.choice([16, 64, 100])
+    order, runs, own = _checked(rows, positions, page, min_keys, width=max(len(t) for t in rows) + rng.randint(0, 2))
+    # Whatever two rows share stands in runs of both, but for less than `min_keys` at its end.
+    for a in range(len(rows)):
+        for b in range(a):
+            alike = 0
+            while alike < min((positions[a] + 1) // page, (positions[b] + 1) // page) and rows[a][alike] == rows[b][alike]:
+                alike += 1
+            both = max([0] + [r.key_end for r in runs if a in r.rows and b in r.rows])
+            assert both <= alike * page and alike * page - both < min_keys
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_the_work_list_covers_every_query_and_key_once(seed):
+    rng = random.Random(100 + seed)
+    group, n_kv, page = rng.choice([1, 3, 7, 40]), rng.choice([1, 2, 4]), 16
+    shared = list(range(rng.randint(0, 90)))
+    rows = [shared + list(range(1000 * (r + 1), 1000 * (r + 1) + rng.randint(1, 5))) for r in range(rng.randint(1, 40))]
+    for r in rows[:len(rows) // 2]:
+        r[len(shared):len(shared)] = list(range(500, 500 + 9))
+    positions = [len(t) * page - 1 - rng.randint(0, page - 1) for t in rows]
+    plan = SharedPrefixes(_table(rows), positions, page, group * n_kv, n_kv, 64, torch.bfloat16, "cpu")
+    items = plan.items.reshape(-1, 8).tolist()
+    order, own, parts = plan.order_dev.tolist(), plan.own_begin_dev.tolist(), plan.parts_dev.tolist()
+    assert len(items) == plan.n_items and order == plan.order and own == plan.own_begin.tolist()
+    seen = {}                                               # (row, head in its group) -> {slot: (begin, end)}
+    for rows_at, columns, first, begin, end, slot, _, _ in items:
+        assert 0 <= first < columns and columns % group == 0 and rows_at + columns // group <= len(rows)
+        assert begin < end <= plan.keys_end and begin % page == 0 and (begin - items[0][3]) % 16 == 0
+        for column in range(first, min(columns, first + plan.COLUMNS)):
+            slots = seen.setdefault((order[rows_at + column // group], column % group), {})
+            assert slot not in slots
+            slots[slot] = (begin, end)
+    for row in range(len(rows)):
+        for head in range(group):
+            slots = seen.get((row, head), {})
+            assert sorted(slots) == list(range(parts[row])) and parts[row] <= plan.shared_parts
+            ranges = [slots[s] for s in sorted(slots)]
+            assert [b for b, _ in ranges] + [own[row]] == [0] + [e for _, e in ranges] if ranges else own[row] == 0

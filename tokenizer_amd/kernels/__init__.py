@@ -14,6 +14,7 @@ import threading
 import torch
 
 from . import build as _build
+from .shared_prefix import SharedPrefixes
 
 _F32, _BF16 = 0, 1
 _CODES = {torch.float32: _F32, torch.bfloat16: _BF16}
@@ -62,6 +63,13 @@ def _dev(*tensors: torch.Tensor | None) -> None:
         if tensor is not None:
             _need(tensor.is_cuda, "kernel operands must live on the GPU")
             _need(tensor.is_contiguous(), "kernel operands must be contiguous")
+
+
+def _here(*tensors: torch.Tensor | None) -> None:
+    """All operands on the current device: its stream is the one a kernel is launched on."""
+    current = torch.cuda.current_device()
+    for tensor in tensors:
+        _need(tensor is None or tensor.device.index == current, "kernel operands must live on the current device")
 
 
 def _parts_of_k(k: int, splits: int, step: int) -> int:
@@ -171,7 +179,7 @@ class Ops:
                      "ta_talking_prefill_parts", "ta_retention_scan", "ta_retention_chunked", "ta_temper_store",
                      "ta_add_slabs_rmsnorm", "ta_experts_few", "ta_experts_few_shared_parts",
                      "ta_fused_qk_temper",
-                     "ta_expert_gate_slots"):
+                     "ta_expert_gate_slots", "ta_sample_filtered", "ta_copy_pages", "ta_shared_prefix_attention"):
             getattr(self.lib, name).restype = ctypes.c_int
         self.lib.ta_grouped_gemm_bf16.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
                                                   ctypes.c_int, ctypes.c_void_p, ctypes.c_long, ctypes.c_int, ctypes.c_void_p,
@@ -1505,6 +1513,73 @@ class Ops:
             ctypes.c_float(softcap or 0.0), int(bool(tied_values)), self._stream()), "decode_attention")
         return out
 
+    def plan_shared_prefixes(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int,
+                             dtype: torch.dtype, device="cuda:0") -> SharedPrefixes:
+        """What the requests of a batch of single tokens share, laid out for `shared_prefix_attention`.
+
+        block_table (on the host) int [B, P]: row i's pages, -1 where there is none; positions (on the host) int [B]: where the rows'
+        newest tokens stand.  A plan holds as long as the rows keep their order, their leading pages and do not go back."""
+        import numpy as np
+        table, positions = np.asarray(block_table), np.asarray(positions)
+        _need(table.ndim == 2 and table.shape[1] >= 1 and positions.shape == (table.shape[0],), "one block table row and one position a request")
+        _need(n_kv > 0 and n_q > 0 and n_q % n_kv == 0, "query heads must be a multiple of kv heads")
+        _need(page_size >= 16 and page_size % 16 == 0, "pages of a multiple of sixteen tokens")
+        _need(head_dim in self.DECODE_HEAD_DIMS, f"head sizes {self.DECODE_HEAD_DIMS}")
+        _code(dtype)
+        return SharedPrefixes(table, positions, page_size, n_q, n_kv, head_dim, dtype, device)
+
+    def shared_prefix_attention(self, qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                                positions: torch.Tensor, block_table: torch.Tensor, plan: SharedPrefixes, n_q: int, n_kv: int,
+                                head_dim: int, scale: float, max_position: int | None = None, sinks: torch.Tensor | None = None,
+                                softcap: float | None = None) -> torch.Tensor:
+        """`paged_attention` of single tokens (row i is request i's newest token) that goes through the keys which several requests
+        share once for all of them (`plan`, from `plan_shared_prefixes` of the same requests).
+
+        qkv [B, >= n_q d] (query heads first); out [B, n_q d]; key pages [n_pages, n_kv, page_size, d], value pages [n_pages, n_kv,
+        d, page_size]; positions int32 [B]; block_table int32 [B, P].  A row sees the keys of all positions up to its own (a row of
+        position -1 none: its result is zero).  `sinks` (float32 [n_q]): exp(sinks[h]) joins the denominator; `softcap` c: a
+        scaled score s becomes c tanh(s / c).  `max_position` (host): the largest position, for the launch's size."""
+        _dev(qkv, out, k_pages, v_pages, positions, block_table, sinks)
+        n_rows = qkv.shape[0]
+        _need(plan.n_rows == n_rows and (plan.n_q, plan.n_kv, plan.head_dim, plan.dtype) == (n_q, n_kv, head_dim, qkv.dtype),
+              "the plan belongs to other rows or to another shape of attention")
+        _need(qkv.dim() == 2 and qkv.shape[1] >= n_q * head_dim and (qkv.shape[1] * qkv.element_size()) % 16 == 0 and qkv.data_ptr() % 16 == 0,
+              "qkv holds the query heads first, in rows of whole 16 bytes")
+        _need(tuple(out.shape) == (n_rows, n_q * head_dim) and out.dtype == qkv.dtype, "attention output shape")
+        _need(k_pages.dtype == qkv.dtype and v_pages.dtype == qkv.dtype, "pages must have the dtype of qkv")
+        page_size = self._page_size(k_pages, v_pages, n_kv, head_dim)
+        _need(page_size == plan.page_size, "the plan belongs to pages of another size")
+        _need(k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0, "pages start at whole 16 bytes")
+        _need(positions.dtype == torch.int32 and positions.numel() == n_rows, "positions must be int32 [B]")
+        _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == n_rows, "block_table must be int32 [B, P]")
+        _need(sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == n_q), "sinks are float32 [n_q]")
+        _need(softcap is None or softcap > 0, "a cap on the scores is positive")
+        _here(qkv, out, k_pages, v_pages, positions, block_table, plan.items, sinks)
+        width = block_table.shape[1]
+        _need(plan.keys_end <= width * page_size, "block table is too narrow for the shared keys")
+        if max_position is None:
+            max_position = width * page_size - 1
+        _need(max_position < width * page_size, "block table is too narrow for the positions")
+        if n_rows == 0:
+            return out
+        # The requests' own keys, in parts that fill the device (as for single tokens that share nothing).
+        longest = max(1, -(-(max_position + 1) // self.PLAN_KEYS) * self.PLAN_KEYS - plan.smallest_own)
+        head_blocks = -(-(n_q // n_kv) // plan.COLUMNS)
+        wanted = max(1, self.target_workgroups // (n_rows * n_kv * head_blocks))
+        own_keys = max(self.min_split_keys, -(-longest // wanted))
+        own_keys = -(-own_keys // 32) * 32
+        own_splits = -(-longest // own_keys)
+        slots = plan.shared_parts + own_splits
+        part_o = torch.empty((n_rows, n_q, slots, head_dim), dtype=torch.float32, device=qkv.device)
+        part_ml = torch.empty((n_rows, n_q, slots, 2), dtype=torch.float32, device=qkv.device)
+        self._check(self.lib.ta_shared_prefix_attention(
+            _ptr(qkv), qkv.shape[1], _ptr(out), _ptr(k_pages), _ptr(v_pages), _ptr(plan.items if plan.n_items else None), plan.n_items,
+            _ptr(plan.order_dev), _ptr(plan.own_begin_dev), _ptr(plan.parts_dev), _ptr(positions), _ptr(block_table), width, _ptr(sinks),
+            _ptr(part_o), _ptr(part_ml), slots, own_splits, own_keys, plan.COLUMNS, n_rows, n_q, n_kv, head_dim, page_size,
+            k_pages.shape[0], ctypes.c_float(scale), ctypes.c_float(softcap or 0.0), _code(qkv.dtype), self._stream()),
+            "shared_prefix_attention")
+        return out
+
     def talking_attention(self, qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                           positions: torch.Tensor, entry_of_token: torch.Tensor, block_table: torch.Tensor, n_q: int, n_kv: int,
                           head_dim: int, value_dim: int, scale: float, talk: torch.Tensor, max_position: int | None = None,
@@ -2341,6 +2416,60 @@ class Ops:
                                        _ptr(workspace), n_rows, logits.shape[1], 1 if any_cut else 0, self._stream()),
                     "sample")
         return out
+
+
+    def sample_filtered(self, logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor,
+                        min_p: torch.Tensor, uniform: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """A draw per row under temperature, top-k, top-p and min-p.  Tokens stand in the order of falling logit, lower index
+        first among equals, and weigh exp((logit - max) / temperature).  Kept are the first top_k of them (top_k <= 0: all), of those
+        the shortest prefix that reaches top_p of their weight (top_p >= 1: all; one token at least), of those the tokens of at
+        least min_p times the first one's weight; the draw is the first kept token whose running weight exceeds uniform times the
+        kept weight (weights are counted in units of 2^-44 of the first one's).  A temperature of 0 takes the first maximum, and
+        so does a row whose largest logit is infinite; NaN is never taken; a row without a number above -inf gives 0.
+
+        logits float32 or bfloat16 [B, V], V up to 2^19, rows that may lie further apart than V; temperature, top_p, min_p, uniform
+        (in [0, 1)) float32 [B]; top_k int32 [B]; returns int32 [B]."""
+        _need(logits.is_cuda, "kernel operands must live on the GPU")
+        _dev(temperature, top_k, top_p, min_p, uniform, out)
+        _need(logits.dim() == 2 and logits.dtype in _CODES, "logits must be float32 or bfloat16 [B, V]")
+        n_rows, vocab = logits.shape
+        _need(1 <= vocab <= self.FILTERED_VOCAB, f"a row has 1 to {self.FILTERED_VOCAB} logits")
+        _need((vocab == 1 or logits.stride(1) == 1) and logits.stride(0) >= 0, "a row's logits lie side by side")
+        for name, t in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("uniform", uniform)):
+            _need(t.dtype == torch.float32 and t.numel() == n_rows, f"{name} must be float32 [B]")
+        _need(top_k.dtype == torch.int32 and top_k.numel() == n_rows, "top_k must be int32 [B]")
+        if out is None:
+            out = torch.empty(n_rows, dtype=torch.int32, device=logits.device)
+        _need(out.dtype == torch.int32 and out.numel() == n_rows, "sample output must be int32 [B]")
+        _here(logits, temperature, top_k, top_p, min_p, uniform, out)
+        self._check(self.lib.ta_sample_filtered(_ptr(logits), ctypes.c_int64(logits.stride(0)), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                                                _ptr(min_p), _ptr(uniform), _ptr(out), n_rows, vocab, _code(logits.dtype), self._stream()),
+                    "sample_filtered")
+        return out
+
+    FILTERED_VOCAB = 1 << 19      # logits of a row that `sample_filtered` takes: so many weights' sum fits 63 bits
+
+    # -------------------------------------------------------------------- pages
+    def copy_pages(self, pages: torch.Tensor, n_pages: int, widths, src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
+        """Copy page src[i] of a pool to page dst[i], in every layer and plane, in place; returns `pages`.
+
+        pages [layers, n_pages * sum(widths)]: in a layer the planes (keys, values) one behind the other, plane j as n_pages pages of
+        widths[j] elements (up to four planes).  src, dst: int32 [n] on the device.  A page may be copied to several others; a page
+        that is written is named once, and is no source (which of the two would win is not said).  A pair that names a page
+        outside the pool is passed over."""
+        _dev(pages, src, dst)
+        widths = tuple(int(w) for w in widths)
+        _need(1 <= len(widths) <= 4 and all(w >= 1 for w in widths), "one to four planes of at least one element a page")
+        _need(pages.dtype in _CODES and pages.dim() == 2 and n_pages >= 1 and pages.shape[1] == n_pages * sum(widths),
+              "a pool is float32 or bfloat16 [layers, n_pages * sum(widths)]")
+        _need(1 <= pages.shape[0] <= 65535, "a pool has 1 to 65535 layers")
+        _need(max(widths) * pages.element_size() < 2 ** 31, "a page's plane holds fewer than 2^31 bytes")
+        _need(src.dtype == torch.int32 and dst.dtype == torch.int32 and src.dim() == 1 and src.shape == dst.shape, "src and dst must be int32 [n]")
+        _here(pages, src, dst)
+        if src.numel():
+            self._check(self.lib.ta_copy_pages(_ptr(pages), _ptr(src), _ptr(dst), src.numel(), n_pages, pages.shape[0], len(widths),
+                                               *(widths + (0, 0, 0))[:4], _code(pages.dtype), self._stream()), "copy_pages")
+        return pages
 
 
 _OPS: Ops | None = None

@@ -1,0 +1,103 @@
+"""What the requests of a batch share: runs of leading pages that several block tables have in common, and the list of work
+that the attention kernel makes of them (`csrc/attention_shared_prefix.hip`).  Host side, NumPy."""
+from __future__ import annotations
+
+import dataclasses
+
+import numpy as np
+import torch
+
+
+@dataclasses.dataclass
+class SharedRun:
+    """Keys `key_begin` .. `key_end` - 1 are the same for the `rows` (indices into the batch)."""
+    rows: list[int]
+    key_begin: int
+    key_end: int
+
+
+def find_shared_runs(block_table, positions, page_size: int, min_keys: int):
+    """The runs of keys that at least two rows share, and where each row's own keys begin.
+
+    block_table int [B, P], positions (of the rows' newest tokens) int [B].  Two rows share a page when their tables name it at the
+    same place and everything before it too; only pages that are full for every row count, so a plan holds as long as the rows'
+    positions do not fall.  Sharing may branch: all rows share a first part, some of them a further one.  A run of fewer than
+    `min_keys` keys is not one of its own: the keys stay with the runs behind it, or with the rows.
+
+    Returns (order, runs, own_begin): the rows so that those of any run stand side by side; the runs, those of shorter prefixes
+    first; int32 [B]."""
+    table = np.ascontiguousarray(block_table, dtype=np.int32)
+    n_rows, width = table.shape
+    full = np.minimum((np.asarray(positions, dtype=np.int64) + 1) // page_size, width).clip(min=0)
+    # A page that is not full, or not there, is like no other row's.
+    known = (np.arange(width)[None] < full[:, None]) & (table >= 0)
+    full = np.where(known.all(axis=1), width, known.argmin(axis=1)) if width else full
+    marked = np.where(np.arange(width)[None] < full[:, None], table, -1 - np.arange(n_rows, dtype=np.int32)[:, None])
+    sortable = marked.astype(">u4")                       # (as unsigned bytes, the highest first: equal rows meet)
+    order = sorted(range(n_rows), key=lambda row: sortable[row].tobytes())
+    sorted_rows = marked[order]
+    common = np.zeros(max(0, n_rows - 1), dtype=np.int64)           # pages that neighbours in the order have in common
+    if n_rows > 1:
+        differs = sorted_rows[1:] != sorted_rows[:-1]
+        common = np.where(differs.any(axis=1), differs.argmax(axis=1), width)
+    runs, own_pages = [], np.zeros(n_rows, dtype=np.int32)
+    open_ranges = [(0, n_rows, 0)]
+    while open_ranges:
+        low, high, depth = open_ranges.pop()
+        if high - low < 2:
+            own_pages[order[low:high]] = depth
+            continue
+        shared = int(common[low:high - 1].min())
+        if (shared - depth) * page_size >= min_keys:
+            runs.append(SharedRun([int(r) for r in order[low:high]], depth * page_size, shared * page_size))
+            depth = shared
+        if shared == width:                               # (rows that are all alike)
+            own_pages[order[low:high]] = depth
+            continue
+        starts = [low] + [low + 1 + int(i) for i in np.nonzero(common[low:high - 1] == shared)[0]] + [high]
+        open_ranges += [(a, b, depth) for a, b in zip(starts, starts[1:])]
+    runs.sort(key=lambda run: (run.key_begin, -len(run.rows)))
+    return order, runs, own_pages * page_size
+
+
+class SharedPrefixes:
+    """A batch's sharing laid out for the attention kernel: made once (`Ops.plan_shared_prefixes`) for requests that stay the same,
+    used at every layer and step.  It belongs to rows in this order with these leading pages, and to one shape of attention."""
+
+    COLUMNS = 32                  # query columns (requests x query heads of a kv head) that a workgroup takes
+    MIN_KEYS = 64                 # a shorter run is not worth a pass and a part to be joined of its own
+    MIN_PART = 128                # keys of a workgroup's part of a run, at least (a block of 32 for each of its four waves)
+    TARGET = 1024                 # workgroups that the parts aim at
+
+    def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device):
+        table = np.asarray(block_table, dtype=np.int32)
+        self.n_rows, self.page_size, self.n_q, self.n_kv, self.head_dim, self.dtype = (
+            table.shape[0], int(page_size), int(n_q), int(n_kv), int(head_dim), dtype)
+        self.order, self.runs, own_begin = find_shared_runs(table, positions, page_size, self.MIN_KEYS)
+        place = {row: at for at, row in enumerate(self.order)}
+        group = n_q // n_kv
+        tiles = [-(-len(run.rows) * group // self.COLUMNS) for run in self.runs]
+        # Parts of so many keys that all runs together make about TARGET workgroups.
+        work = sum(t * (run.key_end - run.key_begin) for t, run in zip(tiles, self.runs)) * n_kv
+        part = max(self.MIN_PART, -(-work // self.TARGET))
+        items, parts_of = [], np.zeros(self.n_rows, dtype=np.int32)
+        for count, run in zip(tiles, self.runs):
+            splits = max(1, -(-(run.key_end - run.key_begin) // part))
+            keys = -(-(run.key_end - run.key_begin) // (32 * splits)) * 32
+            first = int(parts_of[run.rows[0]])
+            for split, begin in enumerate(range(run.key_begin, run.key_end, keys)):
+                for tile in range(count):
+                    items.append((place[run.rows[0]], len(run.rows) * group, tile * self.COLUMNS, begin,
+                                  min(run.key_end, begin + keys), first + split, 0, 0))
+            parts_of[run.rows] = first + -(-(run.key_end - run.key_begin) // keys)
+        items.sort(key=lambda item: item[3] - item[4])    # long ones first
+        self.n_items = len(items)
+        self.shared_parts = int(parts_of.max(initial=0))
+        self.own_begin = own_begin                        # int32 [B] on the host
+        self.keys_end = max((run.key_end for run in self.runs), default=0)
+        self.smallest_own = int(own_begin.min(initial=0)) if self.n_rows else 0
+        packed = np.concatenate([np.asarray(items, dtype=np.int32).reshape(-1), np.asarray(self.order, dtype=np.int32), own_begin,
+                                 parts_of]).astype(np.int32)
+        on_device = torch.from_numpy(packed).to(device)
+        sizes = [8 * self.n_items] + [self.n_rows] * 3
+        self.items, self.order_dev, self.own_begin_dev, self.parts_dev = torch.split(on_device, sizes)
