@@ -1,0 +1,196 @@
+"""Several answers to one prompt through the engine on the GPU: forks that share their prompt's pages, attention that goes through
+those once for all, draws under top-k and min-p, replayed steps."""
+from __future__ import annotations
+
+import dataclasses
+import importlib
+
+import pytest
+import torch
+
+from tiny_configs import TINY, random_ids
+
+pytestmark = pytest.mark.gpu
+
+# Logits of the two ways through the same keys: sums in another order, in float32 as the engine's other tests hold them; in bfloat16 a
+# layer's result that falls on the other side of a rounding moves what follows by the same few percent.
+TOL = {"float32": 2e-5, "bfloat16": 4e-2}
+
+WIDE = dict(TINY["A"][0], num_hidden_layers=3, vocab_size=1000, hidden_size=448, num_attention_heads=7, num_key_value_heads=1,
+            intermediate_size=640, max_position_embeddings=4096, sliding_window=4096)
+
+
+def engine_of(dtype, raw=WIDE, **more):
+    from tokenizer_amd.config import Qwen2Config
+    from tokenizer_amd.engine import Engine, random_model
+    key = (dtype, tuple(sorted((k, str(v)) for k, v in raw.items())))
+    if key not in _MODELS:
+        _MODELS[key] = random_model(Qwen2Config.from_dict(raw), 3, dtype)
+    return Engine(_MODELS[key], **{**dict(num_pages=400, max_requests=24), **more})
+
+
+_MODELS: dict = {}
+
+
+def close(got, want, dtype):
+    err, scale = float((got - want).abs().max()), float(want.abs().max())
+    assert err <= TOL[dtype] * max(1.0, scale), f"off by {err} where logits reach {scale}"
+
+
+def forked(engine, prompt, n):
+    """`n` requests behind one prompt; their logits at its end."""
+    from tokenizer_amd.engine import StepEntry
+    engine.add_request(0)
+    first = engine.step([StepEntry(0, prompt, [len(prompt) - 1])]).clone()
+    engine.fork_request(0, list(range(1, n)))
+    return first
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("length", [5, 64, 200, 1100])
+def test_steps_of_forks_are_those_of_requests_alone(dtype, length):
+    from tokenizer_amd.engine import StepEntry
+    prompt, n = random_ids(1000, length, 1), 6
+    engines = [engine_of(dtype), engine_of(dtype, use_graphs=False), engine_of(dtype, shared_attention=False)]
+    for e in engines:
+        forked(e, prompt, n)
+    for turn in range(40):
+        entries = [StepEntry(r, [int(t)], [0]) for r, t in enumerate(random_ids(1000, n, 50 + turn))]
+        shared, eager, apart = (e.step([dataclasses.replace(x) for x in entries]).clone() for e in engines)
+        assert bool(engines[0].sharing(entries)) == (length >= 64)
+        assert engines[2].sharing(entries) == {}
+        assert torch.equal(shared, eager)                   # a replayed step is the step itself
+        close(shared, apart, dtype)
+    assert engines[0].steps_replayed >= 40
+    for e in engines:
+        for r in range(n):
+            e.end_request(r)
+        e.cache.check_invariants()
+
+
+def test_plans_change_with_the_requests():
+    from tokenizer_amd.engine import StepEntry
+    engines = [engine_of("float32"), engine_of("float32", shared_attention=False)]
+    for e in engines:
+        forked(e, random_ids(1000, 150, 2), 9)
+    live = list(range(9))
+    for turn in range(24):
+        if turn in (5, 11, 17):
+            gone = live.pop(turn % len(live))
+            for e in engines:
+                e.end_request(gone)
+        if turn == 8:                                       # a fork of a fork shares what that one has made of its own
+            for e in engines:
+                e.fork_request(live[2], [100, 101])
+            live += [100, 101]
+        if turn == 14:
+            assert len({e.compact_cache() > 0 for e in engines}) == 1
+        if turn == 15:
+            live.reverse()
+        entries = [StepEntry(r, [int(t)], [0]) for r, t in zip(live, random_ids(1000, len(live), 90 + turn))]
+        got, want = (e.step([dataclasses.replace(x) for x in entries]).clone() for e in engines)
+        close(got, want, "float32")
+    for e in engines:
+        e.cache.check_invariants()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_requests_that_share_through_the_prefix_cache(dtype):
+    from tokenizer_amd.engine import GenerateParams, Scheduler, SchedulerConfig
+    system = random_ids(1000, 330, 4)
+    results = []
+    for shared in (True, None):
+        engine = engine_of(dtype, prefix_cache=True, shared_attention=shared)
+        seen = []
+        inner = engine.sharing
+        engine.sharing = lambda entries: (lambda plans: (seen.append(len(plans)), plans)[1])(inner(entries))
+        scheduler = Scheduler(engine, SchedulerConfig(num_blocks=400, max_batch_size=8))
+        first = scheduler.add_request(system + [7], GenerateParams.greedy(1))
+        scheduler.run()
+        ids = [scheduler.add_request(system + random_ids(1000, 3 + 5 * i, i), GenerateParams.greedy(24)) for i in range(6)]
+        done = scheduler.run()
+        assert any(seen) == (shared is True) and first in done
+        results.append([done[i].tokens for i in ids])
+        scheduler.assert_idle()
+    if dtype == "float32":                                  # (greedy picks of these weights are no near ties in 32 bits)
+        assert results[0] == results[1]
+
+
+@pytest.mark.parametrize("params", [dict(temperature=1.0, top_k=20), dict(temperature=0.8, top_p=0.9, min_p=0.01), dict(temperature=1.0, top_p=0.9),
+                                    dict(temperature=0.0)], ids=["top-k", "min-p", "top-p", "greedy"])
+def test_answers_are_those_of_single_requests(params):
+    from tokenizer_amd.engine import GenerateParams, generate, generate_answers
+    prompt = random_ids(1000, 90, 8)
+    asked = GenerateParams(max_tokens=40, seed=5, **params)
+    got = generate_answers(engine_of("float32"), prompt, asked, 7)
+    for i, answer in enumerate(got):
+        want = generate(engine_of("float32"), prompt, dataclasses.replace(asked, seed=5 + i))
+        # A draw whose border lies between the two sums' roundings would differ: of these 280 none does.
+        assert answer.tokens == want.tokens and answer.reason == want.reason
+
+
+def test_draws_in_a_run_of_steps_keep_each_request_its_settings():
+    # One run with rows under top-k, rows under temperature and top_p alone and greedy rows: each gets what it gets among its like.
+    from tokenizer_amd.engine import StepEntry
+    rows = [(1.0, 1.0, 5, 0.0), (0.9, 0.8, 0, 0.0), (0.0, 1.0, 0, 0.0), (1.3, 1.0, 0, 0.2), (1.0, 0.95, 40, 0.05), (0.7, 1.0, 0, 0.0)]
+    prompt = random_ids(1000, 70, 3)
+
+    def run(which):
+        engine = engine_of("float32", shared_attention=False)
+        forked(engine, prompt, len(which))
+        draw = lambda k: ([rows[i][0] for i in which], [rows[i][1] for i in which], [((7 * i + 3 * k) % 16) / 16 for i in which],
+                          [rows[i][2] for i in which], [rows[i][3] for i in which])
+        out = engine.decode_sampled(list(range(len(which))), [11 + i for i in which], 20, draw)
+        last = [StepEntry(r, [5], [0]) for r in range(len(which))]
+        engine.step(last)
+        return [[ids[at] for ids in out] for at in range(len(which))]
+
+    together = run(range(6))
+    assert run([0, 3, 4]) == [together[i] for i in (0, 3, 4)]
+    assert run([1, 5]) == [together[i] for i in (1, 5)]
+    assert run([2]) == [together[2]]
+    steps = engine_of("float32", shared_attention=False, use_graphs=False)
+    forked(steps, prompt, 6)
+    current = [11 + i for i in range(6)]
+    for k in range(20):
+        logits = steps.step([StepEntry(r, [t], [0]) for r, t in enumerate(current)])
+        drawn = steps.sample(logits, list(range(6)), [r[0] or 1.0 for r in rows], [r[1] for r in rows],
+                             [((7 * i + 3 * k) % 16) / 16 for i in range(6)], [r[2] for r in rows], [r[3] for r in rows])
+        drawn[2] = steps.argmax(logits, [2])[0]
+        assert drawn == [together[i][k] for i in range(6)]
+        current = drawn
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("module,table,name", [("zomavik_configs", "ZOMAVIK", "C"), ("napadra_configs", "NAPADRA", "P"), ("bokulorn_configs", "BOKULORN", "A"),
+                                               ("gafonex_configs", "GAFONEX", "A"), ("dolidra_configs", "DOLIDRA", "A"), ("zeridra_configs", "ZERIDRA", "A")])
+def test_forks_of_other_designs(module, table, name, dtype, tmp_path):
+    # State in the slot, windows, borrowed pages and latents are taken along: a fork goes on as the request itself would.
+    from tokenizer_amd.engine import Engine, StepEntry, load_model
+    configs = importlib.import_module(module)
+    held = getattr(configs, table)[name]
+    raw, seed = held if isinstance(held, tuple) else (held, 1)
+    model = load_model(configs.write_model(raw, seed, str(tmp_path / "m")), dtype)
+    vocab = model.vocab_size
+    engine = Engine(model, num_pages=64, max_requests=6, use_graphs=False, shared_attention=False)
+    prompt = random_ids(vocab, 41, 1)
+    engine.add_request("a")
+    engine.step([StepEntry("a", prompt)])
+    engine.fork_request("a", ["b", "c"])
+    engine.pools.manager.check_invariants()
+    for turn in range(8):
+        tokens = random_ids(vocab, 2, 20 + turn)
+        # "a" and "b" get the same tokens, "c" others: the first two stay alike to the last bit.
+        got = engine.step([StepEntry("a", tokens[:1], [0]), StepEntry("c", tokens[1:], [0]), StepEntry("b", tokens[:1], [0])])
+        assert torch.equal(got[0], got[2]) and not torch.equal(got[0], got[1])
+    shared = Engine(model, num_pages=64, max_requests=6)
+    shared.add_request("a")
+    shared.step([StepEntry("a", prompt + random_ids(vocab, 30, 2))])
+    shared.fork_request("a", ["b", "c"])
+    apart = Engine(model, num_pages=64, max_requests=6, shared_attention=False)
+    apart.add_request("a")
+    apart.step([StepEntry("a", prompt + random_ids(vocab, 30, 2))])
+    apart.fork_request("a", ["b", "c"])
+    for turn in range(6):
+        entries = [StepEntry(r, [t], [0]) for r, t in zip("abc", random_ids(vocab, 3, 70 + turn))]
+        close(shared.step([dataclasses.replace(e) for e in entries]), apart.step(entries), dtype)

@@ -15,8 +15,8 @@ package is set up, so a user's own architecture reaches them without a change to
 from . import models  # noqa: F401  (registers the architectures)
 from .config import ConfigError, Qwen2Config, load_config, register_architecture, registered_architectures
 from .engine import (Control, Engine, EngineStats, Failure, GenerateParams, Generated, Model, QueueFull, SampleCursor,
-                     Sampled, Scheduler, SchedulerConfig, StepEntry, StopReason, StreamDecoder, generate, generate_with,
-                     greedy_tokens, load_eos_token_ids, load_model, parse_eos_token_ids, random_model)
+                     Sampled, Scheduler, SchedulerConfig, StepEntry, StopReason, StreamDecoder, generate, generate_answers,
+                     generate_with, greedy_tokens, load_eos_token_ids, load_model, parse_eos_token_ids, random_model)
 from .sampling import Rng, SampleError, greedy_token, sample_token
 from .tokenizer import Tokenizer, TokenizerError, load_tokenizer, register_tokenizer
 from .weights import WeightError, write_random_model
@@ -24,7 +24,7 @@ from .weights import WeightError, write_random_model
 __all__ = ["ConfigError", "Qwen2Config", "load_config", "register_architecture", "registered_architectures",
            "Control", "Engine", "EngineStats", "Failure", "GenerateParams", "Generated", "Model", "QueueFull",
            "SampleCursor", "Sampled", "Scheduler", "SchedulerConfig", "StepEntry", "StopReason", "StreamDecoder",
-           "generate", "generate_with", "greedy_tokens", "load_eos_token_ids", "load_model", "parse_eos_token_ids",
+           "generate", "generate_answers", "generate_with", "greedy_tokens", "load_eos_token_ids", "load_model", "parse_eos_token_ids",
            "random_model", "Rng", "SampleError", "greedy_token", "sample_token", "Tokenizer", "TokenizerError",
            "WeightError", "write_random_model", "load_tokenizer", "register_tokenizer"]
 

@@ -266,6 +266,39 @@ class CacheManager:
         keep, pointer = _host.token_array(tokens)
         self._lib.ta_cache_publish(self._core, self._handle_of(rid), pointer, len(keep))
 
+    # --------------------------------------------------------------------- forks
+    def fork(self, rid, new_rid) -> tuple[list[tuple[int, int, int]], tuple[int, int]]:
+        """`new_rid` becomes a live request that holds what `rid` holds: they share the full pages, and the page that is not full
+        (one in every group) is the new request's own.  Returns the pages whose contents are to be copied, as (group, from, to), and
+        the two requests' state slots (from, to).  `OutOfPages` with nothing changed if a slot or a page is missing."""
+        handle = self._handle_of(rid)
+        if self.has_request(new_rid):
+            raise KeyError(f"request {new_rid!r} is already live")
+        child = new_rid if _is_handle(new_rid) else self._next_handle
+        room = max(1, 3 * len(self.groups))
+        copies, count, slots = (ctypes.c_int32 * room)(), ctypes.c_int32(0), (ctypes.c_int32 * 2)()
+        status = self._lib.ta_cache_fork(self._core, handle, child, copies, ctypes.byref(count), slots)
+        if status == -2:
+            raise OutOfPages(f"all {self.max_requests} request slots are taken")
+        if status == -5:
+            raise OutOfPages(f"no page left for a fork of request {rid!r}")
+        if not _is_handle(new_rid):
+            self._next_handle += 1
+            self._ids[new_rid] = child
+        return [tuple(copies[3 * i:3 * i + 3]) for i in range(count.value)], (slots[0], slots[1])
+
+    def compact(self) -> list[tuple[int, int, int]]:
+        """Bring the pages in use (those of live requests and those kept for their prefix) to the lowest ids.  Returns the pages whose
+        contents are to be copied, as (group, from, to); no page is both."""
+        moves = (ctypes.c_int32 * max(1, 3 * self.num_pages * len(self.groups)))()
+        count = self._lib.ta_cache_compact(self._core, moves)
+        return [tuple(moves[3 * i:3 * i + 3]) for i in range(count)]
+
+    @property
+    def epoch(self) -> int:
+        """Changes whenever requests come, go or take pages over."""
+        return self._lib.ta_cache_epoch(self._core)
+
     # ------------------------------------------------------------------- packing
     def pack_batch(self, rids, token_lists, want_lists, out: np.ndarray, table_width: int | None = None,
                    padded: tuple | None = None):

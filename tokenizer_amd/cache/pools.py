@@ -57,6 +57,29 @@ class CachePools:
         return (pages[index, :keys].view(*shape, page_size, need.head_dim),
                 pages[index, keys:].view(shape[0], need.v_heads, need.v_dim, page_size))
 
+    def copy_pages(self, copies, ops) -> None:
+        """Copy the pages' contents, (group, from, to) each, in all layers of their groups: a launch a group.  No page that is written
+        is named twice or is a source."""
+        for g, group in enumerate(self.manager.groups):
+            pairs = [(src, dst) for at, src, dst in copies if at == g]
+            if not pairs:
+                continue
+            src, dst = [p[0] for p in pairs], [p[1] for p in pairs]
+            pages = range(self.manager.num_pages)
+            if len(set(dst)) != len(dst) or set(dst) & set(src) or not all(p in pages for p in src + dst):
+                raise ValueError("a page that is written must be in the pool, named once, and be no source")
+            need, page_size = group.need, self.manager.page_size
+            widths = (need.n_kv_heads * need.head_dim * page_size,)
+            if not need.tied_values:
+                widths += (need.v_heads * need.v_dim * page_size,)
+            both = torch.tensor([src, dst], dtype=torch.int32).to(self.pages[g].device)
+            ops.copy_pages(self.pages[g], self.manager.num_pages, widths, both[0], both[1])
+
+    def copy_states(self, src: int, dst: int) -> None:
+        """What the request in slot `src` keeps beside its pages, copied to slot `dst`."""
+        for tensor in list(self.states.values()) + list(self.block_states.values()):
+            tensor[dst].copy_(tensor[src])
+
     def keep_states(self) -> list:
         """Copies of every state tensor (for a run whose effect on them is to be undone)."""
         return [(t, t.clone()) for t in list(self.states.values()) + list(self.block_states.values())]

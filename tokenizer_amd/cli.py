@@ -2,6 +2,9 @@
 
     qwen-infer --model DIR [--max-tokens N] [--temperature T] [--top-p P] [--seed N] [--stop STRING]... <prompt>
 
+Beyond the reference's flags: `--top-k N` and `--min-p P` narrow what is drawn from, `--answers N` draws N answers with the seeds from
+`--seed` on from one run of the prompt.
+
 Flags, defaults and the lines printed are the reference's: the generated text on standard
 output; prompt ids, parameters, generated ids, the stop reason and the timings on standard
 error.  The model comes from a folder (config.json, model.safetensors, tokenizer.json and,
@@ -16,7 +19,8 @@ import sys
 import time
 
 USAGE = ("usage: qwen-infer --model DIR [--dtype bf16|fp32] [--num-blocks N] [--random-weights SEED] [--max-tokens N] "
-         "[--temperature T] [--top-p P] [--seed N] [--stop STRING]... [--token-ids] <prompt>")
+         "[--temperature T] [--top-p P] [--top-k N] [--min-p P] [--seed N] [--answers N] [--stop STRING]... "
+         "[--token-ids] <prompt>")
 
 
 class ArgError(ValueError):
@@ -26,7 +30,7 @@ class ArgError(ValueError):
 def parse_args(argv: list[str]) -> dict:
     args = {"prompt": None, "max_tokens": 20, "temperature": 0.0, "top_p": 1.0, "seed": 0, "stop": [],
             "model": None, "dtype": "bfloat16", "num_blocks": 256, "token_ids": False, "help": False,
-            "random_weights": None}
+            "random_weights": None, "top_k": 0, "min_p": 0.0, "answers": 1}
     it = iter(argv)
 
     def value(flag: str) -> str:
@@ -57,6 +61,25 @@ def parse_args(argv: list[str]) -> dict:
                 args["top_p"] = float(value(arg))
             except ValueError:
                 raise ArgError("--top-p wants a number") from None
+        elif arg == "--top-k":
+            try:
+                args["top_k"] = int(value(arg))
+                if args["top_k"] < 0:
+                    raise ValueError
+            except ValueError:
+                raise ArgError("--top-k wants a count of tokens") from None
+        elif arg == "--min-p":
+            try:
+                args["min_p"] = float(value(arg))
+            except ValueError:
+                raise ArgError("--min-p wants a number") from None
+        elif arg == "--answers":
+            try:
+                args["answers"] = int(value(arg))
+                if args["answers"] < 1:
+                    raise ValueError
+            except ValueError:
+                raise ArgError("--answers wants a count of at least one") from None
         elif arg == "--seed":
             try:
                 args["seed"] = int(value(arg))
@@ -96,6 +119,27 @@ def _plain_number(value: float) -> str:
     return text[:-2] if text.endswith(".0") else text
 
 
+def _several_answers(engine, prompt_ids: list[int], params, count: int, token_bytes) -> int:
+    """`--answers N`: the answers one after the other on standard output, each answer's ids and stop reason on standard error."""
+    from .cache import OutOfPages
+    from .engine import generate_answers
+    started = time.perf_counter()
+    try:
+        answers = generate_answers(engine, prompt_ids, params, count, token_bytes)
+    except (ValueError, OutOfPages) as err:
+        print(f"error: {err}", file=sys.stderr)
+        return 1
+    elapsed = time.perf_counter() - started
+    for answer in answers:
+        print(answer.text)
+        print(f"generated ids: {answer.tokens}", file=sys.stderr)
+        print(f"stop: {answer.reason.value}", file=sys.stderr)
+    total = sum(len(answer.tokens) for answer in answers)
+    print(f"prefill {answers[0].prefill:.4f} s, decode {answers[0].decode:.4f} s ({total} tokens, {count} answers, KV cache, "
+          f"total {elapsed:.4f} s)", file=sys.stderr)
+    return 0
+
+
 def main(argv: list[str] | None = None) -> int:
     try:
         args = parse_args(sys.argv[1:] if argv is None else argv)
@@ -128,6 +172,7 @@ def main(argv: list[str] | None = None) -> int:
     params = GenerateParams.greedy(args["max_tokens"])
     params.temperature, params.top_p, params.seed, params.stop = (args["temperature"], args["top_p"],
                                                                    args["seed"], args["stop"])
+    params.top_k, params.min_p = args["top_k"], args["min_p"]
     eos_path = os.path.join(folder, "generation_config.json")
     if os.path.exists(eos_path):
         params.eos = load_eos_token_ids(eos_path)
@@ -138,10 +183,12 @@ def main(argv: list[str] | None = None) -> int:
         model = random_model(load_config(folder), args["random_weights"], args["dtype"])
     else:
         model = load_model(folder, args["dtype"])
-    engine = Engine(model, num_pages=args["num_blocks"], max_requests=1)
+    engine = Engine(model, num_pages=args["num_blocks"], max_requests=args["answers"])
     token_bytes = (lambda token: tokenizer.decode_bytes([token])) if tokenizer else \
         (lambda token: f"{token} ".encode())
     started = time.perf_counter()
+    if args["answers"] > 1:
+        return _several_answers(engine, prompt_ids, params, args["answers"], token_bytes)
     # The request takes the way every request of a serving engine takes: queued, admitted with pages for its whole
     # prompt, the prompt run in portions under the token budget, decoded (greedy steps in bursts), finished, freed.
     request = engine.add_request(prompt_ids, params, token_bytes=token_bytes)

@@ -147,6 +147,23 @@ int ta_cache_attach_shared_prefix(void* c, int64_t id, const int32_t* tokens, in
 int ta_cache_publish(void* c, int64_t id, const int32_t* tokens, int count) {
   return ((CacheCore*)c)->publish(id, tokens, count);
 }
+// `child` becomes a fork of `id`: per copied page three numbers (group, from, to) into copies (room for 3 * groups), their count
+// in n_copies, the two state slots in slots.  Returns a CacheStatus.
+int ta_cache_fork(void* c, int64_t id, int64_t child, int* copies, int* n_copies, int* slots) {
+  std::vector<int> made;
+  const int status = ((CacheCore*)c)->fork(id, child, &made, slots);
+  std::copy(made.begin(), made.end(), copies);
+  *n_copies = (int)made.size() / 3;
+  return status;
+}
+// Pages to the lowest ids: per moved page three numbers (group, from, to) into moves (room for 3 * groups * pages); how many.
+int ta_cache_compact(void* c, int* moves) {
+  std::vector<int> made;
+  ((CacheCore*)c)->compact(&made);
+  std::copy(made.begin(), made.end(), moves);
+  return (int)made.size() / 3;
+}
+int64_t ta_cache_epoch(void* c) { return ((const CacheCore*)c)->epoch(); }
 int ta_cache_check(void* c) {
   g_message = ((CacheCore*)c)->check_invariants();
   return g_message.empty() ? 0 : 1;
@@ -229,6 +246,9 @@ int ta_sched_finish(void* s, int64_t id) { return ((SchedulerCore*)s)->finish(id
 // ----------------------------------------------------------------------------------------- sampling
 float ta_uniform_f32(uint64_t seed, uint64_t counter) { return uniform_f32(seed, counter); }
 int ta_greedy_token(const float* logits, int64_t count) { return greedy_token(logits, count); }
+int ta_sample_filtered_host(const float* logits, int64_t count, float temperature, int top_k, float top_p, float min_p, float uniform) {
+  return sample_filtered(logits, count, temperature, top_k, top_p, min_p, uniform);
+}
 int ta_sample_with_uniform(const float* logits, int64_t count, float temperature, float top_p, float uniform) {
   return sample_with_uniform(logits, count, temperature, top_p, uniform);
 }

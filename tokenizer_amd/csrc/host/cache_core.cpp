@@ -46,6 +46,7 @@ int CacheCore::add_request(int64_t id) {
   request.tables.resize(groups_.size());
   const int slot = request.slot;
   requests_.emplace(id, std::move(request));
+  ++epoch_;
   return slot;
 }
 
@@ -115,6 +116,7 @@ int CacheCore::release(int64_t id) {
   for (size_t g = 0; g < groups_.size(); ++g) free_table(*groups_[g], found->second.tables[g]);
   free_slots_.push_back(found->second.slot);
   requests_.erase(found);
+  ++epoch_;
   return CACHE_OK;
 }
 
@@ -126,6 +128,7 @@ int CacheCore::detach(int64_t id) {
     request->tables[g].clear();
   }
   request->seq_len = 0;
+  ++epoch_;
   return CACHE_OK;
 }
 
@@ -154,6 +157,7 @@ int CacheCore::attach_shared_prefix(int64_t id, const int32_t* tokens, int count
     request->tables[g].insert(request->tables[g].end(), taken[g].begin(), taken[g].begin() + shared);
   }
   request->seq_len = (int)shared * page_size_;
+  ++epoch_;
   return request->seq_len;
 }
 
@@ -166,6 +170,52 @@ int CacheCore::publish(int64_t id, const int32_t* tokens, int count) {
     groups_[g]->allocator.publish_prompt_pages(tokens, written, request->tables[g].data(),
                                                (int)request->tables[g].size());
   return CACHE_OK;
+}
+
+int CacheCore::fork(int64_t id, int64_t child, std::vector<int>* copies, int* slots) {
+  if (!find(id)) return CACHE_UNKNOWN_REQUEST;
+  if (find(child)) return CACHE_ALREADY_LIVE;
+  if (free_slots_.empty()) return CACHE_NO_SLOT;
+  const int length = find(id)->seq_len, full = length / page_size_, held = pages_for_len(length, page_size_);
+  for (auto& group : groups_)
+    if (held > full && group->allocator.available() < 1) return CACHE_TOO_FEW_PAGES;
+  const int slot = add_request(child);
+  const Request* from = find(id);                          // (a new request may move the others)
+  Request* to = find(child);
+  for (size_t g = 0; g < groups_.size(); ++g) {
+    const std::vector<int>& table = from->tables[g];
+    for (int index = 0; index < held; ++index) {
+      int page = table[index];                             // -1: given back behind the window
+      if (index < full) {
+        if (page >= 0) groups_[g]->allocator.incref(page);
+      } else if (page >= 0) {
+        const int own = groups_[g]->allocator.alloc();
+        copies->insert(copies->end(), {(int)g, page, own});
+        page = own;
+      }
+      to->tables[g].push_back(page);
+    }
+  }
+  to->seq_len = length;
+  slots[0] = from->slot;
+  slots[1] = slot;
+  return CACHE_OK;
+}
+
+void CacheCore::compact(std::vector<int>* moves) {
+  for (size_t g = 0; g < groups_.size(); ++g) {
+    std::vector<std::pair<int, int>> moved;
+    groups_[g]->allocator.compact(&moved);
+    if (moved.empty()) continue;
+    std::unordered_map<int, int> now(moved.begin(), moved.end());
+    for (const auto& move : moved) moves->insert(moves->end(), {(int)g, move.first, move.second});
+    for (auto& item : requests_)
+      for (int& page : item.second.tables[g]) {
+        auto found = now.find(page);
+        if (found != now.end()) page = found->second;
+      }
+    ++epoch_;
+  }
 }
 
 std::string CacheCore::check_invariants() const {

@@ -66,6 +66,15 @@ class CacheCore {
   int attach_shared_prefix(int64_t id, const int32_t* tokens, int count);   // tokens covered, or a CacheStatus
   int detach(int64_t id);
   int publish(int64_t id, const int32_t* tokens, int count);
+  // A new request `child` that holds what `id` holds: it shares the pages that are full, and gets pages of its own for those that are
+  // not (one a group at most), whose contents the caller copies: `copies` gets (group, from, to) for each, `slots` the two
+  // requests' state slots.  CACHE_OK, or a CacheStatus and nothing changed (CACHE_TOO_FEW_PAGES: no page left for a copy).
+  int fork(int64_t id, int64_t child, std::vector<int>* copies, int* slots);
+  // Bring every group's pages to the lowest ids, in the tables and the prefix index; `moves` gets (group, from, to) for each page whose
+  // contents the caller then copies.
+  void compact(std::vector<int>* moves);
+  // Changes whenever requests come, go or take pages over: what is known of the requests' leading pages holds until then.
+  int64_t epoch() const { return epoch_; }
   std::string check_invariants() const;
 
   // One step's batch description.  Entry i is request ids[i] with n_tokens[i] new tokens (flattened in
@@ -88,6 +97,7 @@ class CacheCore {
  private:
   Request* find(int64_t id);
   int page_size_, max_requests_;
+  int64_t epoch_ = 0;
   bool prefix_cache_;
   std::vector<std::unique_ptr<Group>> groups_;
   std::vector<int> free_slots_;

@@ -1,6 +1,7 @@
 #include "page_allocator.h"
 
 #include <algorithm>
+#include <functional>
 #include <cstring>
 
 namespace ta {
@@ -174,6 +175,42 @@ void PageAllocator::reclaim_cached() {
     unindex(page);
     free_.push_back(page);
   }
+}
+
+void PageAllocator::compact(std::vector<std::pair<int, int>>* moves) {
+  const int kept = occupied();
+  std::vector<int> targets;
+  for (int page : free_)
+    if (page < kept) targets.push_back(page);
+  std::sort(targets.begin(), targets.end(), std::greater<int>());      // back() is the lowest
+  if (targets.empty()) return;
+  std::vector<int> now(capacity_);
+  for (int page = 0; page < capacity_; ++page) now[page] = page;
+  for (int page = kept; page < capacity_; ++page) {
+    if (refcount_[page] == 0 && !is_cached_[page]) continue;
+    const int to = targets.back();
+    targets.pop_back();
+    now[page] = to;
+    moves->emplace_back(page, to);
+    refcount_[to] = refcount_[page];
+    has_hash_[to] = has_hash_[page];
+    hash_of_[to] = hash_of_[page];
+    is_cached_[to] = is_cached_[page];
+    if (is_cached_[page]) {
+      cached_at_[to] = cached_at_[page];
+      *cached_at_[to] = to;                                            // (its place in the order of age stays)
+    }
+    refcount_[page] = 0;
+    has_hash_[page] = 0;
+    is_cached_[page] = 0;
+  }
+  for (auto& item : index_) {
+    Entry& e = item.second;
+    e.page = now[e.page];
+    if (e.parent_page >= 0) e.parent_page = now[e.parent_page];
+  }
+  free_.clear();
+  for (int page = capacity_ - 1; page >= kept; --page) free_.push_back(page);
 }
 
 std::string PageAllocator::check_invariants() const {

@@ -8,6 +8,7 @@
 #include <list>
 #include <string>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 namespace ta {
@@ -45,6 +46,9 @@ class PageAllocator {
   void take_shared_prefix(const int32_t* tokens, int count, std::vector<int>* out);
   void publish_prompt_pages(const int32_t* tokens, int count, const int* pages, int n_pages);
   void reclaim_cached();
+  // Bring the live and the cached pages to the lowest ids: appends the moves (from, to) that bring a page there, whose contents the
+  // caller then copies and whose holders it renames.  The targets were free, the pages left are free afterwards.
+  void compact(std::vector<std::pair<int, int>>* moves);
   std::string check_invariants() const;                   // empty when all is well
 
   // The index under a given hash value (what the calls above do after hashing; tests use them to make two

@@ -85,4 +85,47 @@ int sample_with_uniform(const float* logits, int64_t count, float temperature, f
   return (int)order[cutoff - 1];
 }
 
+int sample_filtered(const float* logits, int64_t count, float temperature, int top_k, float top_p, float min_p, float uniform) {
+  if (count <= 0) return -1;
+  if (!std::isfinite(temperature) || temperature < 0) return -2;
+  if (!std::isfinite(top_p) || top_p < 0) return -3;
+  if (count > (1 << 19)) return -4;                       // so many weights' sum fits 63 bits
+  std::vector<int64_t> order;
+  for (int64_t i = 0; i < count; ++i)
+    if (!std::isnan(logits[i])) order.push_back(i);
+  std::stable_sort(order.begin(), order.end(), [&](int64_t a, int64_t b) { return logits[a] > logits[b]; });
+  if (order.empty() || std::isinf(logits[order[0]]) || temperature == 0) return greedy_token(logits, count);
+  const double top = logits[order[0]], rate = 1.0 / (double)temperature;
+  size_t kept = order.size(), over = 0;
+  if (top_k > 0) kept = std::min(kept, (size_t)top_k);
+  std::vector<uint64_t> weight(order.size());
+  uint64_t total = 0;
+  for (size_t i = 0; i < order.size(); ++i) {
+    const double share = std::exp(((double)logits[order[i]] - top) * rate);
+    weight[i] = (uint64_t)std::rint(share * 17592186044416.0);
+    if (i < kept) total += weight[i];
+    if (i == 0 || !(share < (double)min_p)) over = i + 1;
+  }
+  if (top_p < 1.0f) {
+    const uint64_t need = std::max<uint64_t>(1, (uint64_t)std::ceil((double)top_p * (double)total));
+    uint64_t run = 0;
+    for (size_t i = 0; i < kept; ++i) {
+      run += weight[i];
+      if (run >= need) { kept = i + 1; break; }
+    }
+  }
+  kept = std::min(kept, over);
+  total = 0;
+  for (size_t i = 0; i < kept; ++i) total += weight[i];
+  const double target = (double)uniform * (double)total;
+  uint64_t need = target >= 0.0 ? (target < (double)total ? (uint64_t)std::floor(target) + 1 : total) : 1;
+  need = std::min(need, total);
+  uint64_t run = 0;
+  for (size_t i = 0; i < kept; ++i) {
+    run += weight[i];
+    if (run >= need) return (int)order[i];
+  }
+  return (int)order[0];
+}
+
 }  // namespace ta

@@ -2,10 +2,12 @@
 `generate`, `generate_with`, `greedy_tokens`."""
 from __future__ import annotations
 
+import dataclasses
 import time
 
 from .batch import StepEntry
-from .generate import Control, GenerateParams, Generated, SampleCursor, Sampled, StopReason, _go_on, _no_bytes
+from .generate import (Control, GenerateParams, Generated, SampleCursor, Sampled, StopReason, _go_on, _no_bytes,
+                       filters_of)
 
 
 def _next(engine, cursor: SampleCursor, logits, token_bytes, on_chunk):
@@ -17,7 +19,7 @@ def _next(engine, cursor: SampleCursor, logits, token_bytes, on_chunk):
         token = engine.argmax(logits, [0])[0]
     elif hasattr(engine, "sample"):
         token = engine.sample(logits, [0], [cursor.params.temperature], [cursor.params.top_p],
-                              [cursor.next_uniform()])[0]
+                              [cursor.next_uniform()], *filters_of([cursor]))[0]
     else:
         return cursor.push_logits(engine.rows_to_host(logits, [0])[0], token_bytes, on_chunk)
     return cursor.push_token(token, token_bytes, on_chunk)
@@ -76,7 +78,7 @@ def generate_with(engine, prompt: list[int], params: GenerateParams, token_bytes
                 if cursor.is_greedy:
                     engine.decode_greedy([rid], [int(outcome)], params.max_tokens - cursor.produced, on_step)
                 else:
-                    draw = lambda _k: ([params.temperature], [params.top_p], [cursor.next_uniform()])
+                    draw = lambda _k: ([params.temperature], [params.top_p], [cursor.next_uniform()], *filters_of([cursor]))
                     engine.decode_sampled([rid], [int(outcome)], params.max_tokens - cursor.produced, draw, on_step)
                 outcome = ended[0]
             while not isinstance(outcome, Sampled):
@@ -99,6 +101,101 @@ def generate(engine, prompt, params: GenerateParams, token_bytes=_no_bytes, toke
     if tokenizer is not None and token_bytes is _no_bytes:
         token_bytes = lambda token: tokenizer.decode_bytes([token])
     return generate_with(engine, prompt, params, token_bytes, _go_on)
+
+
+def generate_answers(engine, prompt, params: GenerateParams, n: int, token_bytes=_no_bytes, tokenizer=None) -> list[Generated]:
+    """`n` answers to one prompt, decoded together: the prompt is run once, its request forked (the answers share its pages of the
+    cache, which every decode step goes through once for all of them), and answer i is drawn with the seed `params.seed` + i.
+    `engine`: an `Engine` with room for `n` requests, or a bare model; `prompt`, `token_bytes`, `tokenizer` as for `generate`.
+    The times of an answer are those of all."""
+    if n < 1:
+        raise ValueError("at least one answer")
+    if isinstance(prompt, str):
+        if tokenizer is None:
+            raise ValueError("a text prompt needs a tokenizer")
+        prompt = tokenizer.encode(prompt)
+    if not prompt:
+        raise ValueError("prompt encoded to no tokens")
+    if tokenizer is not None and token_bytes is _no_bytes:
+        token_bytes = lambda token: tokenizer.decode_bytes([token])
+    cursors = [SampleCursor(dataclasses.replace(params, seed=params.seed + i)) for i in range(n)]
+    if not hasattr(engine, "step"):
+        from .engine import Engine
+        page = 16
+        engine = Engine(engine, num_pages=-(-len(prompt) // page) + n * (params.max_tokens // page + 2), page_size=page, max_requests=n)
+    rids = [("answer", id(cursors[0]), i) for i in range(n)]
+    done: list[Sampled | None] = [None] * n
+    started = time.perf_counter()
+    engine.add_request(rids[0])
+    live = [rids[0]]
+    try:
+        logits = engine.step([StepEntry(rids[0], list(prompt), [len(prompt) - 1] if params.max_tokens > 0 else [])])
+        if params.max_tokens == 0:
+            first = []
+            done = [cursor.finish_without_sample() for cursor in cursors]
+        elif cursors[0].is_greedy:
+            first = engine.argmax(logits, [0]) * n
+        else:
+            first = engine.sample(logits, [0] * n, [params.temperature] * n, [params.top_p] * n, [c.next_uniform() for c in cursors],
+                                  *filters_of(cursors))
+        prefill = time.perf_counter() - started
+        started = time.perf_counter()
+        tokens: dict[int, int] = {}                       # the answers that go on, and their next tokens
+
+        def take(answers, ids) -> bool:
+            """Hands every answer that goes on its new token; False if one ended."""
+            before = len(tokens)
+            for i, token in zip(answers, ids):
+                if done[i] is None:
+                    outcome = cursors[i].push_token(int(token), token_bytes)
+                    if isinstance(outcome, Sampled):
+                        done[i] = outcome
+                        tokens.pop(i, None)
+                    else:
+                        tokens[i] = int(outcome)
+            return len(tokens) >= before
+
+        take(range(n), first)
+        going_on = sorted(tokens)
+        if going_on:
+            # (The prompt's own request is the first answer that goes on.)
+            names = {i: rids[0] if at == 0 else rids[i] if i else rids[going_on[0]] for at, i in enumerate(going_on)}
+            others = [names[i] for i in going_on[1:]]
+            if others:
+                engine.fork_request(rids[0], others)
+                live += others
+        while tokens:
+            answers = sorted(tokens)
+            steps = min(min(params.max_tokens - cursors[i].produced for i in answers), ANSWER_BURST)
+            handled = 0
+
+            def on_step(_k, ids):
+                nonlocal handled
+                handled += 1
+                return take(answers, ids)
+
+            given = [cursors[i] for i in answers]
+            rows, ids = [names[i] for i in answers], [tokens[i] for i in answers]
+            if cursors[0].is_greedy:
+                picked = engine.decode_greedy(rows, ids, steps, on_step)
+            else:
+                draw = lambda _k: ([params.temperature] * len(given), [params.top_p] * len(given), [c.next_uniform() for c in given],
+                                   *filters_of(given))
+                picked = engine.decode_sampled(rows, ids, steps, draw, on_step)
+            for ids in picked[handled:]:                  # the step that was under way when an answer ended
+                take(answers, ids)
+            for i in answers:
+                if done[i] is not None:
+                    engine.end_request(names[i])
+                    live.remove(names[i])
+    finally:
+        for rid in live:
+            engine.end_request(rid)
+    decode = time.perf_counter() - started
+    return [Generated(d.tokens, d.text, d.chunks, d.reason, d.completion_tokens, prefill, decode) for d in done]
+
+
+ANSWER_BURST = 16       # decode steps of answers that run back to back before finished ones leave
 
 
 def greedy_tokens(engine, prompt: list[int], new_tokens: int) -> list[int]:

@@ -82,8 +82,18 @@ class StepContext:
     max_position: int                # largest position in the batch
     page_size: int
     n_wanted: int = -1               # wanted places of the real entries (the leading rows of the step's logits)
+    sharing: dict = dataclasses.field(default_factory=dict, repr=False, compare=False)   # plans of shared prefixes (`kernels.
+    #                                  SharedPrefixes`) by (cache group, query heads, kv heads, head size); single tokens only
     shared: dict = dataclasses.field(default_factory=dict, repr=False, compare=False)   # what a layer leaves for later
     #                                  layers of the same forward (emptied when a forward starts)
+
+
+    def sharing_of(self, block_table: torch.Tensor, n_q: int, n_kv: int, head_dim: int):
+        """The plan for attention of this shape over the cache group that this block table belongs to, or None."""
+        for group, table in enumerate(self.block_tables):
+            if table is block_table:
+                return self.sharing.get((group, n_q, n_kv, head_dim))
+        return None
 
 
 def build_context(entries: list[StepEntry], manager, device, table_width: int | None = None,

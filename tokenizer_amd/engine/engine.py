@@ -64,6 +64,9 @@ def random_model(config: ModelConfig, seed: int, dtype="bfloat16", device="cuda:
     return Model(config, tensors, dtype, device, ops)
 
 
+NOTHING_SHARED: dict = {}       # what `Engine.sharing` returns where requests share nothing
+
+
 class StepGraph:
     """One captured HIP graph of a step of one shape (a decode step: so many requests with one token each; any
     other step: the counts of tokens, entries, wanted places, prompt tiles and single rows its description is
@@ -83,6 +86,9 @@ class StepGraph:
         self.dev = torch.empty(size, dtype=torch.int32, device=device)
         self.ctx = build_context(entries, engine.cache, device, table_width=self.width, into=(self.host, self.dev), fill=True)
         self.ctx.max_position = bucket - 1          # what the kernels' launch sizes are planned for
+        # What the requests share is filled in again too, where it has changed (plans of one signature: they are in the graph's key).
+        self.sharing_now = engine.sharing(entries)
+        self.ctx.sharing = {shape: plan.standing_copy() for shape, plan in self.sharing_now.items()}
         ops = engine.model.runtime.ops
         before = getattr(ops, "capturing", False)
         ops.capturing = True                        # kernels are chosen by their time on the device alone
@@ -121,44 +127,47 @@ class StepGraph:
         self.draws = None                           # captured graphs of the sampler over these logits, made on demand
 
     def draw_on_device(self, engine: "Engine", temperature: list[float], top_p: list[float], uniform: list[float],
-                       any_cut: bool) -> torch.Tensor:
-        """Temperature / nucleus draws for every row of this graph's logits, left on the device (int32, one per
-        row; the rows past the given ones only fill the step up): the sampler's twenty small launches are captured
-        once (per kind: with or without the rounds of the nucleus cut) and replayed.  Nothing waits for the result
-        here."""
+                       any_cut: bool, top_k: list[int] | None = None, min_p: list[float] | None = None) -> torch.Tensor:
+        """Draws for every row of this graph's logits, left on the device (int32, one per row; the rows past the given
+        ones only fill the step up): the sampler's launches are captured once per kind (`Engine.draw_rows`: with or without the rounds
+        of the nucleus cut, with or without rows under top-k or min-p) and replayed.  Nothing waits for the result here."""
         rows = self.logits.shape[0]
         given = len(temperature)
         fill = [1.0] * (rows - given)
         temperature, top_p, uniform = list(temperature) + fill, list(top_p) + fill, list(uniform) + [0.5] * (rows - given)
+        top_k = list(top_k or [0] * given) + [0] * (rows - given)
+        min_p = list(min_p or [0.0] * given) + [0.0] * (rows - given)
+        filtered = [k > 0 or p > 0 for k, p in zip(top_k, min_p)]
+        # (Rows that only fill the step up are drawn with the others: what they get is not looked at.)
+        kind = (any_cut, "none" if not any(filtered) else "all" if all(filtered[:given]) else "some")
         if self.draws is None:
             self.draws = {}
-            self.draw_host = torch.empty((3, rows), dtype=torch.float32).pin_memory()
-            self.draw_params = torch.empty((3, rows), dtype=torch.float32, device=self.logits.device)
+            self.draw_host = torch.empty((6, rows), dtype=torch.float32).pin_memory()
+            self.draw_params = torch.empty((6, rows), dtype=torch.float32, device=self.logits.device)
             self.draw_ids = torch.zeros(rows, dtype=torch.int32, device=self.logits.device)
             self.draw_uploaded = torch.cuda.Event()
         self.draw_uploaded.synchronize()              # the last draw's numbers have left the pinned buffer
-        self.draw_host.copy_(torch.tensor([temperature, top_p, uniform], dtype=torch.float32))
+        self.draw_host[:5].copy_(torch.tensor([temperature, top_p, uniform, min_p, [float(f) for f in filtered]], dtype=torch.float32))
+        self.draw_host[5].view(torch.int32).copy_(torch.tensor(top_k, dtype=torch.int32))
         self.draw_params.copy_(self.draw_host, non_blocking=True)
         self.draw_uploaded.record()
-        ops = engine.model.runtime.ops
-        launch = lambda: ops.sample(self.logits, self.draw_params[0], self.draw_params[1], self.draw_params[2],
-                                    out=self.draw_ids, any_cut=any_cut)
-        captured = self.draws.get(any_cut)
+        launch = lambda: engine.draw_rows(self.logits, self.draw_params, kind, out=self.draw_ids)
+        captured = self.draws.get(kind)
         if captured is None:
             launch()                                      # once eagerly: the draw of this call, and a warm-up
             torch.cuda.synchronize(self.logits.device)
             captured = torch.cuda.CUDAGraph()
             with torch.cuda.graph(captured, pool=engine.graph_pool):
                 launch()
-            self.draws[any_cut] = captured
+            self.draws[kind] = captured
         else:
             captured.replay()
         return self.draw_ids
 
     def draw(self, engine: "Engine", temperature: list[float], top_p: list[float], uniform: list[float],
-             any_cut: bool) -> list[int]:
+             any_cut: bool, top_k: list[int] | None = None, min_p: list[float] | None = None) -> list[int]:
         """The same draws, brought to the host: one id for each of the given rows."""
-        ids = self.draw_on_device(engine, temperature, top_p, uniform, any_cut)
+        ids = self.draw_on_device(engine, temperature, top_p, uniform, any_cut, top_k, min_p)
         return [int(v) for v in ids.cpu().tolist()][:len(temperature)]
 
     def run(self, engine: "Engine", entries: list[StepEntry], tokens_on_device: torch.Tensor | None = None) -> torch.Tensor:
@@ -185,6 +194,11 @@ class StepGraph:
             self.uploads += 1
             if tokens_on_device is not None:
                 self.dev[:count].copy_(tokens_on_device[:count], non_blocking=True)
+        plans = engine.sharing(entries)
+        if plans is not self.sharing_now:
+            for shape, plan in plans.items():
+                self.ctx.sharing[shape].take(plan)
+            self.sharing_now = plans
         self.graph.replay()
         if self.advances:
             self.on_device = next_decode_description(packed, count, manager.page_size, self.width, len(self.ctx.slots))
@@ -238,8 +252,12 @@ class Engine:
     def __init__(self, model: Model, num_pages: int | None = None, page_size: int = 16, max_requests: int = 8,
                  max_tokens: int | None = None, prefix_cache: bool = False, use_graphs: bool | None = None,
                  num_blocks: int | None = None, max_batch_size: int | None = None,
-                 max_num_batched_tokens: int = 2048):
-        """`num_blocks` and `max_batch_size` are the reference's names (qwen-server/src/lib.rs:33-56) for
+                 max_num_batched_tokens: int = 2048, shared_attention: bool | None = None):
+        """`shared_attention`: whether decode steps go through keys that several of their requests share once for all of them
+        (attention that sees every key; sums fall apart differently then, so logits differ in their last bits).  None: where
+        requests are forks of one (`fork_request`); True: wherever leading pages are shared, by the prefix cache too; False: never.
+
+        `num_blocks` and `max_batch_size` are the reference's names (qwen-server/src/lib.rs:33-56) for
         `num_pages` and `max_requests`; `max_num_batched_tokens` is the token budget of `run()`.  Without
         `num_pages` the pool is made for `max_tokens`: the most tokens that live requests hold at any time, each
         request's count rounded up to a multiple of 64."""
@@ -265,6 +283,10 @@ class Engine:
                                                 block_state=self.pools.block_states.get(
                                                     entry.layer if entry.unit is None else entry.unit),
                                                 writes=entry.cache_of is None))
+        self.shared_attention = shared_attention
+        self._family: set = set()    # requests that were forked or are forks
+        self._sharing: tuple | None = None        # (epoch, requests), their plans
+        self._shared_shapes = self._shapes_that_share()
         self.steps = 0
         self._landing: dict[int, tuple] = {}     # pinned rows and events of `decode_greedy` / `decode_sampled`, by batch size
         self.steps_replayed = 0      # steps (decode steps and others) that replayed a captured graph
@@ -292,17 +314,43 @@ class Engine:
             picked = self.model.runtime.ops.argmax(logits).cpu().tolist()
         return picked if rows is None else [picked[row] for row in rows]
 
+    def draw_rows(self, logits: torch.Tensor, numbers: torch.Tensor, kind: tuple, out: torch.Tensor) -> torch.Tensor:
+        """Draws for all rows of `logits` into `out`, without a wait.  `numbers` float32 [6, rows] on the device: temperature, top_p,
+        uniform number, min_p, whether the row has top-k or min-p, and top_k (int32 bits).  `kind`: whether a row cuts by top_p, and
+        which rows have top-k or min-p ("none", "some", "all"): those are drawn in whole weights (`Ops.sample_filtered`), the others as
+        they are without such rows beside them, so a request's draw does not depend on who else is in the batch."""
+        ops, (any_cut, which) = self.model.runtime.ops, kind
+        temperature, top_p, uniform, min_p, filtered = numbers[:5]
+        if which != "all":
+            ops.sample(logits, temperature, top_p, uniform, out=out, any_cut=any_cut)
+        if which != "none":
+            top_k = numbers[5].view(torch.int32)
+            if which == "all":
+                ops.sample_filtered(logits, temperature, top_k, top_p, min_p, uniform, out=out)
+            else:
+                drawn = ops.sample_filtered(logits, temperature, top_k, top_p, min_p, uniform)
+                out.copy_(torch.where(filtered > 0, drawn, out))
+        return out
+
     def sample(self, logits: torch.Tensor, rows: list[int], temperature: list[float], top_p: list[float],
-               uniform: list[float]) -> list[int]:
-        """Temperature / nucleus draws for the given rows of a step's logits, on the device; one uniform
-        number per row (from the request's own generator).  Draws for all rows of a replayed step's logits
+               uniform: list[float], top_k: list[int] | None = None, min_p: list[float] | None = None) -> list[int]:
+        """Draws under temperature and top_p (and, where they are given, top_k and min_p) for the given rows of a step's logits,
+        on the device; one uniform number per row (from the request's own generator).  Draws for all rows of a replayed step's logits
         replay a captured graph of the sampler's launches as well."""
         device = logits.device
         any_cut = any(p < 1.0 for p in top_p)
+        top_k, min_p = top_k or [0] * len(rows), min_p or [0.0] * len(rows)
+        filtered = [k > 0 or p > 0 for k, p in zip(top_k, min_p)]
         graph = self._graph_result
         if graph is not None and self._is_result_of(logits, graph) and rows == list(range(logits.shape[0])):
-            return graph.draw(self, temperature, top_p, uniform, any_cut)
+            return graph.draw(self, temperature, top_p, uniform, any_cut, top_k, min_p)
         picked = logits if rows == list(range(logits.shape[0])) else logits[torch.tensor(rows, device=device)]
+        if any(filtered):
+            packed = torch.tensor([temperature, top_p, uniform, min_p, [float(f) for f in filtered], [0.0] * len(rows)], dtype=torch.float32)
+            packed[5].view(torch.int32).copy_(torch.tensor(top_k, dtype=torch.int32))
+            out = torch.empty(len(rows), dtype=torch.int32, device=device)
+            ids = self.draw_rows(picked.contiguous(), packed.to(device, non_blocking=True), (any_cut, "all" if all(filtered) else "some"), out)
+            return [int(v) for v in ids.cpu().tolist()]
         # One copy to the device for the three vectors.
         packed = torch.tensor([temperature, top_p, uniform], dtype=torch.float32).to(device, non_blocking=True)
         ids = self.model.runtime.ops.sample(picked.contiguous(), packed[0], packed[1], packed[2], any_cut=any_cut)
@@ -332,8 +380,8 @@ class Engine:
 
     def decode_sampled(self, rids: list, tokens: list[int], n_steps: int, draw, on_step=None) -> list[list[int]]:
         """The same run of decode steps with temperature / nucleus draws in place of the greedy pick.  `draw(k)`
-        gives step k's (temperature, top_p, uniform) lists, one number of each per request; it is asked when step
-        k is launched, once for every step that runs (so a request's generator hands out exactly one uniform
+        gives step k's (temperature, top_p, uniform) lists, one number of each per request, or these and (top_k, min_p) behind them; it is
+        asked when step k is launched, once for every step that runs (so a request's generator hands out exactly one uniform
         number per token it is given, also when the run ends early).  A request whose temperature is 0 keeps the
         greedy pick (its other two numbers are not looked at)."""
         return self._decode_run(rids, tokens, n_steps, on_step, draw)
@@ -361,8 +409,9 @@ class Engine:
                 logits = self.step([StepEntry(rid, [int(t)], [0]) for rid, t in zip(rids, current)])
                 current = self.argmax(logits)
                 if draw is not None:
-                    temperature, top_p, uniform, greedy = self._warm_numbers(*draw(k))
-                    drawn = self.sample(logits, list(range(count)), temperature, top_p, uniform)
+                    temperature, top_p, uniform, *filters = draw(k)
+                    temperature, top_p, uniform, greedy = self._warm_numbers(temperature, top_p, uniform)
+                    drawn = self.sample(logits, list(range(count)), temperature, top_p, uniform, *filters)
                     current = [pick if g else token for g, pick, token in zip(greedy, current, drawn)]
                 picked.append(list(current))
                 if on_step is not None and on_step(k, picked[-1]) is False:
@@ -391,8 +440,9 @@ class Engine:
             if draw is None:
                 previous = graph.ids
             else:
-                temperature, top_p, uniform, greedy = self._warm_numbers(*draw(k))
-                previous = graph.draw_on_device(self, temperature, top_p, uniform, any(p < 1.0 for p in top_p))
+                temperature, top_p, uniform, *filters = draw(k)
+                temperature, top_p, uniform, greedy = self._warm_numbers(temperature, top_p, uniform)
+                previous = graph.draw_on_device(self, temperature, top_p, uniform, any(p < 1.0 for p in top_p), *filters)
                 if any(greedy):
                     if greedy != greedy_rows:
                         greedy_rows, greedy_mask = greedy, torch.tensor(greedy, device=previous.device)
@@ -430,6 +480,9 @@ class Engine:
         # (The bucket is what the kernels' launch shapes are planned for, with any page size: an eager step plans
         # for its context rounded up in the same way, so both cut their sums alike.)
         bucket = -(-longest // self.GRAPH_BUCKET) * self.GRAPH_BUCKET
+        plans = self.sharing(entries)
+        if plans:
+            return (self._shape_of(entries), bucket, tuple((shape, plans[shape].signature) for shape in sorted(plans)))
         return (self._shape_of(entries), bucket)
 
     def _graph_for(self, entries: list[StepEntry]) -> "StepGraph":
@@ -481,7 +534,72 @@ class Engine:
         self._graph_result = graph
         return logits
 
+    # -------------------------------------------------------------------- sharing
+    SHARED_FILL = 32        # a plan's list of work is filled up to a multiple of this, so that plans can share a captured graph
+
+    def _shapes_that_share(self) -> list[tuple]:
+        """(cache group, query heads, kv heads, head size) of the attention that can use a plan of shared prefixes."""
+        ops, shapes = self.model.runtime.ops, set()
+        if not hasattr(ops, "shared_prefix_attention") or self.cache.page_size % 16:
+            return []
+        for entry, cache in zip(self.model.spec.schedule, self.layer_caches):
+            mixer = getattr(self.model.decoder.blocks[entry.layer], "mixer", None)
+            shape = getattr(mixer, "shared_shape", lambda: None)()
+            if shape is not None and cache.group is not None and shape[2] in ops.DECODE_HEAD_DIMS:
+                shapes.add((cache.group, *shape))
+        return sorted(shapes)
+
+    def sharing(self, entries: list[StepEntry]) -> dict:
+        """The plans of what the requests of a step of single tokens share, by the shape of the attention that takes them; empty where
+        nothing is shared.  Worked out when the requests of a step change, and kept while they stay."""
+        if self.shared_attention is False or not self._shared_shapes or len(entries) < 2 or any(len(e.tokens) != 1 for e in entries):
+            return NOTHING_SHARED
+        if self.shared_attention is None and sum(e.rid in self._family for e in entries) < 2:
+            return NOTHING_SHARED
+        key = (self.cache.epoch, tuple(e.rid for e in entries))
+        if self._sharing is not None and self._sharing[0] == key:
+            return self._sharing[1]
+        positions = [self.cache.seq_len(e.rid) for e in entries]
+        plans = {}
+        for group, n_q, n_kv, head_dim in self._shared_shapes:
+            tables = [self.cache.table(e.rid, group) for e in entries]
+            width = max([1] + [len(t) for t in tables])
+            table = np.array([t + [-1] * (width - len(t)) for t in tables], dtype=np.int32)
+            plan = self.model.runtime.ops.plan_shared_prefixes(table, positions, self.cache.page_size, n_q, n_kv, head_dim, self.model.dtype,
+                                                               self.model.device, fill=self.SHARED_FILL)
+            if plan.runs:
+                plans[(group, n_q, n_kv, head_dim)] = plan
+        plans = plans or NOTHING_SHARED
+        self._sharing = (key, plans)
+        return plans
+
     # ------------------------------------------------------------------ requests
+    def fork_request(self, rid, new_rids) -> None:
+        """Make every one of `new_rids` a live request that holds what `rid` holds: the same tokens, to be continued on their own.  Full
+        pages are shared; the last one, where it is not full, is copied for each, and so is what layers keep in the request's slot.
+        `OutOfPages` with nothing changed if a slot or a page is missing."""
+        new_rids, made, copies, slots = list(new_rids), [], [], []
+        try:
+            for new_rid in new_rids:
+                pages, pair = self.cache.fork(rid, new_rid)
+                made.append(new_rid)
+                copies += pages
+                slots.append(pair)
+        except (OutOfPages, KeyError):
+            for new_rid in made:
+                self.cache.release(new_rid)
+            raise
+        self.pools.copy_pages(copies, self.model.runtime.ops)
+        for src, dst in slots:
+            self.pools.copy_states(src, dst)
+        self._family.update(new_rids, [rid])
+
+    def compact_cache(self) -> int:
+        """Bring the pages in use to the lowest ids of their pools; returns how many moved.  Requests go on as before."""
+        moves = self.cache.compact()
+        self.pools.copy_pages(moves, self.model.runtime.ops)
+        return len(moves)
+
     def add_request(self, rid, params=None, **callbacks):
         """`add_request(rid)` makes `rid` a live request for `step()`.  `add_request(prompt_ids, GenerateParams)`
         queues a generation for `run()` instead and returns its id (a scheduler over this engine is made at the
@@ -507,6 +625,7 @@ class Engine:
 
     def end_request(self, rid) -> None:
         self.cache.release(rid)
+        self._family.discard(rid)
 
     def has_request(self, rid) -> bool:
         return self.cache.has_request(rid)
@@ -564,6 +683,7 @@ class Engine:
             logits = self._graph_step(entries)
         else:
             ctx = build_context(entries, self.cache, self.model.device, fill=True)
+            ctx.sharing = self.sharing(entries)
             logits = self.model.decoder.forward(ctx, self.layer_caches)
         if logits.shape[0] != wanted:
             logits = logits[:wanted]        # the rows behind them belong to what the step was filled up with

@@ -11,7 +11,8 @@ import dataclasses
 import enum
 from typing import Callable
 
-from ..sampling.host import Rng, SampleError, check_params, sample_with_uniform, greedy_token
+from ..sampling.host import (Rng, SampleError, check_filters, check_params, greedy_token, sample_filtered,
+                             sample_with_uniform)
 from .stream import StreamDecoder
 
 
@@ -35,6 +36,13 @@ class GenerateParams:
     seed: int = 0
     eos: list[int] = dataclasses.field(default_factory=list)
     stop: list[str] = dataclasses.field(default_factory=list)
+    top_k: int = 0              # draws come from the so many likeliest tokens; 0: from all
+    min_p: float = 0.0          # ... and from those of at least this share of the likeliest one's probability
+
+    @property
+    def filtered(self) -> bool:
+        """Whether draws go beyond temperature and top_p."""
+        return self.top_k > 0 or self.min_p > 0
 
     @classmethod
     def greedy(cls, max_tokens: int) -> "GenerateParams":
@@ -64,6 +72,7 @@ class Generated:
 def validate(params: GenerateParams) -> None:
     """generate.rs:409-426."""
     check_params(params.temperature, params.top_p)
+    check_filters(params.top_k, params.min_p)
     if params.max_tokens < 0:
         raise SampleError("max_tokens is negative")
     if any(stop == "" for stop in params.stop):
@@ -171,6 +180,9 @@ class SampleCursor:
             return self.finish(StopReason.MaxTokens, on_chunk)
         if self.is_greedy:
             token = greedy_token(logits)
+        elif self.params.filtered:
+            token = sample_filtered(logits, self.params.temperature, self.params.top_k, self.params.top_p, self.params.min_p,
+                                    self.next_uniform())
         else:
             token = sample_with_uniform(logits, self.params.temperature, self.params.top_p, self.next_uniform())
         return self.push_token(token, token_bytes, on_chunk)
@@ -227,6 +239,14 @@ class SampleCursor:
             self.chunks.append(piece)
             self.text += piece
         return on_chunk(piece) or Control.Continue
+
+
+def filters_of(cursors) -> tuple:
+    """The cursors' top_k and min_p as `Engine.sample` and `Engine.decode_sampled` take them behind the other numbers; nothing if no
+    cursor has any (an engine that knows temperature and top_p alone is then asked as ever)."""
+    if not any(c.params.filtered for c in cursors):
+        return ()
+    return ([0 if c.is_greedy else c.params.top_k for c in cursors], [0.0 if c.is_greedy else c.params.min_p for c in cursors])
 
 
 def parse_eos_token_ids(text: str) -> list[int]:

@@ -31,7 +31,7 @@ import numpy as np
 from .. import host as _host
 from .batch import StepEntry
 from .generate import (Control, GenerateParams, Generated, SampleCursor, Sampled, StopReason, _go_on,
-                       _no_bytes)
+                       _no_bytes, filters_of)
 
 
 @dataclasses.dataclass
@@ -249,7 +249,7 @@ class Scheduler:
             # who else is in the batch.
             cursors = [wanting[row].cursor for row in warm_rows]
             tokens = self.engine.sample(logits, warm_rows, [c.params.temperature for c in cursors],
-                                        [c.params.top_p for c in cursors], [c.next_uniform() for c in cursors])
+                                        [c.params.top_p for c in cursors], [c.next_uniform() for c in cursors], *filters_of(cursors))
             for row, token in zip(warm_rows, tokens):
                 picked[row] = int(token)
         elif warm_rows:
@@ -357,7 +357,7 @@ class Scheduler:
         else:
             # (A greedy sequence among them has temperature 0, keeps the greedy pick and has no number to give.)
             draw = lambda k: ([c.params.temperature for c in cursors], [c.params.top_p for c in cursors],
-                              [0.5 if c.is_greedy else c.next_uniform() for c in cursors])
+                              [0.5 if c.is_greedy else c.next_uniform() for c in cursors], *filters_of(cursors))
             picked = self.engine.decode_sampled(rids, tokens, burst, draw, on_step=lambda k, ids: take(ids))
         for ids in picked[handled:]:      # the step that was under way when a sequence ended
             take(ids)

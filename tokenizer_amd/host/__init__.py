@@ -55,6 +55,9 @@ _SIGNATURES = {
     "ta_cache_detach": (_int, [_vp, _i64]),
     "ta_cache_attach_shared_prefix": (_int, [_vp, _i64, _i32p, _int]),
     "ta_cache_publish": (_int, [_vp, _i64, _i32p, _int]),
+    "ta_cache_fork": (_int, [_vp, _i64, _i64, _i32p, _i32p, _i32p]),
+    "ta_cache_compact": (_int, [_vp, _i32p]),
+    "ta_cache_epoch": (_i64, [_vp]),
     "ta_cache_check": (_int, [_vp]),
     "ta_cache_pack_batch": (_i64, [_vp, _int, _i64p, _i32p, _i32p, _i32p, _i32p, _int, _i64p, _i32p, _i64, _i64p,
                                    _i32p, _i32p]),
@@ -78,6 +81,7 @@ _SIGNATURES = {
     "ta_bpe_decode": (_i64, [_vp, _i32p, _int, ctypes.c_char_p, _i64, _i32p]),
     "ta_uniform_f32": (_f32, [_u64, _u64]),
     "ta_greedy_token": (_int, [_f32p, _i64]),
+    "ta_sample_filtered_host": (_int, [_f32p, _i64, _f32, _int, _f32, _f32, _f32]),
     "ta_sample_with_uniform": (_int, [_f32p, _i64, _f32, _f32, _f32]),
 }
 

@@ -1302,7 +1302,8 @@ class Ops:
         positions, entry_of_token int32 [T]; block_table int32 [E, P]; a token at position p sees keys
         max(0, p - window)..p.  `max_position` (host) lets the wrapper check that the table is wide enough.
         `batch` (a StepContext of the same tokens) lets the tiled kernel run on prompt portions and the split
-        kernel on single tokens; without it every token goes through the latter.
+        kernel on single tokens; without it every token goes through the latter.  A batch of single tokens that says what its
+        requests share (`StepContext.sharing`) goes through `shared_prefix_attention` where the form allows it.
         """
         _dev(qkv, out, k_pages, v_pages, positions, entry_of_token, block_table)
         n_tokens = qkv.shape[0]
@@ -1312,6 +1313,12 @@ class Ops:
             _need(extra is None or (extra.dtype == torch.float32 and extra.numel() == n_q), "slopes and sinks are float32 [n_q]")
         _need(chunk is None or chunk > 0, "a chunk has at least one position")
         plain = value_dim == head_dim and chunk is None and slopes is None     # (but for the sinks)
+        if batch is not None and getattr(batch, "sharing", None) and self.use_fast_attention:
+            plan = batch.sharing_of(block_table, n_q, n_kv, head_dim)
+            if (plan is not None and plain and window is None and not tied_values and value_heads in (None, n_kv)
+                    and (qkv.shape[1] * qkv.element_size()) % 16 == 0):
+                return self.shared_prefix_attention(qkv, out, k_pages, v_pages, positions, block_table, plan, n_q, n_kv, head_dim, scale,
+                                                    max_position, sinks, softcap)
         value_heads = n_kv if value_heads is None else int(value_heads)
         keep_first = int(keep_first) if window is not None else 0
         _need(value_heads > 0 and n_kv % value_heads == 0 and keep_first >= 0, "value heads divide the key heads")
@@ -1514,11 +1521,12 @@ class Ops:
         return out
 
     def plan_shared_prefixes(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int,
-                             dtype: torch.dtype, device="cuda:0") -> SharedPrefixes:
+                             dtype: torch.dtype, device="cuda:0", fill: int = 0) -> SharedPrefixes:
         """What the requests of a batch of single tokens share, laid out for `shared_prefix_attention`.
 
         block_table (on the host) int [B, P]: row i's pages, -1 where there is none; positions (on the host) int [B]: where the rows'
-        newest tokens stand.  A plan holds as long as the rows keep their order, their leading pages and do not go back."""
+        newest tokens stand.  A plan holds as long as the rows keep their order, their leading pages and do not go back.  `fill`: the list
+        of work is filled up to a multiple of so many items, so that plans that differ a little have one size."""
         import numpy as np
         table, positions = np.asarray(block_table), np.asarray(positions)
         _need(table.ndim == 2 and table.shape[1] >= 1 and positions.shape == (table.shape[0],), "one block table row and one position a request")
@@ -1526,7 +1534,7 @@ class Ops:
         _need(page_size >= 16 and page_size % 16 == 0, "pages of a multiple of sixteen tokens")
         _need(head_dim in self.DECODE_HEAD_DIMS, f"head sizes {self.DECODE_HEAD_DIMS}")
         _code(dtype)
-        return SharedPrefixes(table, positions, page_size, n_q, n_kv, head_dim, dtype, device)
+        return SharedPrefixes(table, positions, page_size, n_q, n_kv, head_dim, dtype, device, fill)
 
     def shared_prefix_attention(self, qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                                 positions: torch.Tensor, block_table: torch.Tensor, plan: SharedPrefixes, n_q: int, n_kv: int,

@@ -69,7 +69,8 @@ class SharedPrefixes:
     MIN_PART = 128                # keys of a workgroup's part of a run, at least (a block of 32 for each of its four waves)
     TARGET = 1024                 # workgroups that the parts aim at
 
-    def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device):
+    def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device,
+                 fill: int = 0):
         table = np.asarray(block_table, dtype=np.int32)
         self.n_rows, self.page_size, self.n_q, self.n_kv, self.head_dim, self.dtype = (
             table.shape[0], int(page_size), int(n_q), int(n_kv), int(head_dim), dtype)
@@ -92,12 +93,37 @@ class SharedPrefixes:
             parts_of[run.rows] = first + -(-(run.key_end - run.key_begin) // keys)
         items.sort(key=lambda item: item[3] - item[4])    # long ones first
         self.n_items = len(items)
+        if fill:                                          # (up to a multiple, with items without columns: plans of one size)
+            items += [(0,) * 8] * (-len(items) % fill)
+            self.n_items = len(items)
         self.shared_parts = int(parts_of.max(initial=0))
         self.own_begin = own_begin                        # int32 [B] on the host
         self.keys_end = max((run.key_end for run in self.runs), default=0)
         self.smallest_own = int(own_begin.min(initial=0)) if self.n_rows else 0
         packed = np.concatenate([np.asarray(items, dtype=np.int32).reshape(-1), np.asarray(self.order, dtype=np.int32), own_begin,
                                  parts_of]).astype(np.int32)
-        on_device = torch.from_numpy(packed).to(device)
+        self._on_device(torch.from_numpy(packed).to(device))
+
+    def _on_device(self, packed: torch.Tensor) -> None:
+        self.packed = packed
         sizes = [8 * self.n_items] + [self.n_rows] * 3
-        self.items, self.order_dev, self.own_begin_dev, self.parts_dev = torch.split(on_device, sizes)
+        self.items, self.order_dev, self.own_begin_dev, self.parts_dev = torch.split(packed, sizes)
+
+    @property
+    def signature(self) -> tuple:
+        """What a launch depends on beside the tables: plans of one signature may take each other's place in a captured graph."""
+        return (self.n_rows, self.n_items, self.shared_parts, self.smallest_own, self.n_q, self.n_kv, self.head_dim, self.page_size,
+                self.dtype)
+
+    def standing_copy(self) -> "SharedPrefixes":
+        """The same plan in memory of its own, which `take` fills with others of its signature (for a captured graph)."""
+        copy = SharedPrefixes.__new__(SharedPrefixes)
+        copy.__dict__.update(self.__dict__)
+        copy._on_device(self.packed.clone())
+        return copy
+
+    def take(self, other: "SharedPrefixes") -> None:
+        if other.signature != self.signature:
+            raise ValueError("a plan of another make")
+        self.order, self.runs, self.own_begin, self.keys_end = other.order, other.runs, other.own_begin, other.keys_end
+        self.packed.copy_(other.packed, non_blocking=True)

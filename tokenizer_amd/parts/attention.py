@@ -227,6 +227,16 @@ class GQAttention(Mixer):
         return CacheNeed(kind=kind, n_kv_heads=spec.n_kv_heads, head_dim=spec.head_dim, window=spec.window,
                          tied_values=spec.tied_values, value_dim=spec.value_dim or 0, keep_first=int(spec.keep_first) if spec.window is not None else 0)
 
+    def shared_shape(self):
+        """Every key of the sequence, one softmax a head, values of the keys' number and size; sinks and a cap are no hindrance."""
+        if self.window is not None or self.dv != self.d:
+            return None
+        if self.extended:
+            takes = self.maps == 1 and not self.tied and self.talk is None
+        else:
+            takes = self.chunk is None and self.slopes is None
+        return (self.n_q, self.n_kv, self.d) if takes else None
+
     def repeatable(self):
         position = repeatable_of(self.position)
         if position is None or not self.plain or self.extended:

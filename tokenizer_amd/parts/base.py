@@ -167,6 +167,11 @@ class Mixer(Part):
     def forward(self, x: torch.Tensor, ctx, cache) -> torch.Tensor:
         raise NotImplementedError
 
+    def shared_shape(self) -> tuple[int, int, int] | None:
+        """(query heads, kv heads, head size) of a mixer whose attention of single tokens can go through keys that several requests
+        share once for all of them (`ctx.sharing`); None for every other."""
+        return None
+
     def forward_normed(self, residual, delta, norm: Norm, ctx, cache):
         """The sub-layer from the residual stream on: add `delta`, normalise, mix.  Returns the output still
         to be added to the stream, or None if the part added it itself.  A part may override this to fold

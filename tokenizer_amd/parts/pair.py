@@ -51,6 +51,10 @@ class SideBySide(Mixer):
             need = dataclasses.replace(need, state_shape=stateful[0].state_shape, state_dtype=stateful[0].state_dtype)
         return need
 
+    def shared_shape(self):
+        shapes = [shape for shape in (part.shared_shape() for part in self.parts) if shape is not None]
+        return shapes[0] if shapes else None              # (at most one of the two keeps pages)
+
     def forward(self, x, ctx, cache):
         ops = self.runtime.ops
         out = ScaledSum(ops)

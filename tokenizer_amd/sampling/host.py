@@ -57,6 +57,16 @@ def check_params(temperature: float, top_p: float) -> None:
         raise SampleError(f"top_p {top_p} is negative")
 
 
+def check_filters(top_k: int, min_p: float) -> None:
+    """top-k counts tokens (0 keeps all of them), min-p is a share of the largest weight (0 keeps all)."""
+    if isinstance(top_k, bool) or int(top_k) != top_k or not 0 <= top_k < 2 ** 31:
+        raise SampleError(f"top_k {top_k} is not a count of tokens")
+    if not math.isfinite(min_p):
+        raise SampleError(f"min_p {min_p} is not finite")
+    if not 0 <= min_p <= 1:
+        raise SampleError(f"min_p {min_p} is not between 0 and 1")
+
+
 def greedy_token(logits) -> int:
     """Lowest index among the maxima; NaN never wins (a scan with `>` from -inf, sample.rs:43-56)."""
     values = _logits(logits)
@@ -74,10 +84,29 @@ def sample_with_uniform(logits, temperature: float, top_p: float, uniform: float
                                                   uniform))
 
 
-def sample_token(logits, temperature: float, top_p: float, rng: Rng) -> int:
-    """Draw one token (sample.rs:68-137).  Temperature 0 is greedy and draws nothing from `rng`."""
+def sample_filtered(logits, temperature: float, top_k: int, top_p: float, min_p: float, uniform: float) -> int:
+    """The draw under temperature, top-k, top-p and min-p for a given uniform number in [0, 1), as `Ops.sample_filtered` makes it on the
+    device: weights exp((x - max) / T) in whole units of 2^-44, falling logit with the lower index first among equals; kept are the
+    first top_k tokens (0: all), of those the shortest prefix that reaches top_p of their weight, of those the ones of at
+    least min_p times the largest weight."""
     values = _logits(logits)
     check_params(temperature, top_p)
+    check_filters(top_k, min_p)
+    token = int(_host.lib().ta_sample_filtered_host(values.ctypes.data_as(_f32p), values.size, temperature, int(top_k), top_p, min_p,
+                                                    uniform))
+    if token < 0:
+        raise SampleError(f"{values.size} logits are more than a draw takes")
+    return token
+
+
+def sample_token(logits, temperature: float, top_p: float, rng: Rng, top_k: int = 0, min_p: float = 0.0) -> int:
+    """Draw one token (sample.rs:68-137).  Temperature 0 is greedy and draws nothing from `rng`.  With `top_k` or `min_p` the draw is
+    `sample_filtered`'s."""
+    values = _logits(logits)
+    check_params(temperature, top_p)
+    check_filters(top_k, min_p)
     if temperature == 0:
         return greedy_token(values)
+    if top_k or min_p:
+        return sample_filtered(values, temperature, top_k, top_p, min_p, rng.random_f32())
     return sample_with_uniform(values, temperature, top_p, rng.random_f32())
