@@ -179,7 +179,7 @@ class Ops:
                      "ta_talking_prefill_parts", "ta_retention_scan", "ta_retention_chunked", "ta_temper_store",
                      "ta_add_slabs_rmsnorm", "ta_experts_few", "ta_experts_few_shared_parts",
                      "ta_fused_qk_temper",
-                     "ta_expert_gate_slots", "ta_sample_filtered", "ta_copy_pages", "ta_shared_prefix_attention"):
+                     "ta_expert_gate_slots", "ta_sample_filtered", "ta_sample_filtered_workspace", "ta_copy_pages", "ta_shared_prefix_attention"):
             getattr(self.lib, name).restype = ctypes.c_int
         self.lib.ta_grouped_gemm_bf16.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
                                                   ctypes.c_int, ctypes.c_void_p, ctypes.c_long, ctypes.c_int, ctypes.c_void_p,
@@ -2450,8 +2450,11 @@ class Ops:
             out = torch.empty(n_rows, dtype=torch.int32, device=logits.device)
         _need(out.dtype == torch.int32 and out.numel() == n_rows, "sample output must be int32 [B]")
         _here(logits, temperature, top_k, top_p, min_p, uniform, out)
+        _need(n_rows <= 65535, "at most 65535 rows")
+        row_bytes = self.lib.ta_sample_filtered_workspace(vocab)
+        workspace = torch.empty(n_rows * row_bytes, dtype=torch.uint8, device=logits.device) if row_bytes else None
         self._check(self.lib.ta_sample_filtered(_ptr(logits), ctypes.c_int64(logits.stride(0)), _ptr(temperature), _ptr(top_k), _ptr(top_p),
-                                                _ptr(min_p), _ptr(uniform), _ptr(out), n_rows, vocab, _code(logits.dtype), self._stream()),
+                                                _ptr(min_p), _ptr(uniform), _ptr(out), _ptr(workspace), n_rows, vocab, _code(logits.dtype), self._stream()),
                     "sample_filtered")
         return out
 
