@@ -153,6 +153,37 @@ def test_most_of_a_row_in_one_place(ops):
     check_draws(ops, logits.cuda(), uniform=[0.2, 0.5, 0.9, 0.99, 0.4, 0.7], top_p=[1, 0.9, 0.95, 1, 1, 0.6], top_k=[0, 0, 0, 30000, 50001, 0])
 
 
+@pytest.mark.parametrize("vocab", [300, 40000, 151936])
+@pytest.mark.parametrize("masked", [float("-inf"), torch.finfo(torch.float32).min, -1e30, -1000.0])
+def test_masked_rows(ops, vocab, masked):
+    # Most of a row ruled out, by what no number is below or by a number far below: few tokens are left, and fewer than top-k asks for.
+    logits = hills(12, vocab, torch.float32, 9)
+    gen = torch.Generator().manual_seed(vocab)
+    for row, left in enumerate([1, 2, 3, 7, 40, 41, 64, 100, 150, 250, 299, 300]):
+        keep = torch.randperm(vocab, generator=gen)[:left].cuda()
+        mask = torch.ones(vocab, dtype=torch.bool).cuda()
+        mask[keep] = False
+        logits[row, mask] = masked
+    uniform = np.random.default_rng(3).uniform(0, 1, 12)
+    for given in (dict(), dict(top_k=40), dict(top_k=200), dict(top_k=40, top_p=0.9), dict(min_p=0.02), dict(top_k=20, min_p=0.3), dict(top_p=0.8),
+                  dict(top_k=60, temperature=30.0)):
+        check_draws(ops, logits, uniform=uniform, **given)
+
+
+@pytest.mark.parametrize("vocab", [20481, 30000, 151936])
+def test_draws_under_counts_around_those_of_the_waves(ops, vocab):
+    # (A row in pieces of 4,096 logits has four waves a piece.)
+    waves = 4 * -(-vocab // 4096)
+    counts = [1, 2, waves - 1, waves, waves + 1, 2 * waves, 1000, 8191, 8192, 8193, vocab - 1, vocab, vocab + 1]
+    logits = hills(len(counts), vocab, torch.float32, 10)
+    logits[3] = logits[3].sort().values                       # the largest side by side, at the end and at the start
+    logits[4] = logits[4].sort(descending=True).values
+    logits[1, :] = 1.0
+    logits[1, 5] = 2.0
+    for given in (dict(), dict(top_p=0.9), dict(min_p=0.05), dict(top_p=0.95, min_p=0.01)):
+        check_draws(ops, logits, top_k=counts, uniform=np.linspace(0, 0.9999, len(counts)), **given)
+
+
 def test_draws_from_rows_that_lie_apart_and_into_a_given_place(ops):
     wide = hills(9, 3001, torch.float32, 4)
     numbers = settings(9, uniform=np.arange(9) / 9.0, top_k=30)

@@ -12,22 +12,29 @@
 // by 2^-45 of the row's largest at most: 32-bit weights would move the border between two tokens of a flat row of 150,000 by a good
 // part of a token.  Tokens that weigh nothing then (31.2 T below the maximum) are never drawn.
 //
-// No row is sorted whole.  Its tokens fall into FS_BINS ranges of logit, equal parts of what lies between the maximum and the lowest
-// logit that weighs anything, each with its count and weight; the three questions then lie in a few ranges (what is not known
-// yet of an earlier answer is at most a range's weight), whose tokens, some hundreds, are gathered and sorted in LDS.  Should there
-// be more than FS_LIST of them (thousands of equal logits), a range is narrowed by counting instead, key by key.
+// No row is sorted whole: the tokens among which the answers lie, some hundreds, are gathered and sorted in LDS.
+//   * Where the first k tokens are all that counts, or those that min-p keeps, a logit is known below which nothing does
+//     (`fs_cut`): the k-th largest of the maxima that the row's waves found, of which at least k tokens are no smaller, or
+//     max + T ln(min_p).  What is not below it is the list.
+//   * Else every token's weight matters.  The tokens fall into FS_BINS ranges of logit, equal parts of what lies between the maximum and the
+//     lowest logit that weighs anything, each with its count and weight; the answers then lie in a few ranges (what is not known
+//     yet of an earlier answer is at most a range's weight), whose tokens are the list.
+// Should there be more than FS_LIST of them (thousands of equal logits), one workgroup goes through the row again and again and
+// narrows the answer's range by counting, key by key.
 //
 // NaN is no token.  A row without a finite maximum, and a row whose temperature is not positive, gets its first maximum (0 if it
 // holds no number).
 #include "common.h"
 
-#define FS_THREADS 1024
-#define FS_WAVES (FS_THREADS / WAVE)
-#define FS_EACH 20                      // logits a thread holds
+#define FS_THREADS 256                  // of a long row's workgroups
+#define FS_EACH 16                      // logits a thread holds
 #define FS_PIECE (FS_THREADS * FS_EACH)
+#define FS_SHORT_THREADS 512            // of a short row's
+#define FS_SHORT_EACH 32
 #define FS_BINS 256                     // four a lane
 #define FS_LIST 8192
-#define FS_SLOTS 1024                   // ranges a round of narrowing tells apart, one a thread
+#define FS_SLOTS 256                    // ranges that a round of narrowing tells apart
+#define FS_MAX_WAVES (FS_SHORT_THREADS / WAVE)
 #define FS_UNIT 17592186044416.0        // 2^44
 #define FS_REACH 31.3f                  // beyond so many T below the maximum a weight is less than half a unit: nothing
 
@@ -86,22 +93,26 @@ __device__ __forceinline__ int fs_bin(float v, const FsRow& r) {
 
 struct FsAsked { float temperature, top_p, min_p, uniform; int top_k; };
 
-struct FsShared {
+struct FsSmall {
+  u64 mass[FS_BINS];                    // the bins, of a piece or of the whole row
+  uint32_t count[FS_BINS];
+  u64 wave_mass[FS_MAX_WAVES], wave_over[FS_MAX_WAVES];
+  uint32_t wave_count[FS_MAX_WAVES];
+  float wave_low[FS_MAX_WAVES], wave_high[FS_MAX_WAVES];
+  int wave_at[FS_MAX_WAVES];
+  int n_listed;
+};
+
+struct FsShared : FsSmall {
   union {
     u64 list[FS_LIST];                  // the gathered tokens, key in the upper half, the index's complement in the lower
     struct { u64 mass[FS_SLOTS]; uint32_t count[FS_SLOTS]; } slots;      // a round of narrowing
   };
-  u64 mass[FS_BINS];                    // the bins, whole row
-  uint32_t count[FS_BINS];
   u64 missing_mass[FS_BINS];            // of bins that were not gathered, in front of this one
   uint32_t missing_count[FS_BINS];
-  u64 wave_mass[FS_WAVES];
-  uint32_t wave_count[FS_WAVES];
-  float wave_low[FS_WAVES], wave_high[FS_WAVES];
-  int wave_at[FS_WAVES];
   u64 found_mass, kept;
   uint32_t found_count;
-  int found, n_listed;
+  int found;
   uint32_t key_low, key_high;
 };
 
@@ -111,60 +122,68 @@ __device__ __forceinline__ u64 fs_up(u64 v, int off, int lane) {          // the
 }
 
 // Sum over the workgroup, to every thread.
-__device__ __forceinline__ u64 fs_sum(u64 v, FsShared& s) {
+template <int THREADS>
+__device__ __forceinline__ u64 fs_sum(u64 v, FsSmall& s) {
   for (int off = WAVE / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, WAVE);
   __syncthreads();
   if ((threadIdx.x & (WAVE - 1)) == 0) s.wave_mass[threadIdx.x / WAVE] = v;
   __syncthreads();
   u64 total = 0;
-  for (int w = 0; w < FS_WAVES; ++w) total += s.wave_mass[w];
+#pragma unroll
+  for (int w = 0; w < THREADS / WAVE; ++w) total += s.wave_mass[w];
   return total;
 }
 
-// The logits of a piece in registers: thread i has logits i, i + FS_THREADS, ...; NaN where there is none.
-template <typename T>
-__device__ __forceinline__ void fs_load(const T* __restrict__ row, int begin, int vocab, float (&v)[FS_EACH]) {
+// The logits of a piece in registers: thread i has logits i, i + THREADS, ...; NaN where there is none.
+template <int THREADS, int EACH, typename T>
+__device__ __forceinline__ void fs_load(const T* __restrict__ row, int begin, int vocab, float (&v)[EACH]) {
 #pragma unroll
-  for (int j = 0; j < FS_EACH; ++j) v[j] = ld(row + min(begin + j * FS_THREADS + (int)threadIdx.x, vocab - 1));
+  for (int j = 0; j < EACH; ++j) v[j] = ld(row + min(begin + j * THREADS + (int)threadIdx.x, vocab - 1));
 #pragma unroll
-  for (int j = 0; j < FS_EACH; ++j)
-    if (begin + j * FS_THREADS + (int)threadIdx.x >= vocab) v[j] = __uint_as_float(0x7fc00000u);
+  for (int j = 0; j < EACH; ++j)
+    if (begin + j * THREADS + (int)threadIdx.x >= vocab) v[j] = __uint_as_float(0x7fc00000u);
 }
 
-// The largest of a piece's logits, its lowest index, and the smallest above -inf, to every thread.
-__device__ __forceinline__ void fs_extent(const float (&v)[FS_EACH], int begin, float& high, int& at, float& low, FsShared& s) {
+// The largest of a piece's logits, its lowest index, and the smallest above -inf, to every thread.  `of_wave`: the largest of the wave's.
+template <int THREADS, int EACH>
+__device__ __forceinline__ void fs_extent(const float (&v)[EACH], int begin, float& high, int& at, float& low, float& of_wave, FsSmall& s) {
   high = -INFINITY;
   low = INFINITY;
-  at = 0x7fffffff;
 #pragma unroll
-  for (int j = 0; j < FS_EACH; ++j) {
-    if (v[j] > high) { high = v[j]; at = begin + j * FS_THREADS + (int)threadIdx.x; }
-    if (v[j] > -INFINITY) low = fminf(low, v[j]);
+  for (int j = 0; j < EACH; ++j) {
+    high = fmaxf(high, v[j]);
+    low = fminf(low, v[j] > -INFINITY ? v[j] : INFINITY);
   }
-  for (int off = WAVE / 2; off > 0; off >>= 1) {
-    const float other = __shfl_xor(high, off, WAVE);
-    const int other_at = __shfl_xor(at, off, WAVE);
-    if (other > high || (other == high && other_at < at)) { high = other; at = other_at; }
-    low = fminf(low, __shfl_xor(low, off, WAVE));
+  high = of_wave = wave_max(high);
+  low = -wave_max(-low);
+  at = 0x7fffffff;
+  if (high > -INFINITY) {
+#pragma unroll
+    for (int j = EACH - 1; j >= 0; --j) {
+      const unsigned long long equal = __ballot(v[j] == high);
+      if (equal) at = begin + j * THREADS + (int)(threadIdx.x & ~(WAVE - 1)) + __ffsll(equal) - 1;
+    }
   }
   const int wave = threadIdx.x / WAVE;
   if ((threadIdx.x & (WAVE - 1)) == 0) { s.wave_high[wave] = high; s.wave_at[wave] = at; s.wave_low[wave] = low; }
   __syncthreads();
-  for (int w = 0; w < FS_WAVES; ++w) {
+#pragma unroll
+  for (int w = 0; w < THREADS / WAVE; ++w) {
     if (s.wave_high[w] > high || (s.wave_high[w] == high && s.wave_at[w] < at)) { high = s.wave_high[w]; at = s.wave_at[w]; }
     low = fminf(low, s.wave_low[w]);
   }
 }
 
 // A piece's bins into `s.mass` and (if `counted`) `s.count`, and the weight of its tokens that min-p keeps, to every thread.
-__device__ __forceinline__ u64 fs_fill_bins(const float (&v)[FS_EACH], const FsRow& r, const FsAsked& asked, FsShared& s) {
+template <int THREADS, int EACH>
+__device__ __forceinline__ u64 fs_fill_bins(const float (&v)[EACH], const FsRow& r, const FsAsked& asked, FsSmall& s) {
   const bool counted = asked.top_k > 0, floored = asked.min_p > 0.f;
   const double floor_share = (double)asked.min_p * FS_UNIT;
   if (threadIdx.x < FS_BINS) { s.mass[threadIdx.x] = 0; s.count[threadIdx.x] = 0; }
   __syncthreads();
   u64 over = 0;
 #pragma unroll
-  for (int j = 0; j < FS_EACH; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     if (r.top - v[j] <= r.reach) {                         // (false for NaN)
       const double share = fs_share(v[j], r);
       const u64 w = fs_whole(share);
@@ -174,14 +193,14 @@ __device__ __forceinline__ u64 fs_fill_bins(const float (&v)[FS_EACH], const FsR
       if (!floored || !(share < floor_share) || v[j] == r.top) over += w;
     }
   }
-  return fs_sum(over, s);                                  // (its barriers stand behind the bins, too)
+  return fs_sum<THREADS>(over, s);                         // (its barriers stand behind the bins, too)
 }
 
 // A wave's view of the bins: running counts and weights, bins 4 lane .. + 3.
 struct FsRunning {
   u64 mass[4];
   uint32_t count[4];
-  __device__ __forceinline__ void of(const FsShared& s) {
+  __device__ __forceinline__ void of(const FsSmall& s) {
     const int lane = threadIdx.x & (WAVE - 1);
     u64 m = 0, c = 0;
 #pragma unroll
@@ -276,31 +295,44 @@ __device__ __forceinline__ FsRanges fs_ranges(const FsRunning& run, const FsAske
 }
 
 // ------------------------------------------------------------------------------------------------
-// Narrowing, for ranges of more tokens than are sorted: the row is read again for every round.
+// Narrowing, for more tokens than are sorted: the row is read again for every round.
 
-// Where the order of the slots, the last one first, reaches a number (the running count if `counting`, else the running mass).  Returns the
-// slot, and what lies before it in `count` and `mass`; -1 if the whole order does not reach it.
+// Where the order of the slots, the last one first unless `forwards`, reaches a number (the running count if `counting`, else the running
+// mass).  Returns the slot, and what lies before it in `count` and `mass`; -1 if the whole order does not reach it.
 __device__ int fs_reach(FsShared& s, bool forwards, bool counting, u64 need, uint32_t& count, u64& mass) {
-  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  const int slot = forwards ? threadIdx.x : FS_SLOTS - 1 - threadIdx.x;
-  const u64 m = s.slots.mass[slot];
-  const u64 c = s.slots.count[slot];
-  u64 run_m = m, run_c = c;
-  for (int off = 1; off < WAVE; off <<= 1) {
-    run_m += fs_up(run_m, off, lane);
-    run_c += fs_up(run_c, off, lane);
-  }
+  static_assert(FS_SLOTS == 4 * WAVE, "four slots a lane of one wave");
+  const int lane = threadIdx.x & (WAVE - 1);
   __syncthreads();
-  if (threadIdx.x == 0) s.found = -1;
-  if (lane == WAVE - 1) { s.wave_mass[wave] = run_m; s.wave_count[wave] = (uint32_t)run_c; }
-  __syncthreads();
-  u64 before_m = run_m - m, before_c = run_c - c;
-  for (int w = 0; w < wave; ++w) { before_m += s.wave_mass[w]; before_c += s.wave_count[w]; }
-  const u64 before = counting ? before_c : before_m, here = counting ? c : m;
-  if (before < need && before + here >= need) {            // one thread
-    s.found = slot;
-    s.found_mass = before_m;
-    s.found_count = (uint32_t)before_c;
+  if (threadIdx.x < WAVE) {
+    u64 m[4], c[4], all_m = 0, all_c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int slot = forwards ? 4 * lane + j : FS_SLOTS - 1 - 4 * lane - j;
+      m[j] = s.slots.mass[slot];
+      c[j] = s.slots.count[slot];
+      all_m += m[j];
+      all_c += c[j];
+    }
+    u64 run_m = all_m, run_c = all_c;
+    for (int off = 1; off < WAVE; off <<= 1) {
+      run_m += fs_up(run_m, off, lane);
+      run_c += fs_up(run_c, off, lane);
+    }
+    run_m -= all_m;
+    run_c -= all_c;
+    if (lane == 0) s.found = -1;
+    wave_exchange();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const u64 before = counting ? run_c : run_m, here = counting ? c[j] : m[j];
+      if (before < need && before + here >= need) {        // one slot of one lane
+        s.found = forwards ? 4 * lane + j : FS_SLOTS - 1 - 4 * lane - j;
+        s.found_mass = run_m;
+        s.found_count = (uint32_t)run_c;
+      }
+      run_m += m[j];
+      run_c += c[j];
+    }
   }
   __syncthreads();
   const int at = s.found;
@@ -312,21 +344,20 @@ __device__ int fs_reach(FsShared& s, bool forwards, bool counting, u64 need, uin
 
 __device__ __forceinline__ void fs_clear_slots(FsShared& s) {
   __syncthreads();
-  s.slots.mass[threadIdx.x] = 0;
-  s.slots.count[threadIdx.x] = 0;
+  if (threadIdx.x < FS_SLOTS) { s.slots.mass[threadIdx.x] = 0; s.slots.count[threadIdx.x] = 0; }
   __syncthreads();
 }
 
-// Calls use(value, index) for every number of the row, a thread every FS_THREADS-th one, eight loads asked for at a time.
-template <typename T, typename Use>
+// Calls use(value, index) for every number of the row, a thread every THREADS-th one, sixteen loads asked for at a time.
+template <int THREADS, typename T, typename Use>
 __device__ __forceinline__ void fs_numbers(const T* __restrict__ row, int vocab, Use use) {
-  for (int base = threadIdx.x; base < vocab; base += 8 * FS_THREADS) {
-    float v[8];
+  for (int base = threadIdx.x; base < vocab; base += 16 * THREADS) {
+    float v[16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = ld(row + min(base + j * FS_THREADS, vocab - 1));
+    for (int j = 0; j < 16; ++j) v[j] = ld(row + min(base + j * THREADS, vocab - 1));
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (base + j * FS_THREADS < vocab && v[j] == v[j]) use(v[j], base + j * FS_THREADS);
+    for (int j = 0; j < 16; ++j)
+      if (base + j * THREADS < vocab && v[j] == v[j]) use(v[j], base + j * THREADS);
   }
 }
 
@@ -336,11 +367,11 @@ struct FsCrossing {
   u64 before_mass, each;
 };
 
-template <typename T>
+template <int THREADS, typename T>
 __device__ FsCrossing fs_narrow(FsShared& s, const T* row, int vocab, const FsRow& r, int bin, bool counting, u64 need, uint32_t before_count,
                                 u64 before_mass) {
   uint32_t low = 0xffffffffu, high = 0;
-  fs_numbers(row, vocab, [&](float v, int) {
+  fs_numbers<THREADS>(row, vocab, [&](float v, int) {
     if (r.top - v <= r.reach && fs_bin(v, r) == bin) {
       const uint32_t key = fs_key(v);
       low = min(low, key);
@@ -359,7 +390,7 @@ __device__ FsCrossing fs_narrow(FsShared& s, const T* row, int vocab, const FsRo
     int shift = 0;
     while (((high - low) >> shift) >= FS_SLOTS) ++shift;
     fs_clear_slots(s);
-    fs_numbers(row, vocab, [&](float v, int) {
+    fs_numbers<THREADS>(row, vocab, [&](float v, int) {
       if (r.top - v <= r.reach && fs_bin(v, r) == bin) {
         const uint32_t key = fs_key(v);
         if (key >= low && key <= high) {
@@ -368,7 +399,6 @@ __device__ FsCrossing fs_narrow(FsShared& s, const T* row, int vocab, const FsRo
         }
       }
     });
-    __syncthreads();
     uint32_t inner_count = 0;
     u64 inner_mass = 0;
     const int slot = fs_reach(s, false, counting, need - (counting ? (u64)before_count : before_mass), inner_count, inner_mass);
@@ -386,10 +416,29 @@ __device__ FsCrossing fs_narrow(FsShared& s, const T* row, int vocab, const FsRo
   return x;
 }
 
-template <typename T>
-__device__ int fs_draw_by_narrowing(FsShared& s, const T* row, int vocab, const FsRow& r, const FsAsked& asked, const FsRunning& run, u64 over) {
+template <int THREADS, typename T>
+__device__ int fs_draw_by_narrowing(FsShared& s, const T* row, int vocab, const FsRow& r, const FsAsked& asked) {
+  // The bins of the whole row, weights and counts, anew (the row may have come here without any).
+  __syncthreads();
+  if (threadIdx.x < FS_BINS) { s.mass[threadIdx.x] = 0; s.count[threadIdx.x] = 0; }
+  __syncthreads();
+  const double floor_share = (double)asked.min_p * FS_UNIT;
+  u64 over = 0;
+  fs_numbers<THREADS>(row, vocab, [&](float v, int) {
+    if (r.top - v <= r.reach) {
+      const double share = fs_share(v, r);
+      const u64 w = fs_whole(share);
+      const int bin = fs_bin(v, r);
+      atomicAdd(&s.mass[bin], w);
+      atomicAdd(&s.count[bin], 1u);
+      if (!(asked.min_p > 0.f) || !(share < floor_share) || v == r.top) over += w;
+    }
+  });
+  over = fs_sum<THREADS>(over, s);
+  FsRunning run;
+  run.of(s);
   auto crossing = [&](int bin, bool counting, u64 need) {
-    return fs_narrow(s, row, vocab, r, bin, counting, need, run.count_to(bin - 1), run.mass_to(bin - 1));
+    return fs_narrow<THREADS>(s, row, vocab, r, bin, counting, need, run.count_to(bin - 1), run.mass_to(bin - 1));
   };
   u64 kept = run.mass_to(FS_BINS - 1);
   if (asked.top_k > 0 && run.count_to(FS_BINS - 1) >= (uint32_t)asked.top_k) {
@@ -411,73 +460,60 @@ __device__ int fs_draw_by_narrowing(FsShared& s, const T* row, int vocab, const 
   // The rank-th token of the key: which run of indices has it, then which of the run.
   const int per = (vocab + FS_SLOTS - 1) / FS_SLOTS;
   fs_clear_slots(s);
-  fs_numbers(row, vocab, [&](float v, int at) {
+  fs_numbers<THREADS>(row, vocab, [&](float v, int at) {
     if (fs_key(v) == x.key) atomicAdd(&s.slots.count[at / per], 1u);
   });
-  __syncthreads();
   uint32_t before = 0;
   u64 unused;
   const int part = fs_reach(s, true, true, rank, before, unused);
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < WAVE) {                                // a wave looks through the run, sixty-four tokens at a time
+    const int lane = threadIdx.x;
+    const int end = part < 0 ? 0 : min(vocab, (part + 1) * per);
+    uint32_t left = (uint32_t)(rank - before);
     int pick = 0;
-    u64 left = rank - before;
-    for (int i = part < 0 ? vocab : part * per; i < min(vocab, (part + 1) * per); ++i) {
-      const float v = ld(row + i);
-      if (v == v && fs_key(v) == x.key && --left == 0) { pick = i; break; }
+    for (int i = max(part, 0) * per; i < end; i += WAVE) {
+      const float v = ld(row + min(i + lane, vocab - 1));
+      const bool is = i + lane < end && v == v && fs_key(v) == x.key;
+      const unsigned long long votes = __ballot(is);
+      const uint32_t here = (uint32_t)__popcll(votes);
+      if (left <= here) {
+        const bool mine = is && (uint32_t)__popcll(votes & ((1ull << lane) - 1ull)) + 1 == left;
+        pick = i + __ffsll(__ballot(mine)) - 1;
+        break;
+      }
+      left -= here;
     }
-    s.found = pick;
+    if (lane == 0) s.found = pick;
   }
   __syncthreads();
   return s.found;
 }
 
 // ------------------------------------------------------------------------------------------------
-// The draw, with the bins of the whole row in `s.mass` and `s.count`: from the `n` gathered tokens in `s.list` (in any order) if they all
-// found room there, else by narrowing.
-template <typename T>
-__device__ int fs_draw(FsShared& s, const T* row, int vocab, const FsRow& r, const FsAsked& asked, const FsRunning& run,
-                       const FsRanges& ranges, u64 over, int n) {
-  if (n > FS_LIST) return fs_draw_by_narrowing(s, row, vocab, r, asked, run, over);
-  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  if (wave == 0) {                                         // what lies between the gathered bins
-    u64 m[4], c[4], run_m = 0, run_c = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool gathered = ranges.has(4 * lane + j);
-      m[j] = run_m;
-      c[j] = run_c;
-      run_m += gathered ? 0 : s.mass[4 * lane + j];
-      run_c += gathered ? 0 : s.count[4 * lane + j];
-    }
-    const u64 all_m = run_m, all_c = run_c;
-    for (int off = 1; off < WAVE; off <<= 1) {
-      run_m += fs_up(run_m, off, lane);
-      run_c += fs_up(run_c, off, lane);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s.missing_mass[4 * lane + j] = m[j] + run_m - all_m;
-      s.missing_count[4 * lane + j] = (uint32_t)(c[j] + run_c - all_c);
-    }
-  }
-  int size = WAVE;
-  while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += FS_THREADS) s.list[i] = 0;        // (behind every token)
-  __syncthreads();
-  // Sorted by exchanges, the largest first: runs of `run_of` fall and rise in turn until one is left.
+// `size` (a power of two, at least 128) numbers of `s.list`, the largest first: runs of `run_of` fall and rise in turn until one is
+// left.  Numbers at most 64 apart lie in a stretch of 128 that one wave sees to alone: no barrier between such steps.
+template <int THREADS>
+__device__ __forceinline__ void fs_sort(FsShared& s, int size) {
   for (int run_of = 2; run_of <= size; run_of <<= 1)
     for (int apart = run_of >> 1; apart > 0; apart >>= 1) {
-      for (int i = threadIdx.x; i < size / 2; i += FS_THREADS) {
+      for (int i = threadIdx.x; i < size / 2; i += THREADS) {
         const int a = 2 * i - (i & (apart - 1)), b = a + apart;
         const u64 x = s.list[a], y = s.list[b];
         if ((x < y) == ((a & run_of) == 0)) { s.list[a] = y; s.list[b] = x; }
       }
-      __syncthreads();
+      if (apart > 64 || (apart == 1 && run_of >= 128)) __syncthreads();      // (behind the last step of a run the next is wider than a wave's)
+      else wave_exchange();
     }
-  // Running weights: a thread has `per` neighbours of the list.
-  constexpr int MOST = FS_LIST / FS_THREADS;
-  const int per = max(1, size / FS_THREADS);
-  u64 token[MOST], w[MOST], sum = 0;
+  __syncthreads();
+}
+
+// The three answers from the sorted list; a thread has up to MOST neighbours of it.
+template <int THREADS, int MOST>
+__device__ __forceinline__ int fs_answers(FsShared& s, const FsRow& r, const FsAsked& asked, u64 all, bool k_here, u64 over, bool over_known,
+                                          bool all_listed, int n, int per) {
+  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  const double floor_share = (double)asked.min_p * FS_UNIT;
+  u64 token[MOST], w[MOST], sum = 0, above = 0;
 #pragma unroll
   for (int j = 0; j < MOST; ++j) {
     const int i = threadIdx.x * per + j;
@@ -485,7 +521,10 @@ __device__ int fs_draw(FsShared& s, const T* row, int vocab, const FsRow& r, con
     w[j] = 0;
     if (j < per && i < n) {
       token[j] = s.list[i];
-      w[j] = fs_weight(fs_value((uint32_t)(token[j] >> 32)), r);
+      const float v = fs_value((uint32_t)(token[j] >> 32));
+      const double share = fs_share(v, r);
+      w[j] = fs_whole(share);
+      if (!(asked.min_p > 0.f) || !(share < floor_share) || v == r.top) above += w[j];
     }
     sum += w[j];
   }
@@ -493,22 +532,37 @@ __device__ int fs_draw(FsShared& s, const T* row, int vocab, const FsRow& r, con
   for (int off = 1; off < WAVE; off <<= 1) before += fs_up(before, off, lane);
   if (lane == WAVE - 1) s.wave_mass[wave] = before;
   before -= sum;
-  const u64 total = run.mass_to(FS_BINS - 1);              // (the whole wave takes part)
-  if (threadIdx.x == 0) {
-    s.kept = total;
-    s.found = (int)~(uint32_t)s.list[0];
+  if (!over_known) {                                       // (what min-p keeps is in the list, or ends behind it)
+    for (int off = WAVE / 2; off > 0; off >>= 1) above += __shfl_xor(above, off, WAVE);
+    if (lane == 0) s.wave_over[wave] = above;
   }
   __syncthreads();
-  for (int i = 0; i < wave; ++i) before += s.wave_mass[i];
+  u64 listed = 0, floored = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / WAVE; ++i) {
+    if (i < wave) before += s.wave_mass[i];
+    listed += s.wave_mass[i];
+    floored += over_known ? 0 : s.wave_over[i];
+  }
+  if (!over_known) over = floored;
+  if (threadIdx.x == 0) {
+    s.kept = all_listed ? listed : all;
+    s.found = n > 0 ? (int)~(uint32_t)s.list[0] : 0;
+  }
+  __syncthreads();
   u64 at_mass[MOST];                                       // what stands before a token in the whole order
 #pragma unroll
   for (int j = 0; j < MOST; ++j) {
     at_mass[j] = before;
     before += w[j];
     if (token[j]) {
-      const int bin = fs_bin(fs_value((uint32_t)(token[j] >> 32)), r);
-      at_mass[j] += s.missing_mass[bin];
-      if (ranges.k_bin >= 0 && s.missing_count[bin] + threadIdx.x * per + j + 1 == (uint32_t)asked.top_k) s.kept = at_mass[j] + w[j];
+      uint32_t at = threadIdx.x * per + j;
+      if (!all_listed) {
+        const int bin = fs_bin(fs_value((uint32_t)(token[j] >> 32)), r);
+        at_mass[j] += s.missing_mass[bin];
+        at += s.missing_count[bin];
+      }
+      if (k_here && at + 1 == (uint32_t)asked.top_k) s.kept = at_mass[j] + w[j];
     }
   }
   __syncthreads();
@@ -531,6 +585,50 @@ __device__ int fs_draw(FsShared& s, const T* row, int vocab, const FsRow& r, con
   return s.found;
 }
 
+// The draw from the `n` tokens in `s.list` (in any order), if they all found room there, else by narrowing.  `ranges`: the list holds
+// these bins of the whole row's, which are in `s.mass` and `s.count`; null: it holds the order's first tokens, as many as count.
+template <int THREADS, typename T>
+__device__ int fs_draw(FsShared& s, const T* row, int vocab, const FsRow& r, const FsAsked& asked, const FsRanges* ranges, u64 over, int n) {
+  if (n > FS_LIST) return fs_draw_by_narrowing<THREADS>(s, row, vocab, r, asked);
+  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  u64 all = 0;
+  if (ranges) {
+    FsRunning run;
+    run.of(s);
+    all = run.mass_to(FS_BINS - 1);
+    if (wave == 0) {                                       // what lies between the gathered bins
+      u64 m[4], c[4], run_m = 0, run_c = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool gathered = ranges->has(4 * lane + j);
+        m[j] = run_m;
+        c[j] = run_c;
+        run_m += gathered ? 0 : s.mass[4 * lane + j];
+        run_c += gathered ? 0 : s.count[4 * lane + j];
+      }
+      const u64 all_m = run_m, all_c = run_c;
+      for (int off = 1; off < WAVE; off <<= 1) {
+        run_m += fs_up(run_m, off, lane);
+        run_c += fs_up(run_c, off, lane);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s.missing_mass[4 * lane + j] = m[j] + run_m - all_m;
+        s.missing_count[4 * lane + j] = (uint32_t)(c[j] + run_c - all_c);
+      }
+    }
+  }
+  int size = 2 * WAVE;
+  while (size < n) size <<= 1;
+  for (int i = n + threadIdx.x; i < size; i += THREADS) s.list[i] = 0;           // (behind every token)
+  __syncthreads();
+  fs_sort<THREADS>(s, size);
+  const int per = max(1, size / THREADS);
+  const bool k_here = asked.top_k > 0 && (!ranges || ranges->k_bin >= 0);
+  if (per <= 4) return fs_answers<THREADS, 4>(s, r, asked, all, k_here, over, ranges != nullptr, ranges == nullptr, n, per);
+  return fs_answers<THREADS, FS_LIST / THREADS>(s, r, asked, all, k_here, over, ranges != nullptr, ranges == nullptr, n, per);
+}
+
 struct FsArgs {
   const void* logits;
   int64_t stride;
@@ -544,166 +642,160 @@ struct FsArgs {
 
 __device__ __forceinline__ FsAsked fs_asked(const FsArgs& a, int row) {
   FsAsked q;
-  q.temperature = a.temperature[row];
-  q.top_p = a.top_p[row];
-  q.min_p = a.min_p[row];
-  q.uniform = a.uniform[row];
-  q.top_k = a.top_k[row];
+  q.temperature = scalar_float(a.temperature + row);
+  q.top_p = scalar_float(a.top_p + row);
+  q.min_p = scalar_float(a.min_p + row);
+  q.uniform = scalar_float(a.uniform + row);
+  q.top_k = scalar_int(a.top_k + row);
   return q;
 }
 
-// A row of at most FS_PIECE logits: one workgroup, one launch.
+// A row of at most FS_SHORT_THREADS * FS_SHORT_EACH logits: one workgroup, one launch.
 template <typename T>
-__global__ void __launch_bounds__(FS_THREADS)
+__global__ void __launch_bounds__(FS_SHORT_THREADS)
 sample_filtered_short(FsArgs a) {
+  constexpr int THREADS = FS_SHORT_THREADS;
   __shared__ FsShared s;
   const int row_at = blockIdx.x;
   const T* row = (const T*)a.logits + (size_t)row_at * a.stride;
   const FsAsked asked = fs_asked(a, row_at);
-  float v[FS_EACH], high, low;
+  float v[FS_SHORT_EACH], high, low, of_wave;
   int at;
-  fs_load(row, 0, a.vocab, v);
-  fs_extent(v, 0, high, at, low, s);
+  fs_load<THREADS>(row, 0, a.vocab, v);
+  fs_extent<THREADS>(v, 0, high, at, low, of_wave, s);
   if (!fs_is_drawn(asked.temperature, high)) {
     if (threadIdx.x == 0) a.out[row_at] = at == 0x7fffffff ? 0 : at;
     return;
   }
   const FsRow r = fs_row(asked.temperature, high, low);
-  const u64 over = fs_fill_bins(v, r, asked, s);
+  const u64 over = fs_fill_bins<THREADS>(v, r, asked, s);
   FsRunning run;
   run.of(s);
   const FsRanges ranges = fs_ranges(run, asked, over);
   if (threadIdx.x == 0) s.n_listed = 0;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < FS_EACH; ++j)
+  for (int j = 0; j < FS_SHORT_EACH; ++j)
     if (r.top - v[j] <= r.reach && ranges.has(fs_bin(v[j], r))) {
       const int place = atomicAdd(&s.n_listed, 1);
-      if (place < FS_LIST) s.list[place] = (u64)fs_key(v[j]) << 32 | (uint32_t)~(uint32_t)(j * FS_THREADS + (int)threadIdx.x);
+      if (place < FS_LIST) s.list[place] = (u64)fs_key(v[j]) << 32 | (uint32_t)~(uint32_t)(j * THREADS + (int)threadIdx.x);
     }
   __syncthreads();
-  const int pick = fs_draw(s, row, a.vocab, r, asked, run, ranges, over, s.n_listed);
+  const int pick = fs_draw<THREADS>(s, row, a.vocab, r, asked, &ranges, over, s.n_listed);
   if (threadIdx.x == 0) a.out[row_at] = pick;
 }
 
+// ------------------------------------------------------------------------------------------------
 // A longer row: its pieces' workgroups leave what they found in the workspace, a launch a step.
-struct FsExtent { float high, low; int at, unused; };
-__device__ __host__ __forceinline__ size_t fs_bins_at(int pieces) { return 16 + sizeof(FsExtent) * (size_t)pieces; }
-__device__ __host__ __forceinline__ size_t fs_whole_at(int pieces) { return fs_bins_at(pieces) + (size_t)pieces * (12 * FS_BINS + 8); }
-__device__ __host__ __forceinline__ size_t fs_list_at(int pieces) { return fs_whole_at(pieces) + 12 * FS_BINS + 8; }
-// Per row: how many tokens were gathered (and 12 bytes of nothing); the pieces' extents; the pieces' bins (weights, then counts, then the
-// weight that min-p keeps); those of the whole row; the gathered tokens.
+#define FS_PIECE_WAVES (FS_THREADS / WAVE)
+struct FsExtent { float high, low; int at, unused; float of_wave[FS_PIECE_WAVES]; };
+struct FsHead { int n_listed; int ranges[5]; int unused[2]; u64 over; u64 unused2; };      // of a row
+struct FsBinned { u64 mass[FS_BINS]; uint32_t count[FS_BINS]; u64 over; u64 unused; };    // of a piece, or of a row
+// Per row: its head, its bins, its list, the pieces' extents and the pieces' bins.
 struct FsSpace {
   char* base;
   int pieces;
-  __device__ __forceinline__ int* n_listed() const { return (int*)base; }
-  __device__ __forceinline__ FsExtent* extents() const { return (FsExtent*)(base + 16); }
-  __device__ __forceinline__ u64* mass(int piece) const { return (u64*)(base + fs_bins_at(pieces) + (size_t)piece * (12 * FS_BINS + 8)); }
-  __device__ __forceinline__ u64* whole() const { return (u64*)(base + fs_whole_at(pieces)); }
-  __device__ __forceinline__ u64* list() const { return (u64*)(base + fs_list_at(pieces)); }
+  __device__ __forceinline__ FsHead* head() const { return (FsHead*)base; }
+  __device__ __forceinline__ FsBinned* whole() const { return (FsBinned*)(base + sizeof(FsHead)); }
+  __device__ __forceinline__ u64* list() const { return (u64*)(whole() + 1); }
+  __device__ __forceinline__ FsExtent* extents() const { return (FsExtent*)(list() + FS_LIST); }
+  __device__ __forceinline__ FsBinned* binned() const { return (FsBinned*)(extents() + pieces); }
 };
+static size_t fs_row_bytes(int pieces) {
+  return sizeof(FsHead) + sizeof(FsBinned) + 8 * FS_LIST + (sizeof(FsExtent) + sizeof(FsBinned)) * (size_t)pieces;
+}
+static_assert(sizeof(FsHead) % 16 == 0 && sizeof(FsBinned) % 16 == 0 && sizeof(FsExtent) % 16 == 0, "pieces of sixteen bytes");
 __device__ __forceinline__ FsSpace fs_space(const FsArgs& a, int row) { return FsSpace{a.workspace + (size_t)row * a.row_bytes, a.pieces}; }
 
+// The row's extent from its pieces' (a lane of every wave looks at one piece of sixty-four), to every thread.
 __device__ __forceinline__ void fs_row_extent(const FsSpace& w, float& high, int& at, float& low) {
+  const int lane = threadIdx.x & (WAVE - 1);
   high = -INFINITY;
   low = INFINITY;
   at = 0x7fffffff;
-  for (int p = 0; p < w.pieces; ++p) {
-    const FsExtent e = w.extents()[p];
+  for (int p = lane; p < w.pieces; p += WAVE) {
+    const FsExtent& e = w.extents()[p];
     if (e.high > high) { high = e.high; at = e.at; }       // (pieces in the order of their indices)
     low = fminf(low, e.low);
   }
+  const float mine = high;
+  high = wave_max(high);
+  low = -wave_max(-low);
+  if (mine != high) at = 0x7fffffff;
+  for (int off = WAVE / 2; off > 0; off >>= 1) at = min(at, __shfl_xor(at, off, WAVE));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(FS_THREADS)
-sample_filtered_extents(FsArgs a) {
-  __shared__ FsShared s;
-  const FsSpace w = fs_space(a, blockIdx.y);
-  float v[FS_EACH], high, low;
-  int at;
-  fs_load((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
-  fs_extent(v, blockIdx.x * FS_PIECE, high, at, low, s);
-  if (threadIdx.x == 0) {
-    w.extents()[blockIdx.x] = FsExtent{high, low, at, 0};
-    if (blockIdx.x == 0) *w.n_listed() = 0;
-  }
+// Whether a row's list can be made without its bins.
+__device__ __forceinline__ bool fs_listed_at_once(const FsAsked& asked, int pieces) {
+  return (asked.top_k > 0 && asked.top_k <= pieces * FS_PIECE_WAVES) || (!(asked.top_p < 1.f) && asked.min_p > 0.f);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(FS_THREADS)
-sample_filtered_bins(FsArgs a) {
-  __shared__ FsShared s;
-  const FsSpace w = fs_space(a, blockIdx.y);
-  const FsAsked asked = fs_asked(a, blockIdx.y);
-  float v[FS_EACH], high, low;
-  int at;
-  fs_load((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
-  fs_row_extent(w, high, at, low);
-  if (!fs_is_drawn(asked.temperature, high)) return;
-  const u64 over = fs_fill_bins(v, fs_row(asked.temperature, high, low), asked, s);
-  u64* mass = w.mass(blockIdx.x);
-  uint32_t* count = (uint32_t*)(mass + FS_BINS + 1);
-  if (threadIdx.x < FS_BINS) {
-    mass[threadIdx.x] = s.mass[threadIdx.x];
-    count[threadIdx.x] = s.count[threadIdx.x];
-  }
-  if (threadIdx.x == 0) mass[FS_BINS] = over;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(FS_THREADS)
-sample_filtered_gather(FsArgs a) {
-  __shared__ FsShared s;
-  const FsSpace w = fs_space(a, blockIdx.y);
-  const FsAsked asked = fs_asked(a, blockIdx.y);
-  float v[FS_EACH], high, low;
-  int at;
-  fs_load((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
-  fs_row_extent(w, high, at, low);
-  if (!fs_is_drawn(asked.temperature, high)) return;
-  const FsRow r = fs_row(asked.temperature, high, low);
-  if (threadIdx.x < FS_BINS) {
-    u64 m = 0;
-    uint32_t c = 0;
-    for (int p = 0; p < a.pieces; ++p) {
-      m += w.mass(p)[threadIdx.x];
-      c += ((const uint32_t*)(w.mass(p) + FS_BINS + 1))[threadIdx.x];
+// A logit so that every token that counts is no smaller.
+//   top-k: at least k of the waves' maxima are no smaller; found by halving between the largest and the smallest logit that weighs
+//   anything, and what the halvings leave undecided stays above the cut.
+//   min-p (where top-p cuts nothing): max + T ln(min_p), less what 32 bits may be off by: 4 roundings of each of its parts.
+__device__ __forceinline__ float fs_cut(const FsSpace& w, const FsAsked& asked, const FsRow& r, float low) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  const float high = r.top;
+  float cut = -INFINITY;
+  if (asked.top_k > 0 && asked.top_k <= w.pieces * FS_PIECE_WAVES) {
+    constexpr int MOST = 8;                                // of 64 lanes: up to 128 pieces of four waves
+    float m[MOST];
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) {
+      const int i = j * WAVE + lane;
+      m[j] = i < w.pieces * FS_PIECE_WAVES ? w.extents()[i / FS_PIECE_WAVES].of_wave[i % FS_PIECE_WAVES] : -INFINITY;
     }
-    s.mass[threadIdx.x] = m;
-    s.count[threadIdx.x] = c;
-    if (blockIdx.x == 0) {
-      w.whole()[threadIdx.x] = m;
-      ((uint32_t*)(w.whole() + FS_BINS + 1))[threadIdx.x] = c;
+    auto no_smaller = [&](float t) {
+      int count = 0;
+#pragma unroll
+      for (int j = 0; j < MOST; ++j)
+        if (j * WAVE < w.pieces * FS_PIECE_WAVES) count += __popcll(__ballot(m[j] >= t));
+      return count;
+    };
+    float least = fmaxf(low, high - r.reach), most = high;   // (what lies further below weighs nothing)
+    if (no_smaller(least) >= asked.top_k) {
+      for (int turn = 0; turn < 12; ++turn) {
+        const float middle = 0.5f * least + 0.5f * most;
+        if (no_smaller(middle) >= asked.top_k) least = middle; else most = middle;
+      }
+      cut = least;
     }
   }
-  u64 over = 0;
-  for (int p = 0; p < a.pieces; ++p) over += w.mass(p)[FS_BINS];
-  if (blockIdx.x == 0 && threadIdx.x == 0) w.whole()[FS_BINS] = over;
-  __syncthreads();
-  FsRunning run;
-  run.of(s);
-  const FsRanges ranges = fs_ranges(run, asked, over);
-  // Each thread's tokens in the ranges, their place in the workgroup's, and the workgroup's place in the row's list.
-  uint32_t mine = 0, held = 0;
+  if (!(asked.top_p < 1.f) && asked.min_p > 0.f) {
+    const float down = -asked.temperature * logf(fminf(asked.min_p, 1.f));
+    const float floor_cut = high - down - 4.8e-7f * (fabsf(high) + 2.f * down) - 1e-6f * asked.temperature;
+    cut = fmaxf(cut, floor_cut);
+  }
+  return cut;
+}
+
+// The tokens of a piece that `wanted` names, to the row's list: each thread's, their place among the workgroup's, and the
+// workgroup's place in the list.
+template <typename Wanted>
+__device__ __forceinline__ void fs_append(const FsSpace& w, const float (&v)[FS_EACH], FsSmall& s, Wanted wanted) {
+  uint32_t held = 0;
 #pragma unroll
   for (int j = 0; j < FS_EACH; ++j)
-    if (r.top - v[j] <= r.reach && ranges.has(fs_bin(v[j], r))) { ++mine; held |= 1u << j; }
+    if (wanted(v[j])) held |= 1u << j;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  int place = (int)mine;
+  const int mine = __popc(held);
+  int place = mine;
   for (int off = 1; off < WAVE; off <<= 1) {
     const int got = __shfl_up(place, off, WAVE);
     if (lane >= off) place += got;
   }
   if (lane == WAVE - 1) s.wave_count[wave] = (uint32_t)place;
   __syncthreads();
-  place -= (int)mine;
+  place -= mine;
   uint32_t all = 0;
-  for (int i = 0; i < FS_WAVES; ++i) {
+#pragma unroll
+  for (int i = 0; i < FS_PIECE_WAVES; ++i) {
     if (i < wave) place += (int)s.wave_count[i];
     all += s.wave_count[i];
   }
-  if (threadIdx.x == 0) s.n_listed = all ? atomicAdd(w.n_listed(), (int)all) : 0;
+  if (all == 0) return;                                    // (the same for the whole workgroup)
+  if (threadIdx.x == 0) s.n_listed = atomicAdd(&w.head()->n_listed, (int)all);
   __syncthreads();
   place += s.n_listed;
 #pragma unroll
@@ -717,7 +809,53 @@ sample_filtered_gather(FsArgs a) {
 
 template <typename T>
 __global__ void __launch_bounds__(FS_THREADS)
-sample_filtered_draw(FsArgs a) {
+sample_filtered_extents(FsArgs a) {
+  __shared__ FsSmall s;
+  const FsSpace w = fs_space(a, blockIdx.y);
+  float v[FS_EACH], high, low, of_wave;
+  int at;
+  fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
+  fs_extent<FS_THREADS>(v, blockIdx.x * FS_PIECE, high, at, low, of_wave, s);
+  FsExtent& e = w.extents()[blockIdx.x];
+  if ((threadIdx.x & (WAVE - 1)) == 0) e.of_wave[threadIdx.x / WAVE] = of_wave;
+  if (threadIdx.x == 0) {
+    e.high = high;
+    e.low = low;
+    e.at = at;
+    if (blockIdx.x == 0) w.head()->n_listed = 0;
+  }
+}
+
+// The list, where it can be made at once; else the piece's bins.
+template <typename T>
+__global__ void __launch_bounds__(FS_THREADS)
+sample_filtered_bins(FsArgs a) {
+  __shared__ FsSmall s;
+  const FsSpace w = fs_space(a, blockIdx.y);
+  const FsAsked asked = fs_asked(a, blockIdx.y);
+  float v[FS_EACH], high, low;
+  int at;
+  fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
+  fs_row_extent(w, high, at, low);
+  if (!fs_is_drawn(asked.temperature, high)) return;
+  const FsRow r = fs_row(asked.temperature, high, low);
+  if (fs_listed_at_once(asked, a.pieces)) {
+    const float cut = fs_cut(w, asked, r, low);
+    fs_append(w, v, s, [&](float x) { return x >= cut && r.top - x <= r.reach; });
+    return;
+  }
+  const u64 over = fs_fill_bins<FS_THREADS>(v, r, asked, s);
+  FsBinned& mine = w.binned()[blockIdx.x];
+  mine.mass[threadIdx.x] = s.mass[threadIdx.x];
+  mine.count[threadIdx.x] = s.count[threadIdx.x];
+  if (threadIdx.x == 0) mine.over = over;
+}
+static_assert(FS_THREADS == FS_BINS, "a thread a bin");
+
+// A row whose list is there: its draw.  Another: its bins, and the ranges of them in which the answers lie.
+template <typename T>
+__global__ void __launch_bounds__(FS_THREADS)
+sample_filtered_settle(FsArgs a) {
   __shared__ FsShared s;
   const int row_at = blockIdx.x;
   const FsSpace w = fs_space(a, row_at);
@@ -729,36 +867,95 @@ sample_filtered_draw(FsArgs a) {
     if (threadIdx.x == 0) a.out[row_at] = at == 0x7fffffff ? 0 : at;
     return;
   }
-  const int n = *w.n_listed();
-  if (threadIdx.x < FS_BINS) {
-    s.mass[threadIdx.x] = w.whole()[threadIdx.x];
-    s.count[threadIdx.x] = ((const uint32_t*)(w.whole() + FS_BINS + 1))[threadIdx.x];
+  if (fs_listed_at_once(asked, a.pieces)) {
+    const int n = w.head()->n_listed;
+    for (int i = threadIdx.x; i < min(n, FS_LIST); i += FS_THREADS) s.list[i] = w.list()[i];
+    const int pick = fs_draw<FS_THREADS>(s, (const T*)a.logits + (size_t)row_at * a.stride, a.vocab, fs_row(asked.temperature, high, low), asked,
+                                         nullptr, 0, n);
+    if (threadIdx.x == 0) a.out[row_at] = pick;
+    return;
   }
-  for (int i = threadIdx.x; i < min(n, FS_LIST); i += FS_THREADS) s.list[i] = w.list()[i];
-  const u64 over = w.whole()[FS_BINS];
-  __syncthreads();
+  u64 m = 0, over = 0;
+  uint32_t c = 0;
+#pragma unroll 4
+  for (int p = 0; p < a.pieces; ++p) {
+    m += w.binned()[p].mass[threadIdx.x];
+    c += w.binned()[p].count[threadIdx.x];
+  }
+  for (int p = threadIdx.x; p < a.pieces; p += FS_THREADS) over += w.binned()[p].over;
+  s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x] = m;
+  s.count[threadIdx.x] = w.whole()->count[threadIdx.x] = c;
+  over = fs_sum<FS_THREADS>(over, s);
   FsRunning run;
   run.of(s);
   const FsRanges ranges = fs_ranges(run, asked, over);
-  const int pick = fs_draw(s, (const T*)a.logits + (size_t)row_at * a.stride, a.vocab, fs_row(asked.temperature, high, low), asked, run, ranges,
-                           over, n);
+  if (threadIdx.x == 0) {
+    FsHead& head = *w.head();
+    head.ranges[0] = ranges.k_bin; head.ranges[1] = ranges.p_first; head.ranges[2] = ranges.p_last;
+    head.ranges[3] = ranges.draw_first; head.ranges[4] = ranges.draw_last;
+    head.over = over;
+  }
+}
+
+__device__ __forceinline__ FsRanges fs_kept_ranges(const FsSpace& w) {
+  const int* kept = w.head()->ranges;
+  return FsRanges{scalar_int(kept), scalar_int(kept + 1), scalar_int(kept + 2), scalar_int(kept + 3), scalar_int(kept + 4)};
+}
+
+template <typename T>
+__global__ void __launch_bounds__(FS_THREADS)
+sample_filtered_gather(FsArgs a) {
+  __shared__ FsSmall s;
+  const FsSpace w = fs_space(a, blockIdx.y);
+  const FsAsked asked = fs_asked(a, blockIdx.y);
+  if (fs_listed_at_once(asked, a.pieces)) return;
+  float v[FS_EACH], high, low;
+  int at;
+  fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
+  fs_row_extent(w, high, at, low);
+  if (!fs_is_drawn(asked.temperature, high)) return;
+  const FsRow r = fs_row(asked.temperature, high, low);
+  const FsRanges ranges = fs_kept_ranges(w);
+  fs_append(w, v, s, [&](float x) { return r.top - x <= r.reach && ranges.has(fs_bin(x, r)); });
+}
+
+template <typename T>
+__global__ void __launch_bounds__(FS_THREADS)
+sample_filtered_draw(FsArgs a) {
+  __shared__ FsShared s;
+  const int row_at = blockIdx.x;
+  const FsSpace w = fs_space(a, row_at);
+  const FsAsked asked = fs_asked(a, row_at);
+  if (fs_listed_at_once(asked, a.pieces)) return;
+  float high, low;
+  int at;
+  fs_row_extent(w, high, at, low);
+  if (!fs_is_drawn(asked.temperature, high)) return;
+  const int n = w.head()->n_listed;
+  s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x];
+  s.count[threadIdx.x] = w.whole()->count[threadIdx.x];
+  for (int i = threadIdx.x; i < min(n, FS_LIST); i += FS_THREADS) s.list[i] = w.list()[i];
+  const u64 over = w.head()->over;
+  const FsRanges ranges = fs_kept_ranges(w);
+  __syncthreads();
+  const int pick = fs_draw<FS_THREADS>(s, (const T*)a.logits + (size_t)row_at * a.stride, a.vocab, fs_row(asked.temperature, high, low), asked,
+                                       &ranges, over, n);
   if (threadIdx.x == 0) a.out[row_at] = pick;
 }
 
 #define FS_MAX_VOCAB (1 << 19)
+static_assert((FS_MAX_VOCAB / FS_PIECE) * FS_PIECE_WAVES <= 8 * WAVE, "the waves' maxima that fs_cut holds");
 
+static bool fs_is_short(int vocab) { return vocab <= FS_SHORT_THREADS * FS_SHORT_EACH; }
 static int fs_pieces(int vocab) { return (vocab + FS_PIECE - 1) / FS_PIECE; }
 
-// Bytes of workspace a row needs (a multiple of 16; none up to FS_PIECE logits).
-extern "C" int ta_sample_filtered_workspace(int vocab) {
-  const int pieces = fs_pieces(vocab);
-  return pieces <= 1 ? 0 : (int)((fs_list_at(pieces) + 8 * FS_LIST + 15) / 16 * 16);
-}
+// Bytes of workspace a row needs (a multiple of 16; none for a short row).
+extern "C" int ta_sample_filtered_workspace(int vocab) { return fs_is_short(vocab) ? 0 : (int)fs_row_bytes(fs_pieces(vocab)); }
 
 template <typename T>
 static int launch_filtered(FsArgs a, int n_rows, hipStream_t stream) {
-  if (a.pieces <= 1) {
-    sample_filtered_short<T><<<n_rows, FS_THREADS, 0, stream>>>(a);
+  if (fs_is_short(a.vocab)) {
+    sample_filtered_short<T><<<n_rows, FS_SHORT_THREADS, 0, stream>>>(a);
     return LAUNCH_STATUS();
   }
   const dim3 grid(a.pieces, n_rows);
@@ -766,6 +963,9 @@ static int launch_filtered(FsArgs a, int n_rows, hipStream_t stream) {
   int status = LAUNCH_STATUS();
   if (status) return status;
   sample_filtered_bins<T><<<grid, FS_THREADS, 0, stream>>>(a);
+  status = LAUNCH_STATUS();
+  if (status) return status;
+  sample_filtered_settle<T><<<n_rows, FS_THREADS, 0, stream>>>(a);
   status = LAUNCH_STATUS();
   if (status) return status;
   sample_filtered_gather<T><<<grid, FS_THREADS, 0, stream>>>(a);
@@ -782,11 +982,11 @@ extern "C" int ta_sample_filtered(const void* logits, int64_t stride, const void
                                   hipStream_t stream) {
   if (n_rows <= 0) return 0;
   if (vocab < 1 || vocab > FS_MAX_VOCAB || stride < 0 || n_rows > 65535) return -1;
-  if (!logits || !temperature || !top_k || !top_p || !min_p || !uniform || !out || (!workspace && fs_pieces(vocab) > 1)) return -1;
+  if (!logits || !temperature || !top_k || !top_p || !min_p || !uniform || !out || (!workspace && !fs_is_short(vocab))) return -1;
   FsArgs a;
   a.logits = logits; a.stride = stride; a.temperature = (const float*)temperature; a.top_p = (const float*)top_p;
   a.min_p = (const float*)min_p; a.uniform = (const float*)uniform; a.top_k = (const int*)top_k; a.out = (int*)out;
   a.vocab = vocab; a.pieces = fs_pieces(vocab); a.workspace = (char*)workspace;
-  a.row_bytes = (size_t)ta_sample_filtered_workspace(vocab);
+  a.row_bytes = fs_row_bytes(a.pieces);
   return dtype == DT_F32 ? launch_filtered<float>(a, n_rows, stream) : launch_filtered<bf16_t>(a, n_rows, stream);
 }
