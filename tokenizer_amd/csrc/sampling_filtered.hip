@@ -14,7 +14,7 @@
 //
 // No row is sorted whole: the tokens among which the answers lie, some hundreds, are gathered and sorted in LDS.
 //   * Where the first k tokens are all that counts, or those that min-p keeps, a logit is known below which nothing does
-//     (`fs_cut`): the k-th largest of the maxima that the row's waves found, of which at least k tokens are no smaller, or
+//     (`fs_cut`): the k-th largest of the maxima of the row's parts, of which at least k tokens are no smaller, or
 //     max + T ln(min_p).  What is not below it is the list.
 //   * Else every token's weight matters.  The tokens fall into FS_BINS ranges of logit, equal parts of what lies between the maximum and the
 //     lowest logit that weighs anything, each with its count and weight; the answers then lie in a few ranges (what is not known
@@ -33,6 +33,7 @@
 #define FS_SHORT_EACH 32
 #define FS_BINS 256                     // four a lane
 #define FS_LIST 8192
+#define FS_FEW 128
 #define FS_SLOTS 256                    // ranges that a round of narrowing tells apart
 #define FS_MAX_WAVES (FS_SHORT_THREADS / WAVE)
 #define FS_UNIT 17592186044416.0        // 2^44
@@ -101,16 +102,22 @@ struct FsSmall {
   float wave_low[FS_MAX_WAVES], wave_high[FS_MAX_WAVES];
   int wave_at[FS_MAX_WAVES];
   int n_listed;
+  float cut;
 };
 
+struct FsFew { u64 token, w; };
+
 struct FsShared : FsSmall {
+  FsFew few[FS_FEW];                    // a short list with its weights, and what its parts add up
+  u64 part_mass[FS_SHORT_THREADS];
+  uint32_t part_count[FS_SHORT_THREADS];
   union {
     u64 list[FS_LIST];                  // the gathered tokens, key in the upper half, the index's complement in the lower
     struct { u64 mass[FS_SLOTS]; uint32_t count[FS_SLOTS]; } slots;      // a round of narrowing
   };
   u64 missing_mass[FS_BINS];            // of bins that were not gathered, in front of this one
   uint32_t missing_count[FS_BINS];
-  u64 found_mass, kept;
+  u64 found_mass, kept, over;
   uint32_t found_count;
   int found;
   uint32_t key_low, key_high;
@@ -144,9 +151,11 @@ __device__ __forceinline__ void fs_load(const T* __restrict__ row, int begin, in
     if (begin + j * THREADS + (int)threadIdx.x >= vocab) v[j] = __uint_as_float(0x7fc00000u);
 }
 
-// The largest of a piece's logits, its lowest index, and the smallest above -inf, to every thread.  `of_wave`: the largest of the wave's.
+// The largest of a piece's logits, its lowest index, and the smallest above -inf, to every thread.  `of_wave`, `of_row`: the
+// largest of the wave's, and of those of the thread's sixteen lanes.
 template <int THREADS, int EACH>
-__device__ __forceinline__ void fs_extent(const float (&v)[EACH], int begin, float& high, int& at, float& low, float& of_wave, FsSmall& s) {
+__device__ __forceinline__ void fs_extent(const float (&v)[EACH], int begin, float& high, int& at, float& low, float& of_wave, float& of_row,
+                                          FsSmall& s) {
   high = -INFINITY;
   low = INFINITY;
 #pragma unroll
@@ -154,7 +163,8 @@ __device__ __forceinline__ void fs_extent(const float (&v)[EACH], int begin, flo
     high = fmaxf(high, v[j]);
     low = fminf(low, v[j] > -INFINITY ? v[j] : INFINITY);
   }
-  high = of_wave = wave_max(high);
+  of_row = wave_max_repeated<16>(high);
+  high = of_wave = wave_max_across<32>(wave_max_across<16>(of_row));
   low = -wave_max(-low);
   at = 0x7fffffff;
   if (high > -INFINITY) {
@@ -507,82 +517,117 @@ __device__ __forceinline__ void fs_sort(FsShared& s, int size) {
   __syncthreads();
 }
 
-// The three answers from the sorted list; a thread has up to MOST neighbours of it.
-template <int THREADS, int MOST>
-__device__ __forceinline__ int fs_answers(FsShared& s, const FsRow& r, const FsAsked& asked, u64 all, bool k_here, u64 over, bool over_known,
-                                          bool all_listed, int n, int per) {
-  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+// The three answers.  `each(use)` calls use(token, weight, weight before it on the list, place on the list) for every token of the
+// list, each by one thread.  `all`: the weight of the whole row (of the list, if that holds the order's first tokens: `all_listed`);
+// `over`: the weight of what min-p keeps, if it is known.
+template <typename Each>
+__device__ __forceinline__ int fs_answers(FsShared& s, const FsRow& r, const FsAsked& asked, u64 all, bool k_here, u64 over, bool all_listed,
+                                          Each each) {
   const double floor_share = (double)asked.min_p * FS_UNIT;
-  u64 token[MOST], w[MOST], sum = 0, above = 0;
-#pragma unroll
-  for (int j = 0; j < MOST; ++j) {
-    const int i = threadIdx.x * per + j;
-    token[j] = 0;
-    w[j] = 0;
-    if (j < per && i < n) {
-      token[j] = s.list[i];
-      const float v = fs_value((uint32_t)(token[j] >> 32));
-      const double share = fs_share(v, r);
-      w[j] = fs_whole(share);
-      if (!(asked.min_p > 0.f) || !(share < floor_share) || v == r.top) above += w[j];
-    }
-    sum += w[j];
-  }
-  u64 before = sum;
-  for (int off = 1; off < WAVE; off <<= 1) before += fs_up(before, off, lane);
-  if (lane == WAVE - 1) s.wave_mass[wave] = before;
-  before -= sum;
-  if (!over_known) {                                       // (what min-p keeps is in the list, or ends behind it)
-    for (int off = WAVE / 2; off > 0; off >>= 1) above += __shfl_xor(above, off, WAVE);
-    if (lane == 0) s.wave_over[wave] = above;
-  }
-  __syncthreads();
-  u64 listed = 0, floored = 0;
-#pragma unroll
-  for (int i = 0; i < THREADS / WAVE; ++i) {
-    if (i < wave) before += s.wave_mass[i];
-    listed += s.wave_mass[i];
-    floored += over_known ? 0 : s.wave_over[i];
-  }
-  if (!over_known) over = floored;
   if (threadIdx.x == 0) {
-    s.kept = all_listed ? listed : all;
-    s.found = n > 0 ? (int)~(uint32_t)s.list[0] : 0;
+    s.kept = all;
+    s.found = 0;
+    s.over = 0;
   }
   __syncthreads();
-  u64 at_mass[MOST];                                       // what stands before a token in the whole order
-#pragma unroll
-  for (int j = 0; j < MOST; ++j) {
-    at_mass[j] = before;
-    before += w[j];
-    if (token[j]) {
-      uint32_t at = threadIdx.x * per + j;
-      if (!all_listed) {
-        const int bin = fs_bin(fs_value((uint32_t)(token[j] >> 32)), r);
-        at_mass[j] += s.missing_mass[bin];
-        at += s.missing_count[bin];
-      }
-      if (k_here && at + 1 == (uint32_t)asked.top_k) s.kept = at_mass[j] + w[j];
-    }
-  }
+  auto missing = [&](u64 token) { return all_listed ? 0ull : s.missing_mass[fs_bin(fs_value((uint32_t)(token >> 32)), r)]; };
+  u64 above = 0;
+  each([&](u64 token, u64 w, u64 before, uint32_t at) {
+    const float v = fs_value((uint32_t)(token >> 32));
+    before += missing(token);
+    if (!all_listed) at += s.missing_count[fs_bin(v, r)];
+    else if (!(asked.min_p > 0.f) || !(fs_share(v, r) < floor_share) || v == r.top)
+      above = max(above, before + w);                      // (what min-p keeps is in the list, or ends behind it)
+    if (k_here && at + 1 == (uint32_t)asked.top_k) s.kept = before + w;
+  });
+  if (above) atomicMax(&s.over, above);
   __syncthreads();
   u64 kept = s.kept;
+  if (all_listed) over = s.over;
   if (asked.top_p < 1.f) {
     __syncthreads();
     const u64 need = fs_need_of_share(asked.top_p, kept);
-#pragma unroll
-    for (int j = 0; j < MOST; ++j)
-      if (token[j] && at_mass[j] < need && at_mass[j] + w[j] >= need) s.kept = at_mass[j] + w[j];
+    each([&](u64 token, u64 w, u64 before, uint32_t) {
+      before += missing(token);
+      if (before < need && before + w >= need) s.kept = before + w;
+    });
     __syncthreads();
     kept = s.kept;
   }
   kept = over < kept ? over : kept;
   const u64 need = fs_need_of_draw(asked.uniform, kept);
-#pragma unroll
-  for (int j = 0; j < MOST; ++j)
-    if (token[j] && at_mass[j] < need && at_mass[j] + w[j] >= need) s.found = (int)~(uint32_t)token[j];
+  each([&](u64 token, u64 w, u64 before, uint32_t) {
+    before += missing(token);
+    if (before < need && before + w >= need) s.found = (int)~(uint32_t)token;
+  });
   __syncthreads();
   return s.found;
+}
+
+// Up to FS_FEW tokens: each is held against all others, THREADS / FS_FEW threads a token (64 tokens in 0.3 us, 128 in 0.9, where
+// sorting takes 2 and 2.6).
+template <int THREADS>
+__device__ __forceinline__ int fs_answers_of_few(FsShared& s, const FsRow& r, const FsAsked& asked, u64 all, bool k_here, u64 over, bool all_listed,
+                                                 int n) {
+  const int size = n <= WAVE ? WAVE : FS_FEW, parts = THREADS / size;
+  const int at = threadIdx.x & (size - 1), part = threadIdx.x / size;
+  u64 token = at < n ? s.list[at] : 0;
+  const u64 w = token ? fs_weight(fs_value((uint32_t)(token >> 32)), r) : 0;
+  if (part == 0) s.few[at] = FsFew{token, w};
+  __syncthreads();
+  u64 before = 0, listed = 0;
+  uint32_t place = 0;
+  const int of_part = size / parts;
+  for (int i = part * of_part; i < (part + 1) * of_part; ++i) {          // (the same for a whole wave)
+    const FsFew other = s.few[i];
+    const bool first = other.token > token;
+    before += first ? other.w : 0;
+    place += first ? 1 : 0;
+    listed += other.w;
+  }
+  s.part_mass[threadIdx.x] = before;
+  s.part_count[threadIdx.x] = place;
+  if (at == 0) s.wave_over[part] = listed;
+  __syncthreads();
+  before = listed = 0;
+  place = 0;
+  for (int i = 0; i < parts; ++i) {
+    before += s.part_mass[i * size + at];
+    place += s.part_count[i * size + at];
+    listed += s.wave_over[i];
+  }
+  const bool goes_on = token && part == 0;                 // (one thread a token)
+  return fs_answers(s, r, asked, all_listed ? listed : all, k_here, over, all_listed, [&](auto use) { if (goes_on) use(token, w, before, place); });
+}
+
+// More: from the sorted list, of which a thread has `per` neighbours.  (Their weights are worked out again for every answer: keeping
+// those of 32 tokens would take the registers of all kernels that come here.)
+template <int THREADS>
+__device__ __forceinline__ int fs_answers_of_sorted(FsShared& s, const FsRow& r, const FsAsked& asked, u64 all, bool k_here, u64 over,
+                                                    bool all_listed, int n, int per) {
+  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  const int first = threadIdx.x * per, last = min(n, first + per);
+  u64 sum = 0;
+  for (int i = first; i < last; ++i) sum += fs_weight(fs_value((uint32_t)(s.list[i] >> 32)), r);
+  u64 run = sum;
+  for (int off = 1; off < WAVE; off <<= 1) run += fs_up(run, off, lane);
+  if (lane == WAVE - 1) s.wave_mass[wave] = run;
+  run -= sum;
+  __syncthreads();
+  u64 listed = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / WAVE; ++i) {
+    if (i < wave) run += s.wave_mass[i];
+    listed += s.wave_mass[i];
+  }
+  return fs_answers(s, r, asked, all_listed ? listed : all, k_here, over, all_listed, [&](auto use) {
+    u64 before = run;
+    for (int i = first; i < last; ++i) {
+      const u64 token = s.list[i], w = fs_weight(fs_value((uint32_t)(token >> 32)), r);
+      use(token, w, before, (uint32_t)i);
+      before += w;
+    }
+  });
 }
 
 // The draw from the `n` tokens in `s.list` (in any order), if they all found room there, else by narrowing.  `ranges`: the list holds
@@ -618,15 +663,16 @@ __device__ int fs_draw(FsShared& s, const T* row, int vocab, const FsRow& r, con
       }
     }
   }
-  int size = 2 * WAVE;
+  const bool k_here = asked.top_k > 0 && (!ranges || ranges->k_bin >= 0);
+  __syncthreads();
+  if (n <= FS_FEW) return fs_answers_of_few<THREADS>(s, r, asked, all, k_here, over, ranges == nullptr, n);
+  int size = 2 * FS_FEW;
   while (size < n) size <<= 1;
   for (int i = n + threadIdx.x; i < size; i += THREADS) s.list[i] = 0;           // (behind every token)
   __syncthreads();
   fs_sort<THREADS>(s, size);
   const int per = max(1, size / THREADS);
-  const bool k_here = asked.top_k > 0 && (!ranges || ranges->k_bin >= 0);
-  if (per <= 4) return fs_answers<THREADS, 4>(s, r, asked, all, k_here, over, ranges != nullptr, ranges == nullptr, n, per);
-  return fs_answers<THREADS, FS_LIST / THREADS>(s, r, asked, all, k_here, over, ranges != nullptr, ranges == nullptr, n, per);
+  return fs_answers_of_sorted<THREADS>(s, r, asked, all, k_here, over, ranges == nullptr, n, per);
 }
 
 struct FsArgs {
@@ -659,10 +705,10 @@ sample_filtered_short(FsArgs a) {
   const int row_at = blockIdx.x;
   const T* row = (const T*)a.logits + (size_t)row_at * a.stride;
   const FsAsked asked = fs_asked(a, row_at);
-  float v[FS_SHORT_EACH], high, low, of_wave;
+  float v[FS_SHORT_EACH], high, low, of_wave, of_row;
   int at;
   fs_load<THREADS>(row, 0, a.vocab, v);
-  fs_extent<THREADS>(v, 0, high, at, low, of_wave, s);
+  fs_extent<THREADS>(v, 0, high, at, low, of_wave, of_row, s);
   if (!fs_is_drawn(asked.temperature, high)) {
     if (threadIdx.x == 0) a.out[row_at] = at == 0x7fffffff ? 0 : at;
     return;
@@ -688,10 +734,12 @@ sample_filtered_short(FsArgs a) {
 // ------------------------------------------------------------------------------------------------
 // A longer row: its pieces' workgroups leave what they found in the workspace, a launch a step.
 #define FS_PIECE_WAVES (FS_THREADS / WAVE)
-struct FsExtent { float high, low; int at, unused; float of_wave[FS_PIECE_WAVES]; };
+#define FS_PIECE_ROWS (FS_THREADS / 16)
+struct FsExtent { float high, low; int at, unused; };
 struct FsHead { int n_listed; int ranges[5]; int unused[2]; u64 over; u64 unused2; };      // of a row
 struct FsBinned { u64 mass[FS_BINS]; uint32_t count[FS_BINS]; u64 over; u64 unused; };    // of a piece, or of a row
-// Per row: its head, its bins, its list, the pieces' extents and the pieces' bins.
+// Per row: its head, its bins, its list, the pieces' extents, the maxima of their waves and of these waves' rows of sixteen lanes, and the
+// pieces' bins.
 struct FsSpace {
   char* base;
   int pieces;
@@ -699,68 +747,83 @@ struct FsSpace {
   __device__ __forceinline__ FsBinned* whole() const { return (FsBinned*)(base + sizeof(FsHead)); }
   __device__ __forceinline__ u64* list() const { return (u64*)(whole() + 1); }
   __device__ __forceinline__ FsExtent* extents() const { return (FsExtent*)(list() + FS_LIST); }
-  __device__ __forceinline__ FsBinned* binned() const { return (FsBinned*)(extents() + pieces); }
+  __device__ __forceinline__ float* of_waves() const { return (float*)(extents() + pieces); }
+  __device__ __forceinline__ float* of_rows() const { return of_waves() + pieces * FS_PIECE_WAVES; }
+  __device__ __forceinline__ FsBinned* binned() const { return (FsBinned*)(of_rows() + pieces * FS_PIECE_ROWS); }
 };
 static size_t fs_row_bytes(int pieces) {
-  return sizeof(FsHead) + sizeof(FsBinned) + 8 * FS_LIST + (sizeof(FsExtent) + sizeof(FsBinned)) * (size_t)pieces;
+  return sizeof(FsHead) + sizeof(FsBinned) + 8 * FS_LIST + (sizeof(FsExtent) + 4 * (FS_PIECE_WAVES + FS_PIECE_ROWS) + sizeof(FsBinned)) * (size_t)pieces;
 }
-static_assert(sizeof(FsHead) % 16 == 0 && sizeof(FsBinned) % 16 == 0 && sizeof(FsExtent) % 16 == 0, "pieces of sixteen bytes");
+static_assert(sizeof(FsHead) % 16 == 0 && sizeof(FsBinned) % 16 == 0 && sizeof(FsExtent) % 16 == 0 && (FS_PIECE_WAVES + FS_PIECE_ROWS) % 4 == 0, "pieces of sixteen bytes");
 __device__ __forceinline__ FsSpace fs_space(const FsArgs& a, int row) { return FsSpace{a.workspace + (size_t)row * a.row_bytes, a.pieces}; }
 
 // The row's extent from its pieces' (a lane of every wave looks at one piece of sixty-four), to every thread.
-__device__ __forceinline__ void fs_row_extent(const FsSpace& w, float& high, int& at, float& low) {
+__device__ __forceinline__ void fs_row_extent(const FsSpace& w, float& high, float& low) {
   const int lane = threadIdx.x & (WAVE - 1);
   high = -INFINITY;
   low = INFINITY;
-  at = 0x7fffffff;
   for (int p = lane; p < w.pieces; p += WAVE) {
-    const FsExtent& e = w.extents()[p];
-    if (e.high > high) { high = e.high; at = e.at; }       // (pieces in the order of their indices)
-    low = fminf(low, e.low);
+    high = fmaxf(high, w.extents()[p].high);
+    low = fminf(low, w.extents()[p].low);
   }
-  const float mine = high;
   high = wave_max(high);
   low = -wave_max(-low);
-  if (mine != high) at = 0x7fffffff;
+}
+// The lowest index of the row's largest logit, to every thread; 0 if there is none above -inf.
+__device__ __forceinline__ int fs_row_top(const FsSpace& w, float high) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  int at = 0x7fffffff;
+  for (int p = lane; p < w.pieces; p += WAVE)
+    if (w.extents()[p].high == high) at = min(at, w.extents()[p].at);
   for (int off = WAVE / 2; off > 0; off >>= 1) at = min(at, __shfl_xor(at, off, WAVE));
+  return at == 0x7fffffff ? 0 : at;
 }
 
 // Whether a row's list can be made without its bins.
 __device__ __forceinline__ bool fs_listed_at_once(const FsAsked& asked, int pieces) {
-  return (asked.top_k > 0 && asked.top_k <= pieces * FS_PIECE_WAVES) || (!(asked.top_p < 1.f) && asked.min_p > 0.f);
+  return (asked.top_k > 0 && asked.top_k <= pieces * FS_PIECE_ROWS) || (!(asked.top_p < 1.f) && asked.min_p > 0.f);
+}
+
+// A logit not below `least` of which at least k of the `count` maxima are no smaller, close to the k-th largest of them; -inf if there are
+// not so many.
+template <int MOST>
+__device__ __forceinline__ float fs_cut_of_maxima(const float* __restrict__ maxima, int count, int k, float least, float most) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  float m[MOST];                                           // of 64 lanes
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) {
+    m[j] = -INFINITY;
+    if (j * WAVE + lane < count) m[j] = maxima[j * WAVE + lane];
+  }
+  auto no_smaller = [&](float t) {
+    int found = 0;
+#pragma unroll
+    for (int j = 0; j < MOST; ++j)
+      if (j * WAVE < count) found += __popcll(__ballot(m[j] >= t));
+    return found;
+  };
+  if (no_smaller(least) < k) return -INFINITY;
+  for (int turn = 0; turn < 8; ++turn) {
+    const float middle = 0.5f * least + 0.5f * most;
+    if (no_smaller(middle) >= k) least = middle; else most = middle;
+  }
+  return least;
 }
 
 // A logit so that every token that counts is no smaller.
-//   top-k: at least k of the waves' maxima are no smaller; found by halving between the largest and the smallest logit that weighs
+//   top-k: at least k of the maxima are no smaller; found by halving between the largest and the smallest logit that weighs
 //   anything, and what the halvings leave undecided stays above the cut.
 //   min-p (where top-p cuts nothing): max + T ln(min_p), less what 32 bits may be off by: 4 roundings of each of its parts.
 __device__ __forceinline__ float fs_cut(const FsSpace& w, const FsAsked& asked, const FsRow& r, float low) {
-  const int lane = threadIdx.x & (WAVE - 1);
   const float high = r.top;
   float cut = -INFINITY;
-  if (asked.top_k > 0 && asked.top_k <= w.pieces * FS_PIECE_WAVES) {
-    constexpr int MOST = 8;                                // of 64 lanes: up to 128 pieces of four waves
-    float m[MOST];
-#pragma unroll
-    for (int j = 0; j < MOST; ++j) {
-      const int i = j * WAVE + lane;
-      m[j] = i < w.pieces * FS_PIECE_WAVES ? w.extents()[i / FS_PIECE_WAVES].of_wave[i % FS_PIECE_WAVES] : -INFINITY;
-    }
-    auto no_smaller = [&](float t) {
-      int count = 0;
-#pragma unroll
-      for (int j = 0; j < MOST; ++j)
-        if (j * WAVE < w.pieces * FS_PIECE_WAVES) count += __popcll(__ballot(m[j] >= t));
-      return count;
-    };
-    float least = fmaxf(low, high - r.reach), most = high;   // (what lies further below weighs nothing)
-    if (no_smaller(least) >= asked.top_k) {
-      for (int turn = 0; turn < 12; ++turn) {
-        const float middle = 0.5f * least + 0.5f * most;
-        if (no_smaller(middle) >= asked.top_k) least = middle; else most = middle;
-      }
-      cut = least;
-    }
+  if (asked.top_k > 0 && asked.top_k <= w.pieces * FS_PIECE_ROWS) {
+    const float least = fmaxf(low, high - r.reach);        // (what lies further below weighs nothing)
+    // Few maxima while k is small beside their number (k = 40 of 152: some 50 tokens are no smaller; 150 of them: 700).
+    cut = 2 * asked.top_k <= w.pieces * FS_PIECE_WAVES ? fs_cut_of_maxima<8>(w.of_waves(), w.pieces * FS_PIECE_WAVES, asked.top_k, least, high)
+                                                       : w.pieces * FS_PIECE_ROWS <= 12 * WAVE
+              ? fs_cut_of_maxima<12>(w.of_rows(), w.pieces * FS_PIECE_ROWS, asked.top_k, least, high)
+              : fs_cut_of_maxima<32>(w.of_rows(), w.pieces * FS_PIECE_ROWS, asked.top_k, least, high);
   }
   if (!(asked.top_p < 1.f) && asked.min_p > 0.f) {
     const float down = -asked.temperature * logf(fminf(asked.min_p, 1.f));
@@ -812,12 +875,13 @@ __global__ void __launch_bounds__(FS_THREADS)
 sample_filtered_extents(FsArgs a) {
   __shared__ FsSmall s;
   const FsSpace w = fs_space(a, blockIdx.y);
-  float v[FS_EACH], high, low, of_wave;
+  float v[FS_EACH], high, low, of_wave, of_row;
   int at;
   fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
-  fs_extent<FS_THREADS>(v, blockIdx.x * FS_PIECE, high, at, low, of_wave, s);
+  fs_extent<FS_THREADS>(v, blockIdx.x * FS_PIECE, high, at, low, of_wave, of_row, s);
   FsExtent& e = w.extents()[blockIdx.x];
-  if ((threadIdx.x & (WAVE - 1)) == 0) e.of_wave[threadIdx.x / WAVE] = of_wave;
+  if ((threadIdx.x & (WAVE - 1)) == 0) w.of_waves()[blockIdx.x * FS_PIECE_WAVES + threadIdx.x / WAVE] = of_wave;
+  if ((threadIdx.x & 15) == 0) w.of_rows()[blockIdx.x * FS_PIECE_ROWS + threadIdx.x / 16] = of_row;
   if (threadIdx.x == 0) {
     e.high = high;
     e.low = low;
@@ -834,13 +898,18 @@ sample_filtered_bins(FsArgs a) {
   const FsSpace w = fs_space(a, blockIdx.y);
   const FsAsked asked = fs_asked(a, blockIdx.y);
   float v[FS_EACH], high, low;
-  int at;
   fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
-  fs_row_extent(w, high, at, low);
+  fs_row_extent(w, high, low);
   if (!fs_is_drawn(asked.temperature, high)) return;
   const FsRow r = fs_row(asked.temperature, high, low);
   if (fs_listed_at_once(asked, a.pieces)) {
-    const float cut = fs_cut(w, asked, r, low);
+    // (One wave works it out: eight halvings among six hundred maxima by every wave of 2,432 workgroups took 14 us of their time.)
+    if (threadIdx.x < WAVE) {
+      const float found = fs_cut(w, asked, r, low);
+      if (threadIdx.x == 0) s.cut = found;
+    }
+    __syncthreads();
+    const float cut = s.cut;
     fs_append(w, v, s, [&](float x) { return x >= cut && r.top - x <= r.reach; });
     return;
   }
@@ -861,10 +930,10 @@ sample_filtered_settle(FsArgs a) {
   const FsSpace w = fs_space(a, row_at);
   const FsAsked asked = fs_asked(a, row_at);
   float high, low;
-  int at;
-  fs_row_extent(w, high, at, low);
+  fs_row_extent(w, high, low);
   if (!fs_is_drawn(asked.temperature, high)) {
-    if (threadIdx.x == 0) a.out[row_at] = at == 0x7fffffff ? 0 : at;
+    const int at = fs_row_top(w, high);
+    if (threadIdx.x == 0) a.out[row_at] = at;
     return;
   }
   if (fs_listed_at_once(asked, a.pieces)) {
@@ -877,10 +946,18 @@ sample_filtered_settle(FsArgs a) {
   }
   u64 m = 0, over = 0;
   uint32_t c = 0;
-#pragma unroll 4
-  for (int p = 0; p < a.pieces; ++p) {
-    m += w.binned()[p].mass[threadIdx.x];
-    c += w.binned()[p].count[threadIdx.x];
+  for (int first = 0; first < a.pieces; first += 16) {     // (sixteen pieces asked for at a time)
+    u64 of_mass[16];
+    uint32_t of_count[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const FsBinned& piece = w.binned()[min(first + j, a.pieces - 1)];
+      of_mass[j] = piece.mass[threadIdx.x];
+      of_count[j] = piece.count[threadIdx.x];
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (first + j < a.pieces) { m += of_mass[j]; c += of_count[j]; }
   }
   for (int p = threadIdx.x; p < a.pieces; p += FS_THREADS) over += w.binned()[p].over;
   s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x] = m;
@@ -910,9 +987,8 @@ sample_filtered_gather(FsArgs a) {
   const FsAsked asked = fs_asked(a, blockIdx.y);
   if (fs_listed_at_once(asked, a.pieces)) return;
   float v[FS_EACH], high, low;
-  int at;
   fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
-  fs_row_extent(w, high, at, low);
+  fs_row_extent(w, high, low);
   if (!fs_is_drawn(asked.temperature, high)) return;
   const FsRow r = fs_row(asked.temperature, high, low);
   const FsRanges ranges = fs_kept_ranges(w);
@@ -928,8 +1004,7 @@ sample_filtered_draw(FsArgs a) {
   const FsAsked asked = fs_asked(a, row_at);
   if (fs_listed_at_once(asked, a.pieces)) return;
   float high, low;
-  int at;
-  fs_row_extent(w, high, at, low);
+  fs_row_extent(w, high, low);
   if (!fs_is_drawn(asked.temperature, high)) return;
   const int n = w.head()->n_listed;
   s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x];
@@ -944,7 +1019,8 @@ sample_filtered_draw(FsArgs a) {
 }
 
 #define FS_MAX_VOCAB (1 << 19)
-static_assert((FS_MAX_VOCAB / FS_PIECE) * FS_PIECE_WAVES <= 8 * WAVE, "the waves' maxima that fs_cut holds");
+static_assert((FS_MAX_VOCAB / FS_PIECE) * FS_PIECE_WAVES <= 8 * WAVE && (FS_MAX_VOCAB / FS_PIECE) * FS_PIECE_ROWS <= 32 * WAVE,
+              "the maxima that fs_cut holds");
 
 static bool fs_is_short(int vocab) { return vocab <= FS_SHORT_THREADS * FS_SHORT_EACH; }
 static int fs_pieces(int vocab) { return (vocab + FS_PIECE - 1) / FS_PIECE; }
