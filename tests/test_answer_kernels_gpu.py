@@ -437,6 +437,18 @@ def test_attention_over_lengths(ops, rows, prefix_keys, page):
     batch.check(batch.run(ops)[0])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,n_q,n_kv", [(33, 2, 1), (13, 14, 2), (19, 28, 4), (60, 12, 2), (129, 1, 1), (40, 40, 1)])
+@pytest.mark.parametrize("keys,page", [(64, 16), (80, 16), (1008, 16), (96, 32), (1056, 48), (1600, 64)])
+def test_attention_of_many_columns(ops, keys, page, rows, n_q, n_kv, d):
+    # (More than 64 query columns of a kv head go through the shared keys together; parts and blocks of them end anywhere.)
+    tables, positions = shared_tables(rows, keys // page, page, [1 + (13 * r) % 40 for r in range(rows)])
+    batch = Batch(tables, positions, n_q, n_kv, d, page, torch.bfloat16, rows + keys)
+    got, plan = batch.run(ops)
+    assert any(plan.items.reshape(-1, 8)[:, 6].tolist())
+    batch.check(got)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_behind_branches(ops, dtype):
     tables, positions = shared_tables(23, 13, 16, [1 + (29 * r) % 200 for r in range(23)], branch=(4, 7))

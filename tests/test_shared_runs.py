@@ -113,10 +113,10 @@ def test_the_work_list_covers_every_query_and_key_once(seed):
     order, own, parts = plan.order_dev.tolist(), plan.own_begin_dev.tolist(), plan.parts_dev.tolist()
     assert len(items) == plan.n_items and order == plan.order and own == plan.own_begin.tolist()
     seen = {}                                               # (row, head in its group) -> {slot: (begin, end)}
-    for rows_at, columns, first, begin, end, slot, _, _ in items:
+    for rows_at, columns, first, begin, end, slot, wide, _ in items:
         assert 0 <= first < columns and columns % group == 0 and rows_at + columns // group <= len(rows)
         assert begin < end <= plan.keys_end and begin % page == 0 and (begin - items[0][3]) % 16 == 0
-        for column in range(first, min(columns, first + plan.COLUMNS)):
+        for column in range(first, min(columns, first + (plan.WIDE_COLUMNS if wide else plan.COLUMNS))):
             slots = seen.setdefault((order[rows_at + column // group], column % group), {})
             assert slot not in slots
             slots[slot] = (begin, end)

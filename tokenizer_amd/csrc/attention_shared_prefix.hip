@@ -19,6 +19,9 @@ typedef float sp_floatx16 __attribute__((ext_vector_type(16)));
 
 #define SP_WAVES 4
 #define SP_BLOCK 32                    // keys of a step of a wave
+#define SP_WIDE_COLUMNS 128
+#define SP_WIDE_BLOCK 64               // keys of a step of a workgroup that shares them through LDS
+#define LOG2E 1.4426950408889634f
 
 // A run of shared keys and some of the queries that read them, as the host lists them.
 struct SharedItem {
@@ -27,7 +30,8 @@ struct SharedItem {
   int first_column;                    // of this item
   int key_begin, key_end;              // positions; key_end - 1 is the last
   int slot;                            // which of a query's partial results this one is
-  int unused0, unused1;
+  int wide;                            // whether it takes SP_WIDE_COLUMNS columns, a block of 32 a wave (else 32, the keys shared out)
+  int unused;
 };
 
 struct SharedArgs {
@@ -153,6 +157,185 @@ struct Frag<float, D> {
   }
 };
 
+// A step of the softmax: `s` holds BLOCKS blocks of 32 scores a column (a lane half's sixteen each), of which the first `there` keys count;
+// they become weights.  m: the largest score so far, in units of 1 / log2(e) (a weight is then one instruction of the exponent's),
+// l: this lane's sum of weights, o: the weighed values, all brought to the new maximum where it has grown for any of the wave's columns.
+template <int BLOCKS, int ROWS>
+__device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)[BLOCKS], int there, int half, float& m, float& l,
+                                           sp_floatx16 (&o)[ROWS]) {
+  float scale = a.scale * LOG2E;
+  if (a.softcap > 0.f) {
+    const float inner = 2.f * LOG2E * a.scale / a.softcap;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = a.softcap * (1.f - 2.f / (1.f + __builtin_amdgcn_exp2f(inner * s[b][i])));
+    scale = LOG2E;
+  }
+  if (there < BLOCKS * SP_BLOCK) {
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (SP_BLOCK * b + 16 * (i >> 3) + 8 * half + (i & 7) >= there) s[b][i] = -INFINITY;
+  }
+  float high = s[0][0];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) high = fmaxf(high, s[b][i]);
+  high = wave_max_across<32>(high) * scale;                // (the scale is positive)
+  if (__any(high > m)) {
+    const float m_new = fmaxf(m, high);
+    const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+    m = m_new;
+    l *= corr;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[r][i] *= corr;
+  }
+  const float from = m == -INFINITY ? 0.f : m;             // (no key yet: weights of exp(-inf))
+  float sum = 0.f;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], scale, -from));
+      sum += s[b][i];
+    }
+  l += sum;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Many columns: a wave has 32 of the workgroup's SP_WIDE_COLUMNS, and all of them go through the same keys, a block of 64 at a time, which
+// the workgroup brings into LDS while it works on the block before.  Loads write LDS in the order of their lanes, so the lanes ask for
+// pieces of sixteen bytes in the order in which the reads find them in different banks: a unit of sixteen keys lies key by key, piece p of
+// key k at place p ^ (k, or k / 2 where a key is half as long as the banks are wide); its values lie coordinate by coordinate, the two
+// pieces of a coordinate d changing places with d / 8.
+template <int D>
+struct Wide {
+  static constexpr int PIECES = D / 8, KEY = 2 * D, UNIT = 16 * KEY, TILE = 4 * UNIT;      // pieces of a key; bytes of keys (values alike)
+  static constexpr int ROUNDS = TILE / 4096, STEPS = D / 16, ROWS = D / 32;
+  static_assert(D == 64 || D == 128, "the order of the pieces is made for keys of 128 and of 256 bytes");
+  typedef const char __attribute__((address_space(1)))* from_t;
+  typedef char __attribute__((address_space(3)))* lds_t;
+
+  static __device__ __forceinline__ int turn(int key) { return D == 128 ? key & 15 : (key >> 1) & 7; }
+  // Which of the block's four units of sixteen keys a wave brings in round j.
+  static __device__ __forceinline__ int unit_of(int j, int wave) { return D == 128 ? j : 2 * j + (wave >> 1); }
+
+  // Bytes from a unit's start in its page to what this thread brings, for keys and for values.
+  static __device__ __forceinline__ uint32_t key_place(int thread) {
+    const int key = thread / PIECES % 16, place = thread % PIECES;
+    return key * KEY + 16 * (place ^ turn(key));
+  }
+  static __device__ __forceinline__ uint32_t value_place(int thread, int page_size) {
+    const int d = thread / 2 % D;
+    return d * page_size * 2 + 16 * ((thread & 1) ^ ((d >> 3) & 1));
+  }
+  static __device__ __forceinline__ sp_bf16x8 key_piece(const char* keys, int key, int piece) {
+    return *reinterpret_cast<const sp_bf16x8*>(keys + key * KEY + 16 * (piece ^ turn(key & 15)));
+  }
+  static __device__ __forceinline__ sp_bf16x8 value_piece(const char* values, int unit, int d, int half) {
+    return *reinterpret_cast<const sp_bf16x8*>(values + unit * UNIT + d * 32 + 16 * (half ^ ((d >> 3) & 1)));
+  }
+};
+
+template <int D>
+__device__ __forceinline__ void sp_wide(const SharedArgs& a, int rows_at, int columns, int first_column, int begin, int end, int slot, char* even,
+                                        char* odd) {
+  typedef Wide<D> W;
+  typedef Frag<bf16_t, D> F;
+  constexpr int ROWS = W::ROWS;
+  const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 31, half = lane >> 5;
+  const int kvh = blockIdx.y, group = a.n_q / a.n_kv;
+  const int column = first_column + 32 * wave + col;
+  const bool there = column < columns, wave_there = first_column + 32 * wave < columns;
+  const int row = there ? a.order[rows_at + column / group] : -1, head = kvh * group + column % group;
+  typename F::Query q;
+  F::load_query(q, (const bf16_t*)a.q + (size_t)max(row, 0) * a.q_stride + (size_t)head * D, there, half);
+  const int* table = a.block_table + (size_t)scalar_int(a.order + rows_at) * a.table_stride;
+  const uint32_t key_place = W::key_place(threadIdx.x), value_place = W::value_place(threadIdx.x, a.page_size);
+  const size_t page_bytes = (size_t)a.page_size * D * 2;
+  // Where round j's unit of a block starts in the pages (the run's last unit stands in for one behind it, of which nothing counts).
+  int page[W::ROUNDS], at[W::ROUNDS];
+  auto look_up = [&](int kb) {
+#pragma unroll
+    for (int j = 0; j < W::ROUNDS; ++j) {
+      const int key = min(kb + 16 * W::unit_of(j, wave), end - 16);
+      page[j] = min(max(scalar_int(table + key / a.page_size), 0), a.n_pages - 1);
+      at[j] = key % a.page_size;
+    }
+  };
+  auto fetch = [&](char* to) {
+#pragma unroll
+    for (int j = 0; j < W::ROUNDS; ++j) {
+      const size_t start = ((size_t)page[j] * a.n_kv + kvh) * page_bytes;
+      __builtin_amdgcn_global_load_lds((typename W::from_t)((const char*)a.k_pages + start + (size_t)at[j] * W::KEY + key_place),
+                                       (typename W::lds_t)(to + j * 4096 + wave * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((typename W::from_t)((const char*)a.vt_pages + start + (size_t)at[j] * 2 + value_place),
+                                       (typename W::lds_t)(to + W::TILE + j * 4096 + wave * 1024), 16, 0, 0);
+    }
+  };
+  sp_floatx16 o[ROWS];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) o[r] = (sp_floatx16){};
+  const int my_key = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
+  auto work = [&](const char* keys, int kb) {
+    const char* values = keys + W::TILE;
+    sp_floatx16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = (sp_floatx16){};
+#pragma unroll
+      for (int i = 0; i < W::STEPS; ++i)
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(W::key_piece(keys, SP_BLOCK * b + my_key, 2 * i + half), q.f[i], s[b], 0, 0, 0);
+    }
+    sp_softmax<2, ROWS>(a, s, end - kb, half, m, l, o);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      sp_bf16x8 w[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = (__bf16)s[b][i];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          o[r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(W::value_piece(values, 2 * b + t, 32 * r + col, half), w[t], o[r], 0, 0, 0);
+    }
+  };
+  // A block's loads are asked for a block ahead; the barrier behind the wait for them is also the one that frees the other buffer.
+  look_up(begin);
+  fetch(even);
+  look_up(begin + SP_WIDE_BLOCK);
+  for (int kb = begin; kb < end; kb += 2 * SP_WIDE_BLOCK) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);                    // all that this wave fetched has arrived (vmcnt 0)
+    __syncthreads();
+    if (kb + SP_WIDE_BLOCK < end) fetch(odd);
+    look_up(kb + 2 * SP_WIDE_BLOCK);
+    if (wave_there) work(even, kb);
+    if (kb + SP_WIDE_BLOCK >= end) break;                  // (the same for the whole workgroup)
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    if (kb + 2 * SP_WIDE_BLOCK < end) fetch(even);
+    look_up(kb + 3 * SP_WIDE_BLOCK);
+    if (wave_there) work(odd, kb + SP_WIDE_BLOCK);
+  }
+  l = wave_add_across<32>(l);
+  if (row < 0) return;
+  const size_t to = ((size_t)row * a.n_q + head) * a.slots + slot;
+  if (half == 0) { a.part_ml[2 * to] = m; a.part_ml[2 * to + 1] = l; }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<sp_floatx4*>(a.part_o + to * D + 32 * r + 8 * j + 4 * half) =
+          (sp_floatx4){o[r][4 * j], o[r][4 * j + 1], o[r][4 * j + 2], o[r][4 * j + 3]};
+}
+
+// ------------------------------------------------------------------------------------------------
 // One workgroup: some columns (COLS blocks of 32) of one kv head and a run of keys, which its waves share out block by block.  The
 // workgroups from `n_items` on take the requests' own keys.
 template <typename T, int D, int COLS>
@@ -160,7 +343,12 @@ __global__ void __launch_bounds__(SP_WAVES * WAVE)
 shared_prefix_kernel(SharedArgs a) {
   typedef Frag<T, D> F;
   constexpr int ROWS = F::ROWS;
-  __shared__ float o_s[SP_WAVES / 2][COLS][ROWS * 32][33];
+  constexpr bool WIDE = sizeof(T) == 2 && (D == 64 || D == 128);
+  constexpr int SUMS = SP_WAVES / 2 * COLS * ROWS * 32 * 33 * 4, TILES = WIDE ? 2 * SP_WIDE_BLOCK * D * 2 : 0;
+  // (The two buffers are arrays of their own, each named where it is used: a read of one then waits for no load into the other.)
+  __shared__ __attribute__((aligned(1024))) char even_s[SUMS > TILES ? SUMS : TILES];
+  __shared__ __attribute__((aligned(1024))) char odd_s[TILES ? TILES : 16];
+  float (*o_s)[COLS][ROWS * 32][33] = reinterpret_cast<float (*)[COLS][ROWS * 32][33]>(even_s);
   __shared__ float m_s[SP_WAVES][COLS * 32], l_s[SP_WAVES][COLS * 32];
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int col = lane & 31, half = lane >> 5;
@@ -171,6 +359,12 @@ shared_prefix_kernel(SharedArgs a) {
     rows_at = scalar_int(item); columns = scalar_int(item + 1); first_column = scalar_int(item + 2);
     begin = scalar_int(item + 3); end = scalar_int(item + 4); slot = scalar_int(item + 5);
     if (columns <= 0) return;                              // an item that only fills the list up
+    if constexpr (WIDE) {
+      if (scalar_int(item + 6)) {
+        sp_wide<D>(a, rows_at, columns, first_column, begin, end, slot, even_s, odd_s);
+        return;
+      }
+    }
   } else {
     const int tiles = (group + COLS * 32 - 1) / (COLS * 32);
     const int at = blockIdx.x - a.n_items, split = at % a.own_splits, tile = at / a.own_splits % tiles;
@@ -224,31 +418,9 @@ shared_prefix_kernel(SharedArgs a) {
     if (there < SP_BLOCK) f.cut_values(there, half);
 #pragma unroll
     for (int c = 0; c < COLS; ++c) {
-      sp_floatx16 s = f.scores(q[c]);
-      float high = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] *= a.scale;
-        if (a.softcap > 0.f) s[i] = a.softcap * (1.f - 2.f / (1.f + __expf(2.f * s[i] / a.softcap)));
-        if (there < SP_BLOCK && 16 * (i >> 3) + 8 * half + (i & 7) >= there) s[i] = -INFINITY;
-        high = fmaxf(high, s[i]);
-      }
-      high = wave_max_across<32>(high);
-      const float m_new = fmaxf(m[c], high);
-      const float corr = m_new == -INFINITY ? 1.f : __expf(m[c] - m_new);
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = m_new == -INFINITY ? 0.f : __expf(s[i] - m_new);
-        sum += s[i];
-      }
-      l[c] = l[c] * corr + sum;
-      m[c] = m_new;
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[c][r][i] *= corr;
-      f.add_values(s, o[c]);
+      sp_floatx16 s[1] = {f.scores(q[c])};
+      sp_softmax<1, ROWS>(a, s, there, half, m[c], l[c], o[c]);
+      f.add_values(s[0], o[c]);
     }
   }
   // The waves' results brought together: two halves of the waves, then one wave takes what the other left.
@@ -265,8 +437,8 @@ shared_prefix_kernel(SharedArgs a) {
     all_l[c] = 0.f;
     for (int w = 0; w < SP_WAVES; ++w) all_m[c] = fmaxf(all_m[c], m_s[w][32 * c + col]);
     for (int w = 0; w < SP_WAVES; ++w)
-      all_l[c] += all_m[c] == -INFINITY ? 0.f : l_s[w][32 * c + col] * __expf(m_s[w][32 * c + col] - all_m[c]);
-    const float mine = m[c] == -INFINITY ? 0.f : __expf(m[c] - all_m[c]);
+      all_l[c] += all_m[c] == -INFINITY ? 0.f : l_s[w][32 * c + col] * __builtin_amdgcn_exp2f(m_s[w][32 * c + col] - all_m[c]);
+    const float mine = m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[c] - all_m[c]);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
 #pragma unroll
@@ -323,16 +495,16 @@ shared_prefix_join(SharedArgs a, T* __restrict__ out) {
   const int parts = min(a.slots, scalar_int(a.shared_parts + row) + (own > 0 ? (own + a.own_keys - 1) / a.own_keys : 0));
   const float* ml = a.part_ml + (size_t)at * a.slots * 2;
   const float* part = a.part_o + (size_t)at * a.slots * D;
-  float m = a.sinks ? a.sinks[head] : -INFINITY;
+  float m = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;
   const float sink = m;
   for (int p = 0; p < parts; ++p) m = fmaxf(m, ml[2 * p]);
-  float below = a.sinks && m > -INFINITY ? __expf(sink - m) : 0.f;
+  float below = a.sinks && m > -INFINITY ? __builtin_amdgcn_exp2f(sink - m) : 0.f;
   constexpr int PER = (D + WAVE - 1) / WAVE;
   float o[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) o[j] = 0.f;
   for (int p = 0; p < parts; ++p) {
-    const float w = ml[2 * p] == -INFINITY ? 0.f : __expf(ml[2 * p] - m);
+    const float w = ml[2 * p] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * p] - m);
     below += w * ml[2 * p + 1];
 #pragma unroll
     for (int j = 0; j < PER; ++j)

@@ -1315,7 +1315,7 @@ class Ops:
         plain = value_dim == head_dim and chunk is None and slopes is None     # (but for the sinks)
         if batch is not None and getattr(batch, "sharing", None) and self.use_fast_attention:
             plan = batch.sharing_of(block_table, n_q, n_kv, head_dim)
-            if (plan is not None and plain and window is None and not tied_values and value_heads in (None, n_kv)
+            if (plan is not None and plain and window is None and not tied_values and value_heads in (None, n_kv) and scale > 0
                     and (qkv.shape[1] * qkv.element_size()) % 16 == 0):
                 return self.shared_prefix_attention(qkv, out, k_pages, v_pages, positions, block_table, plan, n_q, n_kv, head_dim, scale,
                                                     max_position, sinks, softcap)
@@ -1562,6 +1562,7 @@ class Ops:
         _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == n_rows, "block_table must be int32 [B, P]")
         _need(sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == n_q), "sinks are float32 [n_q]")
         _need(softcap is None or softcap > 0, "a cap on the scores is positive")
+        _need(scale > 0, "the scores' scale is positive")
         _here(qkv, out, k_pages, v_pages, positions, block_table, plan.items, sinks)
         width = block_table.shape[1]
         _need(plan.keys_end <= width * page_size, "block table is too narrow for the shared keys")

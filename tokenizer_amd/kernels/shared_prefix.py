@@ -64,10 +64,13 @@ class SharedPrefixes:
     """A batch's sharing laid out for the attention kernel: made once (`Ops.plan_shared_prefixes`) for requests that stay the same,
     used at every layer and step.  It belongs to rows in this order with these leading pages, and to one shape of attention."""
 
-    COLUMNS = 32                  # query columns (requests x query heads of a kv head) that a workgroup takes
+    COLUMNS = 32                  # query columns (requests x query heads of a kv head) of a narrow item, whose waves share out the keys
+    WIDE_COLUMNS = 128            # ... and of a wide one, whose waves have 32 each
+    WIDE_HEADS = (64, 128)        # head sizes of bfloat16 that have wide items
     MIN_KEYS = 64                 # a shorter run is not worth a pass and a part to be joined of its own
-    MIN_PART = 128                # keys of a workgroup's part of a run, at least (a block of 32 for each of its four waves)
-    TARGET = 1024                 # workgroups that the parts aim at
+    MIN_PART = 128                # keys of a narrow part of a run, at least (a block of 32 for each of its four waves)
+    MIN_WIDE_PART = 512
+    TARGET = 512                  # workgroups that the parts aim at: two a compute unit
 
     def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device,
                  fill: int = 0):
@@ -77,20 +80,29 @@ class SharedPrefixes:
         self.order, self.runs, own_begin = find_shared_runs(table, positions, page_size, self.MIN_KEYS)
         place = {row: at for at, row in enumerate(self.order)}
         group = n_q // n_kv
-        tiles = [-(-len(run.rows) * group // self.COLUMNS) for run in self.runs]
-        # Parts of so many keys that all runs together make about TARGET workgroups.
-        work = sum(t * (run.key_end - run.key_begin) for t, run in zip(tiles, self.runs)) * n_kv
-        part = max(self.MIN_PART, -(-work // self.TARGET))
+        # A run's columns in wide tiles, and what is left, if that is at most half of one, in narrow ones.
+        wide = dtype == torch.bfloat16 and head_dim in self.WIDE_HEADS
+        tiles = []                                        # per run: (first column, wide)
+        for run in self.runs:
+            columns, at, found = len(run.rows) * group, 0, []
+            while at < columns:
+                takes_wide = wide and columns - at > self.WIDE_COLUMNS // 2
+                found.append((at, int(takes_wide)))
+                at += self.WIDE_COLUMNS if takes_wide else self.COLUMNS
+            tiles.append(found)
+        # Parts of so many keys that all runs together make about TARGET workgroups (no more: they would wait for a second round).
+        work = sum(len(t) * (run.key_end - run.key_begin) for t, run in zip(tiles, self.runs)) * n_kv
         items, parts_of = [], np.zeros(self.n_rows, dtype=np.int32)
-        for count, run in zip(tiles, self.runs):
-            splits = max(1, -(-(run.key_end - run.key_begin) // part))
-            keys = -(-(run.key_end - run.key_begin) // (32 * splits)) * 32
+        for found, run in zip(tiles, self.runs):
+            length = run.key_end - run.key_begin
+            part = max(self.MIN_WIDE_PART if any(w for _, w in found) else self.MIN_PART, -(-work // self.TARGET))
+            keys = -(-length // (32 * max(1, length // part))) * 32
             first = int(parts_of[run.rows[0]])
             for split, begin in enumerate(range(run.key_begin, run.key_end, keys)):
-                for tile in range(count):
-                    items.append((place[run.rows[0]], len(run.rows) * group, tile * self.COLUMNS, begin,
-                                  min(run.key_end, begin + keys), first + split, 0, 0))
-            parts_of[run.rows] = first + -(-(run.key_end - run.key_begin) // keys)
+                for column, takes_wide in found:
+                    items.append((place[run.rows[0]], len(run.rows) * group, column, begin, min(run.key_end, begin + keys), first + split,
+                                  takes_wide, 0))
+            parts_of[run.rows] = first + -(-length // keys)
         items.sort(key=lambda item: item[3] - item[4])    # long ones first
         self.n_items = len(items)
         if fill:                                          # (up to a multiple, with items without columns: plans of one size)
