@@ -445,7 +445,7 @@ def test_attention_of_many_columns(ops, keys, page, rows, n_q, n_kv, d):
     tables, positions = shared_tables(rows, keys // page, page, [1 + (13 * r) % 40 for r in range(rows)])
     batch = Batch(tables, positions, n_q, n_kv, d, page, torch.bfloat16, rows + keys)
     got, plan = batch.run(ops)
-    assert any(plan.items.reshape(-1, 8)[:, 6].tolist())
+    assert plan.n_many > 0
     batch.check(got)
 
 

@@ -111,12 +111,13 @@ def test_the_work_list_covers_every_query_and_key_once(seed):
     plan = SharedPrefixes(_table(rows), positions, page, group * n_kv, n_kv, 64, torch.bfloat16, "cpu")
     items = plan.items.reshape(-1, 8).tolist()
     order, own, parts = plan.order_dev.tolist(), plan.own_begin_dev.tolist(), plan.parts_dev.tolist()
-    assert len(items) == plan.n_items and order == plan.order and own == plan.own_begin.tolist()
+    assert len(items) == plan.n_few + plan.n_many and order == plan.order and own == plan.own_begin.tolist()
     seen = {}                                               # (row, head in its group) -> {slot: (begin, end)}
-    for rows_at, columns, first, begin, end, slot, wide, _ in items:
+    for at, (rows_at, columns, first, begin, end, slot, _, _) in enumerate(items):
+        takes = plan.FEW_COLUMNS if at < plan.n_few else plan.WIDE_COLUMNS
         assert 0 <= first < columns and columns % group == 0 and rows_at + columns // group <= len(rows)
         assert begin < end <= plan.keys_end and begin % page == 0 and (begin - items[0][3]) % 16 == 0
-        for column in range(first, min(columns, first + (plan.WIDE_COLUMNS if wide else plan.COLUMNS))):
+        for column in range(first, min(columns, first + takes)):
             slots = seen.setdefault((order[rows_at + column // group], column % group), {})
             assert slot not in slots
             slots[slot] = (begin, end)

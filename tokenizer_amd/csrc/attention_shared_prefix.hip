@@ -6,11 +6,17 @@
 // So the keys that several requests share are gone through once, for the queries of all of them (a column of the products each, all
 // query heads of a kv head side by side), and each request's own keys behind them on their own; a second kernel joins a query's runs.
 //
-// Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T, on the 32x32 matrix instructions: a lane then holds one
-// column of scores and outputs alike (column lane % 32), and rescaling takes nothing from other lanes.  The rows of the
-// first product are taken in the order in which the second wants its keys, so the weights go from the one to the other in
-// registers: row r of a block of 32 keys is key 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4, and lane half h then holds
-// keys 16 s + 8 h .. + 7 of step s of the second product, which are sixteen contiguous bytes of a page of V^T.
+// Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T: a lane then holds one column of scores and outputs alike, and
+// rescaling takes nothing from other lanes.  The rows of the first product are taken in the order in which the second wants its
+// keys, so the weights go from the one to the other in registers, and what a lane contracts over is contiguous in a page of V^T.
+//
+// Three kernels share the work, by how many columns go through a run of keys:
+//   * few (a request's own keys; up to 64 columns): sixteen columns a workgroup, whose waves share the keys out;
+//   * more, in bfloat16 at head sizes 64 and 128: 128 columns a workgroup, 32 a wave, keys and values through LDS;
+//   * more, of other types and sizes: 32 columns a workgroup, whose waves share the keys out.
+// Fragments of the 32x32 instructions: row r of a block of 32 keys is key 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4, and lane
+// half h then holds keys 16 s + 8 h .. + 7 of step s of the second product.  Of the 16x16 ones: row r of the first product's
+// instruction t is key 8 (r / 4) + 4 t + r % 4, and lane group g then holds keys 8 g .. 8 g + 7.
 #include "common.h"
 
 typedef __bf16 sp_bf16x8 __attribute__((ext_vector_type(8)));
@@ -30,19 +36,30 @@ struct SharedItem {
   int first_column;                    // of this item
   int key_begin, key_end;              // positions; key_end - 1 is the last
   int slot;                            // which of a query's partial results this one is
-  int wide;                            // whether it takes SP_WIDE_COLUMNS columns, a block of 32 a wave (else 32, the keys shared out)
-  int unused;
+  int unused[2];
 };
 
 struct SharedArgs {
   const void *q, *k_pages, *vt_pages;
   float *part_o, *part_ml;             // [rows, n_q, slots, D], [rows, n_q, slots, 2]
-  const SharedItem* items;
+  const SharedItem* items;             // those of few columns first, then those of many
   const int *order, *own_begin, *shared_parts, *positions, *block_table;
   const float* sinks;
-  int q_stride, table_stride, n_items, n_rows, n_q, n_kv, page_size, n_pages, slots, own_splits, own_keys;
+  int q_stride, table_stride, n_narrow, n_many, n_rows, n_q, n_kv, page_size, n_pages, slots, own_splits, own_keys;
+  int page_shift;                      // page_size as a power of two, -1 if it is none
   float scale, softcap;
 };
+
+// Which page of a table holds a key, and where in it (for a whole wave; a division takes some twenty instructions of the scalar unit).
+__device__ __forceinline__ void sp_page_of(const SharedArgs& a, int key, int& index, int& slot) {
+  if (a.page_shift >= 0) {
+    index = key >> a.page_shift;
+    slot = key & (a.page_size - 1);
+  } else {
+    index = key / a.page_size;
+    slot = key - index * a.page_size;
+  }
+}
 
 // The fragments of one type: how a block of 32 keys, the queries and the weights lie in registers, and the products.
 template <typename T, int D> struct Frag;
@@ -160,6 +177,9 @@ struct Frag<float, D> {
 // A step of the softmax: `s` holds BLOCKS blocks of 32 scores a column (a lane half's sixteen each), of which the first `there` keys count;
 // they become weights.  m: the largest score so far, in units of 1 / log2(e) (a weight is then one instruction of the exponent's),
 // l: this lane's sum of weights, o: the weighed values, all brought to the new maximum where it has grown for any of the wave's columns.
+//   The maximum is a reference alone: a weight may be up to 2^SP_SLACK as long as no rescaling has been due (rescaling at every new maximum
+//   of any of 32 columns came up in nearly every block: 64 of 220 vector instructions of a block of 64 keys at head size 128).
+#define SP_SLACK 8.f
 template <int BLOCKS, int ROWS>
 __device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)[BLOCKS], int there, int half, float& m, float& l,
                                            sp_floatx16 (&o)[ROWS]) {
@@ -169,7 +189,7 @@ __device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[b][i] = a.softcap * (1.f - 2.f / (1.f + __builtin_amdgcn_exp2f(inner * s[b][i])));
+      for (int i = 0; i < 16; ++i) s[b][i] = a.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(inner * s[b][i])));
     scale = LOG2E;
   }
   if (there < BLOCKS * SP_BLOCK) {
@@ -185,8 +205,8 @@ __device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)
 #pragma unroll
     for (int i = 0; i < 16; ++i) high = fmaxf(high, s[b][i]);
   high = wave_max_across<32>(high) * scale;                // (the scale is positive)
-  if (__any(high > m)) {
-    const float m_new = fmaxf(m, high);
+  if (__any(high > m + SP_SLACK)) {
+    const float m_new = high > m + SP_SLACK ? high : m;       // (each column for itself: what stands beside it changes nothing)
     const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
     m = m_new;
     l *= corr;
@@ -243,9 +263,12 @@ struct Wide {
 };
 
 template <int D>
-__device__ __forceinline__ void sp_wide(const SharedArgs& a, int rows_at, int columns, int first_column, int begin, int end, int slot, char* even,
-                                        char* odd) {
+__device__ __forceinline__ void sp_wide(const SharedArgs& a, char* even, char* odd) {
   typedef Wide<D> W;
+  const int* item = reinterpret_cast<const int*>(a.items + a.n_narrow + blockIdx.x);
+  const int rows_at = scalar_int(item), columns = scalar_int(item + 1), first_column = scalar_int(item + 2);
+  const int begin = scalar_int(item + 3), end = scalar_int(item + 4), slot = scalar_int(item + 5);
+  if (columns <= 0) return;                                // an item that only fills the list up
   typedef Frag<bf16_t, D> F;
   constexpr int ROWS = W::ROWS;
   const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 31, half = lane >> 5;
@@ -257,24 +280,26 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, int rows_at, int co
   F::load_query(q, (const bf16_t*)a.q + (size_t)max(row, 0) * a.q_stride + (size_t)head * D, there, half);
   const int* table = a.block_table + (size_t)scalar_int(a.order + rows_at) * a.table_stride;
   const uint32_t key_place = W::key_place(threadIdx.x), value_place = W::value_place(threadIdx.x, a.page_size);
-  const size_t page_bytes = (size_t)a.page_size * D * 2;
+  // (A layer's keys are fewer than 2^31 elements: places in bytes fit 32 bits.)
+  const uint32_t page_bytes = (uint32_t)a.page_size * D * 2, all_heads = page_bytes * a.n_kv, of_head = page_bytes * kvh;
+  const typename W::from_t k_from = (typename W::from_t)a.k_pages, v_from = (typename W::from_t)a.vt_pages;
   // Where round j's unit of a block starts in the pages (the run's last unit stands in for one behind it, of which nothing counts).
   int page[W::ROUNDS], at[W::ROUNDS];
   auto look_up = [&](int kb) {
 #pragma unroll
     for (int j = 0; j < W::ROUNDS; ++j) {
-      const int key = min(kb + 16 * W::unit_of(j, wave), end - 16);
-      page[j] = min(max(scalar_int(table + key / a.page_size), 0), a.n_pages - 1);
-      at[j] = key % a.page_size;
+      int index;
+      sp_page_of(a, min(kb + 16 * W::unit_of(j, wave), end - 16), index, at[j]);
+      page[j] = scalar_int(table + index);
     }
   };
   auto fetch = [&](char* to) {
 #pragma unroll
     for (int j = 0; j < W::ROUNDS; ++j) {
-      const size_t start = ((size_t)page[j] * a.n_kv + kvh) * page_bytes;
-      __builtin_amdgcn_global_load_lds((typename W::from_t)((const char*)a.k_pages + start + (size_t)at[j] * W::KEY + key_place),
+      const uint32_t start = (uint32_t)min(max(page[j], 0), a.n_pages - 1) * all_heads + of_head;
+      __builtin_amdgcn_global_load_lds(k_from + (start + (uint32_t)at[j] * W::KEY + key_place),
                                        (typename W::lds_t)(to + j * 4096 + wave * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((typename W::from_t)((const char*)a.vt_pages + start + (size_t)at[j] * 2 + value_place),
+      __builtin_amdgcn_global_load_lds(v_from + (start + (uint32_t)at[j] * 2 + value_place),
                                        (typename W::lds_t)(to + W::TILE + j * 4096 + wave * 1024), 16, 0, 0);
     }
   };
@@ -335,49 +360,31 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, int rows_at, int co
           (sp_floatx4){o[r][4 * j], o[r][4 * j + 1], o[r][4 * j + 2], o[r][4 * j + 3]};
 }
 
+template <int D>
+__global__ void __launch_bounds__(SP_WAVES * WAVE)
+shared_prefix_wide(SharedArgs a) {
+  // (The two buffers are arrays of their own, each named where it is used: a read of one then waits for no load into the other.)
+  __shared__ __attribute__((aligned(1024))) char even[2 * Wide<D>::TILE];
+  __shared__ __attribute__((aligned(1024))) char odd[2 * Wide<D>::TILE];
+  sp_wide<D>(a, even, odd);
+}
+
 // ------------------------------------------------------------------------------------------------
-// One workgroup: some columns (COLS blocks of 32) of one kv head and a run of keys, which its waves share out block by block.  The
-// workgroups from `n_items` on take the requests' own keys.
+// One workgroup: some columns (COLS blocks of 32) of one kv head and a run of keys, which its waves share out block by block.
 template <typename T, int D, int COLS>
 __global__ void __launch_bounds__(SP_WAVES * WAVE)
 shared_prefix_kernel(SharedArgs a) {
   typedef Frag<T, D> F;
   constexpr int ROWS = F::ROWS;
-  constexpr bool WIDE = sizeof(T) == 2 && (D == 64 || D == 128);
-  constexpr int SUMS = SP_WAVES / 2 * COLS * ROWS * 32 * 33 * 4, TILES = WIDE ? 2 * SP_WIDE_BLOCK * D * 2 : 0;
-  // (The two buffers are arrays of their own, each named where it is used: a read of one then waits for no load into the other.)
-  __shared__ __attribute__((aligned(1024))) char even_s[SUMS > TILES ? SUMS : TILES];
-  __shared__ __attribute__((aligned(1024))) char odd_s[TILES ? TILES : 16];
-  float (*o_s)[COLS][ROWS * 32][33] = reinterpret_cast<float (*)[COLS][ROWS * 32][33]>(even_s);
+  __shared__ float o_s[SP_WAVES / 2][COLS][ROWS * 32][33];
   __shared__ float m_s[SP_WAVES][COLS * 32], l_s[SP_WAVES][COLS * 32];
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int col = lane & 31, half = lane >> 5;
   const int kvh = blockIdx.y, group = a.n_q / a.n_kv;
-  int rows_at, columns, first_column, begin, end, slot;
-  if ((int)blockIdx.x < a.n_items) {
-    const int* item = reinterpret_cast<const int*>(a.items + blockIdx.x);
-    rows_at = scalar_int(item); columns = scalar_int(item + 1); first_column = scalar_int(item + 2);
-    begin = scalar_int(item + 3); end = scalar_int(item + 4); slot = scalar_int(item + 5);
-    if (columns <= 0) return;                              // an item that only fills the list up
-    if constexpr (WIDE) {
-      if (scalar_int(item + 6)) {
-        sp_wide<D>(a, rows_at, columns, first_column, begin, end, slot, even_s, odd_s);
-        return;
-      }
-    }
-  } else {
-    const int tiles = (group + COLS * 32 - 1) / (COLS * 32);
-    const int at = blockIdx.x - a.n_items, split = at % a.own_splits, tile = at / a.own_splits % tiles;
-    rows_at = at / a.own_splits / tiles;
-    const int row = scalar_int(a.order + rows_at);
-    columns = group;
-    first_column = tile * COLS * 32;
-    begin = scalar_int(a.own_begin + row) + split * a.own_keys;
-    end = min(scalar_int(a.positions + row), a.table_stride * a.page_size - 1) + 1;
-    if (begin >= end) return;                              // a short request: its last parts are empty, and not asked for
-    end = min(end, begin + a.own_keys);
-    slot = scalar_int(a.shared_parts + row) + split;
-  }
+  const int* item = reinterpret_cast<const int*>(a.items + a.n_narrow + blockIdx.x);
+  const int rows_at = scalar_int(item), columns = scalar_int(item + 1), first_column = scalar_int(item + 2);
+  const int begin = scalar_int(item + 3), end = scalar_int(item + 4), slot = scalar_int(item + 5);
+  if (columns <= 0) return;                                // an item that only fills the list up
   // This lane's columns: request (row of the batch) and query head of each.
   int row_of[COLS], head_of[COLS];
   typename F::Query q[COLS];
@@ -407,10 +414,12 @@ shared_prefix_kernel(SharedArgs a) {
     // Runs of shared keys begin and end with pages, whose sizes are multiples of sixteen: a half of a block lies in one page.  The second
     // half may have no key: the first one's page stands in for it, and nothing that is read there counts.
     const int second = kb + 16 < end ? kb + 16 : kb;
-    const int page0 = min(max(scalar_int(table + kb / a.page_size), 0), a.n_pages - 1);
-    const int page1 = min(max(scalar_int(table + second / a.page_size), 0), a.n_pages - 1);
+    int index0, index1, slot0, slot1;
+    sp_page_of(a, kb, index0, slot0);
+    sp_page_of(a, second, index1, slot1);
+    const int page0 = min(max(scalar_int(table + index0), 0), a.n_pages - 1);
+    const int page1 = min(max(scalar_int(table + index1), 0), a.n_pages - 1);
     const size_t at0 = ((size_t)page0 * a.n_kv + kvh) * page_elems, at1 = ((size_t)page1 * a.n_kv + kvh) * page_elems;
-    const int slot0 = kb % a.page_size, slot1 = second % a.page_size;
     F f;
     f.load_keys(k_pages + (my_key < 16 ? at0 + (size_t)(slot0 + my_key) * D : at1 + (size_t)(slot1 + my_key - 16) * D), half);
     f.load_values(vt_pages + at0 + slot0, vt_pages + at1 + slot1, a.page_size, col, half);
@@ -483,6 +492,240 @@ shared_prefix_kernel(SharedArgs a) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Few columns: sixteen, the waves share out the keys.  The workgroups from `n_narrow` on take the requests' own keys.
+template <typename T, int D> struct Frag16;
+
+template <int D>
+struct Frag16<bf16_t, D> {
+  static constexpr int STEPS = (D + 31) / 32, ROWS = D / 16;
+  sp_bf16x8 k[2][STEPS];
+  sp_bf16x8 v[ROWS];
+  struct Query { sp_bf16x8 f[STEPS]; };
+  static __device__ __forceinline__ sp_bf16x8 none() {
+    sp_bf16x8 z;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = (__bf16)0.f;
+    return z;
+  }
+  static __device__ __forceinline__ void load_query(Query& q, const bf16_t* row, bool there, int g) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      q.f[s] = none();
+      if (there && (D % 32 == 0 || 32 * s + 8 * g < D)) q.f[s] = *reinterpret_cast<const sp_bf16x8*>(row + 32 * s + 8 * g);
+    }
+  }
+  __device__ __forceinline__ void load_keys(int t, const bf16_t* row, int g) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (D % 32) k[t][s] = none();
+      if (D % 32 == 0 || 32 * s + 8 * g < D) k[t][s] = *reinterpret_cast<const sp_bf16x8*>(row + 32 * s + 8 * g);
+    }
+  }
+  __device__ __forceinline__ void load_values(const bf16_t* from, int page_size, int col) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) v[r] = *reinterpret_cast<const sp_bf16x8*>(from + (16 * r + col) * page_size);
+  }
+  __device__ __forceinline__ void cut_values(int there) {  // as above; `there` counted from the lane's first key
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >= there) v[r][i] = (__bf16)0.f;
+  }
+  __device__ __forceinline__ sp_floatx4 scores(int t, const Query& q) const {
+    sp_floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[t][i], q.f[i], s, 0, 0, 0);
+    return s;
+  }
+  __device__ __forceinline__ void add_values(const float (&p)[8], sp_floatx4 (&o)[ROWS]) const {
+    sp_bf16x8 w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = (__bf16)p[i];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) o[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[r], w, o[r], 0, 0, 0);
+  }
+};
+
+// In 32 bits a step takes four coordinates or four keys, one a lane group: group g has coordinates 16 e + 4 g .. + 3 of every sixteen.
+template <int D>
+struct Frag16<float, D> {
+  static constexpr int STEPS = D / 16, ROWS = D / 16;
+  sp_floatx4 k[2][STEPS];
+  sp_floatx4 v[ROWS][2];
+  struct Query { sp_floatx4 f[STEPS]; };
+  static __device__ __forceinline__ void load_query(Query& q, const float* row, bool there, int g) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      q.f[s] = (sp_floatx4){0.f, 0.f, 0.f, 0.f};
+      if (there) q.f[s] = *reinterpret_cast<const sp_floatx4*>(row + 16 * s + 4 * g);
+    }
+  }
+  __device__ __forceinline__ void load_keys(int t, const float* row, int g) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) k[t][s] = *reinterpret_cast<const sp_floatx4*>(row + 16 * s + 4 * g);
+  }
+  __device__ __forceinline__ void load_values(const float* from, int page_size, int col) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[r][i] = *reinterpret_cast<const sp_floatx4*>(from + (16 * r + col) * page_size + 4 * i);
+  }
+  __device__ __forceinline__ void cut_values(int there) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >= there) v[r][i >> 2][i & 3] = 0.f;
+  }
+  __device__ __forceinline__ sp_floatx4 scores(int t, const Query& q) const {
+    sp_floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < STEPS; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][e][i], q.f[e][i], s, 0, 0, 0);
+    return s;
+  }
+  __device__ __forceinline__ void add_values(const float (&p)[8], sp_floatx4 (&o)[ROWS]) const {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i >> 2][i & 3], p[i], o[r], 0, 0, 0);
+  }
+};
+
+#define SP_FEW_COLUMNS 16
+
+template <typename T, int D>
+__global__ void __launch_bounds__(SP_WAVES * WAVE)
+shared_prefix_few(SharedArgs a) {
+  typedef Frag16<T, D> F;
+  constexpr int ROWS = F::ROWS;
+  __shared__ float o_s[SP_WAVES][SP_FEW_COLUMNS][D + 4];
+  __shared__ float m_s[SP_WAVES][SP_FEW_COLUMNS], l_s[SP_WAVES][SP_FEW_COLUMNS];
+  __shared__ int row_s[SP_FEW_COLUMNS], head_s[SP_FEW_COLUMNS];
+  const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.y, group = a.n_q / a.n_kv;
+  int rows_at, columns, first_column, begin, end, slot;
+  if ((int)blockIdx.x < a.n_narrow) {
+    const int* item = reinterpret_cast<const int*>(a.items + blockIdx.x);
+    rows_at = scalar_int(item); columns = scalar_int(item + 1); first_column = scalar_int(item + 2);
+    begin = scalar_int(item + 3); end = scalar_int(item + 4); slot = scalar_int(item + 5);
+    if (columns <= 0) return;                              // an item that only fills the list up
+  } else {
+    const int tiles = (group + SP_FEW_COLUMNS - 1) / SP_FEW_COLUMNS;
+    const int at = blockIdx.x - a.n_narrow, split = at % a.own_splits, tile = at / a.own_splits % tiles;
+    rows_at = at / a.own_splits / tiles;
+    const int row = scalar_int(a.order + rows_at);
+    columns = group;
+    first_column = tile * SP_FEW_COLUMNS;
+    begin = scalar_int(a.own_begin + row) + split * a.own_keys;
+    end = min(scalar_int(a.positions + row), a.table_stride * a.page_size - 1) + 1;
+    if (begin >= end) return;                              // a short request: its last parts are empty, and not asked for
+    end = min(end, begin + a.own_keys);
+    slot = scalar_int(a.shared_parts + row) + split;
+  }
+  const int column = first_column + col;
+  const bool there = column < columns;
+  const int row = there ? a.order[rows_at + column / group] : -1, head = kvh * group + column % group;
+  const int* table = a.block_table + (size_t)scalar_int(a.order + rows_at) * a.table_stride;
+  typename F::Query q;
+  F::load_query(q, (const T*)a.q + (size_t)max(row, 0) * a.q_stride + (size_t)head * D, there, g);
+  sp_floatx4 o[ROWS];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) o[r] = (sp_floatx4){0.f, 0.f, 0.f, 0.f};
+  const uint32_t page_elems = (uint32_t)a.page_size * D;
+  const T *k_pages = (const T*)a.k_pages, *vt_pages = (const T*)a.vt_pages;
+  float scale = a.scale * LOG2E;
+  if (a.softcap > 0.f) scale = LOG2E;
+  const float inner = a.softcap > 0.f ? 2.f * LOG2E * a.scale / a.softcap : 0.f;
+  for (int kb = begin + SP_BLOCK * wave; kb < end; kb += SP_BLOCK * SP_WAVES) {
+    // (Halves of a block as above.)
+    const int second = kb + 16 < end ? kb + 16 : kb;
+    int index0, index1, slot0, slot1;
+    sp_page_of(a, kb, index0, slot0);
+    sp_page_of(a, second, index1, slot1);
+    const uint32_t page0 = min(max(scalar_int(table + index0), 0), a.n_pages - 1), page1 = min(max(scalar_int(table + index1), 0), a.n_pages - 1);
+    F f;
+    {
+      const uint32_t at = ((col >> 3 ? page1 : page0) * a.n_kv + kvh) * page_elems + ((col >> 3 ? slot1 : slot0) + 8 * ((col >> 2) & 1) + (col & 3)) * D;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) f.load_keys(t, k_pages + at + 4 * t * D, g);
+    }
+    f.load_values(vt_pages + ((g >> 1 ? page1 : page0) * a.n_kv + kvh) * page_elems + (g >> 1 ? slot1 : slot0) + 8 * (g & 1), a.page_size, col);
+    const int here = end - kb;                             // keys of the block that count
+    if (here < SP_BLOCK) f.cut_values(here - 8 * g);
+    float s[8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const sp_floatx4 st = f.scores(t, q);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[4 * t + r] = st[r];
+    }
+    if (a.softcap > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = a.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(inner * s[i])));
+    }
+    if (here < SP_BLOCK) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (8 * g + i >= here) s[i] = -INFINITY;
+    }
+    float high = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) high = fmaxf(high, s[i]);
+    high = wave_max_across<32>(wave_max_across<16>(high)) * scale;
+    if (__any(high > m + SP_SLACK)) {
+      const float m_new = high > m + SP_SLACK ? high : m;
+      const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= corr;
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) o[r] *= corr;
+    }
+    const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], scale, -from));
+      l += s[i];
+    }
+    f.add_values(s, o);
+  }
+  // The waves' sums brought together through LDS, column by column.
+  l = wave_add_across<32>(wave_add_across<16>(l));
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) *reinterpret_cast<sp_floatx4*>(&o_s[wave][col][16 * r + 4 * g]) = o[r];
+  if (g == 0) { m_s[wave][col] = m; l_s[wave][col] = l; }
+  if (wave == 0 && g == 0) { row_s[col] = row; head_s[col] = head; }
+  __syncthreads();
+  const int heads_here = min(SP_FEW_COLUMNS, columns - first_column);
+  for (int c = wave; c < heads_here; c += SP_WAVES) {
+    float top = m_s[0][c];
+#pragma unroll
+    for (int w = 1; w < SP_WAVES; ++w) top = fmaxf(top, m_s[w][c]);
+    float factor[SP_WAVES], below = 0.f;
+#pragma unroll
+    for (int w = 0; w < SP_WAVES; ++w) {
+      factor[w] = m_s[w][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_s[w][c] - top);
+      below += l_s[w][c] * factor[w];
+    }
+    const size_t to = ((size_t)row_s[c] * a.n_q + head_s[c]) * a.slots + slot;
+    if (lane == 0) { a.part_ml[2 * to] = top; a.part_ml[2 * to + 1] = below; }
+#pragma unroll
+    for (int j = 0; j < (D + WAVE - 1) / WAVE; ++j) {
+      const int d = lane + j * WAVE;
+      if (d < D) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < SP_WAVES; ++w) sum += o_s[w][c][d] * factor[w];
+        a.part_o[to * D + d] = sum;
+      }
+    }
+  }
+}
+
 // A wave joins the runs of one query: `parts` of shared keys, then its own.
 template <typename T, int D>
 __global__ void __launch_bounds__(SP_WAVES * WAVE)
@@ -517,12 +760,22 @@ shared_prefix_join(SharedArgs a, T* __restrict__ out) {
     if (lane + j * WAVE < D) st(out + (size_t)at * D + lane + j * WAVE, o[j] * share);
 }
 
+// Whether many columns of this type and head size go through LDS, 128 a workgroup (else 32 a workgroup).
 template <typename T, int D>
-static int launch_shared(const SharedArgs& a, void* out, int columns, hipStream_t stream) {
-  const int group = a.n_q / a.n_kv, tiles = (group + columns - 1) / columns;
-  const dim3 grid((unsigned)a.n_items + (unsigned)a.n_rows * tiles * a.own_splits, a.n_kv);
-  if (columns == 32) shared_prefix_kernel<T, D, 1><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
-  else return -2;
+constexpr bool sp_is_wide() { return sizeof(T) == 2 && (D == 64 || D == 128); }
+
+template <typename T, int D>
+static int launch_shared(const SharedArgs& a, void* out, hipStream_t stream) {
+  const int group = a.n_q / a.n_kv, tiles = (group + SP_FEW_COLUMNS - 1) / SP_FEW_COLUMNS;
+  if (a.n_many > 0) {
+    const dim3 grid(a.n_many, a.n_kv);
+    if constexpr (sp_is_wide<T, D>()) shared_prefix_wide<D><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
+    else shared_prefix_kernel<T, D, 1><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
+    const int status = LAUNCH_STATUS();
+    if (status) return status;
+  }
+  const dim3 grid((unsigned)a.n_narrow + (unsigned)a.n_rows * tiles * a.own_splits, a.n_kv);
+  shared_prefix_few<T, D><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
   const int status = LAUNCH_STATUS();
   if (status) return status;
   const int queries = a.n_rows * a.n_q;
@@ -531,30 +784,31 @@ static int launch_shared(const SharedArgs& a, void* out, int columns, hipStream_
 }
 
 // q: the query heads of every row at its start, rows q_stride elements apart; pages as in the other attention kernels; items int32
-// [n_items, 8] (`SharedItem`); order int32 [n_rows]: the rows, those of a run of shared keys side by side; own_begin,
+// [n_narrow + n_many, 8] (`SharedItem`; sixteen columns each, then 128 or 32); order int32 [n_rows]: the rows, those of a run of shared keys side by side; own_begin,
 // shared_parts int32 [n_rows]: where a request's own keys begin, and how many partial results its shared keys leave; positions
 // int32 [n_rows]; block_table int32 [n_rows, table_stride].  part_o float [n_rows, n_q, slots, head_dim], part_ml float
 // [n_rows, n_q, slots, 2].  -2: a head size without an instance.
 extern "C" int ta_shared_prefix_attention(const void* q, int q_stride, void* out, const void* k_pages, const void* vt_pages,
-                                          const void* items, int n_items, const void* order, const void* own_begin,
+                                          const void* items, int n_narrow, int n_many, const void* order, const void* own_begin,
                                           const void* shared_parts, const void* positions, const void* block_table,
                                           int table_stride, const void* sinks, void* part_o, void* part_ml, int slots,
-                                          int own_splits, int own_keys, int columns, int n_rows, int n_q, int n_kv, int head_dim,
+                                          int own_splits, int own_keys, int n_rows, int n_q, int n_kv, int head_dim,
                                           int page_size, int n_pages, float scale, float softcap, int dtype, hipStream_t stream) {
   if (n_rows <= 0) return 0;
   if (!q || !out || !k_pages || !vt_pages || !order || !own_begin || !shared_parts || !positions || !block_table || !part_o || !part_ml)
     return -1;
-  if (n_items < 0 || (n_items && !items) || n_kv < 1 || n_kv > 65535 || n_q < n_kv || n_q % n_kv || page_size < 16 || page_size % 16 || n_pages < 1 ||
+  if (n_narrow < 0 || n_many < 0 || (n_narrow + n_many && !items) || n_kv < 1 || n_kv > 65535 || n_q < n_kv || n_q % n_kv || page_size < 16 || page_size % 16 || n_pages < 1 ||
       slots < 1 || own_splits < 1 || own_keys < SP_BLOCK || own_keys % SP_BLOCK || table_stride < 1) return -1;
   SharedArgs a = {};
   a.q = q; a.k_pages = k_pages; a.vt_pages = vt_pages; a.part_o = (float*)part_o; a.part_ml = (float*)part_ml;
   a.items = (const SharedItem*)items; a.order = (const int*)order; a.own_begin = (const int*)own_begin;
   a.shared_parts = (const int*)shared_parts; a.positions = (const int*)positions; a.block_table = (const int*)block_table;
-  a.sinks = (const float*)sinks; a.q_stride = q_stride; a.table_stride = table_stride; a.n_items = n_items; a.n_rows = n_rows;
+  a.sinks = (const float*)sinks; a.q_stride = q_stride; a.table_stride = table_stride; a.n_narrow = n_narrow; a.n_many = n_many; a.n_rows = n_rows;
   a.n_q = n_q; a.n_kv = n_kv; a.page_size = page_size; a.n_pages = n_pages; a.slots = slots; a.own_splits = own_splits;
+  a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size);
   a.own_keys = own_keys; a.scale = scale; a.softcap = softcap;
 #define SHARED_CASE(D) \
-  case D: return dtype == DT_F32 ? launch_shared<float, D>(a, out, columns, stream) : launch_shared<bf16_t, D>(a, out, columns, stream);
+  case D: return dtype == DT_F32 ? launch_shared<float, D>(a, out, stream) : launch_shared<bf16_t, D>(a, out, stream);
   switch (head_dim) {
     SHARED_CASE(16) SHARED_CASE(32) SHARED_CASE(48) SHARED_CASE(64) SHARED_CASE(80) SHARED_CASE(96) SHARED_CASE(112)
     SHARED_CASE(128) SHARED_CASE(160) SHARED_CASE(192) SHARED_CASE(224) SHARED_CASE(256)

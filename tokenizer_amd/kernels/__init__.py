@@ -1573,7 +1573,7 @@ class Ops:
             return out
         # The requests' own keys, in parts that fill the device (as for single tokens that share nothing).
         longest = max(1, -(-(max_position + 1) // self.PLAN_KEYS) * self.PLAN_KEYS - plan.smallest_own)
-        head_blocks = -(-(n_q // n_kv) // plan.COLUMNS)
+        head_blocks = -(-(n_q // n_kv) // plan.FEW_COLUMNS)
         wanted = max(1, self.target_workgroups // (n_rows * n_kv * head_blocks))
         own_keys = max(self.min_split_keys, -(-longest // wanted))
         own_keys = -(-own_keys // 32) * 32
@@ -1582,9 +1582,9 @@ class Ops:
         part_o = torch.empty((n_rows, n_q, slots, head_dim), dtype=torch.float32, device=qkv.device)
         part_ml = torch.empty((n_rows, n_q, slots, 2), dtype=torch.float32, device=qkv.device)
         self._check(self.lib.ta_shared_prefix_attention(
-            _ptr(qkv), qkv.shape[1], _ptr(out), _ptr(k_pages), _ptr(v_pages), _ptr(plan.items if plan.n_items else None), plan.n_items,
+            _ptr(qkv), qkv.shape[1], _ptr(out), _ptr(k_pages), _ptr(v_pages), _ptr(plan.items if plan.n_few + plan.n_many else None), plan.n_few, plan.n_many,
             _ptr(plan.order_dev), _ptr(plan.own_begin_dev), _ptr(plan.parts_dev), _ptr(positions), _ptr(block_table), width, _ptr(sinks),
-            _ptr(part_o), _ptr(part_ml), slots, own_splits, own_keys, plan.COLUMNS, n_rows, n_q, n_kv, head_dim, page_size,
+            _ptr(part_o), _ptr(part_ml), slots, own_splits, own_keys, n_rows, n_q, n_kv, head_dim, page_size,
             k_pages.shape[0], ctypes.c_float(scale), ctypes.c_float(softcap or 0.0), _code(qkv.dtype), self._stream()),
             "shared_prefix_attention")
         return out

@@ -64,11 +64,12 @@ class SharedPrefixes:
     """A batch's sharing laid out for the attention kernel: made once (`Ops.plan_shared_prefixes`) for requests that stay the same,
     used at every layer and step.  It belongs to rows in this order with these leading pages, and to one shape of attention."""
 
-    COLUMNS = 32                  # query columns (requests x query heads of a kv head) of a narrow item, whose waves share out the keys
-    WIDE_COLUMNS = 128            # ... and of a wide one, whose waves have 32 each
-    WIDE_HEADS = (64, 128)        # head sizes of bfloat16 that have wide items
+    FEW_COLUMNS = 16              # query columns (requests x query heads of a kv head) of an item of few; its waves share out the keys
+    MANY_COLUMNS = 32             # ... of one of many, likewise
+    WIDE_COLUMNS = 128            # ... of one of many in bfloat16 at head sizes WIDE_HEADS: its waves have 32 each
+    WIDE_HEADS = (64, 128)
     MIN_KEYS = 64                 # a shorter run is not worth a pass and a part to be joined of its own
-    MIN_PART = 128                # keys of a narrow part of a run, at least (a block of 32 for each of its four waves)
+    MIN_PART = 128                # keys of a part of a run, at least (a block of 32 for each of its four waves)
     MIN_WIDE_PART = 512
     TARGET = 512                  # workgroups that the parts aim at: two a compute unit
 
@@ -80,51 +81,52 @@ class SharedPrefixes:
         self.order, self.runs, own_begin = find_shared_runs(table, positions, page_size, self.MIN_KEYS)
         place = {row: at for at, row in enumerate(self.order)}
         group = n_q // n_kv
-        # A run's columns in wide tiles, and what is left, if that is at most half of one, in narrow ones.
+        # A run's columns in tiles of many, and what is left, if that is little, in tiles of few.
         wide = dtype == torch.bfloat16 and head_dim in self.WIDE_HEADS
-        tiles = []                                        # per run: (first column, wide)
+        size, little = (self.WIDE_COLUMNS, self.WIDE_COLUMNS // 2) if wide else (self.MANY_COLUMNS, self.FEW_COLUMNS)
+        tiles = []                                        # per run: (first column, whether it is one of many)
         for run in self.runs:
             columns, at, found = len(run.rows) * group, 0, []
             while at < columns:
-                takes_wide = wide and columns - at > self.WIDE_COLUMNS // 2
-                found.append((at, int(takes_wide)))
-                at += self.WIDE_COLUMNS if takes_wide else self.COLUMNS
+                many = columns - at > little
+                found.append((at, many))
+                at += size if many else self.FEW_COLUMNS
             tiles.append(found)
         # Parts of so many keys that all runs together make about TARGET workgroups (no more: they would wait for a second round).
         work = sum(len(t) * (run.key_end - run.key_begin) for t, run in zip(tiles, self.runs)) * n_kv
-        items, parts_of = [], np.zeros(self.n_rows, dtype=np.int32)
+        items, parts_of = {False: [], True: []}, np.zeros(self.n_rows, dtype=np.int32)
         for found, run in zip(tiles, self.runs):
             length = run.key_end - run.key_begin
-            part = max(self.MIN_WIDE_PART if any(w for _, w in found) else self.MIN_PART, -(-work // self.TARGET))
+            part = max(self.MIN_WIDE_PART if wide and found[0][1] else self.MIN_PART, -(-work // self.TARGET))
             keys = -(-length // (32 * max(1, length // part))) * 32
             first = int(parts_of[run.rows[0]])
             for split, begin in enumerate(range(run.key_begin, run.key_end, keys)):
-                for column, takes_wide in found:
-                    items.append((place[run.rows[0]], len(run.rows) * group, column, begin, min(run.key_end, begin + keys), first + split,
-                                  takes_wide, 0))
+                for column, many in found:
+                    items[many].append((place[run.rows[0]], len(run.rows) * group, column, begin, min(run.key_end, begin + keys),
+                                        first + split, 0, 0))
             parts_of[run.rows] = first + -(-length // keys)
-        items.sort(key=lambda item: item[3] - item[4])    # long ones first
-        self.n_items = len(items)
-        if fill:                                          # (up to a multiple, with items without columns: plans of one size)
-            items += [(0,) * 8] * (-len(items) % fill)
-            self.n_items = len(items)
+        for some in items.values():
+            some.sort(key=lambda item: item[3] - item[4])     # long ones first
+            if fill:                                      # (up to a multiple, with items without columns: plans of one size)
+                some += [(0,) * 8] * (-len(some) % fill)
+        self.n_few, self.n_many = len(items[False]), len(items[True])
         self.shared_parts = int(parts_of.max(initial=0))
         self.own_begin = own_begin                        # int32 [B] on the host
         self.keys_end = max((run.key_end for run in self.runs), default=0)
         self.smallest_own = int(own_begin.min(initial=0)) if self.n_rows else 0
-        packed = np.concatenate([np.asarray(items, dtype=np.int32).reshape(-1), np.asarray(self.order, dtype=np.int32), own_begin,
+        packed = np.concatenate([np.asarray(items[False] + items[True], dtype=np.int32).reshape(-1), np.asarray(self.order, dtype=np.int32), own_begin,
                                  parts_of]).astype(np.int32)
         self._on_device(torch.from_numpy(packed).to(device))
 
     def _on_device(self, packed: torch.Tensor) -> None:
         self.packed = packed
-        sizes = [8 * self.n_items] + [self.n_rows] * 3
+        sizes = [8 * (self.n_few + self.n_many)] + [self.n_rows] * 3
         self.items, self.order_dev, self.own_begin_dev, self.parts_dev = torch.split(packed, sizes)
 
     @property
     def signature(self) -> tuple:
         """What a launch depends on beside the tables: plans of one signature may take each other's place in a captured graph."""
-        return (self.n_rows, self.n_items, self.shared_parts, self.smallest_own, self.n_q, self.n_kv, self.head_dim, self.page_size,
+        return (self.n_rows, self.n_few, self.n_many, self.shared_parts, self.smallest_own, self.n_q, self.n_kv, self.head_dim, self.page_size,
                 self.dtype)
 
     def standing_copy(self) -> "SharedPrefixes":
