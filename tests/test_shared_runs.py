@@ -1,6 +1,7 @@
 """Which leading pages the requests of a batch share, against a look at every pair of rows; no GPU."""
 from __future__ import annotations
 
+import itertools
 import random
 
 import numpy as np
@@ -110,20 +111,25 @@ def test_the_work_list_covers_every_query_and_key_once(seed):
     positions = [len(t) * page - 1 - rng.randint(0, page - 1) for t in rows]
     plan = SharedPrefixes(_table(rows), positions, page, group * n_kv, n_kv, 64, torch.bfloat16, "cpu")
     items = plan.items.reshape(-1, 8).tolist()
-    order, own, parts = plan.order_dev.tolist(), plan.own_begin_dev.tolist(), plan.parts_dev.tolist()
+    order, by_row = plan.order_dev.tolist(), plan.own_of_row_dev.reshape(-1, 4).tolist()
+    own, parts = [r[1] for r in by_row], [r[2] for r in by_row]
+    assert [r[0] for r in by_row] == list(range(len(rows))) and plan.own_dev.reshape(-1, 4).tolist() == [by_row[r] for r in order]
     assert len(items) == plan.n_few + plan.n_many and order == plan.order and own == plan.own_begin.tolist()
-    seen = {}                                               # (row, head in its group) -> {slot: (begin, end)}
-    for at, (rows_at, columns, first, begin, end, slot, _, _) in enumerate(items):
+    seen = {}                                               # (row, kv head, head in its group) -> {slot: (begin, end)}
+    for at, (rows_at, columns, first, begin, end, slot, table_row, kv_head) in enumerate(items):
+        if columns == 0:                                    # an item that only fills the list up
+            continue
+        assert table_row == order[rows_at]
         takes = plan.FEW_COLUMNS if at < plan.n_few else plan.WIDE_COLUMNS
         assert 0 <= first < columns and columns % group == 0 and rows_at + columns // group <= len(rows)
-        assert begin < end <= plan.keys_end and begin % page == 0 and (begin - items[0][3]) % 16 == 0
+        assert begin < end <= plan.keys_end and begin % page == 0 and 0 <= kv_head < n_kv
         for column in range(first, min(columns, first + takes)):
-            slots = seen.setdefault((order[rows_at + column // group], column % group), {})
+            slots = seen.setdefault((order[rows_at + column // group], kv_head, column % group), {})
             assert slot not in slots
             slots[slot] = (begin, end)
-    for row in range(len(rows)):
-        for head in range(group):
-            slots = seen.get((row, head), {})
+    for row, head in itertools.product(range(len(rows)), range(group)):
+        for kv_head in range(n_kv):
+            slots = seen.get((row, kv_head, head), {})
             assert sorted(slots) == list(range(parts[row])) and parts[row] <= plan.shared_parts
             ranges = [slots[s] for s in sorted(slots)]
             assert [b for b, _ in ranges] + [own[row]] == [0] + [e for _, e in ranges] if ranges else own[row] == 0

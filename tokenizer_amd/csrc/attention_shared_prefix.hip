@@ -36,14 +36,18 @@ struct SharedItem {
   int first_column;                    // of this item
   int key_begin, key_end;              // positions; key_end - 1 is the last
   int slot;                            // which of a query's partial results this one is
-  int unused[2];
+  int table_row;                       // a request whose block table names the run's pages
+  int kv_head;
 };
+struct SharedOwn { int row, begin, slot, unused; };   // a request's own keys: where they begin, its first partial result of them
 
 struct SharedArgs {
   const void *q, *k_pages, *vt_pages;
   float *part_o, *part_ml;             // [rows, n_q, slots, D], [rows, n_q, slots, 2]
   const SharedItem* items;             // those of few columns first, then those of many
-  const int *order, *own_begin, *shared_parts, *positions, *block_table;
+  const int* order;                    // the requests, those of a run side by side
+  const SharedOwn *own, *own_of_row;   // in that order, and by request
+  const int *positions, *block_table;
   const float* sinks;
   int q_stride, table_stride, n_narrow, n_many, n_rows, n_q, n_kv, page_size, n_pages, slots, own_splits, own_keys;
   int page_shift;                      // page_size as a power of two, -1 if it is none
@@ -272,13 +276,13 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* even, char* o
   typedef Frag<bf16_t, D> F;
   constexpr int ROWS = W::ROWS;
   const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 31, half = lane >> 5;
-  const int kvh = blockIdx.y, group = a.n_q / a.n_kv;
+  const int kvh = scalar_int(item + 7), group = a.n_q / a.n_kv;
   const int column = first_column + 32 * wave + col;
   const bool there = column < columns, wave_there = first_column + 32 * wave < columns;
   const int row = there ? a.order[rows_at + column / group] : -1, head = kvh * group + column % group;
   typename F::Query q;
   F::load_query(q, (const bf16_t*)a.q + (size_t)max(row, 0) * a.q_stride + (size_t)head * D, there, half);
-  const int* table = a.block_table + (size_t)scalar_int(a.order + rows_at) * a.table_stride;
+  const int* table = a.block_table + (size_t)scalar_int(item + 6) * a.table_stride;
   const uint32_t key_place = W::key_place(threadIdx.x), value_place = W::value_place(threadIdx.x, a.page_size);
   // (A layer's keys are fewer than 2^31 elements: places in bytes fit 32 bits.)
   const uint32_t page_bytes = (uint32_t)a.page_size * D * 2, all_heads = page_bytes * a.n_kv, of_head = page_bytes * kvh;
@@ -380,10 +384,11 @@ shared_prefix_kernel(SharedArgs a) {
   __shared__ float m_s[SP_WAVES][COLS * 32], l_s[SP_WAVES][COLS * 32];
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int col = lane & 31, half = lane >> 5;
-  const int kvh = blockIdx.y, group = a.n_q / a.n_kv;
+  const int group = a.n_q / a.n_kv;
   const int* item = reinterpret_cast<const int*>(a.items + a.n_narrow + blockIdx.x);
   const int rows_at = scalar_int(item), columns = scalar_int(item + 1), first_column = scalar_int(item + 2);
   const int begin = scalar_int(item + 3), end = scalar_int(item + 4), slot = scalar_int(item + 5);
+  const int kvh = scalar_int(item + 7);
   if (columns <= 0) return;                                // an item that only fills the list up
   // This lane's columns: request (row of the batch) and query head of each.
   int row_of[COLS], head_of[COLS];
@@ -396,7 +401,7 @@ shared_prefix_kernel(SharedArgs a) {
     head_of[c] = kvh * group + column % group;
     F::load_query(q[c], (const T*)a.q + (size_t)max(row_of[c], 0) * a.q_stride + (size_t)head_of[c] * D, there, half);
   }
-  const int* table = a.block_table + (size_t)scalar_int(a.order + rows_at) * a.table_stride;
+  const int* table = a.block_table + (size_t)scalar_int(item + 6) * a.table_stride;
   sp_floatx16 o[COLS][ROWS];
   float m[COLS], l[COLS];
 #pragma unroll
@@ -606,55 +611,80 @@ shared_prefix_few(SharedArgs a) {
   __shared__ float m_s[SP_WAVES][SP_FEW_COLUMNS], l_s[SP_WAVES][SP_FEW_COLUMNS];
   __shared__ int row_s[SP_FEW_COLUMNS], head_s[SP_FEW_COLUMNS];
   const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, group = a.n_q / a.n_kv;
-  int rows_at, columns, first_column, begin, end, slot;
-  if ((int)blockIdx.x < a.n_narrow) {
+  const int group = a.n_q / a.n_kv;
+  int columns, first_column, begin, end, slot, table_row, kvh, row = -1;
+  const bool own = (int)blockIdx.x >= a.n_narrow;
+  const int* table;
+  // Which pages the two halves of the wave's next block of keys lie in, asked for a block ahead.  The second half may have no key: the first
+  // one's page stands in for it, and nothing that is read there counts.  (The first block of a request's own keys is looked up beside its
+  // position: an entry of the table past its pages may hold anything, and is not used.)
+  struct Pages { int page0, page1, slot0, slot1; };
+  auto look_up = [&](int kb, int last) {
+    Pages p;
+    int index0, index1;
+    sp_page_of(a, kb, index0, p.slot0);
+    sp_page_of(a, kb + 16 <= last ? kb + 16 : kb, index1, p.slot1);
+    p.page0 = scalar_int(table + min(index0, a.table_stride - 1));
+    p.page1 = scalar_int(table + min(index1, a.table_stride - 1));
+    return p;
+  };
+  Pages next;
+  if (!own) {
     const int* item = reinterpret_cast<const int*>(a.items + blockIdx.x);
-    rows_at = scalar_int(item); columns = scalar_int(item + 1); first_column = scalar_int(item + 2);
+    const int rows_at = scalar_int(item);
+    columns = scalar_int(item + 1); first_column = scalar_int(item + 2);
     begin = scalar_int(item + 3); end = scalar_int(item + 4); slot = scalar_int(item + 5);
+    table_row = scalar_int(item + 6); kvh = scalar_int(item + 7);
     if (columns <= 0) return;                              // an item that only fills the list up
+    table = a.block_table + (size_t)table_row * a.table_stride;
+    next = look_up(begin + SP_BLOCK * wave, end - 1);
+    if (first_column + col < columns) row = a.order[rows_at + (first_column + col) / group];
   } else {
     const int tiles = (group + SP_FEW_COLUMNS - 1) / SP_FEW_COLUMNS;
-    const int at = blockIdx.x - a.n_narrow, split = at % a.own_splits, tile = at / a.own_splits % tiles;
-    rows_at = at / a.own_splits / tiles;
-    const int row = scalar_int(a.order + rows_at);
+    // (First parts of all requests first: the last ones are empty for the short ones.)
+    int at = blockIdx.x - a.n_narrow;
+    kvh = at % a.n_kv;
+    at /= a.n_kv;
+    const int tile = at % tiles;
+    at /= tiles;
+    const int split = at / a.n_rows;
+    const int* mine = reinterpret_cast<const int*>(a.own + (at - split * a.n_rows));
+    table_row = scalar_int(mine);
+    begin = scalar_int(mine + 1) + split * a.own_keys;
+    slot = scalar_int(mine + 2) + split;
     columns = group;
     first_column = tile * SP_FEW_COLUMNS;
-    begin = scalar_int(a.own_begin + row) + split * a.own_keys;
-    end = min(scalar_int(a.positions + row), a.table_stride * a.page_size - 1) + 1;
+    table = a.block_table + (size_t)table_row * a.table_stride;
+    end = min(scalar_int(a.positions + table_row), a.table_stride * a.page_size - 1) + 1;
+    next = look_up(begin + SP_BLOCK * wave, begin + SP_BLOCK * wave + 16);
     if (begin >= end) return;                              // a short request: its last parts are empty, and not asked for
     end = min(end, begin + a.own_keys);
-    slot = scalar_int(a.shared_parts + row) + split;
+    if (begin + SP_BLOCK * wave + 16 >= end) { next.page1 = next.page0; next.slot1 = next.slot0; }
+    if (first_column + col < columns) row = table_row;
   }
-  const int column = first_column + col;
-  const bool there = column < columns;
-  const int row = there ? a.order[rows_at + column / group] : -1, head = kvh * group + column % group;
-  const int* table = a.block_table + (size_t)scalar_int(a.order + rows_at) * a.table_stride;
+  const int column = first_column + col, head = kvh * group + column % group;
   typename F::Query q;
-  F::load_query(q, (const T*)a.q + (size_t)max(row, 0) * a.q_stride + (size_t)head * D, there, g);
+  F::load_query(q, (const T*)a.q + (size_t)max(row, 0) * a.q_stride + (size_t)head * D, row >= 0, g);
   sp_floatx4 o[ROWS];
   float m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) o[r] = (sp_floatx4){0.f, 0.f, 0.f, 0.f};
   const uint32_t page_elems = (uint32_t)a.page_size * D;
   const T *k_pages = (const T*)a.k_pages, *vt_pages = (const T*)a.vt_pages;
-  float scale = a.scale * LOG2E;
-  if (a.softcap > 0.f) scale = LOG2E;
+  const float scale = a.softcap > 0.f ? LOG2E : a.scale * LOG2E;
   const float inner = a.softcap > 0.f ? 2.f * LOG2E * a.scale / a.softcap : 0.f;
-  for (int kb = begin + SP_BLOCK * wave; kb < end; kb += SP_BLOCK * SP_WAVES) {
-    // (Halves of a block as above.)
-    const int second = kb + 16 < end ? kb + 16 : kb;
-    int index0, index1, slot0, slot1;
-    sp_page_of(a, kb, index0, slot0);
-    sp_page_of(a, second, index1, slot1);
-    const uint32_t page0 = min(max(scalar_int(table + index0), 0), a.n_pages - 1), page1 = min(max(scalar_int(table + index1), 0), a.n_pages - 1);
-    F f;
-    {
-      const uint32_t at = ((col >> 3 ? page1 : page0) * a.n_kv + kvh) * page_elems + ((col >> 3 ? slot1 : slot0) + 8 * ((col >> 2) & 1) + (col & 3)) * D;
+  constexpr int STRIDE = SP_BLOCK * SP_WAVES;
+  auto load = [&](F& f, int kb) {
+    const uint32_t page0 = min(max(next.page0, 0), a.n_pages - 1), page1 = min(max(next.page1, 0), a.n_pages - 1);
+    const uint32_t at = ((col >> 3 ? page1 : page0) * a.n_kv + kvh) * page_elems +
+                        ((col >> 3 ? next.slot1 : next.slot0) + 8 * ((col >> 2) & 1) + (col & 3)) * D;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) f.load_keys(t, k_pages + at + 4 * t * D, g);
-    }
-    f.load_values(vt_pages + ((g >> 1 ? page1 : page0) * a.n_kv + kvh) * page_elems + (g >> 1 ? slot1 : slot0) + 8 * (g & 1), a.page_size, col);
+    for (int t = 0; t < 2; ++t) f.load_keys(t, k_pages + at + 4 * t * D, g);
+    f.load_values(vt_pages + ((g >> 1 ? page1 : page0) * a.n_kv + kvh) * page_elems + (g >> 1 ? next.slot1 : next.slot0) + 8 * (g & 1),
+                  a.page_size, col);
+    if (kb + STRIDE < end) next = look_up(kb + STRIDE, end - 1);
+  };
+  auto attend = [&](F& f, int kb) {
     const int here = end - kb;                             // keys of the block that count
     if (here < SP_BLOCK) f.cut_values(here - 8 * g);
     float s[8];
@@ -692,6 +722,31 @@ shared_prefix_few(SharedArgs a) {
       l += s[i];
     }
     f.add_values(s, o);
+  };
+  // Two blocks in turn, where their registers leave two waves a SIMD: the next one's keys and values are on their way meanwhile.
+  constexpr bool AHEAD = sizeof(T) == 2 ? D <= 128 : D <= 64;
+  int kb = begin + SP_BLOCK * wave;
+  if constexpr (AHEAD) {
+    if (kb < end) {
+      F one, two;
+      load(one, kb);
+      while (true) {
+        if (kb + STRIDE < end) load(two, kb + STRIDE);
+        attend(one, kb);
+        kb += STRIDE;
+        if (kb >= end) break;
+        if (kb + STRIDE < end) load(one, kb + STRIDE);
+        attend(two, kb);
+        kb += STRIDE;
+        if (kb >= end) break;
+      }
+    }
+  } else {
+    for (; kb < end; kb += STRIDE) {
+      F one;
+      load(one, kb);
+      attend(one, kb);
+    }
   }
   // The waves' sums brought together through LDS, column by column.
   l = wave_add_across<32>(wave_add_across<16>(l));
@@ -726,33 +781,54 @@ shared_prefix_few(SharedArgs a) {
   }
 }
 
-// A wave joins the runs of one query: `parts` of shared keys, then its own.
+// A wave joins the runs of one query: those of shared keys, then its own.  A lane has one run's maximum and sum (of sixty-four at a
+// time), and the runs' values are asked for eight at a time.
 template <typename T, int D>
 __global__ void __launch_bounds__(SP_WAVES * WAVE)
 shared_prefix_join(SharedArgs a, T* __restrict__ out) {
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int at = blockIdx.x * SP_WAVES + wave;
   if (at >= a.n_rows * a.n_q) return;
-  const int row = at / a.n_q, head = at % a.n_q;
-  const int own = min(scalar_int(a.positions + row), a.table_stride * a.page_size - 1) + 1 - scalar_int(a.own_begin + row);
-  const int parts = min(a.slots, scalar_int(a.shared_parts + row) + (own > 0 ? (own + a.own_keys - 1) / a.own_keys : 0));
-  const float* ml = a.part_ml + (size_t)at * a.slots * 2;
+  const int row = at / a.n_q, head = at - row * a.n_q;
+  const int* mine = reinterpret_cast<const int*>(a.own_of_row + row);
+  const int begin = scalar_int(mine + 1), shared = scalar_int(mine + 2);
+  const int own = min(scalar_int(a.positions + row), a.table_stride * a.page_size - 1) + 1 - begin;
+  const int parts = min(a.slots, shared + (own > 0 ? (own + a.own_keys - 1) / a.own_keys : 0));
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)at * a.slots;
   const float* part = a.part_o + (size_t)at * a.slots * D;
-  float m = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;
-  const float sink = m;
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, ml[2 * p]);
-  float below = a.sinks && m > -INFINITY ? __builtin_amdgcn_exp2f(sink - m) : 0.f;
-  constexpr int PER = (D + WAVE - 1) / WAVE;
+  const float sink = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;
+  float m = sink;
+  for (int p = lane; p < parts; p += WAVE) m = fmaxf(m, ml[p].x);
+  m = wave_max(m);
+  float below = 0.f;
+  constexpr int PER = (D + WAVE - 1) / WAVE, DEEP = 8;
   float o[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) o[j] = 0.f;
-  for (int p = 0; p < parts; ++p) {
-    const float w = ml[2 * p] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * p] - m);
-    below += w * ml[2 * p + 1];
+  for (int first = 0; first < parts; first += WAVE) {
+    const float2 of = first + lane < parts ? ml[first + lane] : make_float2(-INFINITY, 0.f);
+    const float weight = of.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(of.x - m);
+    below += weight * of.y;
+    const int here = min(WAVE, parts - first);
+    for (int p = 0; p < here; p += DEEP) {
+      float got[DEEP][PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (lane + j * WAVE < D) o[j] += w * part[(size_t)p * D + lane + j * WAVE];
+      for (int i = 0; i < DEEP; ++i)
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          got[i][j] = part[(size_t)(first + min(p + i, here - 1)) * D + min(lane + j * WAVE, D - 1)];
+#pragma unroll
+      for (int i = 0; i < DEEP; ++i) {
+        const float w = p + i < here ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), min(p + i, WAVE - 1))) : 0.f;
+        if (p + i < here) {
+#pragma unroll
+          for (int j = 0; j < PER; ++j) o[j] += w * got[i][j];
+        }
+      }
+    }
   }
+  below = wave_sum(below);
+  if (sink > -INFINITY) below += __builtin_amdgcn_exp2f(sink - m);
   // (A query that sees no key gets zeros.)
   const float share = below > 0.f ? 1.f / below : 0.f;
 #pragma unroll
@@ -768,13 +844,13 @@ template <typename T, int D>
 static int launch_shared(const SharedArgs& a, void* out, hipStream_t stream) {
   const int group = a.n_q / a.n_kv, tiles = (group + SP_FEW_COLUMNS - 1) / SP_FEW_COLUMNS;
   if (a.n_many > 0) {
-    const dim3 grid(a.n_many, a.n_kv);
+    const unsigned grid = a.n_many;
     if constexpr (sp_is_wide<T, D>()) shared_prefix_wide<D><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
     else shared_prefix_kernel<T, D, 1><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
     const int status = LAUNCH_STATUS();
     if (status) return status;
   }
-  const dim3 grid((unsigned)a.n_narrow + (unsigned)a.n_rows * tiles * a.own_splits, a.n_kv);
+  const unsigned grid = (unsigned)a.n_narrow + (unsigned)a.n_rows * tiles * a.own_splits * a.n_kv;
   shared_prefix_few<T, D><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
   const int status = LAUNCH_STATUS();
   if (status) return status;
@@ -784,25 +860,25 @@ static int launch_shared(const SharedArgs& a, void* out, hipStream_t stream) {
 }
 
 // q: the query heads of every row at its start, rows q_stride elements apart; pages as in the other attention kernels; items int32
-// [n_narrow + n_many, 8] (`SharedItem`; sixteen columns each, then 128 or 32); order int32 [n_rows]: the rows, those of a run of shared keys side by side; own_begin,
-// shared_parts int32 [n_rows]: where a request's own keys begin, and how many partial results its shared keys leave; positions
+// [n_narrow + n_many, 8] (`SharedItem`; sixteen columns each, then 128 or 32); order int32 [n_rows]: the rows, those of a run of shared keys side by side; own, own_of_row int32 [n_rows, 4]
+// (`SharedOwn`): where a request's own keys begin and how many partial results its shared keys leave, in that order and by row; positions
 // int32 [n_rows]; block_table int32 [n_rows, table_stride].  part_o float [n_rows, n_q, slots, head_dim], part_ml float
 // [n_rows, n_q, slots, 2].  -2: a head size without an instance.
 extern "C" int ta_shared_prefix_attention(const void* q, int q_stride, void* out, const void* k_pages, const void* vt_pages,
-                                          const void* items, int n_narrow, int n_many, const void* order, const void* own_begin,
-                                          const void* shared_parts, const void* positions, const void* block_table,
+                                          const void* items, int n_narrow, int n_many, const void* order, const void* own,
+                                          const void* own_of_row, const void* positions, const void* block_table,
                                           int table_stride, const void* sinks, void* part_o, void* part_ml, int slots,
                                           int own_splits, int own_keys, int n_rows, int n_q, int n_kv, int head_dim,
                                           int page_size, int n_pages, float scale, float softcap, int dtype, hipStream_t stream) {
   if (n_rows <= 0) return 0;
-  if (!q || !out || !k_pages || !vt_pages || !order || !own_begin || !shared_parts || !positions || !block_table || !part_o || !part_ml)
+  if (!q || !out || !k_pages || !vt_pages || !order || !own || !own_of_row || !positions || !block_table || !part_o || !part_ml)
     return -1;
   if (n_narrow < 0 || n_many < 0 || (n_narrow + n_many && !items) || n_kv < 1 || n_kv > 65535 || n_q < n_kv || n_q % n_kv || page_size < 16 || page_size % 16 || n_pages < 1 ||
       slots < 1 || own_splits < 1 || own_keys < SP_BLOCK || own_keys % SP_BLOCK || table_stride < 1) return -1;
   SharedArgs a = {};
   a.q = q; a.k_pages = k_pages; a.vt_pages = vt_pages; a.part_o = (float*)part_o; a.part_ml = (float*)part_ml;
-  a.items = (const SharedItem*)items; a.order = (const int*)order; a.own_begin = (const int*)own_begin;
-  a.shared_parts = (const int*)shared_parts; a.positions = (const int*)positions; a.block_table = (const int*)block_table;
+  a.items = (const SharedItem*)items; a.order = (const int*)order; a.own = (const SharedOwn*)own;
+  a.own_of_row = (const SharedOwn*)own_of_row; a.positions = (const int*)positions; a.block_table = (const int*)block_table;
   a.sinks = (const float*)sinks; a.q_stride = q_stride; a.table_stride = table_stride; a.n_narrow = n_narrow; a.n_many = n_many; a.n_rows = n_rows;
   a.n_q = n_q; a.n_kv = n_kv; a.page_size = page_size; a.n_pages = n_pages; a.slots = slots; a.own_splits = own_splits;
   a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size);

@@ -1583,7 +1583,7 @@ class Ops:
         part_ml = torch.empty((n_rows, n_q, slots, 2), dtype=torch.float32, device=qkv.device)
         self._check(self.lib.ta_shared_prefix_attention(
             _ptr(qkv), qkv.shape[1], _ptr(out), _ptr(k_pages), _ptr(v_pages), _ptr(plan.items if plan.n_few + plan.n_many else None), plan.n_few, plan.n_many,
-            _ptr(plan.order_dev), _ptr(plan.own_begin_dev), _ptr(plan.parts_dev), _ptr(positions), _ptr(block_table), width, _ptr(sinks),
+            _ptr(plan.order_dev), _ptr(plan.own_dev), _ptr(plan.own_of_row_dev), _ptr(positions), _ptr(block_table), width, _ptr(sinks),
             _ptr(part_o), _ptr(part_ml), slots, own_splits, own_keys, n_rows, n_q, n_kv, head_dim, page_size,
             k_pages.shape[0], ctypes.c_float(scale), ctypes.c_float(softcap or 0.0), _code(qkv.dtype), self._stream()),
             "shared_prefix_attention")

@@ -70,7 +70,7 @@ class SharedPrefixes:
     WIDE_HEADS = (64, 128)
     MIN_KEYS = 64                 # a shorter run is not worth a pass and a part to be joined of its own
     MIN_PART = 128                # keys of a part of a run, at least (a block of 32 for each of its four waves)
-    MIN_WIDE_PART = 512
+    MIN_WIDE_PART = 256
     TARGET = 512                  # workgroups that the parts aim at: two a compute unit
 
     def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device,
@@ -94,34 +94,60 @@ class SharedPrefixes:
             tiles.append(found)
         # Parts of so many keys that all runs together make about TARGET workgroups (no more: they would wait for a second round).
         work = sum(len(t) * (run.key_end - run.key_begin) for t, run in zip(tiles, self.runs)) * n_kv
-        items, parts_of = {False: [], True: []}, np.zeros(self.n_rows, dtype=np.int32)
+        groups, parts_of = {False: [], True: []}, np.zeros(self.n_rows, dtype=np.int32)      # items that read the same keys and values
         for found, run in zip(tiles, self.runs):
             length = run.key_end - run.key_begin
             part = max(self.MIN_WIDE_PART if wide and found[0][1] else self.MIN_PART, -(-work // self.TARGET))
             keys = -(-length // (32 * max(1, length // part))) * 32
             first = int(parts_of[run.rows[0]])
             for split, begin in enumerate(range(run.key_begin, run.key_end, keys)):
-                for column, many in found:
-                    items[many].append((place[run.rows[0]], len(run.rows) * group, column, begin, min(run.key_end, begin + keys),
-                                        first + split, 0, 0))
+                end = min(run.key_end, begin + keys)
+                for head in range(n_kv):
+                    for kind in (False, True):
+                        group_items = [(place[run.rows[0]], len(run.rows) * group, column, begin, end, first + split, run.rows[0], head)
+                                       for column, many in found if many is kind]
+                        if group_items:
+                            groups[kind].append((end - begin, group_items))
             parts_of[run.rows] = first + -(-length // keys)
-        for some in items.values():
-            some.sort(key=lambda item: item[3] - item[4])     # long ones first
-            if fill:                                      # (up to a multiple, with items without columns: plans of one size)
-                some += [(0,) * 8] * (-len(some) % fill)
+        items = {kind: self._in_order(some, fill) for kind, some in groups.items()}
         self.n_few, self.n_many = len(items[False]), len(items[True])
         self.shared_parts = int(parts_of.max(initial=0))
         self.own_begin = own_begin                        # int32 [B] on the host
         self.keys_end = max((run.key_end for run in self.runs), default=0)
         self.smallest_own = int(own_begin.min(initial=0)) if self.n_rows else 0
-        packed = np.concatenate([np.asarray(items[False] + items[True], dtype=np.int32).reshape(-1), np.asarray(self.order, dtype=np.int32), own_begin,
-                                 parts_of]).astype(np.int32)
+        rows = np.arange(self.n_rows, dtype=np.int32)
+        own = np.stack([rows, own_begin, parts_of, np.zeros_like(rows)], axis=1).astype(np.int32)
+        packed = np.concatenate([np.asarray(items[False] + items[True], dtype=np.int32).reshape(-1), np.asarray(self.order, dtype=np.int32),
+                                 own[self.order].reshape(-1), own.reshape(-1)]).astype(np.int32)
         self._on_device(torch.from_numpy(packed).to(device))
+
+    CHIPLETS = 8                  # of the device: each gets every eighth workgroup, and has a cache of its own
+
+    @classmethod
+    def _in_order(cls, groups, fill: int) -> list[tuple]:
+        """The items in the order of their workgroups: those of a group, which read the same keys and values, on one chiplet (two, where an
+        even share of the work ends inside a group), the long ones first.  Places that a chiplet has left, and those up to a multiple of
+        `fill` (plans of one size), hold items without columns."""
+        queues = [[] for _ in range(cls.CHIPLETS)]
+        # (A part's last piece may be a little shorter: shares are counted in eighths of the longest, so that equal parts stay equal.)
+        step = max([1] + [-(-keys // 8) for keys, _ in groups])
+        cost = lambda keys: -(-keys // step)
+        total, before = sum(cost(keys) * len(group) for keys, group in groups), 0
+        for keys, group in sorted(groups, key=lambda g: -g[0]):
+            for item in group:
+                queues[min(cls.CHIPLETS - 1, before * cls.CHIPLETS // total)].append(item)
+                before += cost(keys)
+        nothing = (0,) * 8
+        longest = max(len(q) for q in queues)
+        order = [queue[i] if i < len(queue) else nothing for i in range(longest) for queue in queues]
+        while order and order[-1] is nothing:
+            order.pop()
+        return order + [nothing] * (-len(order) % fill if fill else 0)
 
     def _on_device(self, packed: torch.Tensor) -> None:
         self.packed = packed
-        sizes = [8 * (self.n_few + self.n_many)] + [self.n_rows] * 3
-        self.items, self.order_dev, self.own_begin_dev, self.parts_dev = torch.split(packed, sizes)
+        sizes = [8 * (self.n_few + self.n_many)] + [self.n_rows, 4 * self.n_rows, 4 * self.n_rows]
+        self.items, self.order_dev, self.own_dev, self.own_of_row_dev = torch.split(packed, sizes)
 
     @property
     def signature(self) -> tuple:
