@@ -232,15 +232,21 @@ __device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)
 }
 
 // ------------------------------------------------------------------------------------------------
-// Many columns: a wave has 32 of the workgroup's SP_WIDE_COLUMNS, and all of them go through the same keys, a block of 64 at a time, which
-// the workgroup brings into LDS while it works on the block before.  Loads write LDS in the order of their lanes, so the lanes ask for
-// pieces of sixteen bytes in the order in which the reads find them in different banks: a unit of sixteen keys lies key by key, piece p of
-// key k at place p ^ (k, or k / 2 where a key is half as long as the banks are wide); its values lie coordinate by coordinate, the two
-// pieces of a coordinate d changing places with d / 8.
+// Many columns: a wave has 32 of the workgroup's SP_WIDE_COLUMNS, and all of them go through the same keys, which the workgroup brings into
+// LDS in blocks of 64 ahead of their use.  Loads write LDS in the order of their lanes, so the lanes ask for pieces of sixteen bytes in
+// the order in which the reads find them in different banks: a unit of sixteen keys lies key by key, piece p of key k at place p ^ (k, or
+// k / 2 where a key is half as long as the banks are wide); its values lie coordinate by coordinate, the two pieces of a coordinate d
+// changing places with d / 8.
+//
+// The work is a pipeline over steps of 32 keys.  In step k the weights of step k - 1 meet their values while the maximum of step k's scores
+// is looked for, and the scores of step k + 1 are made while those of step k become weights: the matrix instructions of a step wait
+// for no vector instruction of the same step, and the other way round.  (One after the other, a block of 64 keys took 1.6 us of a
+// wave alone on its SIMD at head size 128, of which the matrix cores worked 0.43.)  So in iteration b, steps 2 b + 1 and 2 b + 2, the keys
+// of block b + 1 and the values of block b are read, and the keys of block b + 2 and the values of block b + 1 come in.
 template <int D>
 struct Wide {
   static constexpr int PIECES = D / 8, KEY = 2 * D, UNIT = 16 * KEY, TILE = 4 * UNIT;      // pieces of a key; bytes of keys (values alike)
-  static constexpr int ROUNDS = TILE / 4096, STEPS = D / 16, ROWS = D / 32;
+  static constexpr int ROUNDS = TILE / 4096, STEPS = D / 16, ROWS = D / 32;   // (as many pieces of keys as of values: 2 ROWS = STEPS)
   static_assert(D == 64 || D == 128, "the order of the pieces is made for keys of 128 and of 256 bytes");
   typedef const char __attribute__((address_space(1)))* from_t;
   typedef char __attribute__((address_space(3)))* lds_t;
@@ -266,111 +272,180 @@ struct Wide {
   }
 };
 
-template <int D>
-__device__ __forceinline__ void sp_wide(const SharedArgs& a, char* even, char* odd) {
+template <int D, bool CAPPED>
+__device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* keys1, char* values0, char* values1) {
   typedef Wide<D> W;
+  typedef Frag<bf16_t, D> F;
+  constexpr int ROWS = W::ROWS;
   const int* item = reinterpret_cast<const int*>(a.items + a.n_narrow + blockIdx.x);
   const int rows_at = scalar_int(item), columns = scalar_int(item + 1), first_column = scalar_int(item + 2);
   const int begin = scalar_int(item + 3), end = scalar_int(item + 4), slot = scalar_int(item + 5);
-  if (columns <= 0) return;                                // an item that only fills the list up
-  typedef Frag<bf16_t, D> F;
-  constexpr int ROWS = W::ROWS;
-  const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 31, half = lane >> 5;
+  const int* table = a.block_table + (size_t)scalar_int(item + 6) * a.table_stride;
   const int kvh = scalar_int(item + 7), group = a.n_q / a.n_kv;
+  if (columns <= 0) return;                                // an item that only fills the list up
+  const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 31, half = lane >> 5;
+  const uint32_t key_place = W::key_place(threadIdx.x), value_place = W::value_place(threadIdx.x, a.page_size);
+  // (A layer's keys are fewer than 2^31 elements: places in bytes fit 32 bits.)
+  const uint32_t page_bytes = (uint32_t)a.page_size * D * 2, all_heads = page_bytes * a.n_kv, of_head = page_bytes * kvh;
+  const typename W::from_t k_from = (typename W::from_t)a.k_pages, v_from = (typename W::from_t)a.vt_pages;
+  // Where this wave's units of a block lie in the pages (the run's last unit stands in for one behind it, of which nothing counts).
+  struct Units { int page[W::ROUNDS], at[W::ROUNDS]; };
+  auto look_up = [&](int block) {
+    Units u;
+#pragma unroll
+    for (int j = 0; j < W::ROUNDS; ++j) {
+      int index;
+      sp_page_of(a, min(begin + SP_WIDE_BLOCK * block + 16 * W::unit_of(j, wave), end - 16), index, u.at[j]);
+      u.page[j] = scalar_int(table + index);
+    }
+    return u;
+  };
+  auto start = [&](const Units& u, int j) { return (uint32_t)min(max(u.page[j], 0), a.n_pages - 1) * all_heads + of_head; };
+  auto fetch_keys = [&](const Units& u, char* to) {
+#pragma unroll
+    for (int j = 0; j < W::ROUNDS; ++j)
+      __builtin_amdgcn_global_load_lds(k_from + (start(u, j) + (uint32_t)u.at[j] * W::KEY + key_place),
+                                       (typename W::lds_t)(to + j * 4096 + wave * 1024), 16, 0, 0);
+  };
+  auto fetch_values = [&](const Units& u, char* to) {
+#pragma unroll
+    for (int j = 0; j < W::ROUNDS; ++j)
+      __builtin_amdgcn_global_load_lds(v_from + (start(u, j) + (uint32_t)u.at[j] * 2 + value_place),
+                                       (typename W::lds_t)(to + j * 4096 + wave * 1024), 16, 0, 0);
+  };
+  const int blocks = (end - begin + SP_WIDE_BLOCK - 1) / SP_WIDE_BLOCK;
+  Units before = look_up(0), next = look_up(1);
+  fetch_keys(before, keys0);
+  fetch_values(before, values0);
+  fetch_keys(next, keys1);
+  before = next;                                           // (block b + 1's, whose values come in iteration b; `next`: block b + 2's)
+  next = look_up(2);
+
   const int column = first_column + 32 * wave + col;
   const bool there = column < columns, wave_there = first_column + 32 * wave < columns;
   const int row = there ? a.order[rows_at + column / group] : -1, head = kvh * group + column % group;
   typename F::Query q;
   F::load_query(q, (const bf16_t*)a.q + (size_t)max(row, 0) * a.q_stride + (size_t)head * D, there, half);
-  const int* table = a.block_table + (size_t)scalar_int(item + 6) * a.table_stride;
-  const uint32_t key_place = W::key_place(threadIdx.x), value_place = W::value_place(threadIdx.x, a.page_size);
-  // (A layer's keys are fewer than 2^31 elements: places in bytes fit 32 bits.)
-  const uint32_t page_bytes = (uint32_t)a.page_size * D * 2, all_heads = page_bytes * a.n_kv, of_head = page_bytes * kvh;
-  const typename W::from_t k_from = (typename W::from_t)a.k_pages, v_from = (typename W::from_t)a.vt_pages;
-  // Where round j's unit of a block starts in the pages (the run's last unit stands in for one behind it, of which nothing counts).
-  int page[W::ROUNDS], at[W::ROUNDS];
-  auto look_up = [&](int kb) {
-#pragma unroll
-    for (int j = 0; j < W::ROUNDS; ++j) {
-      int index;
-      sp_page_of(a, min(kb + 16 * W::unit_of(j, wave), end - 16), index, at[j]);
-      page[j] = scalar_int(table + index);
-    }
-  };
-  auto fetch = [&](char* to) {
-#pragma unroll
-    for (int j = 0; j < W::ROUNDS; ++j) {
-      const uint32_t start = (uint32_t)min(max(page[j], 0), a.n_pages - 1) * all_heads + of_head;
-      __builtin_amdgcn_global_load_lds(k_from + (start + (uint32_t)at[j] * W::KEY + key_place),
-                                       (typename W::lds_t)(to + j * 4096 + wave * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(v_from + (start + (uint32_t)at[j] * 2 + value_place),
-                                       (typename W::lds_t)(to + W::TILE + j * 4096 + wave * 1024), 16, 0, 0);
-    }
-  };
   sp_floatx16 o[ROWS];
   float m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) o[r] = (sp_floatx16){};
   const int my_key = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
-  auto work = [&](const char* keys, int kb) {
-    const char* values = keys + W::TILE;
-    sp_floatx16 s[2];
+  const float scale = CAPPED ? LOG2E : a.scale * LOG2E;
+  const float inner = CAPPED ? 2.f * LOG2E * a.scale / a.softcap : 0.f;
+
+  // Pieces of the keys, and of the values, of one half (32 keys) of a block: all asked for before the first is used, ahead of other work
+  // (left to itself the compiler asks for two, waits, and asks for the next two: 0.06 us each time).
+  struct Pieces { sp_bf16x8 p[W::STEPS]; };
+  auto read_keys = [&](const char* keys, int part) {
+    Pieces f;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = (sp_floatx16){};
+    for (int i = 0; i < W::STEPS; ++i) f.p[i] = W::key_piece(keys, SP_BLOCK * part + my_key, 2 * i + half);
+    return f;
+  };
+  auto read_values = [&](const char* values, int part) {
+    Pieces f;
 #pragma unroll
-      for (int i = 0; i < W::STEPS; ++i)
-        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(W::key_piece(keys, SP_BLOCK * b + my_key, 2 * i + half), q.f[i], s[b], 0, 0, 0);
+    for (int i = 0; i < 2 * ROWS; ++i) f.p[i] = W::value_piece(values, 2 * part + (i & 1), 32 * (i >> 1) + col, half);
+    return f;
+  };
+  auto scores = [&](const Pieces& f) {
+    sp_floatx16 s = {};
+#pragma unroll
+    for (int i = 0; i < W::STEPS; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.p[i], q.f[i], s, 0, 0, 0);
+    return s;
+  };
+  auto add_values = [&](const Pieces& f, const sp_bf16x8 (&w)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2 * ROWS; ++i) o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.p[i], w[i & 1], o[i >> 1], 0, 0, 0);
+  };
+  // The reference brought up where a weight would pass 2^SP_SLACK (see `sp_softmax`); `here`: keys of the step that count.
+  auto settle = [&](sp_floatx16& s, int here) {
+    if (CAPPED) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = a.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(inner * s[i])));
     }
-    sp_softmax<2, ROWS>(a, s, end - kb, half, m, l, o);
+    if (here < SP_BLOCK) {
+      asm volatile("");                                    // (a branch: worked out for every step the cuts are 48 instructions of it)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      sp_bf16x8 w[2];
+      for (int i = 0; i < 16; ++i)
+        if (16 * (i >> 3) + 8 * half + (i & 7) >= here) s[i] = -INFINITY;
+    }
+    float high = s[0];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = (__bf16)s[b][i];
+    for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
+    high = wave_max_across<32>(high) * scale;
+    if (__any(high > m + SP_SLACK)) {
+      const float m_new = high > m + SP_SLACK ? high : m;
+      const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= corr;
 #pragma unroll
       for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          o[r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(W::value_piece(values, 2 * b + t, 32 * r + col, half), w[t], o[r], 0, 0, 0);
+        for (int i = 0; i < 16; ++i) o[r][i] *= corr;
     }
   };
-  // A block's loads are asked for a block ahead; the barrier behind the wait for them is also the one that frees the other buffer.
-  look_up(begin);
-  fetch(even);
-  look_up(begin + SP_WIDE_BLOCK);
-  for (int kb = begin; kb < end; kb += 2 * SP_WIDE_BLOCK) {
+  auto weigh = [&](const sp_floatx16& s, sp_bf16x8 (&w)[2]) {
+    const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[i], scale, -from));
+      l += p;
+      w[i >> 3][i & 7] = (__bf16)p;
+    }
+  };
+  sp_floatx16 even, odd;                                   // scores of the steps in turn
+  sp_bf16x8 w[2];
+  // Iteration b: `keys` of block b + 1, `values` of block b; the two buffers that the iteration before has freed are filled.
+  auto iteration = [&](int b, const char* keys, const char* values, char* keys_to, char* values_to) {
     __builtin_amdgcn_s_waitcnt(0x0F70);                    // all that this wave fetched has arrived (vmcnt 0)
     __syncthreads();
-    if (kb + SP_WIDE_BLOCK < end) fetch(odd);
-    look_up(kb + 2 * SP_WIDE_BLOCK);
-    if (wave_there) work(even, kb);
-    if (kb + SP_WIDE_BLOCK >= end) break;                  // (the same for the whole workgroup)
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
-    if (kb + 2 * SP_WIDE_BLOCK < end) fetch(even);
-    look_up(kb + 3 * SP_WIDE_BLOCK);
-    if (wave_there) work(odd, kb + SP_WIDE_BLOCK);
+    if (b + 2 < blocks) fetch_keys(next, keys_to);
+    if (b + 1 < blocks) fetch_values(before, values_to);
+    before = next;
+    next = look_up(b + 3);
+    if (wave_there) {
+      const int here = end - begin - SP_WIDE_BLOCK * b;    // keys from block b on
+      const Pieces v0 = read_values(values, 0), k0 = read_keys(keys, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      add_values(v0, w);
+      settle(odd, here - SP_BLOCK);
+      const Pieces v1 = read_values(values, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      even = scores(k0);
+      weigh(odd, w);
+      const Pieces k1 = read_keys(keys, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      add_values(v1, w);
+      settle(even, here - 2 * SP_BLOCK);
+      odd = scores(k1);
+      weigh(even, w);
+    }
+  };
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  __syncthreads();
+  if (wave_there) {
+    even = scores(read_keys(keys0, 0));
+    odd = scores(read_keys(keys0, 1));
+    settle(even, end - begin);
+    weigh(even, w);
+  }
+  for (int b = 0; b < blocks; b += 2) {
+    iteration(b, keys1, values0, keys0, values1);
+    if (b + 1 >= blocks) break;                            // (the same for the whole workgroup)
+    iteration(b + 1, keys0, values1, keys1, values0);
   }
   l = wave_add_across<32>(l);
   if (row < 0) return;
   const size_t to = ((size_t)row * a.n_q + head) * a.slots + slot;
-  if (half == 0) { a.part_ml[2 * to] = m; a.part_ml[2 * to + 1] = l; }
+  if (half == 0) st_through(reinterpret_cast<uint2*>(a.part_ml + 2 * to), make_uint2(__float_as_uint(m), __float_as_uint(l)));
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       *reinterpret_cast<sp_floatx4*>(a.part_o + to * D + 32 * r + 8 * j + 4 * half) =
           (sp_floatx4){o[r][4 * j], o[r][4 * j + 1], o[r][4 * j + 2], o[r][4 * j + 3]};
-}
-
-template <int D>
-__global__ void __launch_bounds__(SP_WAVES * WAVE)
-shared_prefix_wide(SharedArgs a) {
-  // (The two buffers are arrays of their own, each named where it is used: a read of one then waits for no load into the other.)
-  __shared__ __attribute__((aligned(1024))) char even[2 * Wide<D>::TILE];
-  __shared__ __attribute__((aligned(1024))) char odd[2 * Wide<D>::TILE];
-  sp_wide<D>(a, even, odd);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -602,18 +677,21 @@ struct Frag16<float, D> {
 
 #define SP_FEW_COLUMNS 16
 
+struct FewSums {                         // what the waves leave for each other, beside their outputs
+  float m[SP_WAVES][SP_FEW_COLUMNS], l[SP_WAVES][SP_FEW_COLUMNS];
+  int row[SP_FEW_COLUMNS], head[SP_FEW_COLUMNS];
+};
+template <int D> constexpr int few_outputs() { return SP_FEW_COLUMNS * (D + 4); }      // floats of a wave's outputs, column by column
+
+// `block`: which of the workgroups for few columns; o0 .. o3: LDS for the waves' outputs.
 template <typename T, int D>
-__global__ void __launch_bounds__(SP_WAVES * WAVE)
-shared_prefix_few(SharedArgs a) {
+__device__ __forceinline__ void sp_few(const SharedArgs& a, int block, float* o0, float* o1, float* o2, float* o3, FewSums& sums) {
   typedef Frag16<T, D> F;
-  constexpr int ROWS = F::ROWS;
-  __shared__ float o_s[SP_WAVES][SP_FEW_COLUMNS][D + 4];
-  __shared__ float m_s[SP_WAVES][SP_FEW_COLUMNS], l_s[SP_WAVES][SP_FEW_COLUMNS];
-  __shared__ int row_s[SP_FEW_COLUMNS], head_s[SP_FEW_COLUMNS];
+  constexpr int ROWS = F::ROWS, COLUMN = D + 4;
   const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 15, g = lane >> 4;
   const int group = a.n_q / a.n_kv;
   int columns, first_column, begin, end, slot, table_row, kvh, row = -1;
-  const bool own = (int)blockIdx.x >= a.n_narrow;
+  const bool own = block >= a.n_narrow;
   const int* table;
   // Which pages the two halves of the wave's next block of keys lie in, asked for a block ahead.  The second half may have no key: the first
   // one's page stands in for it, and nothing that is read there counts.  (The first block of a request's own keys is looked up beside its
@@ -630,7 +708,7 @@ shared_prefix_few(SharedArgs a) {
   };
   Pages next;
   if (!own) {
-    const int* item = reinterpret_cast<const int*>(a.items + blockIdx.x);
+    const int* item = reinterpret_cast<const int*>(a.items + block);
     const int rows_at = scalar_int(item);
     columns = scalar_int(item + 1); first_column = scalar_int(item + 2);
     begin = scalar_int(item + 3); end = scalar_int(item + 4); slot = scalar_int(item + 5);
@@ -642,16 +720,16 @@ shared_prefix_few(SharedArgs a) {
   } else {
     const int tiles = (group + SP_FEW_COLUMNS - 1) / SP_FEW_COLUMNS;
     // (First parts of all requests first: the last ones are empty for the short ones.)
-    int at = blockIdx.x - a.n_narrow;
+    int at = block - a.n_narrow;
     kvh = at % a.n_kv;
     at /= a.n_kv;
     const int tile = at % tiles;
     at /= tiles;
     const int split = at / a.n_rows;
-    const int* mine = reinterpret_cast<const int*>(a.own + (at - split * a.n_rows));
-    table_row = scalar_int(mine);
-    begin = scalar_int(mine + 1) + split * a.own_keys;
-    slot = scalar_int(mine + 2) + split;
+    const int* of = reinterpret_cast<const int*>(a.own + (at - split * a.n_rows));
+    table_row = scalar_int(of);
+    begin = scalar_int(of + 1) + split * a.own_keys;
+    slot = scalar_int(of + 2) + split;
     columns = group;
     first_column = tile * SP_FEW_COLUMNS;
     table = a.block_table + (size_t)table_row * a.table_stride;
@@ -750,34 +828,65 @@ shared_prefix_few(SharedArgs a) {
   }
   // The waves' sums brought together through LDS, column by column.
   l = wave_add_across<32>(wave_add_across<16>(l));
+  float* mine = wave < 2 ? (wave == 0 ? o0 : o1) : (wave == 2 ? o2 : o3);
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) *reinterpret_cast<sp_floatx4*>(&o_s[wave][col][16 * r + 4 * g]) = o[r];
-  if (g == 0) { m_s[wave][col] = m; l_s[wave][col] = l; }
-  if (wave == 0 && g == 0) { row_s[col] = row; head_s[col] = head; }
+  for (int r = 0; r < ROWS; ++r) *reinterpret_cast<sp_floatx4*>(mine + col * COLUMN + 16 * r + 4 * g) = o[r];
+  if (g == 0) { sums.m[wave][col] = m; sums.l[wave][col] = l; }
+  if (wave == 0 && g == 0) { sums.row[col] = row; sums.head[col] = head; }
   __syncthreads();
   const int heads_here = min(SP_FEW_COLUMNS, columns - first_column);
   for (int c = wave; c < heads_here; c += SP_WAVES) {
-    float top = m_s[0][c];
+    float top = sums.m[0][c];
 #pragma unroll
-    for (int w = 1; w < SP_WAVES; ++w) top = fmaxf(top, m_s[w][c]);
+    for (int w = 1; w < SP_WAVES; ++w) top = fmaxf(top, sums.m[w][c]);
     float factor[SP_WAVES], below = 0.f;
 #pragma unroll
     for (int w = 0; w < SP_WAVES; ++w) {
-      factor[w] = m_s[w][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_s[w][c] - top);
-      below += l_s[w][c] * factor[w];
+      factor[w] = sums.m[w][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sums.m[w][c] - top);
+      below += sums.l[w][c] * factor[w];
     }
-    const size_t to = ((size_t)row_s[c] * a.n_q + head_s[c]) * a.slots + slot;
-    if (lane == 0) { a.part_ml[2 * to] = top; a.part_ml[2 * to + 1] = below; }
+    const size_t to = ((size_t)sums.row[c] * a.n_q + sums.head[c]) * a.slots + slot;
+    if (lane == 0) st_through(reinterpret_cast<uint2*>(a.part_ml + 2 * to), make_uint2(__float_as_uint(top), __float_as_uint(below)));
 #pragma unroll
     for (int j = 0; j < (D + WAVE - 1) / WAVE; ++j) {
       const int d = lane + j * WAVE;
       if (d < D) {
         float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < SP_WAVES; ++w) sum += o_s[w][c][d] * factor[w];
-        a.part_o[to * D + d] = sum;
+        sum += o0[c * COLUMN + d] * factor[0];
+        sum += o1[c * COLUMN + d] * factor[1];
+        sum += o2[c * COLUMN + d] * factor[2];
+        sum += o3[c * COLUMN + d] * factor[3];
+        st_through(a.part_o + to * D + d, sum);
       }
     }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(SP_WAVES * WAVE)
+shared_prefix_few(SharedArgs a) {
+  __shared__ float o_s[SP_WAVES][few_outputs<D>()];
+  __shared__ FewSums sums;
+  static_assert(SP_WAVES == 4, "outputs of four waves");
+  sp_few<T, D>(a, blockIdx.x, o_s[0], o_s[1], o_s[2], o_s[3], sums);
+}
+
+// Both in one launch: the workgroups for many columns first.  (Neither leaves more than two waves a SIMD room at head size 128, and each
+// alone leaves much of the device idle at its end.)
+template <int D, bool CAPPED>
+__global__ void __launch_bounds__(SP_WAVES * WAVE, 2)      // (two waves a SIMD: half its registers each)
+shared_prefix_both(SharedArgs a) {
+  // (The buffers are arrays of their own, each named where it is used: a read of one then waits for no load into another.)
+  __shared__ __attribute__((aligned(1024))) char keys0[Wide<D>::TILE];
+  __shared__ __attribute__((aligned(1024))) char keys1[Wide<D>::TILE];
+  __shared__ __attribute__((aligned(1024))) char values0[Wide<D>::TILE];
+  __shared__ __attribute__((aligned(1024))) char values1[Wide<D>::TILE];
+  __shared__ FewSums sums;
+  static_assert(few_outputs<D>() * 4 <= Wide<D>::TILE, "a wave's outputs in a buffer");
+  if ((int)blockIdx.x < a.n_many) {
+    sp_wide<D, CAPPED>(a, keys0, keys1, values0, values1);
+  } else {
+    sp_few<bf16_t, D>(a, blockIdx.x - a.n_many, (float*)keys0, (float*)keys1, (float*)values0, (float*)values1, sums);
   }
 }
 
@@ -843,16 +952,22 @@ constexpr bool sp_is_wide() { return sizeof(T) == 2 && (D == 64 || D == 128); }
 template <typename T, int D>
 static int launch_shared(const SharedArgs& a, void* out, hipStream_t stream) {
   const int group = a.n_q / a.n_kv, tiles = (group + SP_FEW_COLUMNS - 1) / SP_FEW_COLUMNS;
-  if (a.n_many > 0) {
-    const unsigned grid = a.n_many;
-    if constexpr (sp_is_wide<T, D>()) shared_prefix_wide<D><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
-    else shared_prefix_kernel<T, D, 1><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
-    const int status = LAUNCH_STATUS();
-    if (status) return status;
+  const unsigned few = (unsigned)a.n_narrow + (unsigned)a.n_rows * tiles * a.own_splits * a.n_kv;
+  int status = 0;
+  if constexpr (sp_is_wide<T, D>()) {
+    if (a.n_many == 0) shared_prefix_few<T, D><<<few, SP_WAVES * WAVE, 0, stream>>>(a);
+    else if (a.softcap > 0.f) shared_prefix_both<D, true><<<a.n_many + few, SP_WAVES * WAVE, 0, stream>>>(a);
+    else shared_prefix_both<D, false><<<a.n_many + few, SP_WAVES * WAVE, 0, stream>>>(a);
+    status = LAUNCH_STATUS();
+  } else {
+    if (a.n_many > 0) {
+      shared_prefix_kernel<T, D, 1><<<a.n_many, SP_WAVES * WAVE, 0, stream>>>(a);
+      status = LAUNCH_STATUS();
+      if (status) return status;
+    }
+    shared_prefix_few<T, D><<<few, SP_WAVES * WAVE, 0, stream>>>(a);
+    status = LAUNCH_STATUS();
   }
-  const unsigned grid = (unsigned)a.n_narrow + (unsigned)a.n_rows * tiles * a.own_splits * a.n_kv;
-  shared_prefix_few<T, D><<<grid, SP_WAVES * WAVE, 0, stream>>>(a);
-  const int status = LAUNCH_STATUS();
   if (status) return status;
   const int queries = a.n_rows * a.n_q;
   shared_prefix_join<T, D><<<(queries + SP_WAVES - 1) / SP_WAVES, SP_WAVES * WAVE, 0, stream>>>(a, (T*)out);
