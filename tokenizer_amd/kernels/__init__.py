@@ -66,10 +66,23 @@ def _dev(*tensors: torch.Tensor | None) -> None:
 
 
 def _here(*tensors: torch.Tensor | None) -> None:
-    """All operands on the current device: its stream is the one a kernel is launched on."""
+    """All operands contiguous and on the current device: its stream is the one a kernel is launched on."""
     current = torch.cuda.current_device()
     for tensor in tensors:
-        _need(tensor is None or tensor.device.index == current, "kernel operands must live on the current device")
+        if tensor is not None:
+            if tensor.get_device() != current:
+                raise KernelError("kernel operands must live on the current GPU")
+            if not tensor.is_contiguous():
+                raise KernelError("kernel operands must be contiguous")
+
+
+def _address(tensor: torch.Tensor | None, offset: int = 0):
+    """A tensor's address (`offset` bytes further) for a function whose argument types are declared: a plain number, which costs a
+    fraction of a ctypes object, but for a thread that records its calls."""
+    if _RECORDING.library is None:
+        return None if tensor is None else tensor.data_ptr() + offset
+    pointer = _ptr(tensor)
+    return ctypes.c_void_p(pointer.value + offset) if offset else pointer
 
 
 def _parts_of_k(k: int, splits: int, step: int) -> int:
@@ -191,6 +204,12 @@ class Ops:
                                                  ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
         self.lib.ta_library_gemm_bf16.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int] * 5 + [
             ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p]
+        pointer, number, real = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+        self.lib.ta_shared_prefix_attention.argtypes = ([pointer, number] + [pointer] * 4 + [number] * 2 + [pointer] * 5 + [number]
+                                                        + [pointer] * 3 + [number] * 9 + [real] * 2 + [number, pointer])
+        self.lib.ta_sample_filtered.argtypes = [pointer, ctypes.c_int64] + [pointer] * 7 + [number] * 3 + [pointer]
+        self.lib.ta_copy_pages.argtypes = [pointer] * 3 + [number] * 9 + [pointer]
+        self._sample_bytes: dict[int, int] = {}    # workspace of a row of so many logits
         self._workspaces: dict[int, torch.Tensor] = {}
         self._filled: dict[int, tuple] = {}        # weights whose K was filled up to a multiple of eight, by address
         self.compute_units = int(self._loaded.ta_compute_units())     # what the splits below aim to fill
@@ -1547,14 +1566,15 @@ class Ops:
         d, page_size]; positions int32 [B]; block_table int32 [B, P].  A row sees the keys of all positions up to its own (a row of
         position -1 none: its result is zero).  `sinks` (float32 [n_q]): exp(sinks[h]) joins the denominator; `softcap` c: a
         scaled score s becomes c tanh(s / c).  `max_position` (host): the largest position, for the launch's size."""
-        _dev(qkv, out, k_pages, v_pages, positions, block_table, sinks)
-        n_rows = qkv.shape[0]
-        _need(plan.n_rows == n_rows and (plan.n_q, plan.n_kv, plan.head_dim, plan.dtype) == (n_q, n_kv, head_dim, qkv.dtype),
+        _here(qkv, out, k_pages, v_pages, positions, block_table, plan.packed, sinks)
+        n_rows, row_elements = qkv.shape
+        dtype = qkv.dtype
+        _need(plan.n_rows == n_rows and (plan.n_q, plan.n_kv, plan.head_dim, plan.dtype) == (n_q, n_kv, head_dim, dtype),
               "the plan belongs to other rows or to another shape of attention")
-        _need(qkv.dim() == 2 and qkv.shape[1] >= n_q * head_dim and (qkv.shape[1] * qkv.element_size()) % 16 == 0 and qkv.data_ptr() % 16 == 0,
+        _need(row_elements >= n_q * head_dim and row_elements * qkv.element_size() % 16 == 0 and qkv.data_ptr() % 16 == 0,
               "qkv holds the query heads first, in rows of whole 16 bytes")
-        _need(tuple(out.shape) == (n_rows, n_q * head_dim) and out.dtype == qkv.dtype, "attention output shape")
-        _need(k_pages.dtype == qkv.dtype and v_pages.dtype == qkv.dtype, "pages must have the dtype of qkv")
+        _need(out.shape == (n_rows, n_q * head_dim) and out.dtype == dtype, "attention output shape")
+        _need(k_pages.dtype == dtype and v_pages.dtype == dtype, "pages must have the dtype of qkv")
         page_size = self._page_size(k_pages, v_pages, n_kv, head_dim)
         _need(page_size == plan.page_size, "the plan belongs to pages of another size")
         _need(k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0, "pages start at whole 16 bytes")
@@ -1563,7 +1583,6 @@ class Ops:
         _need(sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == n_q), "sinks are float32 [n_q]")
         _need(softcap is None or softcap > 0, "a cap on the scores is positive")
         _need(scale > 0, "the scores' scale is positive")
-        _here(qkv, out, k_pages, v_pages, positions, block_table, plan.items, sinks)
         width = block_table.shape[1]
         _need(plan.keys_end <= width * page_size, "block table is too narrow for the shared keys")
         if max_position is None:
@@ -1579,14 +1598,16 @@ class Ops:
         own_keys = -(-own_keys // 32) * 32
         own_splits = -(-longest // own_keys)
         slots = plan.shared_parts + own_splits
-        part_o = torch.empty((n_rows, n_q, slots, head_dim), dtype=torch.float32, device=qkv.device)
-        part_ml = torch.empty((n_rows, n_q, slots, 2), dtype=torch.float32, device=qkv.device)
+        # Partial results: the weighed values, and behind them the maxima and sums.
+        values = n_rows * n_q * slots * head_dim
+        partial = torch.empty(values + 2 * n_rows * n_q * slots, dtype=torch.float32, device=qkv.device)
+        items, order, own, own_of_row = plan.places
+        packed = plan.packed
         self._check(self.lib.ta_shared_prefix_attention(
-            _ptr(qkv), qkv.shape[1], _ptr(out), _ptr(k_pages), _ptr(v_pages), _ptr(plan.items if plan.n_few + plan.n_many else None), plan.n_few, plan.n_many,
-            _ptr(plan.order_dev), _ptr(plan.own_dev), _ptr(plan.own_of_row_dev), _ptr(positions), _ptr(block_table), width, _ptr(sinks),
-            _ptr(part_o), _ptr(part_ml), slots, own_splits, own_keys, n_rows, n_q, n_kv, head_dim, page_size,
-            k_pages.shape[0], ctypes.c_float(scale), ctypes.c_float(softcap or 0.0), _code(qkv.dtype), self._stream()),
-            "shared_prefix_attention")
+            _address(qkv), row_elements, _address(out), _address(k_pages), _address(v_pages), _address(packed, items), plan.n_few, plan.n_many,
+            _address(packed, order), _address(packed, own), _address(packed, own_of_row), _address(positions), _address(block_table), width,
+            _address(sinks), _address(partial), _address(partial, 4 * values), slots, own_splits, own_keys, n_rows, n_q, n_kv, head_dim,
+            page_size, k_pages.shape[0], scale, softcap or 0.0, _code(dtype), self._stream()), "shared_prefix_attention")
         return out
 
     def talking_attention(self, qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -2438,25 +2459,28 @@ class Ops:
 
         logits float32 or bfloat16 [B, V], V up to 2^19, rows that may lie further apart than V; temperature, top_p, min_p, uniform
         (in [0, 1)) float32 [B]; top_k int32 [B]; returns int32 [B]."""
-        _need(logits.is_cuda, "kernel operands must live on the GPU")
-        _dev(temperature, top_k, top_p, min_p, uniform, out)
         _need(logits.dim() == 2 and logits.dtype in _CODES, "logits must be float32 or bfloat16 [B, V]")
+        _here(temperature, top_k, top_p, min_p, uniform, out)
+        _need(logits.get_device() == torch.cuda.current_device(), "kernel operands must live on the current GPU")
         n_rows, vocab = logits.shape
+        apart, beside = logits.stride()
         _need(1 <= vocab <= self.FILTERED_VOCAB, f"a row has 1 to {self.FILTERED_VOCAB} logits")
-        _need((vocab == 1 or logits.stride(1) == 1) and logits.stride(0) >= 0, "a row's logits lie side by side")
+        _need((vocab == 1 or beside == 1) and apart >= 0, "a row's logits lie side by side")
+        _need(n_rows <= 65535, "at most 65535 rows")
         for name, t in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("uniform", uniform)):
-            _need(t.dtype == torch.float32 and t.numel() == n_rows, f"{name} must be float32 [B]")
+            if t.dtype != torch.float32 or t.numel() != n_rows:
+                raise KernelError(f"{name} must be float32 [B]")
         _need(top_k.dtype == torch.int32 and top_k.numel() == n_rows, "top_k must be int32 [B]")
         if out is None:
             out = torch.empty(n_rows, dtype=torch.int32, device=logits.device)
         _need(out.dtype == torch.int32 and out.numel() == n_rows, "sample output must be int32 [B]")
-        _here(logits, temperature, top_k, top_p, min_p, uniform, out)
-        _need(n_rows <= 65535, "at most 65535 rows")
-        row_bytes = self.lib.ta_sample_filtered_workspace(vocab)
+        row_bytes = self._sample_bytes.get(vocab)
+        if row_bytes is None:
+            row_bytes = self._sample_bytes[vocab] = self._loaded.ta_sample_filtered_workspace(vocab)
         workspace = torch.empty(n_rows * row_bytes, dtype=torch.uint8, device=logits.device) if row_bytes else None
-        self._check(self.lib.ta_sample_filtered(_ptr(logits), ctypes.c_int64(logits.stride(0)), _ptr(temperature), _ptr(top_k), _ptr(top_p),
-                                                _ptr(min_p), _ptr(uniform), _ptr(out), _ptr(workspace), n_rows, vocab, _code(logits.dtype), self._stream()),
-                    "sample_filtered")
+        self._check(self.lib.ta_sample_filtered(
+            _address(logits), apart, _address(temperature), _address(top_k), _address(top_p), _address(min_p), _address(uniform), _address(out),
+            _address(workspace), n_rows, vocab, _code(logits.dtype), self._stream()), "sample_filtered")
         return out
 
     FILTERED_VOCAB = 1 << 19      # logits of a row that `sample_filtered` takes: so many weights' sum fits 63 bits
@@ -2469,17 +2493,18 @@ class Ops:
         widths[j] elements (up to four planes).  src, dst: int32 [n] on the device.  A page may be copied to several others; a page
         that is written is named once, and is no source (which of the two would win is not said).  A pair that names a page
         outside the pool is passed over."""
-        _dev(pages, src, dst)
+        _here(pages, src, dst)
         widths = tuple(int(w) for w in widths)
-        _need(1 <= len(widths) <= 4 and all(w >= 1 for w in widths), "one to four planes of at least one element a page")
+        _need(1 <= len(widths) <= 4 and min(widths) >= 1, "one to four planes of at least one element a page")
         _need(pages.dtype in _CODES and pages.dim() == 2 and n_pages >= 1 and pages.shape[1] == n_pages * sum(widths),
               "a pool is float32 or bfloat16 [layers, n_pages * sum(widths)]")
-        _need(1 <= pages.shape[0] <= 65535, "a pool has 1 to 65535 layers")
+        layers = pages.shape[0]
+        _need(1 <= layers <= 65535, "a pool has 1 to 65535 layers")
         _need(max(widths) * pages.element_size() < 2 ** 31, "a page's plane holds fewer than 2^31 bytes")
         _need(src.dtype == torch.int32 and dst.dtype == torch.int32 and src.dim() == 1 and src.shape == dst.shape, "src and dst must be int32 [n]")
-        _here(pages, src, dst)
-        if src.numel():
-            self._check(self.lib.ta_copy_pages(_ptr(pages), _ptr(src), _ptr(dst), src.numel(), n_pages, pages.shape[0], len(widths),
+        pairs = src.numel()
+        if pairs:
+            self._check(self.lib.ta_copy_pages(_address(pages), _address(src), _address(dst), pairs, n_pages, layers, len(widths),
                                                *(widths + (0, 0, 0))[:4], _code(pages.dtype), self._stream()), "copy_pages")
         return pages
 

@@ -146,8 +146,9 @@ class SharedPrefixes:
 
     def _on_device(self, packed: torch.Tensor) -> None:
         self.packed = packed
-        sizes = [8 * (self.n_few + self.n_many)] + [self.n_rows, 4 * self.n_rows, 4 * self.n_rows]
+        sizes = [8 * (self.n_few + self.n_many), self.n_rows, 4 * self.n_rows, 4 * self.n_rows]
         self.items, self.order_dev, self.own_dev, self.own_of_row_dev = torch.split(packed, sizes)
+        self.places = tuple(4 * sum(sizes[:i]) for i in range(4))           # in bytes from the start of `packed`
 
     @property
     def signature(self) -> tuple:
