@@ -78,7 +78,7 @@ def hills(rows, vocab, dtype, seed, spread=2.0):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocab", [1, 2, 63, 64, 65, 1000, 2049, 4096, 32003, 151936])
+@pytest.mark.parametrize("vocab", [1, 2, 63, 64, 65, 1000, 2048, 2049, 4096, 8192, 8193, 32003, 151936])
 def test_draws_over_vocabularies(ops, vocab, dtype):
     rows = 24 if vocab < 100000 else 6
     rng = np.random.default_rng(vocab)
@@ -170,11 +170,11 @@ def test_masked_rows(ops, vocab, masked):
         check_draws(ops, logits, uniform=uniform, **given)
 
 
-@pytest.mark.parametrize("vocab", [20481, 30000, 151936])
+@pytest.mark.parametrize("vocab", [8193, 20481, 30000, 151936])
 def test_draws_under_counts_around_those_of_the_waves(ops, vocab):
     # (A row in pieces of 4,096 logits has four waves a piece.)
     waves = 4 * -(-vocab // 4096)
-    counts = [1, 2, waves - 1, waves, waves + 1, 2 * waves, 1000, 8191, 8192, 8193, vocab - 1, vocab, vocab + 1]
+    counts = [1, 2, waves // 2, waves // 2 + 1, 8 * (vocab // 4096), 8 * (vocab // 4096) + 1, 1000, 8191, 8192, 8193, vocab - 1, vocab, vocab + 1]
     logits = hills(len(counts), vocab, torch.float32, 10)
     logits[3] = logits[3].sort().values                       # the largest side by side, at the end and at the start
     logits[4] = logits[4].sort(descending=True).values
@@ -202,6 +202,16 @@ def test_a_draw_does_not_depend_on_the_batch(ops):
     whole = ops.sample_filtered(logits, **numbers)
     for part in (slice(0, 1), slice(3, 10), slice(30, 70)):
         assert torch.equal(whole[part], ops.sample_filtered(logits[part], **{n: t[part].contiguous() for n, t in numbers.items()}))
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 40])
+def test_draws_of_few_and_many_long_rows(ops, rows):
+    # (Up to eight rows are gathered and drawn in one launch.)
+    logits = hills(rows, 50001, torch.float32, rows, 3.0)
+    rng = np.random.default_rng(rows)
+    for given in (dict(), dict(top_p=0.9), dict(top_k=30), dict(top_k=rng.integers(0, 2, rows) * 40, top_p=rng.uniform(0.5, 1.1, rows)),
+                  dict(temperature=rng.integers(0, 2, rows) * 1.0, top_p=0.8)):
+        check_draws(ops, logits, uniform=rng.uniform(0, 1, rows), **given)
 
 
 def test_draws_on_another_stream_and_replayed(ops):

@@ -30,11 +30,12 @@
 #define FS_EACH 16                      // logits a thread holds
 #define FS_PIECE (FS_THREADS * FS_EACH)
 #define FS_SHORT_THREADS 512            // of a short row's
-#define FS_SHORT_EACH 32
+#define FS_SHORT_EACH 16
 #define FS_BINS 256                     // four a lane
 #define FS_LIST 8192
 #define FS_FEW 128
 #define FS_SLOTS 256                    // ranges that a round of narrowing tells apart
+#define FS_FEW_ROWS 8                   // up to so many long rows are gathered and drawn in one launch
 #define FS_MAX_WAVES (FS_SHORT_THREADS / WAVE)
 #define FS_UNIT 17592186044416.0        // 2^44
 #define FS_REACH 31.3f                  // beyond so many T below the maximum a weight is less than half a unit: nothing
@@ -696,8 +697,8 @@ __device__ __forceinline__ FsAsked fs_asked(const FsArgs& a, int row) {
   return q;
 }
 
-// A row of at most FS_SHORT_THREADS * FS_SHORT_EACH logits: one workgroup, one launch.
-template <typename T>
+// A row of at most FS_SHORT_THREADS * EACH logits: one workgroup, one launch.
+template <typename T, int EACH>
 __global__ void __launch_bounds__(FS_SHORT_THREADS)
 sample_filtered_short(FsArgs a) {
   constexpr int THREADS = FS_SHORT_THREADS;
@@ -705,7 +706,7 @@ sample_filtered_short(FsArgs a) {
   const int row_at = blockIdx.x;
   const T* row = (const T*)a.logits + (size_t)row_at * a.stride;
   const FsAsked asked = fs_asked(a, row_at);
-  float v[FS_SHORT_EACH], high, low, of_wave, of_row;
+  float v[EACH], high, low, of_wave, of_row;
   int at;
   fs_load<THREADS>(row, 0, a.vocab, v);
   fs_extent<THREADS>(v, 0, high, at, low, of_wave, of_row, s);
@@ -721,7 +722,7 @@ sample_filtered_short(FsArgs a) {
   if (threadIdx.x == 0) s.n_listed = 0;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < FS_SHORT_EACH; ++j)
+  for (int j = 0; j < EACH; ++j)
     if (r.top - v[j] <= r.reach && ranges.has(fs_bin(v[j], r))) {
       const int place = atomicAdd(&s.n_listed, 1);
       if (place < FS_LIST) s.list[place] = (u64)fs_key(v[j]) << 32 | (uint32_t)~(uint32_t)(j * THREADS + (int)threadIdx.x);
@@ -736,7 +737,7 @@ sample_filtered_short(FsArgs a) {
 #define FS_PIECE_WAVES (FS_THREADS / WAVE)
 #define FS_PIECE_ROWS (FS_THREADS / 16)
 struct FsExtent { float high, low; int at, unused; };
-struct FsHead { int n_listed; int ranges[5]; int unused[2]; u64 over; u64 unused2; };      // of a row
+struct FsHead { int n_listed; int ranges[5]; int came; int unused; u64 over; u64 unused2; };      // of a row
 struct FsBinned { u64 mass[FS_BINS]; uint32_t count[FS_BINS]; u64 over; u64 unused; };    // of a piece, or of a row
 // Per row: its head, its bins, its list, the pieces' extents, the maxima of their waves and of these waves' rows of sixteen lanes, and the
 // pieces' bins.
@@ -779,9 +780,12 @@ __device__ __forceinline__ int fs_row_top(const FsSpace& w, float high) {
   return at == 0x7fffffff ? 0 : at;
 }
 
-// Whether a row's list can be made without its bins.
-__device__ __forceinline__ bool fs_listed_at_once(const FsAsked& asked, int pieces) {
-  return (asked.top_k > 0 && asked.top_k <= pieces * FS_PIECE_ROWS) || (!(asked.top_p < 1.f) && asked.min_p > 0.f);
+// How many maxima of rows of sixteen lanes stand for 256 logits each.
+__device__ __forceinline__ int fs_full_maxima(int vocab) { return vocab / FS_PIECE * FS_PIECE_ROWS; }
+// Whether a row's list can be made without its bins.  (Half as many tokens as maxima at most: the list is then about
+// k long; close to their number it would be several times as long.)
+__device__ __forceinline__ bool fs_listed_at_once(const FsAsked& asked, int vocab) {
+  return (asked.top_k > 0 && 2 * asked.top_k <= fs_full_maxima(vocab)) || (!(asked.top_p < 1.f) && asked.min_p > 0.f);
 }
 
 // A logit not below `least` of which at least k of the `count` maxima are no smaller, close to the k-th largest of them; -inf if there are
@@ -814,10 +818,10 @@ __device__ __forceinline__ float fs_cut_of_maxima(const float* __restrict__ maxi
 //   top-k: at least k of the maxima are no smaller; found by halving between the largest and the smallest logit that weighs
 //   anything, and what the halvings leave undecided stays above the cut.
 //   min-p (where top-p cuts nothing): max + T ln(min_p), less what 32 bits may be off by: 4 roundings of each of its parts.
-__device__ __forceinline__ float fs_cut(const FsSpace& w, const FsAsked& asked, const FsRow& r, float low) {
+__device__ __forceinline__ float fs_cut(const FsSpace& w, const FsAsked& asked, const FsRow& r, float low, int vocab) {
   const float high = r.top;
   float cut = -INFINITY;
-  if (asked.top_k > 0 && asked.top_k <= w.pieces * FS_PIECE_ROWS) {
+  if (asked.top_k > 0 && 2 * asked.top_k <= fs_full_maxima(vocab)) {
     const float least = fmaxf(low, high - r.reach);        // (what lies further below weighs nothing)
     // Few maxima while k is small beside their number (k = 40 of 152: some 50 tokens are no smaller; 150 of them: 700).
     cut = 2 * asked.top_k <= w.pieces * FS_PIECE_WAVES ? fs_cut_of_maxima<8>(w.of_waves(), w.pieces * FS_PIECE_WAVES, asked.top_k, least, high)
@@ -886,7 +890,7 @@ sample_filtered_extents(FsArgs a) {
     e.high = high;
     e.low = low;
     e.at = at;
-    if (blockIdx.x == 0) w.head()->n_listed = 0;
+    if (blockIdx.x == 0) { w.head()->n_listed = 0; w.head()->came = 0; }
   }
 }
 
@@ -902,10 +906,10 @@ sample_filtered_bins(FsArgs a) {
   fs_row_extent(w, high, low);
   if (!fs_is_drawn(asked.temperature, high)) return;
   const FsRow r = fs_row(asked.temperature, high, low);
-  if (fs_listed_at_once(asked, a.pieces)) {
+  if (fs_listed_at_once(asked, a.vocab)) {
     // (One wave works it out: eight halvings among six hundred maxima by every wave of 2,432 workgroups took 14 us of their time.)
     if (threadIdx.x < WAVE) {
-      const float found = fs_cut(w, asked, r, low);
+      const float found = fs_cut(w, asked, r, low, a.vocab);
       if (threadIdx.x == 0) s.cut = found;
     }
     __syncthreads();
@@ -936,7 +940,7 @@ sample_filtered_settle(FsArgs a) {
     if (threadIdx.x == 0) a.out[row_at] = at;
     return;
   }
-  if (fs_listed_at_once(asked, a.pieces)) {
+  if (fs_listed_at_once(asked, a.vocab)) {
     const int n = w.head()->n_listed;
     for (int i = threadIdx.x; i < min(n, FS_LIST); i += FS_THREADS) s.list[i] = w.list()[i];
     const int pick = fs_draw<FS_THREADS>(s, (const T*)a.logits + (size_t)row_at * a.stride, a.vocab, fs_row(asked.temperature, high, low), asked,
@@ -979,34 +983,25 @@ __device__ __forceinline__ FsRanges fs_kept_ranges(const FsSpace& w) {
   return FsRanges{scalar_int(kept), scalar_int(kept + 1), scalar_int(kept + 2), scalar_int(kept + 3), scalar_int(kept + 4)};
 }
 
+// The piece's tokens in the ranges, to the row's list.  False (for the whole workgroup) for a row that needs none.
 template <typename T>
-__global__ void __launch_bounds__(FS_THREADS)
-sample_filtered_gather(FsArgs a) {
-  __shared__ FsSmall s;
-  const FsSpace w = fs_space(a, blockIdx.y);
-  const FsAsked asked = fs_asked(a, blockIdx.y);
-  if (fs_listed_at_once(asked, a.pieces)) return;
+__device__ __forceinline__ bool fs_gather(const FsArgs& a, const FsSpace& w, const FsAsked& asked, FsSmall& s) {
+  if (fs_listed_at_once(asked, a.vocab)) return false;
   float v[FS_EACH], high, low;
   fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v);
   fs_row_extent(w, high, low);
-  if (!fs_is_drawn(asked.temperature, high)) return;
+  if (!fs_is_drawn(asked.temperature, high)) return false;
   const FsRow r = fs_row(asked.temperature, high, low);
   const FsRanges ranges = fs_kept_ranges(w);
   fs_append(w, v, s, [&](float x) { return r.top - x <= r.reach && ranges.has(fs_bin(x, r)); });
+  return true;
 }
 
+// The draw of a row whose list has been gathered, `n` tokens.
 template <typename T>
-__global__ void __launch_bounds__(FS_THREADS)
-sample_filtered_draw(FsArgs a) {
-  __shared__ FsShared s;
-  const int row_at = blockIdx.x;
-  const FsSpace w = fs_space(a, row_at);
-  const FsAsked asked = fs_asked(a, row_at);
-  if (fs_listed_at_once(asked, a.pieces)) return;
+__device__ __forceinline__ void fs_draw_gathered(const FsArgs& a, const FsSpace& w, const FsAsked& asked, int row_at, int n, FsShared& s) {
   float high, low;
   fs_row_extent(w, high, low);
-  if (!fs_is_drawn(asked.temperature, high)) return;
-  const int n = w.head()->n_listed;
   s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x];
   s.count[threadIdx.x] = w.whole()->count[threadIdx.x];
   for (int i = threadIdx.x; i < min(n, FS_LIST); i += FS_THREADS) s.list[i] = w.list()[i];
@@ -1016,6 +1011,47 @@ sample_filtered_draw(FsArgs a) {
   const int pick = fs_draw<FS_THREADS>(s, (const T*)a.logits + (size_t)row_at * a.stride, a.vocab, fs_row(asked.temperature, high, low), asked,
                                        &ranges, over, n);
   if (threadIdx.x == 0) a.out[row_at] = pick;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(FS_THREADS)
+sample_filtered_gather(FsArgs a) {
+  __shared__ FsSmall s;
+  fs_gather<T>(a, fs_space(a, blockIdx.y), fs_asked(a, blockIdx.y), s);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(FS_THREADS)
+sample_filtered_draw(FsArgs a) {
+  __shared__ FsShared s;
+  const FsSpace w = fs_space(a, blockIdx.x);
+  const FsAsked asked = fs_asked(a, blockIdx.x);
+  float high, low;
+  fs_row_extent(w, high, low);
+  if (fs_listed_at_once(asked, a.vocab) || !fs_is_drawn(asked.temperature, high)) return;
+  fs_draw_gathered<T>(a, w, asked, blockIdx.x, w.head()->n_listed, s);
+}
+
+// Both in one launch: the workgroup that comes last in its row finds the whole list there and draws.  (Nobody waits: each leaves its
+// tokens, then counts itself in.)  For few rows, where a launch counts; the draw's LDS lets one workgroup onto a compute unit.
+template <typename T>
+__global__ void __launch_bounds__(FS_THREADS)
+sample_filtered_gather_draw(FsArgs a) {
+  __shared__ FsShared s;
+  __shared__ int came;
+  const FsSpace w = fs_space(a, blockIdx.y);
+  const FsAsked asked = fs_asked(a, blockIdx.y);
+  if (!fs_gather<T>(a, w, asked, s)) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {                                  // (one thread's fences, between barriers, stand for the workgroup's)
+    __threadfence();                                       // the tokens are there for all that see the count
+    came = atomicAdd(&w.head()->came, 1);
+    __threadfence();                                       // and so is what the others left before they counted themselves in
+  }
+  __syncthreads();
+  if (came != a.pieces - 1) return;                        // (the same for the whole workgroup)
+  const int n = __hip_atomic_load(&w.head()->n_listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  fs_draw_gathered<T>(a, w, asked, blockIdx.y, n, s);
 }
 
 #define FS_MAX_VOCAB (1 << 19)
@@ -1031,7 +1067,10 @@ extern "C" int ta_sample_filtered_workspace(int vocab) { return fs_is_short(voca
 template <typename T>
 static int launch_filtered(FsArgs a, int n_rows, hipStream_t stream) {
   if (fs_is_short(a.vocab)) {
-    sample_filtered_short<T><<<n_rows, FS_SHORT_THREADS, 0, stream>>>(a);
+    if (a.vocab <= FS_SHORT_THREADS * FS_SHORT_EACH / 4)
+      sample_filtered_short<T, FS_SHORT_EACH / 4><<<n_rows, FS_SHORT_THREADS, 0, stream>>>(a);
+    else
+      sample_filtered_short<T, FS_SHORT_EACH><<<n_rows, FS_SHORT_THREADS, 0, stream>>>(a);
     return LAUNCH_STATUS();
   }
   const dim3 grid(a.pieces, n_rows);
@@ -1044,6 +1083,10 @@ static int launch_filtered(FsArgs a, int n_rows, hipStream_t stream) {
   sample_filtered_settle<T><<<n_rows, FS_THREADS, 0, stream>>>(a);
   status = LAUNCH_STATUS();
   if (status) return status;
+  if (n_rows <= FS_FEW_ROWS) {
+    sample_filtered_gather_draw<T><<<grid, FS_THREADS, 0, stream>>>(a);
+    return LAUNCH_STATUS();
+  }
   sample_filtered_gather<T><<<grid, FS_THREADS, 0, stream>>>(a);
   status = LAUNCH_STATUS();
   if (status) return status;
