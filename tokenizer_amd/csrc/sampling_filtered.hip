@@ -12,7 +12,7 @@
 // by 2^-45 of the row's largest at most: 32-bit weights would move the border between two tokens of a flat row of 150,000 by a good
 // part of a token.  Tokens that weigh nothing then (31.2 T below the maximum) are never drawn.
 //
-// No row is sorted whole: the tokens among which the answers lie, some hundreds, are gathered and sorted in LDS.
+// No row is sorted whole: the tokens among which the answers lie, some hundreds, are gathered and ordered in LDS.
 //   * Where the first k tokens are all that counts, or those that min-p keeps, a logit is known below which nothing does
 //     (`fs_cut`): the k-th largest of the maxima of the row's parts, of which at least k tokens are no smaller, or
 //     max + T ln(min_p).  What is not below it is the list.
@@ -35,7 +35,7 @@
 #define FS_LIST 8192
 #define FS_FEW 128
 #define FS_SLOTS 256                    // ranges that a round of narrowing tells apart
-#define FS_FEW_ROWS 8                   // up to so many long rows are gathered and drawn in one launch
+#define FS_FEW_ROWS 8                   // up to so many long rows take three launches instead of five
 #define FS_MAX_WAVES (FS_SHORT_THREADS / WAVE)
 #define FS_UNIT 17592186044416.0        // 2^44
 #define FS_REACH 31.3f                  // beyond so many T below the maximum a weight is less than half a unit: nothing
@@ -840,7 +840,7 @@ sample_filtered_short(FsArgs a) {
 #define FS_PIECE_WAVES (FS_THREADS / WAVE)
 #define FS_PIECE_ROWS (FS_THREADS / 16)
 struct FsExtent { float high, low; int at, unused; };
-struct FsHead { int n_listed; int ranges[5]; int came; int unused; u64 over; u64 unused2; };      // of a row
+struct FsHead { int n_listed; int ranges[5]; int gathered, unused; u64 over, unused2; };      // of a row; `gathered`: pieces that are
 struct FsBinned { u64 mass[FS_BINS]; uint32_t count[FS_BINS]; u64 over; u64 unused; };    // of a piece, or of a row
 // Per row: its head, its bins, its list, the pieces' extents, the maxima of their waves and of these waves' rows of sixteen lanes, and the
 // pieces' bins.
@@ -888,7 +888,7 @@ __device__ __forceinline__ int fs_full_maxima(int vocab) { return vocab / FS_PIE
 // Whether a row's list can be made without its bins.  (Half as many tokens as maxima at most: the list is then about
 // k long; close to their number it would be several times as long.)
 __device__ __forceinline__ bool fs_listed_at_once(const FsAsked& asked, int vocab) {
-  return (asked.top_k > 0 && 2 * asked.top_k <= fs_full_maxima(vocab)) || (!(asked.top_p < 1.f) && asked.min_p > 0.f);
+  return (asked.top_k > 0 && asked.top_k <= fs_full_maxima(vocab) / 2) || (!(asked.top_p < 1.f) && asked.min_p > 0.f);
 }
 
 // A logit not below `least` of which at least k of the `count` maxima are no smaller, close to the k-th largest of them; -inf if there are
@@ -924,7 +924,7 @@ __device__ __forceinline__ float fs_cut_of_maxima(const float* __restrict__ maxi
 __device__ __forceinline__ float fs_cut(const FsSpace& w, const FsAsked& asked, const FsRow& r, float low, int vocab) {
   const float high = r.top;
   float cut = -INFINITY;
-  if (asked.top_k > 0 && 2 * asked.top_k <= fs_full_maxima(vocab)) {
+  if (asked.top_k > 0 && asked.top_k <= fs_full_maxima(vocab) / 2) {
     const float least = fmaxf(low, high - r.reach);        // (what lies further below weighs nothing)
     // Few maxima while k is small beside their number (k = 40 of 152: some 50 tokens are no smaller; 150 of them: 700).
     cut = 2 * asked.top_k <= w.pieces * FS_PIECE_WAVES ? fs_cut_of_maxima<8>(w.of_waves(), w.pieces * FS_PIECE_WAVES, asked.top_k, least, high)
@@ -993,7 +993,7 @@ sample_filtered_extents(FsArgs a) {
     e.high = high;
     e.low = low;
     e.at = at;
-    if (blockIdx.x == 0) { w.head()->n_listed = 0; w.head()->came = 0; }
+    if (blockIdx.x == 0) { w.head()->n_listed = w.head()->gathered = 0; }
   }
 }
 
@@ -1037,7 +1037,55 @@ sample_filtered_bins(FsArgs a) {
 }
 static_assert(FS_THREADS == FS_BINS, "a thread a bin");
 
-// A row whose list is there: its draw.  Another: its bins, and the ranges of them in which the answers lie.
+// The row's bins from its pieces', into `s`; the weight of what min-p keeps; and the ranges of bins in which the answers lie.
+__device__ __forceinline__ FsRanges fs_settle(const FsSpace& w, const FsAsked& asked, u64& over, FsSmall& s) {
+  u64 m = 0;
+  uint32_t c = 0;
+  over = 0;
+  for (int first = 0; first < w.pieces; first += 16) {     // (sixteen pieces asked for at a time)
+    u64 of_mass[16];
+    uint32_t of_count[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const FsBinned& piece = w.binned()[min(first + j, w.pieces - 1)];
+      of_mass[j] = piece.mass[threadIdx.x];
+      of_count[j] = piece.count[threadIdx.x];
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (first + j < w.pieces) { m += of_mass[j]; c += of_count[j]; }
+  }
+  for (int p = threadIdx.x; p < w.pieces; p += FS_THREADS) over += w.binned()[p].over;
+  s.mass[threadIdx.x] = m;
+  s.count[threadIdx.x] = c;
+  over = fs_sum<FS_THREADS>(over, s);
+  FsRunning run;
+  run.of(s);
+  return fs_ranges(run, asked, over);
+}
+
+// The draw from the row's list in the workspace, `n` tokens; `ranges` as in fs_draw.
+template <typename T>
+__device__ __forceinline__ void fs_draw_listed(const FsArgs& a, const FsSpace& w, const FsAsked& asked, const FsRow& r, int row_at,
+                                               const FsRanges* ranges, u64 over, int n, FsShared& s) {
+  for (int i = threadIdx.x; i < min(n, FS_LIST); i += FS_THREADS) s.list[i] = w.list()[i];
+  __syncthreads();
+  const int pick = fs_draw<FS_THREADS>(s, (const T*)a.logits + (size_t)row_at * a.stride, a.vocab, r, asked, ranges, over, n);
+  if (threadIdx.x == 0) a.out[row_at] = pick;
+}
+
+// The piece's tokens in the ranges, to the row's list.
+template <typename T>
+__device__ __forceinline__ void fs_gather(const FsArgs& a, const FsSpace& w, const FsRow& r, const FsRanges& ranges, FsSmall& s) {
+  const float of_row = w.of_rows()[blockIdx.x * FS_PIECE_ROWS + threadIdx.x / 16];
+  float v[FS_EACH];
+  // (A row of sixteen lanes whose maximum lies behind all the ranges has nothing in them.)
+  const bool wanted = r.top - of_row <= r.reach && fs_bin(of_row, r) <= max(ranges.k_bin, max(ranges.p_last, ranges.draw_last));
+  fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v, wanted);
+  fs_append(w, v, s, [&](float x) { return r.top - x <= r.reach && ranges.has(fs_bin(x, r)); });
+}
+
+// Many rows.  A row whose list is there: its draw.  Another: its bins and ranges, left for its pieces, which gather; and its draw.
 template <typename T>
 __global__ void __launch_bounds__(FS_THREADS)
 sample_filtered_settle(FsArgs a) {
@@ -1053,35 +1101,13 @@ sample_filtered_settle(FsArgs a) {
     return;
   }
   if (fs_listed_at_once(asked, a.vocab)) {
-    const int n = w.head()->n_listed;
-    for (int i = threadIdx.x; i < min(n, FS_LIST); i += FS_THREADS) s.list[i] = w.list()[i];
-    const int pick = fs_draw<FS_THREADS>(s, (const T*)a.logits + (size_t)row_at * a.stride, a.vocab, fs_row(asked.temperature, high, low), asked,
-                                         nullptr, 0, n);
-    if (threadIdx.x == 0) a.out[row_at] = pick;
+    fs_draw_listed<T>(a, w, asked, fs_row(asked.temperature, high, low), row_at, nullptr, 0, w.head()->n_listed, s);
     return;
   }
-  u64 m = 0, over = 0;
-  uint32_t c = 0;
-  for (int first = 0; first < a.pieces; first += 16) {     // (sixteen pieces asked for at a time)
-    u64 of_mass[16];
-    uint32_t of_count[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const FsBinned& piece = w.binned()[min(first + j, a.pieces - 1)];
-      of_mass[j] = piece.mass[threadIdx.x];
-      of_count[j] = piece.count[threadIdx.x];
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (first + j < a.pieces) { m += of_mass[j]; c += of_count[j]; }
-  }
-  for (int p = threadIdx.x; p < a.pieces; p += FS_THREADS) over += w.binned()[p].over;
-  s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x] = m;
-  s.count[threadIdx.x] = w.whole()->count[threadIdx.x] = c;
-  over = fs_sum<FS_THREADS>(over, s);
-  FsRunning run;
-  run.of(s);
-  const FsRanges ranges = fs_ranges(run, asked, over);
+  u64 over;
+  const FsRanges ranges = fs_settle(w, asked, over, s);
+  w.whole()->mass[threadIdx.x] = s.mass[threadIdx.x];
+  w.whole()->count[threadIdx.x] = s.count[threadIdx.x];
   if (threadIdx.x == 0) {
     FsHead& head = *w.head();
     head.ranges[0] = ranges.k_bin; head.ranges[1] = ranges.p_first; head.ranges[2] = ranges.p_last;
@@ -1095,44 +1121,16 @@ __device__ __forceinline__ FsRanges fs_kept_ranges(const FsSpace& w) {
   return FsRanges{scalar_int(kept), scalar_int(kept + 1), scalar_int(kept + 2), scalar_int(kept + 3), scalar_int(kept + 4)};
 }
 
-// The piece's tokens in the ranges, to the row's list.  False (for the whole workgroup) for a row that needs none.
-template <typename T>
-__device__ __forceinline__ bool fs_gather(const FsArgs& a, const FsSpace& w, const FsAsked& asked, FsSmall& s) {
-  if (fs_listed_at_once(asked, a.vocab)) return false;
-  const float of_row = w.of_rows()[blockIdx.x * FS_PIECE_ROWS + threadIdx.x / 16];
-  float v[FS_EACH], high, low;
-  fs_row_extent(w, high, low);
-  if (!fs_is_drawn(asked.temperature, high)) return false;
-  const FsRow r = fs_row(asked.temperature, high, low);
-  const FsRanges ranges = fs_kept_ranges(w);
-  // (A row of sixteen lanes whose maximum lies behind all the ranges has nothing in them.)
-  const bool wanted = r.top - of_row <= r.reach && fs_bin(of_row, r) <= max(ranges.k_bin, max(ranges.p_last, ranges.draw_last));
-  fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v, wanted);
-  fs_append(w, v, s, [&](float x) { return r.top - x <= r.reach && ranges.has(fs_bin(x, r)); });
-  return true;
-}
-
-// The draw of a row whose list has been gathered, `n` tokens.
-template <typename T>
-__device__ __forceinline__ void fs_draw_gathered(const FsArgs& a, const FsSpace& w, const FsAsked& asked, int row_at, int n, FsShared& s) {
-  float high, low;
-  fs_row_extent(w, high, low);
-  s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x];
-  s.count[threadIdx.x] = w.whole()->count[threadIdx.x];
-  for (int i = threadIdx.x; i < min(n, FS_LIST); i += FS_THREADS) s.list[i] = w.list()[i];
-  const u64 over = w.head()->over;
-  const FsRanges ranges = fs_kept_ranges(w);
-  __syncthreads();
-  const int pick = fs_draw<FS_THREADS>(s, (const T*)a.logits + (size_t)row_at * a.stride, a.vocab, fs_row(asked.temperature, high, low), asked,
-                                       &ranges, over, n);
-  if (threadIdx.x == 0) a.out[row_at] = pick;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(FS_THREADS)
 sample_filtered_gather(FsArgs a) {
   __shared__ FsSmall s;
-  fs_gather<T>(a, fs_space(a, blockIdx.y), fs_asked(a, blockIdx.y), s);
+  const FsSpace w = fs_space(a, blockIdx.y);
+  const FsAsked asked = fs_asked(a, blockIdx.y);
+  float high, low;
+  fs_row_extent(w, high, low);
+  if (fs_listed_at_once(asked, a.vocab) || !fs_is_drawn(asked.temperature, high)) return;
+  fs_gather<T>(a, w, fs_row(asked.temperature, high, low), fs_kept_ranges(w), s);
 }
 
 template <typename T>
@@ -1144,29 +1142,50 @@ sample_filtered_draw(FsArgs a) {
   float high, low;
   fs_row_extent(w, high, low);
   if (fs_listed_at_once(asked, a.vocab) || !fs_is_drawn(asked.temperature, high)) return;
-  fs_draw_gathered<T>(a, w, asked, blockIdx.x, w.head()->n_listed, s);
+  s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x];
+  s.count[threadIdx.x] = w.whole()->count[threadIdx.x];
+  const FsRanges ranges = fs_kept_ranges(w);
+  fs_draw_listed<T>(a, w, asked, fs_row(asked.temperature, high, low), blockIdx.x, &ranges, w.head()->over, w.head()->n_listed, s);
 }
 
-// Both in one launch: the workgroup that comes last in its row finds the whole list there and draws.  (Nobody waits: each leaves its
-// tokens, then counts itself in.)  For few rows, where a launch counts; the draw's LDS lets one workgroup onto a compute unit.
+// Few rows, where a launch counts: every piece's workgroup adds the row's bins up for itself, gathers, and the one that comes last in its row
+// finds the whole list there and draws.  (Nobody waits: each leaves its tokens, then counts itself in.)  The draw's LDS lets one
+// workgroup onto a compute unit.
 template <typename T>
 __global__ void __launch_bounds__(FS_THREADS)
-sample_filtered_gather_draw(FsArgs a) {
+sample_filtered_finish(FsArgs a) {
   __shared__ FsShared s;
   __shared__ int came;
-  const FsSpace w = fs_space(a, blockIdx.y);
-  const FsAsked asked = fs_asked(a, blockIdx.y);
-  if (!fs_gather<T>(a, w, asked, s)) return;
+  const int row_at = blockIdx.y;
+  const FsSpace w = fs_space(a, row_at);
+  const FsAsked asked = fs_asked(a, row_at);
+  const bool listed = fs_listed_at_once(asked, a.vocab);
+  if (listed && blockIdx.x > 0) return;
+  float high, low;
+  fs_row_extent(w, high, low);
+  if (!fs_is_drawn(asked.temperature, high)) {
+    const int at = fs_row_top(w, high);
+    if (threadIdx.x == 0 && blockIdx.x == 0) a.out[row_at] = at;
+    return;
+  }
+  const FsRow r = fs_row(asked.temperature, high, low);
+  if (listed) {
+    fs_draw_listed<T>(a, w, asked, r, row_at, nullptr, 0, w.head()->n_listed, s);
+    return;
+  }
+  u64 over;
+  const FsRanges ranges = fs_settle(w, asked, over, s);
+  fs_gather<T>(a, w, r, ranges, s);
   __syncthreads();
   if (threadIdx.x == 0) {                                  // (one thread's fences, between barriers, stand for the workgroup's)
     __threadfence();                                       // the tokens are there for all that see the count
-    came = atomicAdd(&w.head()->came, 1);
+    came = atomicAdd(&w.head()->gathered, 1);
     __threadfence();                                       // and so is what the others left before they counted themselves in
   }
   __syncthreads();
   if (came != a.pieces - 1) return;                        // (the same for the whole workgroup)
   const int n = __hip_atomic_load(&w.head()->n_listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  fs_draw_gathered<T>(a, w, asked, blockIdx.y, n, s);
+  fs_draw_listed<T>(a, w, asked, r, row_at, &ranges, over, n, s);
 }
 
 #define FS_MAX_VOCAB (1 << 19)
@@ -1195,13 +1214,13 @@ static int launch_filtered(FsArgs a, int n_rows, hipStream_t stream) {
   sample_filtered_bins<T><<<grid, FS_THREADS, 0, stream>>>(a);
   status = LAUNCH_STATUS();
   if (status) return status;
+  if (n_rows <= FS_FEW_ROWS) {
+    sample_filtered_finish<T><<<grid, FS_THREADS, 0, stream>>>(a);
+    return LAUNCH_STATUS();
+  }
   sample_filtered_settle<T><<<n_rows, FS_THREADS, 0, stream>>>(a);
   status = LAUNCH_STATUS();
   if (status) return status;
-  if (n_rows <= FS_FEW_ROWS) {
-    sample_filtered_gather_draw<T><<<grid, FS_THREADS, 0, stream>>>(a);
-    return LAUNCH_STATUS();
-  }
   sample_filtered_gather<T><<<grid, FS_THREADS, 0, stream>>>(a);
   status = LAUNCH_STATUS();
   if (status) return status;
