@@ -902,7 +902,7 @@ shared_prefix_join(SharedArgs a, T* __restrict__ out) {
   const int* mine = reinterpret_cast<const int*>(a.own_of_row + row);
   const int begin = scalar_int(mine + 1), shared = scalar_int(mine + 2);
   const int own = min(scalar_int(a.positions + row), a.table_stride * a.page_size - 1) + 1 - begin;
-  const int parts = min(a.slots, shared + (own > 0 ? (own + a.own_keys - 1) / a.own_keys : 0));
+  const int parts = shared + (own > 0 ? min((own + a.own_keys - 1) / a.own_keys, a.own_splits) : 0);      // (a.slots at most)
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)at * a.slots;
   const float* part = a.part_o + (size_t)at * a.slots * D;
   const float sink = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;

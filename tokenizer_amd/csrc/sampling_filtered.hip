@@ -22,6 +22,15 @@
 // Should there be more than FS_LIST of them (thousands of equal logits), one workgroup goes through the row again and again and
 // narrows the answer's range by counting, key by key.
 //
+// What bounds it, measured with logits of 32 bits in the caches (the operator's own launches, replayed):
+//   one row of 152,064 under top-k 40: 14.6 us, a chain of three launches (extents 3.6, the list 6.0, the draw 6.0 with the profiler's
+//     share), each a few dependent steps of one workgroup a piece; reading 0.6 MB would take 0.1.  Under top-p alone 22.
+//   64 rows of 152,064, each under other limits: 31 us: the extents 8.8, the second reading 11.5 (weights in 64 bits where the bins are
+//     needed), ordering the lists 9.2, the gathering and the draws 4.6.
+//   256 rows of 152,064 under min-p: 53 us: the extents 25 (156 MB at 6.2 TB/s), the list 13, the draw 9; a row read once at the rate of a
+//     large copy would take 31.  Under top-p alone, where every token's weight and bin is worked out, 134.
+// A workgroup has 4,096 logits, sixteen a thread, all asked for at once; a single row is then 38 workgroups.
+//
 // NaN is no token.  A row without a finite maximum, and a row whose temperature is not positive, gets its first maximum (0 if it
 // holds no number).
 #include "common.h"
@@ -572,8 +581,8 @@ __device__ __forceinline__ int fs_answers(FsShared& s, const FsRow& r, const FsA
   return s.found;
 }
 
-// Up to FS_FEW tokens: each is held against all others, THREADS / FS_FEW threads a token (64 tokens in 0.3 us, 128 in 0.9, where
-// sorting takes 2 and 2.6).
+// Up to FS_FEW tokens: each is held against all others, two to eight threads a token.  (A draw under top-k 40 from 152,064
+// logits 14.6 us so, 15.8 by fs_spread; four rows of 1,000 logits 9.0 and 10.2.)
 template <int THREADS>
 __device__ __forceinline__ int fs_answers_of_few(FsShared& s, const FsRow& r, const FsAsked& asked, u64 all, bool k_here, u64 over, bool all_listed,
                                                  int n) {

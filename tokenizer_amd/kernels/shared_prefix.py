@@ -71,6 +71,7 @@ class SharedPrefixes:
     MIN_KEYS = 64                 # a shorter run is not worth a pass and a part to be joined of its own
     MIN_PART = 128                # keys of a part of a run, at least (a block of 32 for each of its four waves)
     MIN_WIDE_PART = 256
+    OWN_STEP = 128                # `smallest_own` in whole steps: prefixes that differ a little make launches of one shape
     TARGET = 512                  # workgroups that the parts aim at: two a compute unit
 
     def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device,
@@ -114,7 +115,7 @@ class SharedPrefixes:
         self.shared_parts = int(parts_of.max(initial=0))
         self.own_begin = own_begin                        # int32 [B] on the host
         self.keys_end = max((run.key_end for run in self.runs), default=0)
-        self.smallest_own = int(own_begin.min(initial=0)) if self.n_rows else 0
+        self.smallest_own = int(own_begin.min()) // self.OWN_STEP * self.OWN_STEP if self.n_rows else 0
         rows = np.arange(self.n_rows, dtype=np.int32)
         own = np.stack([rows, own_begin, parts_of, np.zeros_like(rows)], axis=1).astype(np.int32)
         packed = np.concatenate([np.asarray(items[False] + items[True], dtype=np.int32).reshape(-1), np.asarray(self.order, dtype=np.int32),
