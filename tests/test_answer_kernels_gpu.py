@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from tokenizer_amd.kernels import KernelError
+from tokenizer_amd.kernels.shared_prefix import SharedPrefixes
 
 pytestmark = pytest.mark.gpu
 
@@ -399,6 +400,14 @@ class Batch:
                 assert off <= 1.0, f"request {r} at {p}, kv head {g}: {off} of the bound"
 
 
+@pytest.fixture(params=["as planned", "many columns"])
+def any_work(request, monkeypatch):
+    """As the plan's rule says for the (small) batches of these tests, and with the items of many columns that larger ones get."""
+    if request.param == "many columns":
+        monkeypatch.setattr(SharedPrefixes, "WIDE_WORK", -1)
+        monkeypatch.setattr(SharedPrefixes, "MANY_WORK", -1)
+
+
 def shared_tables(rows, prefix_pages, page, own, branch=None):
     """`rows` requests behind `prefix_pages` common pages, request r with own[r] keys of its own; branch: (every, pages)."""
     used, tables, positions = prefix_pages, [], []
@@ -421,7 +430,7 @@ def shared_tables(rows, prefix_pages, page, own, branch=None):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128, 160, 192, 224, 256])
-def test_attention_over_head_sizes(ops, d, dtype):
+def test_attention_over_head_sizes(ops, any_work, d, dtype):
     tables, positions = shared_tables(6, 11, 16, [1, 5, 16, 17, 40, 70])
     batch = Batch(tables, positions, 6, 2, d, 16, dtype, d)
     got, plan = batch.run(ops)
@@ -431,7 +440,7 @@ def test_attention_over_head_sizes(ops, d, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n_q,n_kv", [(1, 1), (14, 2), (4, 4), (7, 1), (33, 1), (64, 2), (70, 1)])
-def test_attention_over_heads(ops, n_q, n_kv, dtype):
+def test_attention_over_heads(ops, any_work, n_q, n_kv, dtype):
     tables, positions = shared_tables(11, 9, 16, [3 * r + 1 for r in range(11)])
     batch = Batch(tables, positions, n_q, n_kv, 64, 16, dtype, n_q)
     batch.check(batch.run(ops)[0])
@@ -440,7 +449,7 @@ def test_attention_over_heads(ops, n_q, n_kv, dtype):
 @pytest.mark.parametrize("page", [16, 32, 48, 64])
 @pytest.mark.parametrize("prefix_keys", [0, 48, 64, 192, 960, 2880])
 @pytest.mark.parametrize("rows", [2, 5, 40])
-def test_attention_over_lengths(ops, rows, prefix_keys, page):
+def test_attention_over_lengths(ops, any_work, rows, prefix_keys, page):
     prefix = prefix_keys // page
     tables, positions = shared_tables(rows, prefix, page, [1 + (37 * r) % 150 for r in range(rows)])
     batch = Batch(tables, positions, 14, 2, 64, page, torch.bfloat16, rows + prefix)
@@ -450,7 +459,8 @@ def test_attention_over_lengths(ops, rows, prefix_keys, page):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("rows,n_q,n_kv", [(33, 2, 1), (13, 14, 2), (19, 28, 4), (60, 12, 2), (129, 1, 1), (40, 40, 1)])
 @pytest.mark.parametrize("keys,page", [(64, 16), (80, 16), (1008, 16), (96, 32), (1056, 48), (1600, 64)])
-def test_attention_of_many_columns(ops, keys, page, rows, n_q, n_kv, d):
+def test_attention_of_many_columns(ops, monkeypatch, keys, page, rows, n_q, n_kv, d):
+    monkeypatch.setattr(SharedPrefixes, "WIDE_WORK", -1)
     # (More than 64 query columns of a kv head go through the shared keys together; parts and blocks of them end anywhere.)
     tables, positions = shared_tables(rows, keys // page, page, [1 + (13 * r) % 40 for r in range(rows)])
     batch = Batch(tables, positions, n_q, n_kv, d, page, torch.bfloat16, rows + keys)
@@ -459,8 +469,20 @@ def test_attention_of_many_columns(ops, keys, page, rows, n_q, n_kv, d):
     batch.check(got)
 
 
+@pytest.mark.parametrize("n_q,n_kv,d,dtype,rows,keys", [(14, 2, 64, torch.bfloat16, 40, 12048), (14, 2, 64, torch.float32, 64, 24000),
+                                                        (14, 2, 64, torch.float32, 104, 24000),
+                                                        (14, 2, 96, torch.bfloat16, 100, 16000)])
+def test_attention_with_work_for_many_columns(ops, n_q, n_kv, d, dtype, rows, keys):
+    tables, positions = shared_tables(rows, keys // 16, 16, [1 + (13 * r) % 40 for r in range(rows)])
+    batch = Batch(tables, positions, n_q, n_kv, d, 16, dtype, keys)
+    got, plan = batch.run(ops)
+    wide = dtype == torch.bfloat16 and d in SharedPrefixes.WIDE_HEADS
+    assert (plan.n_many > 0) == (rows * keys * n_q * d > (SharedPrefixes.WIDE_WORK if wide else SharedPrefixes.MANY_WORK))
+    batch.check(got)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_attention_behind_branches(ops, dtype):
+def test_attention_behind_branches(ops, any_work, dtype):
     tables, positions = shared_tables(23, 13, 16, [1 + (29 * r) % 200 for r in range(23)], branch=(4, 7))
     tables += [[900 + i for i in range(12)], [950]]           # two that share nothing, one of them short
     positions += [12 * 16 - 4, 0]
@@ -470,7 +492,7 @@ def test_attention_behind_branches(ops, dtype):
     batch.check(got)
 
 
-def test_attention_with_sinks_and_capped_scores(ops):
+def test_attention_with_sinks_and_capped_scores(ops, any_work):
     tables, positions = shared_tables(9, 20, 16, [1 + 11 * r for r in range(9)])
     for dtype in DTYPES:
         batch = Batch(tables, positions, 10, 2, 64, 16, dtype, 5, sharp=6.0)
@@ -481,7 +503,7 @@ def test_attention_with_sinks_and_capped_scores(ops):
         batch.check(batch.run(ops, sinks=sinks.cuda())[0], sinks)
 
 
-def test_one_row_and_rows_without_keys(ops):
+def test_one_row_and_rows_without_keys(ops, any_work):
     batch = Batch([[4, 2, 0]], [40], 14, 2, 64, 16, torch.bfloat16, 1)
     batch.check(batch.run(ops)[0])
     batch = Batch([[0], [0, 1], [2, 3]], [-1, 20, 31], 6, 3, 32, 16, torch.float32, 1)
@@ -489,7 +511,7 @@ def test_one_row_and_rows_without_keys(ops):
     batch.check(batch.run(ops, sinks=torch.zeros(6).cuda())[0], torch.zeros(6))
 
 
-def test_scores_far_apart_and_equal(ops):
+def test_scores_far_apart_and_equal(ops, any_work):
     # Keys whose scores leave all others behind, in the shared run and in a request's own; then scores that are all zero.
     tables, positions = shared_tables(4, 40, 16, [100, 3, 50, 17])
     batch = Batch(tables, positions, 4, 2, 64, 16, torch.bfloat16, 9, sharp=40.0)
@@ -498,7 +520,7 @@ def test_scores_far_apart_and_equal(ops):
     batch.check(batch.run(ops)[0])
 
 
-def test_a_plan_holds_while_requests_grow(ops):
+def test_a_plan_holds_while_requests_grow(ops, any_work):
     tables, positions = shared_tables(7, 12, 16, [16 * 12] * 7)
     batch = Batch(tables, [12 * 16] * 7, 14, 2, 64, 16, torch.bfloat16, 2)
     plan = batch.run(ops)[1]
@@ -509,7 +531,7 @@ def test_a_plan_holds_while_requests_grow(ops):
         assert torch.equal(later.run(ops, plan, max_position=max(later.positions))[0], narrow.run(ops, plan, max_position=max(later.positions))[0])
 
 
-def test_attention_replayed_on_new_data_and_beside_another_stream(ops):
+def test_attention_replayed_on_new_data_and_beside_another_stream(ops, any_work):
     tables, positions = shared_tables(16, 30, 16, [1 + 7 * r for r in range(16)])
     first, second = (Batch(tables, positions, 14, 2, 64, 16, torch.bfloat16, s) for s in (1, 2))
     plan = first.run(ops)[1]

@@ -100,8 +100,10 @@ def test_any_batch(seed):
             assert both <= alike * page and alike * page - both < min_keys
 
 
+@pytest.mark.parametrize("work", [-1, 4 * 10 ** 8])       # (with items of many columns, and without)
 @pytest.mark.parametrize("seed", range(12))
-def test_the_work_list_covers_every_query_and_key_once(seed):
+def test_the_work_list_covers_every_query_and_key_once(seed, work, monkeypatch):
+    monkeypatch.setattr(SharedPrefixes, "WIDE_WORK", work)
     rng = random.Random(100 + seed)
     group, n_kv, page = rng.choice([1, 3, 7, 40]), rng.choice([1, 2, 4]), 16
     shared = list(range(rng.randint(0, 90)))

@@ -11,9 +11,17 @@
 // keys, so the weights go from the one to the other in registers, and what a lane contracts over is contiguous in a page of V^T.
 //
 // Three kernels share the work, by how many columns go through a run of keys:
-//   * few (a request's own keys; up to 64 columns): sixteen columns a workgroup, whose waves share the keys out;
+//   * few (a request's own keys; all columns where there is little work; up to 64 left of a run's): sixteen columns a workgroup, whose
+//     waves share the keys out;
 //   * more, in bfloat16 at head sizes 64 and 128: 128 columns a workgroup, 32 a wave, keys and values through LDS;
 //   * more, of other types and sizes: 32 columns a workgroup, whose waves share the keys out.
+// What bounds them, measured with keys and values of 16 bits in the caches, head size 128, 4 kv heads of 7 query heads:
+//   256 requests behind 32,000 keys: 145 to 172 us with the clock, 9 of them the join; the products are 118 GFLOP, 0.7 to 0.8 PFLOP/s.  The
+//     matrix instructions share the SIMD's issue with one exponential a score and its weight's rounding.
+//   64 requests behind 4,096 keys, in eight families of 512 more, with 20 to 700 of their own: 29 us, 4.4 GFLOP and 43 MB: the chain of a
+//     workgroup's blocks and the join's launch; two workgroups a compute unit are all there are.
+//   4 requests behind 512 keys (head size 64): 7 us, two launches of a few dependent loads each.
+// In 32 bits, 21 requests behind 1,040 keys of head size 64: 12.7 us.
 // Fragments of the 32x32 instructions: row r of a block of 32 keys is key 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4, and lane
 // half h then holds keys 16 s + 8 h .. + 7 of step s of the second product.  Of the 16x16 ones: row r of the first product's
 // instruction t is key 8 (r / 4) + 4 t + r % 4, and lane group g then holds keys 8 g .. 8 g + 7.
@@ -54,7 +62,7 @@ struct SharedArgs {
   float scale, softcap;
 };
 
-// Which page of a table holds a key, and where in it (for a whole wave; a division takes some twenty instructions of the scalar unit).
+// Which page of a table holds a key, and where in it (for a whole wave; the scalar unit has no division).
 __device__ __forceinline__ void sp_page_of(const SharedArgs& a, int key, int& index, int& slot) {
   if (a.page_shift >= 0) {
     index = key >> a.page_shift;
@@ -240,8 +248,8 @@ __device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)
 //
 // The work is a pipeline over steps of 32 keys.  In step k the weights of step k - 1 meet their values while the maximum of step k's scores
 // is looked for, and the scores of step k + 1 are made while those of step k become weights: the matrix instructions of a step wait
-// for no vector instruction of the same step, and the other way round.  (One after the other, a block of 64 keys took 1.6 us of a
-// wave alone on its SIMD at head size 128, of which the matrix cores worked 0.43.)  So in iteration b, steps 2 b + 1 and 2 b + 2, the keys
+// for no vector instruction of the same step, and the other way round.  (One after the other, a block of 64 keys took a wave alone
+// on its SIMD 1.6 us at head size 128; its 32 instructions of 32x32x16 take 0.43.)  So in iteration b, steps 2 b + 1 and 2 b + 2, the keys
 // of block b + 1 and the values of block b are read, and the keys of block b + 2 and the values of block b + 1 come in.
 template <int D>
 struct Wide {
@@ -334,8 +342,8 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
   const float scale = CAPPED ? LOG2E : a.scale * LOG2E;
   const float inner = CAPPED ? 2.f * LOG2E * a.scale / a.softcap : 0.f;
 
-  // Pieces of the keys, and of the values, of one half (32 keys) of a block: all asked for before the first is used, ahead of other work
-  // (left to itself the compiler asks for two, waits, and asks for the next two: 0.06 us each time).
+  // Pieces of the keys, and of the values, of one half (32 keys) of a block: all asked for before the first is used, ahead of other work (left to itself
+  // the compiler asks for two, waits, and asks for the next two).
   struct Pieces { sp_bf16x8 p[W::STEPS]; };
   auto read_keys = [&](const char* keys, int part) {
     Pieces f;

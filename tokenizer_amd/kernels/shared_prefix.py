@@ -7,6 +7,8 @@ import dataclasses
 import numpy as np
 import torch
 
+WAVE = 64                         # lanes of a wave, which looks at so many parts at a time when they are joined
+
 
 @dataclasses.dataclass
 class SharedRun:
@@ -64,15 +66,29 @@ class SharedPrefixes:
     """A batch's sharing laid out for the attention kernel: made once (`Ops.plan_shared_prefixes`) for requests that stay the same,
     used at every layer and step.  It belongs to rows in this order with these leading pages, and to one shape of attention."""
 
-    FEW_COLUMNS = 16              # query columns (requests x query heads of a kv head) of an item of few; its waves share out the keys
-    MANY_COLUMNS = 32             # ... of one of many, likewise
-    WIDE_COLUMNS = 128            # ... of one of many in bfloat16 at head sizes WIDE_HEADS: its waves have 32 each
+    # Query columns (requests x query heads of a kv head) of an item: of few, whose waves share out the keys; of many, likewise; of many in
+    # bfloat16 at head sizes WIDE_HEADS, whose waves have 32 each and keys and values come through LDS.
+    FEW_COLUMNS, MANY_COLUMNS, WIDE_COLUMNS = 16, 32, 128
     WIDE_HEADS = (64, 128)
-    MIN_KEYS = 64                 # a shorter run is not worth a pass and a part to be joined of its own
-    MIN_PART = 128                # keys of a part of a run, at least (a block of 32 for each of its four waves)
-    MIN_WIDE_PART = 256
+    # Items of many columns read the keys less often but are fewer, so they pay where the runs' scores take so many multiply-adds (columns x
+    # keys x head size of all runs); below, every item is one of few.  Few only | with many, us: head size 128, 4 kv heads, 4,096 shared
+    # keys, 16 requests of 7 heads a kv head 14 | 17, 24 18.5 | 18.8, 32 20.2 | 19.6, 100 44 | 30; 256 requests behind 32,000 554 | 146.
+    # 32-bit keys of head size 64, 2 kv heads, 4,096 keys, 8 requests 12.1 | 17.4, 64 27.9 | 27.9, 128 35.7 | 41.6; behind 16,000
+    # 64 54 | 63, 128 104 | 87.
+    WIDE_WORK, MANY_WORK = 4 * 10 ** 8, 2 ** 31
+    WIDE_LITTLE, MANY_LITTLE = 64, 16          # ... and what is left of a run's columns, up to so many, goes into items of few all the same
+    # A shorter run is not a pass and a part to be joined of its own.  (64 requests, 64 keys shared 14.7 us as a run, 14.0 with the
+    # requests' own; 256 keys 19.2 and 19.2, and the cache is read less.)
+    MIN_KEYS = 64
+    # Keys of a part of a run, at least: a block of 32 for each of its four waves.  (Parts of 64 | 128 | 256 keys, 2 requests of 4,096 keys 13.1 |
+    # 10.6 | 10.6 us, 4 requests of 512 7.4 | 7.1 | 7.8.)  Of a long one a 64th, up to 512: a wave joins 64 parts at a time (2 requests of
+    # 32,000 keys of head size 64 in 250 parts 25.8 us, in 63 12.8).
+    MIN_PART, MIN_WIDE_PART = 128, 256
     OWN_STEP = 128                # `smallest_own` in whole steps: prefixes that differ a little make launches of one shape
-    TARGET = 512                  # workgroups that the parts aim at: two a compute unit
+    # Workgroups that the parts aim at: two a compute unit; one where all items are of few columns.  (256 | 512 | 768: 64 requests behind 4,096
+    # keys 34.6 | 28.7 | 32.7 us, 256 behind 32,000 187 | 145 | 161; few only, 64 behind 512 11.0 | 13.1 | 13.2, 16 behind 4,096
+    # 15.1 | 14.2 | 18.1, 2 behind 32,000 22.0 | 26.7 | 32.7.)
+    TARGET, FEW_TARGET = 512, 256
 
     def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device,
                  fill: int = 0):
@@ -82,9 +98,14 @@ class SharedPrefixes:
         self.order, self.runs, own_begin = find_shared_runs(table, positions, page_size, self.MIN_KEYS)
         place = {row: at for at, row in enumerate(self.order)}
         group = n_q // n_kv
-        # A run's columns in tiles of many, and what is left, if that is little, in tiles of few.
+        # A run's columns in tiles of many, where there is work for them, and what is left, if that is little, in tiles of few.
         wide = dtype == torch.bfloat16 and head_dim in self.WIDE_HEADS
-        size, little = (self.WIDE_COLUMNS, self.WIDE_COLUMNS // 2) if wide else (self.MANY_COLUMNS, self.FEW_COLUMNS)
+        size, little = (self.WIDE_COLUMNS, self.WIDE_LITTLE) if wide else (self.MANY_COLUMNS, self.MANY_LITTLE)
+        products = sum(len(run.rows) * (run.key_end - run.key_begin) for run in self.runs) * n_q * head_dim
+        if products <= (self.WIDE_WORK if wide else self.MANY_WORK):
+            little, target = self.n_rows * group, self.FEW_TARGET
+        else:
+            target = self.TARGET
         tiles = []                                        # per run: (first column, whether it is one of many)
         for run in self.runs:
             columns, at, found = len(run.rows) * group, 0, []
@@ -93,12 +114,12 @@ class SharedPrefixes:
                 found.append((at, many))
                 at += size if many else self.FEW_COLUMNS
             tiles.append(found)
-        # Parts of so many keys that all runs together make about TARGET workgroups (no more: they would wait for a second round).
+        # Parts of so many keys that all runs together make about the workgroups aimed at (no more: they would wait for a second round).
         work = sum(len(t) * (run.key_end - run.key_begin) for t, run in zip(tiles, self.runs)) * n_kv
         groups, parts_of = {False: [], True: []}, np.zeros(self.n_rows, dtype=np.int32)      # items that read the same keys and values
         for found, run in zip(tiles, self.runs):
             length = run.key_end - run.key_begin
-            part = max(self.MIN_WIDE_PART if wide and found[0][1] else self.MIN_PART, -(-work // self.TARGET))
+            part = max(self.MIN_WIDE_PART if wide and found[0][1] else self.MIN_PART, -(-work // target), min(length // WAVE, 4 * self.MIN_PART))
             keys = -(-length // (32 * max(1, length // part))) * 32
             first = int(parts_of[run.rows[0]])
             for split, begin in enumerate(range(run.key_begin, run.key_end, keys)):
