@@ -296,6 +296,17 @@ def test_forked_requests_go_on_as_if_each_had_run_the_prompt(model_folders, name
     engine.cache.check_invariants()
 
 
+def test_a_request_is_no_fork_for_its_name(model_folders):
+    # A fork that leaves by the cache, as a scheduler's requests do; the next request of that name is one of its own.
+    engine = _engine(model_folders["A"])
+    engine.add_request("a")
+    engine.fork_request("a", ["b"])                       # (a request without a token, too)
+    assert engine.cache.seq_len("b") == 0 and engine._family == {"a", "b"}
+    engine.cache.release("b")
+    engine.add_request("b")
+    assert engine._family == {"a"}
+
+
 def test_requests_go_on_behind_a_compaction(model_folders):
     engine, still = _engine(model_folders["A"]), _engine(model_folders["A"])
     vocab = engine.model.vocab_size

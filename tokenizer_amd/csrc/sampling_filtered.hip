@@ -23,9 +23,9 @@
 // narrows the answer's range by counting, key by key.
 //
 // What bounds it, measured with logits of 32 bits in the caches (the operator's own launches, replayed):
-//   one row of 152,064 under top-k 40: 14.6 us, a chain of three launches (extents 3.6, the list 6.0, the draw 6.0 with the profiler's
+//   one row of 151,936 under top-k 40: 14.6 us, a chain of three launches (extents 3.6, the list 6.0, the draw 6.0 with the profiler's
 //     share), each a few dependent steps of one workgroup a piece; reading 0.6 MB would take 0.1.  Under top-p alone 22.
-//   64 rows of 152,064, each under other limits: 31 us: the extents 8.8, the second reading 11.5 (weights in 64 bits where the bins are
+//   64 rows of 151,936, each under other limits: 31 us: the extents 8.8, the second reading 11.5 (weights in 64 bits where the bins are
 //     needed), ordering the lists 9.2, the gathering and the draws 4.6.
 //   256 rows of 152,064 under min-p: 53 us: the extents 25 (156 MB at 6.2 TB/s), the list 13, the draw 9; a row read once at the rate of a
 //     large copy would take 31.  Under top-p alone, where every token's weight and bin is worked out, 134.
@@ -581,7 +581,7 @@ __device__ __forceinline__ int fs_answers(FsShared& s, const FsRow& r, const FsA
   return s.found;
 }
 
-// Up to FS_FEW tokens: each is held against all others, two to eight threads a token.  (A draw under top-k 40 from 152,064
+// Up to FS_FEW tokens: each is held against all others, two to eight threads a token.  (A draw under top-k 40 from 151,936
 // logits 14.6 us so, 15.8 by fs_spread; four rows of 1,000 logits 9.0 and 10.2.)
 template <int THREADS>
 __device__ __forceinline__ int fs_answers_of_few(FsShared& s, const FsRow& r, const FsAsked& asked, u64 all, bool k_here, u64 over, bool all_listed,
@@ -650,7 +650,7 @@ __device__ __forceinline__ int fs_answers_of_sorted(FsShared& s, const FsRow& r,
 // Up to FS_SPREAD tokens, unless many are (nearly) equal: they are spread over 256 ranges between the list's largest and smallest, whose
 // counts and weights are added up in order, and each is held against those of its own range.  s.list: tokens as they came, then in
 // order | weight before each | tokens range by range | their weights, FS_SPREAD each.  Returns false with the list as it was if a range has more
-// than WAVE tokens.  (With 64 rows of 152,064 the settling pass, slowest row, 14.9 us sorted and 9.2 so; one row that lists 128 tokens or
+// than WAVE tokens.  (With 64 rows of 151,936 the settling pass, slowest row, 14.9 us sorted and 9.2 so; one row that lists 128 tokens or
 // fewer takes fs_answers_of_few and pays nothing.)
 #define FS_SPREAD (FS_LIST / 4)
 template <int THREADS>

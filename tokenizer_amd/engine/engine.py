@@ -552,9 +552,11 @@ class Engine:
     def sharing(self, entries: list[StepEntry]) -> dict:
         """The plans of what the requests of a step of single tokens share, by the shape of the attention that takes them; empty where
         nothing is shared.  Worked out when the requests of a step change, and kept while they stay."""
-        if self.shared_attention is False or not self._shared_shapes or len(entries) < 2 or any(len(e.tokens) != 1 for e in entries):
+        if self.shared_attention is False or not self._shared_shapes or len(entries) < 2:
             return NOTHING_SHARED
-        if self.shared_attention is None and sum(e.rid in self._family for e in entries) < 2:
+        if self.shared_attention is None and (len(self._family) < 2 or sum(e.rid in self._family for e in entries) < 2):
+            return NOTHING_SHARED
+        if any(len(e.tokens) != 1 for e in entries):
             return NOTHING_SHARED
         key = (self.cache.epoch, tuple(e.rid for e in entries))
         if self._sharing is not None and self._sharing[0] == key:
@@ -606,6 +608,7 @@ class Engine:
         first such call; `token_bytes` and `on_chunk` may be passed on)."""
         if params is None:
             self.cache.add_request(rid)
+            self._family.discard(rid)        # (a scheduler's requests leave by the cache: the name may be an old fork's)
             return None
         return self.scheduler.add_request(list(rid), params, **callbacks)
 
