@@ -215,6 +215,29 @@ def test_draws_of_few_and_many_long_rows(ops, rows):
         check_draws(ops, logits, uniform=rng.uniform(0, 1, rows), **given)
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [(216, 151936, torch.bfloat16), (830, 40001, torch.float32)])
+def test_draws_of_very_many_long_rows(ops, rows, vocab, dtype):
+    # (A workgroup sees to several pieces of a row then.)  Each row's draw is what it is among eight, and of some by the definition.
+    logits = hills(rows, vocab, dtype, rows, 3.0)
+    logits[::7, 5:] = float("-inf")
+    logits[3::11, 9000:] = float("nan")
+    rng = np.random.default_rng(rows)
+    given = dict(temperature=rng.integers(0, 5, rows) * 0.4, top_k=rng.integers(-1, 3, rows) * 45, top_p=rng.uniform(0.6, 1.3, rows),
+                 min_p=rng.integers(0, 2, rows) * 0.03, uniform=rng.uniform(0, 1, rows))
+    got = ops.sample_filtered(logits, **settings(rows, **given)).tolist()
+    for at in range(0, rows, 8):
+        part = {name: value[at:at + 8] for name, value in given.items()}
+        some = logits[at:at + 8]
+        assert ops.sample_filtered(some, **settings(len(some), **part)).tolist() == got[at:at + 8]
+    some = list(range(0, rows, rows // 9))
+    assert check_draws(ops, logits[some], **{name: value[some] for name, value in given.items()}) == [got[r] for r in some]
+
+
+def test_the_largest_counts(ops):
+    logits = hills(4, 50001, torch.float32, 2)
+    check_draws(ops, logits, top_k=[2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1, -2 ** 31], uniform=[0.1, 0.5, 0.7, 0.9])
+
+
 def test_draws_on_another_stream_and_replayed(ops):
     first, second = hills(5, 20000, torch.float32, 6), hills(5, 20000, torch.float32, 8)
     numbers = settings(5, uniform=[0.1, 0.4, 0.6, 0.8, 0.95], top_k=40, top_p=0.9)

@@ -27,7 +27,7 @@
 //     share), each a few dependent steps of one workgroup a piece; reading 0.6 MB would take 0.1.  Under top-p alone 22.
 //   64 rows of 151,936, each under other limits: 31 us: the extents 8.8, the second reading 11.5 (weights in 64 bits where the bins are
 //     needed), ordering the lists 9.2, the gathering and the draws 4.6.
-//   256 rows of 152,064 under min-p: 53 us: the extents 25 (156 MB at 6.2 TB/s), the list 13, the draw 9; a row read once at the rate of a
+//   256 rows of 152,064 under min-p: 53 us: the extents 25 (156 MB at 6.2 TB/s), the list 14, the draw 9; a row read once at the rate of a
 //     large copy would take 31.  Under top-p alone, where every token's weight and bin is worked out, 134.
 // A workgroup has 4,096 logits, sixteen a thread, all asked for at once; a single row is then 38 workgroups.
 //
@@ -45,6 +45,11 @@
 #define FS_FEW 128
 #define FS_SLOTS 256                    // ranges that a round of narrowing tells apart
 #define FS_FEW_ROWS 8                   // up to so many long rows take three launches instead of five
+#define FS_SPAN 4                       // pieces that a workgroup sees to in the passes behind the first ...
+// ... from so many pieces of all rows on.  (One | four pieces a workgroup, us: rows of 151,936 under min-p, 128 rows 34.8 | 33.9, 256 54.3 |
+// 47.8, 512 104 | 84; under top-k 40 47.5 | 40.5, 77 | 64, 148 | 120; under top-p 81 | 85, 136 | 137, 267 | 239; rows of 32,000 under
+// several limits, 128 rows 35 | 46, 512 86 | 91.)
+#define FS_MANY_PIECES 8192
 #define FS_MAX_WAVES (FS_SHORT_THREADS / WAVE)
 #define FS_UNIT 17592186044416.0        // 2^44
 #define FS_REACH 31.3f                  // beyond so many T below the maximum a weight is less than half a unit: nothing
@@ -201,13 +206,15 @@ __device__ __forceinline__ void fs_extent(const float (&v)[EACH], int begin, flo
   }
 }
 
-// A piece's bins into `s.mass` and (if `counted`) `s.count`, and the weight of its tokens that min-p keeps, to every thread.
-template <int THREADS, int EACH>
+// Bins in `s.mass` and (if `counted`) `s.count`.  A thread's logits are added to them, and the weight of those that min-p keeps is returned.
+__device__ __forceinline__ void fs_clear_bins(FsSmall& s) {
+  if (threadIdx.x < FS_BINS) { s.mass[threadIdx.x] = 0; s.count[threadIdx.x] = 0; }
+  __syncthreads();
+}
+template <int EACH>
 __device__ __forceinline__ u64 fs_fill_bins(const float (&v)[EACH], const FsRow& r, const FsAsked& asked, FsSmall& s) {
   const bool counted = asked.top_k > 0, floored = asked.min_p > 0.f;
   const double floor_share = (double)asked.min_p * FS_UNIT;
-  if (threadIdx.x < FS_BINS) { s.mass[threadIdx.x] = 0; s.count[threadIdx.x] = 0; }
-  __syncthreads();
   u64 over = 0;
 #pragma unroll
   for (int j = 0; j < EACH; ++j) {
@@ -220,7 +227,7 @@ __device__ __forceinline__ u64 fs_fill_bins(const float (&v)[EACH], const FsRow&
       if (!floored || !(share < floor_share) || v[j] == r.top) over += w;
     }
   }
-  return fs_sum<THREADS>(over, s);                         // (its barriers stand behind the bins, too)
+  return over;
 }
 
 // A wave's view of the bins: running counts and weights, bins 4 lane .. + 3.
@@ -794,7 +801,7 @@ struct FsArgs {
   const float *temperature, *top_p, *min_p, *uniform;
   const int* top_k;
   int* out;
-  int vocab, pieces;
+  int vocab, pieces, span;              // span: pieces that a workgroup sees to behind the first pass
   char* workspace;
   size_t row_bytes;
 };
@@ -827,7 +834,8 @@ sample_filtered_short(FsArgs a) {
     return;
   }
   const FsRow r = fs_row(asked.temperature, high, low);
-  const u64 over = fs_fill_bins<THREADS>(v, r, asked, s);
+  fs_clear_bins(s);
+  const u64 over = fs_sum<THREADS>(fs_fill_bins(v, r, asked, s), s);     // (its barriers stand behind the bins, too)
   FsRunning run;
   run.of(s);
   const FsRanges ranges = fs_ranges(run, asked, over);
@@ -855,7 +863,7 @@ struct FsBinned { u64 mass[FS_BINS]; uint32_t count[FS_BINS]; u64 over; u64 unus
 // pieces' bins.
 struct FsSpace {
   char* base;
-  int pieces;
+  int pieces, binned_pieces;
   __device__ __forceinline__ FsHead* head() const { return (FsHead*)base; }
   __device__ __forceinline__ FsBinned* whole() const { return (FsBinned*)(base + sizeof(FsHead)); }
   __device__ __forceinline__ u64* list() const { return (u64*)(whole() + 1); }
@@ -868,7 +876,7 @@ static size_t fs_row_bytes(int pieces) {
   return sizeof(FsHead) + sizeof(FsBinned) + 8 * FS_LIST + (sizeof(FsExtent) + 4 * (FS_PIECE_WAVES + FS_PIECE_ROWS) + sizeof(FsBinned)) * (size_t)pieces;
 }
 static_assert(sizeof(FsHead) % 16 == 0 && sizeof(FsBinned) % 16 == 0 && sizeof(FsExtent) % 16 == 0 && (FS_PIECE_WAVES + FS_PIECE_ROWS) % 4 == 0, "pieces of sixteen bytes");
-__device__ __forceinline__ FsSpace fs_space(const FsArgs& a, int row) { return FsSpace{a.workspace + (size_t)row * a.row_bytes, a.pieces}; }
+__device__ __forceinline__ FsSpace fs_space(const FsArgs& a, int row) { return FsSpace{a.workspace + (size_t)row * a.row_bytes, a.pieces, (a.pieces + a.span - 1) / a.span}; }
 
 // The row's extent from its pieces' (a lane of every wave looks at one piece of sixty-four), to every thread.
 __device__ __forceinline__ void fs_row_extent(const FsSpace& w, float& high, float& low) {
@@ -949,10 +957,10 @@ __device__ __forceinline__ float fs_cut(const FsSpace& w, const FsAsked& asked, 
   return cut;
 }
 
-// The tokens of a piece that `wanted` names, to the row's list: each thread's, their place among the workgroup's, and the
+// The tokens of piece `p` that `wanted` names, to the row's list: each thread's, their place among the workgroup's, and the
 // workgroup's place in the list.
 template <typename Wanted>
-__device__ __forceinline__ void fs_append(const FsSpace& w, const float (&v)[FS_EACH], FsSmall& s, Wanted wanted) {
+__device__ __forceinline__ void fs_append(const FsSpace& w, int p, const float (&v)[FS_EACH], FsSmall& s, Wanted wanted) {
   uint32_t held = 0;
 #pragma unroll
   for (int j = 0; j < FS_EACH; ++j)
@@ -981,7 +989,7 @@ __device__ __forceinline__ void fs_append(const FsSpace& w, const float (&v)[FS_
   for (int j = 0; j < FS_EACH; ++j)
     if (held >> j & 1) {
       if (place < FS_LIST)
-        w.list()[place] = (u64)fs_key(v[j]) << 32 | (uint32_t)~(uint32_t)(blockIdx.x * FS_PIECE + j * FS_THREADS + (int)threadIdx.x);
+        w.list()[place] = (u64)fs_key(v[j]) << 32 | (uint32_t)~(uint32_t)(p * FS_PIECE + j * FS_THREADS + (int)threadIdx.x);
       ++place;
     }
 }
@@ -1006,18 +1014,25 @@ sample_filtered_extents(FsArgs a) {
   }
 }
 
-// The list, where it can be made at once; else the piece's bins.
-template <typename T>
+// The list, where it can be made at once; else the bins of SPAN pieces.
+template <typename T, int SPAN>
 __global__ void __launch_bounds__(FS_THREADS)
 sample_filtered_bins(FsArgs a) {
   __shared__ FsSmall s;
   const FsSpace w = fs_space(a, blockIdx.y);
   const FsAsked asked = fs_asked(a, blockIdx.y);
   const T* row = (const T*)a.logits + (size_t)blockIdx.y * a.stride;
+  const int first = blockIdx.x * SPAN;
   float v[FS_EACH], high, low;
   if (fs_listed_at_once(asked, a.vocab)) {
     // (One wave works the cut out: eight halvings among six hundred maxima by every wave of 2,432 workgroups took 14 us of their time.)
-    const float of_row = w.of_rows()[blockIdx.x * FS_PIECE_ROWS + threadIdx.x / 16], of_piece = w.extents()[blockIdx.x].high;
+    float of_row[SPAN], of_piece[SPAN];
+#pragma unroll
+    for (int j = 0; j < SPAN; ++j) {
+      const int p = min(first + j, a.pieces - 1);
+      of_row[j] = w.of_rows()[p * FS_PIECE_ROWS + threadIdx.x / 16];
+      of_piece[j] = w.extents()[p].high;
+    }
     fs_row_extent(w, high, low);
     if (!fs_is_drawn(asked.temperature, high)) return;
     const FsRow r = fs_row(asked.temperature, high, low);
@@ -1027,18 +1042,30 @@ sample_filtered_bins(FsArgs a) {
     }
     __syncthreads();
     const float cut = s.cut;
-    if (of_piece < cut) return;                            // (the same for the whole workgroup)
-    // Only lanes whose row of sixteen has something at or above the cut read their logits again: of 256 rows of 152,064 under min-p, 13 of
-    // 26 us of this pass were the second reading.
-    fs_load<FS_THREADS>(row, blockIdx.x * FS_PIECE, a.vocab, v, of_row >= cut);
-    fs_append(w, v, s, [&](float x) { return x >= cut && r.top - x <= r.reach; });
+#pragma unroll
+    for (int j = 0; j < SPAN; ++j) {
+      const int p = first + j;
+      if (p >= a.pieces || of_piece[j] < cut) continue;    // (the same for the whole workgroup)
+      // Only lanes whose row of sixteen has something at or above the cut read their logits again: of 256 rows of 152,064 under min-p, 13
+      // of 26 us of this pass were the second reading.
+      fs_load<FS_THREADS>(row, p * FS_PIECE, a.vocab, v, of_row[j] >= cut);
+      fs_append(w, p, v, s, [&](float x) { return x >= cut && r.top - x <= r.reach; });
+      if (SPAN > 1) __syncthreads();
+    }
     return;
   }
-  fs_load<FS_THREADS>(row, blockIdx.x * FS_PIECE, a.vocab, v);
+  fs_load<FS_THREADS>(row, first * FS_PIECE, a.vocab, v);
   fs_row_extent(w, high, low);
   if (!fs_is_drawn(asked.temperature, high)) return;
   const FsRow r = fs_row(asked.temperature, high, low);
-  const u64 over = fs_fill_bins<FS_THREADS>(v, r, asked, s);
+  fs_clear_bins(s);
+  u64 over = 0;
+  for (int p = first;;) {
+    over += fs_fill_bins(v, r, asked, s);
+    if (SPAN == 1 || ++p == min(first + SPAN, a.pieces)) break;
+    fs_load<FS_THREADS>(row, p * FS_PIECE, a.vocab, v);
+  }
+  over = fs_sum<FS_THREADS>(over, s);
   FsBinned& mine = w.binned()[blockIdx.x];
   mine.mass[threadIdx.x] = s.mass[threadIdx.x];
   mine.count[threadIdx.x] = s.count[threadIdx.x];
@@ -1051,20 +1078,20 @@ __device__ __forceinline__ FsRanges fs_settle(const FsSpace& w, const FsAsked& a
   u64 m = 0;
   uint32_t c = 0;
   over = 0;
-  for (int first = 0; first < w.pieces; first += 16) {     // (sixteen pieces asked for at a time)
+  for (int first = 0; first < w.binned_pieces; first += 16) {     // (sixteen pieces asked for at a time)
     u64 of_mass[16];
     uint32_t of_count[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const FsBinned& piece = w.binned()[min(first + j, w.pieces - 1)];
+      const FsBinned& piece = w.binned()[min(first + j, w.binned_pieces - 1)];
       of_mass[j] = piece.mass[threadIdx.x];
       of_count[j] = piece.count[threadIdx.x];
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (first + j < w.pieces) { m += of_mass[j]; c += of_count[j]; }
+      if (first + j < w.binned_pieces) { m += of_mass[j]; c += of_count[j]; }
   }
-  for (int p = threadIdx.x; p < w.pieces; p += FS_THREADS) over += w.binned()[p].over;
+  for (int p = threadIdx.x; p < w.binned_pieces; p += FS_THREADS) over += w.binned()[p].over;
   s.mass[threadIdx.x] = m;
   s.count[threadIdx.x] = c;
   over = fs_sum<FS_THREADS>(over, s);
@@ -1083,15 +1110,19 @@ __device__ __forceinline__ void fs_draw_listed(const FsArgs& a, const FsSpace& w
   if (threadIdx.x == 0) a.out[row_at] = pick;
 }
 
-// The piece's tokens in the ranges, to the row's list.
-template <typename T>
-__device__ __forceinline__ void fs_gather(const FsArgs& a, const FsSpace& w, const FsRow& r, const FsRanges& ranges, FsSmall& s) {
-  const float of_row = w.of_rows()[blockIdx.x * FS_PIECE_ROWS + threadIdx.x / 16];
-  float v[FS_EACH];
-  // (A row of sixteen lanes whose maximum lies behind all the ranges has nothing in them.)
-  const bool wanted = r.top - of_row <= r.reach && fs_bin(of_row, r) <= max(ranges.k_bin, max(ranges.p_last, ranges.draw_last));
-  fs_load<FS_THREADS>((const T*)a.logits + (size_t)blockIdx.y * a.stride, blockIdx.x * FS_PIECE, a.vocab, v, wanted);
-  fs_append(w, v, s, [&](float x) { return r.top - x <= r.reach && ranges.has(fs_bin(x, r)); });
+// The tokens of SPAN pieces in the ranges, to the row's list.
+template <int SPAN, typename T>
+__device__ __forceinline__ void fs_gather(const FsArgs& a, const FsSpace& w, const T* row, const FsRow& r, const FsRanges& ranges, FsSmall& s) {
+  const int last_bin = max(ranges.k_bin, max(ranges.p_last, ranges.draw_last));
+  for (int p = blockIdx.x * SPAN; p < min((int)blockIdx.x * SPAN + SPAN, a.pieces); ++p) {
+    const float of_row = w.of_rows()[p * FS_PIECE_ROWS + threadIdx.x / 16];
+    float v[FS_EACH];
+    // (A row of sixteen lanes whose maximum lies behind all the ranges has nothing in them.)
+    const bool wanted = r.top - of_row <= r.reach && fs_bin(of_row, r) <= last_bin;
+    fs_load<FS_THREADS>(row, p * FS_PIECE, a.vocab, v, wanted);
+    fs_append(w, p, v, s, [&](float x) { return r.top - x <= r.reach && ranges.has(fs_bin(x, r)); });
+    if (SPAN > 1) __syncthreads();
+  }
 }
 
 // Many rows.  A row whose list is there: its draw.  Another: its bins and ranges, left for its pieces, which gather; and its draw.
@@ -1130,7 +1161,7 @@ __device__ __forceinline__ FsRanges fs_kept_ranges(const FsSpace& w) {
   return FsRanges{scalar_int(kept), scalar_int(kept + 1), scalar_int(kept + 2), scalar_int(kept + 3), scalar_int(kept + 4)};
 }
 
-template <typename T>
+template <typename T, int SPAN>
 __global__ void __launch_bounds__(FS_THREADS)
 sample_filtered_gather(FsArgs a) {
   __shared__ FsSmall s;
@@ -1139,7 +1170,7 @@ sample_filtered_gather(FsArgs a) {
   float high, low;
   fs_row_extent(w, high, low);
   if (fs_listed_at_once(asked, a.vocab) || !fs_is_drawn(asked.temperature, high)) return;
-  fs_gather<T>(a, w, fs_row(asked.temperature, high, low), fs_kept_ranges(w), s);
+  fs_gather<SPAN>(a, w, (const T*)a.logits + (size_t)blockIdx.y * a.stride, fs_row(asked.temperature, high, low), fs_kept_ranges(w), s);
 }
 
 template <typename T>
@@ -1184,7 +1215,7 @@ sample_filtered_finish(FsArgs a) {
   }
   u64 over;
   const FsRanges ranges = fs_settle(w, asked, over, s);
-  fs_gather<T>(a, w, r, ranges, s);
+  fs_gather<1>(a, w, (const T*)a.logits + (size_t)row_at * a.stride, r, ranges, s);
   __syncthreads();
   if (threadIdx.x == 0) {                                  // (one thread's fences, between barriers, stand for the workgroup's)
     __threadfence();                                       // the tokens are there for all that see the count
@@ -1192,7 +1223,7 @@ sample_filtered_finish(FsArgs a) {
     __threadfence();                                       // and so is what the others left before they counted themselves in
   }
   __syncthreads();
-  if (came != a.pieces - 1) return;                        // (the same for the whole workgroup)
+  if (came != w.binned_pieces - 1) return;                        // (the same for the whole workgroup)
   const int n = __hip_atomic_load(&w.head()->n_listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   fs_draw_listed<T>(a, w, asked, r, row_at, &ranges, over, n, s);
 }
@@ -1207,6 +1238,28 @@ static int fs_pieces(int vocab) { return (vocab + FS_PIECE - 1) / FS_PIECE; }
 // Bytes of workspace a row needs (a multiple of 16; none for a short row).
 extern "C" int ta_sample_filtered_workspace(int vocab) { return fs_is_short(vocab) ? 0 : (int)fs_row_bytes(fs_pieces(vocab)); }
 
+// The passes of long rows behind the first: so many pieces a workgroup.
+template <typename T, int SPAN>
+static int launch_long(FsArgs a, int n_rows, hipStream_t stream) {
+  a.span = SPAN;
+  const dim3 grid((a.pieces + SPAN - 1) / SPAN, n_rows);
+  sample_filtered_bins<T, SPAN><<<grid, FS_THREADS, 0, stream>>>(a);
+  int status = LAUNCH_STATUS();
+  if (status) return status;
+  if (SPAN == 1 && n_rows <= FS_FEW_ROWS) {
+    sample_filtered_finish<T><<<grid, FS_THREADS, 0, stream>>>(a);
+    return LAUNCH_STATUS();
+  }
+  sample_filtered_settle<T><<<n_rows, FS_THREADS, 0, stream>>>(a);
+  status = LAUNCH_STATUS();
+  if (status) return status;
+  sample_filtered_gather<T, SPAN><<<grid, FS_THREADS, 0, stream>>>(a);
+  status = LAUNCH_STATUS();
+  if (status) return status;
+  sample_filtered_draw<T><<<n_rows, FS_THREADS, 0, stream>>>(a);
+  return LAUNCH_STATUS();
+}
+
 template <typename T>
 static int launch_filtered(FsArgs a, int n_rows, hipStream_t stream) {
   if (fs_is_short(a.vocab)) {
@@ -1216,25 +1269,10 @@ static int launch_filtered(FsArgs a, int n_rows, hipStream_t stream) {
       sample_filtered_short<T, FS_SHORT_EACH><<<n_rows, FS_SHORT_THREADS, 0, stream>>>(a);
     return LAUNCH_STATUS();
   }
-  const dim3 grid(a.pieces, n_rows);
-  sample_filtered_extents<T><<<grid, FS_THREADS, 0, stream>>>(a);
-  int status = LAUNCH_STATUS();
+  sample_filtered_extents<T><<<dim3(a.pieces, n_rows), FS_THREADS, 0, stream>>>(a);
+  const int status = LAUNCH_STATUS();
   if (status) return status;
-  sample_filtered_bins<T><<<grid, FS_THREADS, 0, stream>>>(a);
-  status = LAUNCH_STATUS();
-  if (status) return status;
-  if (n_rows <= FS_FEW_ROWS) {
-    sample_filtered_finish<T><<<grid, FS_THREADS, 0, stream>>>(a);
-    return LAUNCH_STATUS();
-  }
-  sample_filtered_settle<T><<<n_rows, FS_THREADS, 0, stream>>>(a);
-  status = LAUNCH_STATUS();
-  if (status) return status;
-  sample_filtered_gather<T><<<grid, FS_THREADS, 0, stream>>>(a);
-  status = LAUNCH_STATUS();
-  if (status) return status;
-  sample_filtered_draw<T><<<n_rows, FS_THREADS, 0, stream>>>(a);
-  return LAUNCH_STATUS();
+  return (int64_t)a.pieces * n_rows >= FS_MANY_PIECES ? launch_long<T, FS_SPAN>(a, n_rows, stream) : launch_long<T, 1>(a, n_rows, stream);
 }
 
 // logits [n_rows, vocab] (float or bfloat16), rows `stride` elements apart; the others one number a row; workspace: n_rows *
@@ -1248,7 +1286,7 @@ extern "C" int ta_sample_filtered(const void* logits, int64_t stride, const void
   FsArgs a;
   a.logits = logits; a.stride = stride; a.temperature = (const float*)temperature; a.top_p = (const float*)top_p;
   a.min_p = (const float*)min_p; a.uniform = (const float*)uniform; a.top_k = (const int*)top_k; a.out = (int*)out;
-  a.vocab = vocab; a.pieces = fs_pieces(vocab); a.workspace = (char*)workspace;
+  a.vocab = vocab; a.pieces = fs_pieces(vocab); a.span = 1; a.workspace = (char*)workspace;
   a.row_bytes = fs_row_bytes(a.pieces);
   return dtype == DT_F32 ? launch_filtered<float>(a, n_rows, stream) : launch_filtered<bf16_t>(a, n_rows, stream);
 }
