@@ -500,7 +500,7 @@ def test_attention_with_work_for_many_columns(ops, n_q, n_kv, d, dtype, rows, ke
     batch = Batch(tables, positions, n_q, n_kv, d, 16, dtype, keys)
     got, plan = batch.run(ops)
     wide = dtype == torch.bfloat16 and d in SharedPrefixes.WIDE_HEADS
-    assert (plan.n_many > 0) == (rows * keys * n_q * d > (SharedPrefixes.WIDE_WORK if wide else SharedPrefixes.MANY_WORK))
+    assert (plan.n_many > 0) == (rows * keys * n_q > (SharedPrefixes.WIDE_WORK if wide else SharedPrefixes.MANY_WORK))
     batch.check(got)
 
 

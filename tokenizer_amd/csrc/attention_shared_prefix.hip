@@ -11,7 +11,7 @@
 // keys, so the weights go from the one to the other in registers, and what a lane contracts over is contiguous in a page of V^T.
 //
 // Three kernels share the work, by how many columns go through a run of keys:
-//   * few (a request's own keys; all columns where there is little work; up to 64 left of a run's): sixteen columns a workgroup, whose
+//   * few (a request's own keys; all columns where there is little work; up to 48 left of a run's): sixteen columns a workgroup, whose
 //     waves share the keys out;
 //   * more, in bfloat16 at head sizes 64 and 128: 128 columns a workgroup, 32 a wave, keys and values through LDS;
 //   * more, of other types and sizes: 32 columns a workgroup, whose waves share the keys out.

@@ -70,13 +70,16 @@ class SharedPrefixes:
     # bfloat16 at head sizes WIDE_HEADS, whose waves have 32 each and keys and values come through LDS.
     FEW_COLUMNS, MANY_COLUMNS, WIDE_COLUMNS = 16, 32, 128
     WIDE_HEADS = (64, 128)
-    # Items of many columns read the keys less often but are fewer, so they pay where the runs' scores take so many multiply-adds (columns x
-    # keys x head size of all runs); below, every item is one of few.  Few only | with many, us: head size 128, 4 kv heads, 4,096 shared
-    # keys, 16 requests of 7 heads a kv head 14 | 17, 24 18.5 | 18.8, 32 20.2 | 19.6, 100 44 | 30; 256 requests behind 32,000 554 | 146.
-    # 32-bit keys of head size 64, 2 kv heads, 4,096 keys, 8 requests 12.1 | 17.4, 64 27.9 | 27.9, 128 35.7 | 41.6; behind 16,000
-    # 64 54 | 63, 128 104 | 87.
-    WIDE_WORK, MANY_WORK = 4 * 10 ** 8, 2 ** 31
-    WIDE_LITTLE, MANY_LITTLE = 64, 16          # ... and what is left of a run's columns, up to so many, goes into items of few all the same
+    # Items of many columns read the keys less often but are fewer, so they pay where the runs have so many scores (columns x keys x kv
+    # heads, of all runs); below, every item is one of few.  Few only | with many, us: head size 128, 4 kv heads of 7 query heads,
+    # 4,096 shared keys, 16 requests (1.8 million) 14 | 17, 24 15.4 | 18.8, 32 (3.7) 20.2 | 19.6, 100 44 | 30; 256 requests behind 32,000
+    # 554 | 146.  Head size 64, 2 kv heads, 4,096 keys, 64 requests (3.7) 12.9 | 14.0, 100 16.0 | 15.6; 128 behind 2,048 in families
+    # of 512 more (4.6) 20.7 | 14.9.  In 32 bits, 4,096 keys, 8 requests 12.1 | 17.4, 128 (7) 35.7 | 41.6; behind 16,000 64 (14) 54 | 63,
+    # 128 (29) 104 | 87.  Head size 96, 4,096 keys, 256 requests (15) 30.0 | 27.2; behind 16,000 64 (14) 26 | 30, 256 (57) 87 | 56.
+    WIDE_WORK, MANY_WORK = 3_700_000, 16_000_000
+    # ... and what is left of a run's columns, up to so many, goes into items of few all the same.  (64 left, behind 4,096 keys, up to 64 | 48:
+    # 28.1 | 24.7 us.)
+    WIDE_LITTLE, MANY_LITTLE = 48, 16
     # A shorter run is not a pass and a part to be joined of its own.  (64 requests, 64 keys shared 14.7 us as a run, 14.0 with the
     # requests' own; 256 keys 19.2 and 19.2, and the cache is read less.)
     MIN_KEYS = 64
@@ -86,8 +89,8 @@ class SharedPrefixes:
     MIN_PART, MIN_WIDE_PART = 128, 256
     OWN_STEP = 128                # `smallest_own` in whole steps: prefixes that differ a little make launches of one shape
     # Workgroups that the parts aim at: two a compute unit; one where all items are of few columns.  (256 | 512 | 768: 64 requests behind 4,096
-    # keys 34.6 | 28.7 | 32.7 us, 256 behind 32,000 187 | 145 | 161; few only, 64 behind 512 11.0 | 13.1 | 13.2, 16 behind 4,096
-    # 15.1 | 14.2 | 18.1, 2 behind 32,000 22.0 | 26.7 | 32.7.)
+    # keys 34.6 | 28.7 | 32.7 us, 256 behind 32,000 187 | 145 | 161; few only, 64 behind 512 11.0 | 13.1 | 13.2, 24 behind 4,096
+    # 15.5 | 18.5 | 18.2, 16 15.1 | 14.2 | 18.1, 2 behind 32,000 22.0 | 26.7 | 32.7.)
     TARGET, FEW_TARGET = 512, 256
 
     def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device,
@@ -101,8 +104,8 @@ class SharedPrefixes:
         # A run's columns in tiles of many, where there is work for them, and what is left, if that is little, in tiles of few.
         wide = dtype == torch.bfloat16 and head_dim in self.WIDE_HEADS
         size, little = (self.WIDE_COLUMNS, self.WIDE_LITTLE) if wide else (self.MANY_COLUMNS, self.MANY_LITTLE)
-        products = sum(len(run.rows) * (run.key_end - run.key_begin) for run in self.runs) * n_q * head_dim
-        if products <= (self.WIDE_WORK if wide else self.MANY_WORK):
+        scores = sum(len(run.rows) * (run.key_end - run.key_begin) for run in self.runs) * n_q
+        if scores <= (self.WIDE_WORK if wide else self.MANY_WORK):
             little, target = self.n_rows * group, self.FEW_TARGET
         else:
             target = self.TARGET
