@@ -83,10 +83,12 @@ class SharedPrefixes:
     # A shorter run is not a pass and a part to be joined of its own.  (64 requests, 64 keys shared 14.7 us as a run, 14.0 with the
     # requests' own; 256 keys 19.2 and 19.2, and the cache is read less.)
     MIN_KEYS = 64
-    # Keys of a part of a run, at least: a block of 32 for each of its four waves.  (Parts of 64 | 128 | 256 keys, 2 requests of 4,096 keys 13.1 |
-    # 10.6 | 10.6 us, 4 requests of 512 7.4 | 7.1 | 7.8.)  Of a long one a 64th, up to 512: a wave joins 64 parts at a time (2 requests of
-    # 32,000 keys of head size 64 in 250 parts 25.8 us, in 63 12.8).
-    MIN_PART, MIN_WIDE_PART = 128, 256
+    # Keys of a part of a run, at least: a block of 32 for each of its four waves, four blocks of 64 where many columns go through LDS.  (Parts of
+    # 64 | 128 | 256 keys, 2 requests of 4,096 keys 13.1 | 10.6 | 10.6 us, 4 requests of 512 7.4 | 7.1 | 7.8; 128 | 256 | 512 keys, many
+    # columns, 64 requests of 4,096 29.7 | 24.7 | 25.4, of 1,024 17.4 | 17.4 | 21.5.)  Of a long run a 64th (a wave joins 64 parts at a time) or,
+    # through LDS, a 16th, up to LONG_PART: 2 requests of 32,000 keys of head size 64 in 250 parts 25.8 us, in 63 12.8; 64 of 8,192 in parts
+    # of 256 | 512 32.0 | 28.8.
+    MIN_PART, MIN_WIDE_PART, LONG_PART = 128, 256, 512
     OWN_STEP = 128                # `smallest_own` in whole steps: prefixes that differ a little make launches of one shape
     # Workgroups that the parts aim at: two a compute unit; one where all items are of few columns.  (256 | 512 | 768: 64 requests behind 4,096
     # keys 34.6 | 28.7 | 32.7 us, 256 behind 32,000 187 | 145 | 161; few only, 64 behind 512 11.0 | 13.1 | 13.2, 24 behind 4,096
@@ -122,7 +124,8 @@ class SharedPrefixes:
         groups, parts_of = {False: [], True: []}, np.zeros(self.n_rows, dtype=np.int32)      # items that read the same keys and values
         for found, run in zip(tiles, self.runs):
             length = run.key_end - run.key_begin
-            part = max(self.MIN_WIDE_PART if wide and found[0][1] else self.MIN_PART, -(-work // target), min(length // WAVE, 4 * self.MIN_PART))
+            shortest, of_length = (self.MIN_WIDE_PART, length // 16) if wide and found[0][1] else (self.MIN_PART, length // WAVE)
+            part = max(shortest, -(-work // target), min(of_length, self.LONG_PART))
             keys = -(-length // (32 * max(1, length // part))) * 32
             first = int(parts_of[run.rows[0]])
             for split, begin in enumerate(range(run.key_begin, run.key_end, keys)):
