@@ -272,8 +272,10 @@ struct Wide {
     const int d = thread / 2 % D;
     return d * page_size * 2 + 16 * ((thread & 1) ^ ((d >> 3) & 1));
   }
-  static __device__ __forceinline__ sp_bf16x8 key_piece(const char* keys, int key, int piece) {
-    return *reinterpret_cast<const sp_bf16x8*>(keys + key * KEY + 16 * (piece ^ turn(key & 15)));
+  // Where piece `half` of a key (of the block's first half) lies; its piece 2 i + half is at that place with the bits of 32 i turned over.
+  static __device__ __forceinline__ int key_at(int key, int half) { return key * KEY + 16 * (half ^ turn(key & 15)); }
+  static __device__ __forceinline__ sp_bf16x8 key_piece(const char* keys, int part, int at, int i) {
+    return *reinterpret_cast<const sp_bf16x8*>(keys + SP_BLOCK * KEY * part + (at ^ (32 * i)));
   }
   static __device__ __forceinline__ sp_bf16x8 value_piece(const char* values, int unit, int d, int half) {
     return *reinterpret_cast<const sp_bf16x8*>(values + unit * UNIT + d * 32 + 16 * (half ^ ((d >> 3) & 1)));
@@ -292,7 +294,13 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
   const int kvh = scalar_int(item + 7), group = a.n_q / a.n_kv;
   if (columns <= 0) return;                                // an item that only fills the list up
   const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 31, half = lane >> 5;
-  const uint32_t key_place = W::key_place(threadIdx.x), value_place = W::value_place(threadIdx.x, a.page_size);
+  // (At head size 128 worked out anew wherever it is used: kept, such numbers are what no register is left for.  With nine of them in
+  // memory 40 requests behind 32,000 keys took 49 us instead of 44; at 64, kept, 256 requests 62 instead of 64.)
+  auto thread_now = [&] {
+    int of_wave = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    if (D == 128) asm volatile("" : "+v"(of_wave));
+    return wave * WAVE + of_wave;
+  };
   // (A layer's keys are fewer than 2^31 elements: places in bytes fit 32 bits.)
   const uint32_t page_bytes = (uint32_t)a.page_size * D * 2, all_heads = page_bytes * a.n_kv, of_head = page_bytes * kvh;
   const typename W::from_t k_from = (typename W::from_t)a.k_pages, v_from = (typename W::from_t)a.vt_pages;
@@ -310,12 +318,14 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
   };
   auto start = [&](const Units& u, int j) { return (uint32_t)min(max(u.page[j], 0), a.n_pages - 1) * all_heads + of_head; };
   auto fetch_keys = [&](const Units& u, char* to) {
+    const uint32_t key_place = W::key_place(thread_now());
 #pragma unroll
     for (int j = 0; j < W::ROUNDS; ++j)
       __builtin_amdgcn_global_load_lds(k_from + (start(u, j) + (uint32_t)u.at[j] * W::KEY + key_place),
                                        (typename W::lds_t)(to + j * 4096 + wave * 1024), 16, 0, 0);
   };
   auto fetch_values = [&](const Units& u, char* to) {
+    const uint32_t value_place = W::value_place(thread_now(), a.page_size);
 #pragma unroll
     for (int j = 0; j < W::ROUNDS; ++j)
       __builtin_amdgcn_global_load_lds(v_from + (start(u, j) + (uint32_t)u.at[j] * 2 + value_place),
@@ -329,16 +339,19 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
   before = next;                                           // (block b + 1's, whose values come in iteration b; `next`: block b + 2's)
   next = look_up(2);
 
-  const int column = first_column + 32 * wave + col;
-  const bool there = column < columns, wave_there = first_column + 32 * wave < columns;
-  const int row = there ? a.order[rows_at + column / group] : -1, head = kvh * group + column % group;
+  const bool wave_there = first_column + 32 * wave < columns;
   typename F::Query q;
-  F::load_query(q, (const bf16_t*)a.q + (size_t)max(row, 0) * a.q_stride + (size_t)head * D, there, half);
+  {
+    const int column = first_column + 32 * wave + col;
+    const bool there = column < columns;
+    const int row = there ? a.order[rows_at + column / group] : 0, head = kvh * group + column % group;
+    F::load_query(q, (const bf16_t*)a.q + (size_t)row * a.q_stride + (size_t)head * D, there, half);
+  }
   sp_floatx16 o[ROWS];
   float m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) o[r] = (sp_floatx16){};
-  const int my_key = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
+  const int keys_at = W::key_at(16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3), half);
   const float scale = CAPPED ? LOG2E : a.scale * LOG2E;
   const float inner = CAPPED ? 2.f * LOG2E * a.scale / a.softcap : 0.f;
 
@@ -347,8 +360,10 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
   struct Pieces { sp_bf16x8 p[W::STEPS]; };
   auto read_keys = [&](const char* keys, int part) {
     Pieces f;
+    int at = keys_at;
+    if (D == 128) asm volatile("" : "+v"(at));             // (the pieces' places anew as well)
 #pragma unroll
-    for (int i = 0; i < W::STEPS; ++i) f.p[i] = W::key_piece(keys, SP_BLOCK * part + my_key, 2 * i + half);
+    for (int i = 0; i < W::STEPS; ++i) f.p[i] = W::key_piece(keys, part, at, i);
     return f;
   };
   auto read_values = [&](const char* values, int part) {
@@ -445,8 +460,9 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
     iteration(b + 1, keys0, values1, keys1, values0);
   }
   l = wave_add_across<32>(l);
-  if (row < 0) return;
-  const size_t to = ((size_t)row * a.n_q + head) * a.slots + slot;
+  const int column = first_column + 32 * wave + (thread_now() & 31);
+  if (column >= columns) return;
+  const size_t to = ((size_t)a.order[rows_at + column / group] * a.n_q + kvh * group + column % group) * a.slots + slot;
   if (half == 0) st_through(reinterpret_cast<uint2*>(a.part_ml + 2 * to), make_uint2(__float_as_uint(m), __float_as_uint(l)));
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
