@@ -16,12 +16,12 @@
 //   * more, in bfloat16 at head sizes 64 and 128: 128 columns a workgroup, 32 a wave, keys and values through LDS;
 //   * more, of other types and sizes: 32 columns a workgroup, whose waves share the keys out.
 // What bounds them, measured with keys and values of 16 bits in the caches, head size 128, 4 kv heads of 7 query heads:
-//   256 requests behind 32,000 keys: 145 to 172 us with the clock, 9 of them the join; the products are 118 GFLOP, 0.7 to 0.8 PFLOP/s.  The
-//     matrix instructions share the SIMD's issue with one exponential a score and its weight's rounding.
-//   64 requests behind 4,096 keys, in eight families of 512 more, with 20 to 700 of their own: 29 us, 4.4 GFLOP and 43 MB: the chain of a
-//     workgroup's blocks and the join's launch; two workgroups a compute unit are all there are.
+//   256 requests behind 32,000 keys: 150 us, 9 of them the join; the products are 118 GFLOP, 0.79 PFLOP/s.  The matrix instructions share the
+//     SIMD's issue with an exponential a score and its weight's rounding.
+//   64 requests behind 4,096 keys, in eight families of 512 more, with 20 to 700 of their own: 27 us, 4.4 GFLOP and 43 MB: four blocks of
+//     keys a workgroup, some 8 us around them (a chain of loads to the first block, the partial results), and the join, 5.
 //   4 requests behind 512 keys (head size 64): 7 us, two launches of a few dependent loads each.
-// In 32 bits, 21 requests behind 1,040 keys of head size 64: 12.7 us.
+// In 32 bits, 21 requests behind 1,040 keys of head size 64: 12.8 us.
 // Fragments of the 32x32 instructions: row r of a block of 32 keys is key 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4, and lane
 // half h then holds keys 16 s + 8 h .. + 7 of step s of the second product.  Of the 16x16 ones: row r of the first product's
 // instruction t is key 8 (r / 4) + 4 t + r % 4, and lane group g then holds keys 8 g .. 8 g + 7.
