@@ -459,17 +459,31 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
     if (b + 1 >= blocks) break;                            // (the same for the whole workgroup)
     iteration(b + 1, keys0, values1, keys1, values0);
   }
+  // A column's results lie 16 bytes a lane: they go through LDS, so that a store takes whole columns side by side.  Piece p of column c lies at
+  // place p ^ c.
   l = wave_add_across<32>(l);
-  const int column = first_column + 32 * wave + (thread_now() & 31);
-  if (column >= columns) return;
-  const size_t to = ((size_t)a.order[rows_at + column / group] * a.n_q + kvh * group + column % group) * a.slots + slot;
-  if (half == 0) st_through(reinterpret_cast<uint2*>(a.part_ml + 2 * to), make_uint2(__float_as_uint(m), __float_as_uint(l)));
+  const int column = first_column + 32 * wave + col, here = columns - first_column - 32 * wave;
+  int query = 0;
+  if (column < columns) query = a.order[rows_at + column / group] * a.n_q + kvh * group + column % group;
+  if (half == 0 && column < columns)
+    st_through(reinterpret_cast<uint2*>(a.part_ml) + (size_t)query * a.slots + slot, make_uint2(__float_as_uint(m), __float_as_uint(l)));
+  __syncthreads();                                         // the last block has been read
+  char* mine = wave < 2 ? (wave == 0 ? keys0 : keys1) : (wave == 2 ? values0 : values1);
+  constexpr int LANES = D / 2, AT_ONCE = WAVE / LANES;     // of a column; columns a store
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<sp_floatx4*>(a.part_o + to * D + 32 * r + 8 * j + 4 * half) =
+      *reinterpret_cast<sp_floatx4*>(mine + col * 4 * D + 16 * ((8 * r + 2 * j + half) ^ (col & (D / 4 - 1)))) =
           (sp_floatx4){o[r][4 * j], o[r][4 * j + 1], o[r][4 * j + 2], o[r][4 * j + 3]};
+  wave_exchange();
+  const int in_column = lane % LANES;
+#pragma unroll 8
+  for (int c = lane / LANES; c < 32; c += AT_ONCE) {
+    const int to = __shfl(query, c, WAVE);
+    const uint2 v = *reinterpret_cast<const uint2*>(mine + c * 4 * D + 16 * ((in_column >> 1) ^ (c & (D / 4 - 1))) + 8 * (in_column & 1));
+    if (c < here) st_through(reinterpret_cast<uint2*>(a.part_o + ((size_t)to * a.slots + slot) * D) + in_column, v);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
