@@ -333,20 +333,23 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
   };
   const int blocks = (end - begin + SP_WIDE_BLOCK - 1) / SP_WIDE_BLOCK;
   Units before = look_up(0), next = look_up(1);
+  // (The queries are asked for ahead of the keys: which request a column belongs to is looked up while the pages are, and a wait for that would
+  // wait for keys under way as well.)
+  const bool wave_there = first_column + 32 * wave < columns;
+  typename F::Query q;
+  {
+    // (Behind the last column that one stands in: nothing of it is stored.)
+    const int column = min(first_column + 32 * wave + col, columns - 1);
+    const int row = a.order[rows_at + column / group], head = kvh * group + column % group;
+    __builtin_amdgcn_sched_barrier(0);                     // (the pages and the request are asked for by here)
+    F::load_query(q, (const bf16_t*)a.q + (size_t)row * a.q_stride + (size_t)head * D, true, half);
+  }
   fetch_keys(before, keys0);
   fetch_values(before, values0);
   fetch_keys(next, keys1);
   before = next;                                           // (block b + 1's, whose values come in iteration b; `next`: block b + 2's)
   next = look_up(2);
 
-  const bool wave_there = first_column + 32 * wave < columns;
-  typename F::Query q;
-  {
-    const int column = first_column + 32 * wave + col;
-    const bool there = column < columns;
-    const int row = there ? a.order[rows_at + column / group] : 0, head = kvh * group + column % group;
-    F::load_query(q, (const bf16_t*)a.q + (size_t)row * a.q_stride + (size_t)head * D, there, half);
-  }
   sp_floatx16 o[ROWS];
   float m = -INFINITY, l = 0.f;
 #pragma unroll
