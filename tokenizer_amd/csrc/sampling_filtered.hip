@@ -801,7 +801,7 @@ struct FsArgs {
   const float *temperature, *top_p, *min_p, *uniform;
   const int* top_k;
   int* out;
-  int vocab, pieces, span;              // span: pieces that a workgroup sees to behind the first pass
+  int vocab, pieces, shares;            // shares: workgroups of a row behind the first pass, SPAN pieces each
   char* workspace;
   size_t row_bytes;
 };
@@ -863,7 +863,7 @@ struct FsBinned { u64 mass[FS_BINS]; uint32_t count[FS_BINS]; u64 over; u64 unus
 // pieces' bins.
 struct FsSpace {
   char* base;
-  int pieces, binned_pieces;
+  int pieces, shares;
   __device__ __forceinline__ FsHead* head() const { return (FsHead*)base; }
   __device__ __forceinline__ FsBinned* whole() const { return (FsBinned*)(base + sizeof(FsHead)); }
   __device__ __forceinline__ u64* list() const { return (u64*)(whole() + 1); }
@@ -876,7 +876,7 @@ static size_t fs_row_bytes(int pieces) {
   return sizeof(FsHead) + sizeof(FsBinned) + 8 * FS_LIST + (sizeof(FsExtent) + 4 * (FS_PIECE_WAVES + FS_PIECE_ROWS) + sizeof(FsBinned)) * (size_t)pieces;
 }
 static_assert(sizeof(FsHead) % 16 == 0 && sizeof(FsBinned) % 16 == 0 && sizeof(FsExtent) % 16 == 0 && (FS_PIECE_WAVES + FS_PIECE_ROWS) % 4 == 0, "pieces of sixteen bytes");
-__device__ __forceinline__ FsSpace fs_space(const FsArgs& a, int row) { return FsSpace{a.workspace + (size_t)row * a.row_bytes, a.pieces, (a.pieces + a.span - 1) / a.span}; }
+__device__ __forceinline__ FsSpace fs_space(const FsArgs& a, int row) { return FsSpace{a.workspace + (size_t)row * a.row_bytes, a.pieces, a.shares}; }
 
 // The row's extent from its pieces' (a lane of every wave looks at one piece of sixty-four), to every thread.
 __device__ __forceinline__ void fs_row_extent(const FsSpace& w, float& high, float& low) {
@@ -1078,20 +1078,20 @@ __device__ __forceinline__ FsRanges fs_settle(const FsSpace& w, const FsAsked& a
   u64 m = 0;
   uint32_t c = 0;
   over = 0;
-  for (int first = 0; first < w.binned_pieces; first += 16) {     // (sixteen pieces asked for at a time)
+  for (int first = 0; first < w.shares; first += 16) {     // (sixteen pieces asked for at a time)
     u64 of_mass[16];
     uint32_t of_count[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const FsBinned& piece = w.binned()[min(first + j, w.binned_pieces - 1)];
+      const FsBinned& piece = w.binned()[min(first + j, w.shares - 1)];
       of_mass[j] = piece.mass[threadIdx.x];
       of_count[j] = piece.count[threadIdx.x];
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (first + j < w.binned_pieces) { m += of_mass[j]; c += of_count[j]; }
+      if (first + j < w.shares) { m += of_mass[j]; c += of_count[j]; }
   }
-  for (int p = threadIdx.x; p < w.binned_pieces; p += FS_THREADS) over += w.binned()[p].over;
+  for (int p = threadIdx.x; p < w.shares; p += FS_THREADS) over += w.binned()[p].over;
   s.mass[threadIdx.x] = m;
   s.count[threadIdx.x] = c;
   over = fs_sum<FS_THREADS>(over, s);
@@ -1114,7 +1114,10 @@ __device__ __forceinline__ void fs_draw_listed(const FsArgs& a, const FsSpace& w
 template <int SPAN, typename T>
 __device__ __forceinline__ void fs_gather(const FsArgs& a, const FsSpace& w, const T* row, const FsRow& r, const FsRanges& ranges, FsSmall& s) {
   const int last_bin = max(ranges.k_bin, max(ranges.p_last, ranges.draw_last));
-  for (int p = blockIdx.x * SPAN; p < min((int)blockIdx.x * SPAN + SPAN, a.pieces); ++p) {
+#pragma unroll
+  for (int j = 0; j < SPAN; ++j) {
+    const int p = blockIdx.x * SPAN + j;
+    if (SPAN > 1 && p >= a.pieces) break;                  // (the same for the whole workgroup)
     const float of_row = w.of_rows()[p * FS_PIECE_ROWS + threadIdx.x / 16];
     float v[FS_EACH];
     // (A row of sixteen lanes whose maximum lies behind all the ranges has nothing in them.)
@@ -1223,7 +1226,7 @@ sample_filtered_finish(FsArgs a) {
     __threadfence();                                       // and so is what the others left before they counted themselves in
   }
   __syncthreads();
-  if (came != w.binned_pieces - 1) return;                        // (the same for the whole workgroup)
+  if (came != w.shares - 1) return;                        // (the same for the whole workgroup)
   const int n = __hip_atomic_load(&w.head()->n_listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   fs_draw_listed<T>(a, w, asked, r, row_at, &ranges, over, n, s);
 }
@@ -1241,8 +1244,8 @@ extern "C" int ta_sample_filtered_workspace(int vocab) { return fs_is_short(voca
 // The passes of long rows behind the first: so many pieces a workgroup.
 template <typename T, int SPAN>
 static int launch_long(FsArgs a, int n_rows, hipStream_t stream) {
-  a.span = SPAN;
-  const dim3 grid((a.pieces + SPAN - 1) / SPAN, n_rows);
+  a.shares = (a.pieces + SPAN - 1) / SPAN;
+  const dim3 grid(a.shares, n_rows);
   sample_filtered_bins<T, SPAN><<<grid, FS_THREADS, 0, stream>>>(a);
   int status = LAUNCH_STATUS();
   if (status) return status;
@@ -1286,7 +1289,7 @@ extern "C" int ta_sample_filtered(const void* logits, int64_t stride, const void
   FsArgs a;
   a.logits = logits; a.stride = stride; a.temperature = (const float*)temperature; a.top_p = (const float*)top_p;
   a.min_p = (const float*)min_p; a.uniform = (const float*)uniform; a.top_k = (const int*)top_k; a.out = (int*)out;
-  a.vocab = vocab; a.pieces = fs_pieces(vocab); a.span = 1; a.workspace = (char*)workspace;
+  a.vocab = vocab; a.pieces = fs_pieces(vocab); a.shares = a.pieces; a.workspace = (char*)workspace;
   a.row_bytes = fs_row_bytes(a.pieces);
   return dtype == DT_F32 ? launch_filtered<float>(a, n_rows, stream) : launch_filtered<bf16_t>(a, n_rows, stream);
 }
