@@ -205,9 +205,9 @@ def test_a_draw_does_not_depend_on_the_batch(ops):
         assert torch.equal(whole[part], ops.sample_filtered(logits[part], **{n: t[part].contiguous() for n, t in numbers.items()}))
 
 
-@pytest.mark.parametrize("rows", [1, 8, 9, 40])
+@pytest.mark.parametrize("rows", [1, 8, 9, 19, 20, 40])
 def test_draws_of_few_and_many_long_rows(ops, rows):
-    # (Up to eight rows are gathered and drawn in one launch.)
+    # (Rows of up to 256 pieces of 4,096 logits together are gathered and drawn in one launch.)
     logits = hills(rows, 50001, torch.float32, rows, 3.0)
     rng = np.random.default_rng(rows)
     for given in (dict(), dict(top_p=0.9), dict(top_k=30), dict(top_k=rng.integers(0, 2, rows) * 40, top_p=rng.uniform(0.5, 1.1, rows)),

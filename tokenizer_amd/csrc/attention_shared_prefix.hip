@@ -16,10 +16,10 @@
 //   * more, in bfloat16 at head sizes 64 and 128: 128 columns a workgroup, 32 a wave, keys and values through LDS;
 //   * more, of other types and sizes: 32 columns a workgroup, whose waves share the keys out.
 // What bounds them, measured with keys and values of 16 bits in the caches, head size 128, 4 kv heads of 7 query heads:
-//   256 requests behind 32,000 keys: 150 us, 9 of them the join; the products are 118 GFLOP, 0.79 PFLOP/s.  The matrix instructions share the
+//   256 requests behind 32,000 keys: 146 us, 9 of them the join; the products are 118 GFLOP, 0.8 PFLOP/s.  The matrix instructions share the
 //     SIMD's issue with an exponential a score and its weight's rounding.
-//   64 requests behind 4,096 keys, in eight families of 512 more, with 20 to 700 of their own: 27 us, 4.4 GFLOP and 43 MB: four blocks of
-//     keys a workgroup, some 8 us around them (a chain of loads to the first block, the partial results), and the join, 5.
+//   64 requests behind 4,096 keys, in eight families of 512 more, with 20 to 700 of their own: 25 us, 4.4 GFLOP and 43 MB: four blocks of
+//     keys a workgroup, some 7 us around them (a chain of loads to the first block, the partial results), and the join, 5.
 //   4 requests behind 512 keys (head size 64): 7 us, two launches of a few dependent loads each.
 // In 32 bits, 21 requests behind 1,040 keys of head size 64: 12.8 us.
 // Fragments of the 32x32 instructions: row r of a block of 32 keys is key 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4, and lane

@@ -44,7 +44,10 @@
 #define FS_LIST 8192
 #define FS_FEW 128
 #define FS_SLOTS 256                    // ranges that a round of narrowing tells apart
-#define FS_FEW_ROWS 8                   // up to so many long rows take three launches instead of five
+// Long rows of up to so many pieces together (a compute unit each) take three launches instead of five.  (Three | five, us on the device alone:
+// rows of 151,936, 2 rows under top-p 23.2 | 24.7, under top-k 40 15.9 | 18.6, 6 rows 35.5 | 33.5, 15.9 | 18.4; rows of 32,000, 16 rows
+// 22.6 | 24.4, 16.5 | 19.6, 32 rows 26.9 | 24.6, 16.7 | 20.2; and two launches less for the host.)
+#define FS_FEW_PIECES 256
 #define FS_SPAN 4                       // pieces that a workgroup sees to in the passes behind the first ...
 // ... from so many pieces of all rows on.  (One | four pieces a workgroup, us: rows of 151,936 under min-p, 128 rows 34.8 | 33.9, 256 54.3 |
 // 47.8, 512 104 | 84; under top-k 40 47.5 | 40.5, 77 | 64, 148 | 120; under top-p 81 | 85, 136 | 137, 267 | 239; rows of 32,000 under
@@ -1249,7 +1252,7 @@ static int launch_long(FsArgs a, int n_rows, hipStream_t stream) {
   sample_filtered_bins<T, SPAN><<<grid, FS_THREADS, 0, stream>>>(a);
   int status = LAUNCH_STATUS();
   if (status) return status;
-  if (SPAN == 1 && n_rows <= FS_FEW_ROWS) {
+  if (SPAN == 1 && a.pieces * n_rows <= FS_FEW_PIECES) {
     sample_filtered_finish<T><<<grid, FS_THREADS, 0, stream>>>(a);
     return LAUNCH_STATUS();
   }
