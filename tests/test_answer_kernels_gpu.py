@@ -591,7 +591,8 @@ def test_attention_refused(ops):
                 positions=torch.tensor(positions, dtype=torch.int32).cuda(), block_table=batch.table.cuda(), plan=plan, n_q=4, n_kv=2,
                 head_dim=64, scale=0.125)
     ops.shared_prefix_attention(**args)
-    for bad in (dict(qkv=args["qkv"][:2].contiguous()), dict(qkv=args["qkv"].float()), dict(out=args["out"][:, :128].contiguous()), dict(n_q=2),
+    for bad in (dict(qkv=args["qkv"][:2].contiguous()), dict(qkv=args["qkv"][None]), dict(v_pages=args["v_pages"][1:].contiguous()),
+                dict(k_pages=args["k_pages"][1:].contiguous()), dict(block_table=args["block_table"][0]), dict(qkv=args["qkv"].float()), dict(out=args["out"][:, :128].contiguous()), dict(n_q=2),
                 dict(head_dim=32), dict(block_table=args["block_table"][:, :4].contiguous()), dict(block_table=args["block_table"].long()),
                 dict(positions=args["positions"][:2]), dict(k_pages=args["k_pages"].transpose(2, 3)), dict(v_pages=args["k_pages"]),
                 dict(max_position=16 * batch.table.shape[1]), dict(sinks=torch.zeros(3).cuda()), dict(softcap=-1.0),

@@ -73,6 +73,15 @@ __device__ __forceinline__ void sp_page_of(const SharedArgs& a, int key, int& in
   }
 }
 
+// A cap on a score: cap tanh(x), x = `inner` / (2 log2(e)) times the raw one.  1 - 2 / (1 + e^2x) is off by some roundings of one, that is of the
+// cap: for bfloat16 nothing beside the weights' rounding, in 32 bits as much again as all else (1.4e-6 of a result's norm instead of 7e-7), so
+// there tanh itself is called.
+template <typename T>
+__device__ __forceinline__ float sp_capped(float raw, float inner, float cap) {
+  if constexpr (sizeof(T) == 4) return cap * tanhf(raw * (inner * (0.5f / LOG2E)));
+  return cap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(inner * raw)));
+}
+
 // The fragments of one type: how a block of 32 keys, the queries and the weights lie in registers, and the products.
 template <typename T, int D> struct Frag;
 
@@ -171,6 +180,14 @@ struct Frag<float, D> {
         if (16 * (i >> 3) + 8 * half + (i & 7) >= there) v[r][i >> 2][i & 3] = 0.f;
   }
   __device__ __forceinline__ sp_floatx16 scores(const Query& q) const {
+    if constexpr (D <= 96) {                               // (two sums, as below; above there are no registers for them)
+      sp_floatx16 s[2] = {};
+#pragma unroll
+      for (int e = 0; e < EIGHTS; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e][i], q.f[e][i], s[i & 1], 0, 0, 0);
+      return s[0] + s[1];
+    }
     sp_floatx16 s = {};
 #pragma unroll
     for (int e = 0; e < EIGHTS; ++e)
@@ -192,7 +209,7 @@ struct Frag<float, D> {
 //   The maximum is a reference alone: a weight may be up to 2^SP_SLACK as long as no rescaling has been due (rescaling at every new maximum
 //   of any of 32 columns came up in nearly every block: 64 of 220 vector instructions of a block of 64 keys at head size 128).
 #define SP_SLACK 8.f
-template <int BLOCKS, int ROWS>
+template <typename T, int BLOCKS, int ROWS>
 __device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)[BLOCKS], int there, int half, float& m, float& l,
                                            sp_floatx16 (&o)[ROWS]) {
   float scale = a.scale * LOG2E;
@@ -201,7 +218,7 @@ __device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[b][i] = a.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(inner * s[b][i])));
+      for (int i = 0; i < 16; ++i) s[b][i] = sp_capped<T>(s[b][i], inner, a.softcap);
     scale = LOG2E;
   }
   if (there < BLOCKS * SP_BLOCK) {
@@ -389,7 +406,7 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
   auto settle = [&](sp_floatx16& s, int here) {
     if (CAPPED) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = a.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(inner * s[i])));
+      for (int i = 0; i < 16; ++i) s[i] = sp_capped<bf16_t>(s[i], inner, a.softcap);
     }
     if (here < SP_BLOCK) {
       asm volatile("");                                    // (a branch: worked out for every step the cuts are 48 instructions of it)
@@ -549,7 +566,7 @@ shared_prefix_kernel(SharedArgs a) {
 #pragma unroll
     for (int c = 0; c < COLS; ++c) {
       sp_floatx16 s[1] = {f.scores(q[c])};
-      sp_softmax<1, ROWS>(a, s, there, half, m[c], l[c], o[c]);
+      sp_softmax<T, 1, ROWS>(a, s, there, half, m[c], l[c], o[c]);
       f.add_values(s[0], o[c]);
     }
   }
@@ -701,12 +718,13 @@ struct Frag16<float, D> {
         if (i >= there) v[r][i >> 2][i & 3] = 0.f;
   }
   __device__ __forceinline__ sp_floatx4 scores(int t, const Query& q) const {
-    sp_floatx4 s = {0.f, 0.f, 0.f, 0.f};
+    // (Four sums of a quarter of the coordinates each: a sum's roundings grow with its length, and no instruction waits for the one before.)
+    sp_floatx4 s[4] = {};
 #pragma unroll
     for (int e = 0; e < STEPS; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][e][i], q.f[e][i], s, 0, 0, 0);
-    return s;
+      for (int i = 0; i < 4; ++i) s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][e][i], q.f[e][i], s[i], 0, 0, 0);
+    return (s[0] + s[1]) + (s[2] + s[3]);
   }
   __device__ __forceinline__ void add_values(const float (&p)[8], sp_floatx4 (&o)[ROWS]) const {
 #pragma unroll
@@ -815,7 +833,7 @@ __device__ __forceinline__ void sp_few(const SharedArgs& a, int block, float* o0
     }
     if (a.softcap > 0.f) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = a.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(inner * s[i])));
+      for (int i = 0; i < 8; ++i) s[i] = sp_capped<T>(s[i], inner, a.softcap);
     }
     if (here < SP_BLOCK) {
 #pragma unroll

@@ -1567,23 +1567,33 @@ class Ops:
         position -1 none: its result is zero).  `sinks` (float32 [n_q]): exp(sinks[h]) joins the denominator; `softcap` c: a
         scaled score s becomes c tanh(s / c).  `max_position` (host): the largest position, for the launch's size."""
         _here(qkv, out, k_pages, v_pages, positions, block_table, plan.packed, sinks)
-        n_rows, row_elements = qkv.shape
-        dtype = qkv.dtype
-        _need(plan.n_rows == n_rows and (plan.n_q, plan.n_kv, plan.head_dim, plan.dtype) == (n_q, n_kv, head_dim, dtype),
-              "the plan belongs to other rows or to another shape of attention")
-        _need(row_elements >= n_q * head_dim and row_elements * qkv.element_size() % 16 == 0 and qkv.data_ptr() % 16 == 0,
-              "qkv holds the query heads first, in rows of whole 16 bytes")
-        _need(out.shape == (n_rows, n_q * head_dim) and out.dtype == dtype, "attention output shape")
-        _need(k_pages.dtype == dtype and v_pages.dtype == dtype, "pages must have the dtype of qkv")
-        page_size = self._page_size(k_pages, v_pages, n_kv, head_dim)
-        _need(page_size == plan.page_size, "the plan belongs to pages of another size")
-        _need(k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0, "pages start at whole 16 bytes")
-        _need(positions.dtype == torch.int32 and positions.numel() == n_rows, "positions must be int32 [B]")
-        _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == n_rows, "block_table must be int32 [B, P]")
+        # (Every call of an eager step pays for what is asked here: shapes are taken once and compared whole.)
+        shape, dtype, table_shape, k_shape, page_size = qkv.shape, qkv.dtype, block_table.shape, k_pages.shape, plan.page_size
+        _need(len(shape) == 2, "qkv is [B, >= n_q d]")
+        n_rows, row_elements = shape
+        if (n_rows, n_q, n_kv, head_dim, dtype) != plan.belongs_to:
+            raise KernelError("the plan belongs to other rows or to another shape of attention")
+        if row_elements < n_q * head_dim or row_elements * qkv.element_size() % 16 or qkv.data_ptr() % 16:
+            raise KernelError("qkv holds the query heads first, in rows of whole 16 bytes")
+        if out.shape != (n_rows, n_q * head_dim) or out.dtype != dtype:
+            raise KernelError("attention output shape")
+        if k_pages.dtype != dtype or v_pages.dtype != dtype:
+            raise KernelError("pages must have the dtype of qkv")
+        n_pages = k_shape[0]
+        if k_shape != (n_pages, n_kv, page_size, head_dim) or v_pages.shape != (n_pages, n_kv, head_dim, page_size) or \
+                n_pages * n_kv * page_size * head_dim >= 2 ** 31:
+            self._page_size(k_pages, v_pages, n_kv, head_dim)          # (which says what is wrong with the pages, if anything is)
+            raise KernelError("the plan belongs to pages of another size")
+        if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
+            raise KernelError("pages start at whole 16 bytes")
+        if positions.dtype != torch.int32 or positions.numel() != n_rows:
+            raise KernelError("positions must be int32 [B]")
+        if block_table.dtype != torch.int32 or len(table_shape) != 2 or table_shape[0] != n_rows:
+            raise KernelError("block_table must be int32 [B, P]")
         _need(sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == n_q), "sinks are float32 [n_q]")
         _need(softcap is None or softcap > 0, "a cap on the scores is positive")
         _need(scale > 0, "the scores' scale is positive")
-        width = block_table.shape[1]
+        width = table_shape[1]
         _need(plan.keys_end <= width * page_size, "block table is too narrow for the shared keys")
         if max_position is None:
             max_position = width * page_size - 1
@@ -1607,7 +1617,7 @@ class Ops:
             _address(qkv), row_elements, _address(out), _address(k_pages), _address(v_pages), _address(packed, items), plan.n_few, plan.n_many,
             _address(packed, order), _address(packed, own), _address(packed, own_of_row), _address(positions), _address(block_table), width,
             _address(sinks), _address(partial), _address(partial, 4 * values), slots, own_splits, own_keys, n_rows, n_q, n_kv, head_dim,
-            page_size, k_pages.shape[0], scale, softcap or 0.0, _code(dtype), self._stream()), "shared_prefix_attention")
+            page_size, n_pages, scale, softcap or 0.0, _code(dtype), self._stream()), "shared_prefix_attention")
         return out
 
     def talking_attention(self, qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,

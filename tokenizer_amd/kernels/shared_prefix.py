@@ -100,6 +100,7 @@ class SharedPrefixes:
         table = np.asarray(block_table, dtype=np.int32)
         self.n_rows, self.page_size, self.n_q, self.n_kv, self.head_dim, self.dtype = (
             table.shape[0], int(page_size), int(n_q), int(n_kv), int(head_dim), dtype)
+        self.belongs_to = (self.n_rows, self.n_q, self.n_kv, self.head_dim, dtype)
         self.order, self.runs, own_begin = find_shared_runs(table, positions, page_size, self.MIN_KEYS)
         place = {row: at for at, row in enumerate(self.order)}
         group = n_q // n_kv
