@@ -21,7 +21,7 @@
 //   64 requests behind 4,096 keys, in eight families of 512 more, with 20 to 700 of their own: 25 us, 4.4 GFLOP and 43 MB: four blocks of
 //     keys a workgroup, some 7 us around them (a chain of loads to the first block, the partial results), and the join, 5.
 //   4 requests behind 512 keys (head size 64): 7 us, two launches of a few dependent loads each.
-// In 32 bits, 21 requests behind 1,040 keys of head size 64: 12.8 us.
+// In 32 bits, 21 requests behind 1,040 keys of head size 64: 12.5 us.
 // Fragments of the 32x32 instructions: row r of a block of 32 keys is key 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4, and lane
 // half h then holds keys 16 s + 8 h .. + 7 of step s of the second product.  Of the 16x16 ones: row r of the first product's
 // instruction t is key 8 (r / 4) + 4 t + r % 4, and lane group g then holds keys 8 g .. 8 g + 7.
@@ -74,8 +74,8 @@ __device__ __forceinline__ void sp_page_of(const SharedArgs& a, int key, int& in
 }
 
 // A cap on a score: cap tanh(x), x = `inner` / (2 log2(e)) times the raw one.  1 - 2 / (1 + e^2x) is off by some roundings of one, that is of the
-// cap: for bfloat16 nothing beside the weights' rounding, in 32 bits as much again as all else (1.4e-6 of a result's norm instead of 7e-7), so
-// there tanh itself is called.
+// cap: for bfloat16 nothing beside the weights' rounding, in 32 bits more than all else (1.4e-6 of a result's norm instead of 6e-7), so there
+// tanh itself is called.
 template <typename T>
 __device__ __forceinline__ float sp_capped(float raw, float inner, float cap) {
   if constexpr (sizeof(T) == 4) return cap * tanhf(raw * (inner * (0.5f / LOG2E)));
@@ -180,20 +180,15 @@ struct Frag<float, D> {
         if (16 * (i >> 3) + 8 * half + (i & 7) >= there) v[r][i >> 2][i & 3] = 0.f;
   }
   __device__ __forceinline__ sp_floatx16 scores(const Query& q) const {
-    if constexpr (D <= 96) {                               // (two sums, as below; above there are no registers for them)
-      sp_floatx16 s[2] = {};
-#pragma unroll
-      for (int e = 0; e < EIGHTS; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e][i], q.f[e][i], s[i & 1], 0, 0, 0);
-      return s[0] + s[1];
-    }
-    sp_floatx16 s = {};
+    // (Sums of half of the coordinates each, as with few columns; a quarter, where the registers of the one wave a SIMD leave room.)
+    constexpr int SUMS = D >= 112 && D <= 160 ? 4 : 2;
+    sp_floatx16 s[SUMS] = {};
 #pragma unroll
     for (int e = 0; e < EIGHTS; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e][i], q.f[e][i], s, 0, 0, 0);
-    return s;
+      for (int i = 0; i < 4; ++i) s[i % SUMS] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e][i], q.f[e][i], s[i % SUMS], 0, 0, 0);
+    if constexpr (SUMS == 4) return (s[0] + s[1]) + (s[2] + s[3]);
+    return s[0] + s[1];
   }
   __device__ __forceinline__ void add_values(const sp_floatx16& p, sp_floatx16 (&o)[ROWS]) const {
 #pragma unroll
