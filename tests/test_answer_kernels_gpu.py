@@ -138,6 +138,18 @@ def test_a_uniform_number_past_its_range_takes_an_end(ops):
     assert ops.sample_filtered(logits, **numbers).cpu().tolist() == [int(order[0, 8]), int(order[1, 8]), int(order[2, 0]), int(order[3, 0])]
 
 
+@pytest.mark.parametrize("vocab", [7, 3000, 20000, 151936])
+@pytest.mark.parametrize("min_p", [1.0, 1.0 + 2.0 ** -23, 2.0, float("inf")])
+def test_a_share_above_one_leaves_the_first_of_equal_maxima(ops, vocab, min_p):
+    # No token weighs more than the first one: nothing but that is left, whichever of the equal maxima the uniform number would point at.
+    logits = hills(6, vocab, torch.float32, 13)
+    logits[:, 1::2] = 9.0                                    # (a few rows of the long ones reach higher by themselves)
+    first = np.argmax(logits.cpu().numpy(), axis=1).tolist()
+    for given in (dict(), dict(top_k=3), dict(top_p=0.9), dict(top_k=vocab)):
+        got = check_draws(ops, logits, min_p=min_p, uniform=[0.0, 0.2, 0.4, 0.6, 0.8, 0.99], **given)
+        assert min_p == 1.0 or got == first
+
+
 def test_a_flat_row_is_drawn_to_the_token(ops):
     # 150,000 tokens of nearly one weight: 32-bit weights' sums would be tokens away from the border.
     gen = torch.Generator().manual_seed(11)

@@ -112,6 +112,10 @@ __device__ __forceinline__ int fs_bin(float v, const FsRow& r) {
 
 struct FsAsked { float temperature, top_p, min_p, uniform; int top_k; };
 
+// The weight of what min-p keeps, from that of the tokens whose share reaches it and of the maxima: above one no share reaches it, and the order's
+// first token alone is kept (equal maxima weigh 2^44 each).
+__device__ __forceinline__ u64 fs_kept_by_floor(const FsAsked& asked, u64 over) { return asked.min_p > 1.f ? 1ull << 44 : over; }
+
 struct FsSmall {
   u64 mass[FS_BINS];                    // the bins, of a piece or of the whole row
   uint32_t count[FS_BINS];
@@ -471,7 +475,7 @@ __device__ int fs_draw_by_narrowing(FsShared& s, const T* row, int vocab, const 
       if (!(asked.min_p > 0.f) || !(share < floor_share) || v == r.top) over += w;
     }
   });
-  over = fs_sum<THREADS>(over, s);
+  over = fs_kept_by_floor(asked, fs_sum<THREADS>(over, s));
   FsRunning run;
   run.of(s);
   auto crossing = [&](int bin, bool counting, u64 need) {
@@ -570,7 +574,7 @@ __device__ __forceinline__ int fs_answers(FsShared& s, const FsRow& r, const FsA
   if (above) atomicMax(&s.over, above);
   __syncthreads();
   u64 kept = s.kept;
-  if (all_listed) over = s.over;
+  if (all_listed) over = fs_kept_by_floor(asked, s.over);
   if (asked.top_p < 1.f) {
     __syncthreads();
     const u64 need = fs_need_of_share(asked.top_p, kept);
@@ -838,7 +842,7 @@ sample_filtered_short(FsArgs a) {
   }
   const FsRow r = fs_row(asked.temperature, high, low);
   fs_clear_bins(s);
-  const u64 over = fs_sum<THREADS>(fs_fill_bins(v, r, asked, s), s);     // (its barriers stand behind the bins, too)
+  const u64 over = fs_kept_by_floor(asked, fs_sum<THREADS>(fs_fill_bins(v, r, asked, s), s));     // (its barriers stand behind the bins, too)
   FsRunning run;
   run.of(s);
   const FsRanges ranges = fs_ranges(run, asked, over);
@@ -1097,7 +1101,7 @@ __device__ __forceinline__ FsRanges fs_settle(const FsSpace& w, const FsAsked& a
   for (int p = threadIdx.x; p < w.shares; p += FS_THREADS) over += w.binned()[p].over;
   s.mass[threadIdx.x] = m;
   s.count[threadIdx.x] = c;
-  over = fs_sum<FS_THREADS>(over, s);
+  over = fs_kept_by_floor(asked, fs_sum<FS_THREADS>(over, s));
   FsRunning run;
   run.of(s);
   return fs_ranges(run, asked, over);
