@@ -197,6 +197,61 @@ def test_draws_under_counts_around_those_of_the_waves(ops, vocab):
         check_draws(ops, logits, top_k=counts, uniform=np.linspace(0, 0.9999, len(counts)), **given)
 
 
+@pytest.mark.parametrize("rows", [1, 9, 40])
+@pytest.mark.parametrize("vocab", [8193, 60000, 151936])
+def test_draws_where_a_floor_keeps_few_or_thousands(ops, rows, vocab):
+    # Under min-p alone (and under a top-k that fewer parts of the row reach than it asks for) a row is listed only where the list is short.
+    logits = hills(rows, vocab, torch.float32, rows, 2.2)
+    logits[::3, vocab // 7:] = float("-inf")                 # neighbours alone are allowed
+    logits[1::3, ::64] += 7.0                                # some stand out
+    rng = np.random.default_rng(rows)
+    for given in (dict(min_p=1e-9), dict(min_p=1e-3), dict(min_p=0.01, temperature=1.5), dict(min_p=0.05), dict(top_k=40), dict(top_k=200),
+                  dict(top_k=150, min_p=1e-6), dict(min_p=10.0 ** rng.uniform(-8, 0, rows), top_k=rng.integers(0, 2, rows) * 30),
+                  dict(min_p=1e-30, temperature=1e30), dict(min_p=0.5, temperature=1e-3)):
+        check_draws(ops, logits, uniform=rng.uniform(0, 1, rows), **given)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [196609, 256000, 1 << 19])
+def test_draws_from_the_largest_vocabularies(ops, vocab, dtype):
+    logits = hills(5, vocab, dtype, 14, 2.5)
+    logits[3, vocab // 9:] = float("-inf")
+    for given in (dict(top_k=[1, 40, 300, 50, 1000]), dict(top_k=[255, 256, 257, 1023, 1024], top_p=0.9), dict(min_p=[0.1, 0.02, 1e-3, 0.01, 1e-6]),
+                  dict(top_p=0.7), dict(top_k=[0, 60, 0, 500, 512], min_p=0.03, top_p=[1.0, 0.95, 0.9, 1.0, 1.0])):
+        check_draws(ops, logits, uniform=[0.1, 0.9, 0.5, 0.7, 0.3], **given)
+
+
+@pytest.mark.parametrize("name,logits,given", [("a low floor", "flat", dict(min_p=1e-6)), ("a floor that keeps thousands", "flat", dict(min_p=0.01, temperature=1.5)),
+                                               ("neighbours alone", "neighbours", dict(top_k=40))], ids=lambda v: v if isinstance(v, str) else "")
+def test_a_filter_of_many_tokens_costs_about_what_all_tokens_cost(ops, name, logits, given):
+    # (Rows that one workgroup went through again and again took three to thirteen times as long as the same rows without the filter.)
+    rows = hills(8, 151936, torch.float32, 15, 2.2)
+    if logits == "neighbours":
+        rows[:, 20000:] = float("-inf")
+
+    def time_of(numbers):
+        run = lambda: ops.sample_filtered(rows, **numbers)
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        best = float("inf")
+        for _ in range(5):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            for _ in range(10):
+                graph.replay()
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, start.elapsed_time(end))
+        return best
+
+    numbers = settings(8, uniform=np.arange(8) / 8.0, **given)
+    check_draws(ops, rows, uniform=np.arange(8) / 8.0, **given)
+    assert time_of(numbers) < 2.5 * time_of(settings(8, uniform=np.arange(8) / 8.0))
+
+
 def test_draws_from_rows_that_lie_apart_and_into_a_given_place(ops):
     wide = hills(9, 3001, torch.float32, 4)
     numbers = settings(9, uniform=np.arange(9) / 9.0, top_k=30)

@@ -15,20 +15,20 @@
 // No row is sorted whole: the tokens among which the answers lie, some hundreds, are gathered and ordered in LDS.
 //   * Where the first k tokens are all that counts, or those that min-p keeps, a logit is known below which nothing does
 //     (`fs_cut`): the k-th largest of the maxima of the row's parts, of which at least k tokens are no smaller, or
-//     max + T ln(min_p).  What is not below it is the list.
+//     max + T ln(min_p).  What is not below it is the list, where those maxima say that it is short.
 //   * Else every token's weight matters.  The tokens fall into FS_BINS ranges of logit, equal parts of what lies between the maximum and the
 //     lowest logit that weighs anything, each with its count and weight; the answers then lie in a few ranges (what is not known
 //     yet of an earlier answer is at most a range's weight), whose tokens are the list.
-// Should there be more than FS_LIST of them (thousands of equal logits), one workgroup goes through the row again and again and
-// narrows the answer's range by counting, key by key.
+// Should there be more than FS_LIST of them (thousands of logits that are equal, or nearly beside the row's whole range), one workgroup goes
+// through the row again and again and narrows the answer's range by counting, key by key.
 //
 // What bounds it, measured with logits of 32 bits in the caches (the operator's own launches, replayed):
 //   one row of 151,936 under top-k 40: 14.6 us, a chain of three launches (extents 3.6, the list 6.0, the draw 6.0 with the profiler's
 //     share), each a few dependent steps of one workgroup a piece; reading 0.6 MB would take 0.1.  Under top-p alone 22.
 //   64 rows of 151,936, each under other limits: 31 us: the extents 8.8, the second reading 11.5 (weights in 64 bits where the bins are
 //     needed), ordering the lists 9.2, the gathering and the draws 4.6.
-//   256 rows of 152,064 under min-p: 53 us: the extents 25 (156 MB at 6.2 TB/s), the list 14, the draw 9; a row read once at the rate of a
-//     large copy would take 31.  Under top-p alone, where every token's weight and bin is worked out, 134.
+//   256 rows of 152,064 under min-p: 55 us: the extents 25 (156 MB at 6.2 TB/s), the list 16, the draw 9; a row read once at the rate of a
+//     large copy would take 31.  Rows of 151,936 flat logits of which min-p keeps thousands or all: 8 rows 37, 256 rows 144 to 171.  Under top-p alone, where every token's weight and bin is worked out, 134.
 // A workgroup has 4,096 logits, sixteen a thread, all asked for at once; a single row is then 38 workgroups.
 //
 // NaN is no token.  A row without a finite maximum, and a row whose temperature is not positive, gets its first maximum (0 if it
@@ -123,7 +123,7 @@ struct FsSmall {
   uint32_t wave_count[FS_MAX_WAVES];
   float wave_low[FS_MAX_WAVES], wave_high[FS_MAX_WAVES];
   int wave_at[FS_MAX_WAVES];
-  int n_listed;
+  int n_listed, listed;
   float cut;
 };
 
@@ -864,7 +864,7 @@ sample_filtered_short(FsArgs a) {
 #define FS_PIECE_WAVES (FS_THREADS / WAVE)
 #define FS_PIECE_ROWS (FS_THREADS / 16)
 struct FsExtent { float high, low; int at, unused; };
-struct FsHead { int n_listed; int ranges[5]; int gathered, unused; u64 over, unused2; };      // of a row; `gathered`: pieces that are
+struct FsHead { int n_listed; int ranges[5]; int gathered, listed; u64 over, unused; };   // of a row; `gathered`: pieces that are; `listed`: without bins
 struct FsBinned { u64 mass[FS_BINS]; uint32_t count[FS_BINS]; u64 over; u64 unused; };    // of a piece, or of a row
 // Per row: its head, its bins, its list, the pieces' extents, the maxima of their waves and of these waves' rows of sixteen lanes, and the
 // pieces' bins.
@@ -909,11 +909,11 @@ __device__ __forceinline__ int fs_row_top(const FsSpace& w, float high) {
 
 // How many maxima of rows of sixteen lanes stand for 256 logits each.
 __device__ __forceinline__ int fs_full_maxima(int vocab) { return vocab / FS_PIECE * FS_PIECE_ROWS; }
-// Whether a row's list can be made without its bins.  (Half as many tokens as maxima at most: the list is then about
-// k long; close to their number it would be several times as long.)
-__device__ __forceinline__ bool fs_listed_at_once(const FsAsked& asked, int vocab) {
-  return (asked.top_k > 0 && asked.top_k <= fs_full_maxima(vocab) / 2) || (!(asked.top_p < 1.f) && asked.min_p > 0.f);
-}
+// Whether a row's list may be made without its bins: top-k or min-p says below which logit nothing counts.  (Half as many tokens as maxima
+// at most: the list is then about k long; close to their number it would be several times as long.)
+__device__ __forceinline__ bool fs_few_wanted(const FsAsked& asked, int vocab) { return asked.top_k > 0 && asked.top_k <= fs_full_maxima(vocab) / 2; }
+__device__ __forceinline__ bool fs_floor_alone(const FsAsked& asked) { return !(asked.top_p < 1.f) && asked.min_p > 0.f; }
+__device__ __forceinline__ bool fs_may_be_listed(const FsAsked& asked, int vocab) { return fs_few_wanted(asked, vocab) || fs_floor_alone(asked); }
 
 // A logit not below `least` of which at least k of the `count` maxima are no smaller, close to the k-th largest of them; -inf if there are
 // not so many.
@@ -941,27 +941,58 @@ __device__ __forceinline__ float fs_cut_of_maxima(const float* __restrict__ maxi
   return least;
 }
 
-// A logit so that every token that counts is no smaller.
-//   top-k: at least k of the maxima are no smaller; found by halving between the largest and the smallest logit that weighs
-//   anything, and what the halvings leave undecided stays above the cut.
-//   min-p (where top-p cuts nothing): max + T ln(min_p), less what 32 bits may be off by: 4 roundings of each of its parts.
-__device__ __forceinline__ float fs_cut(const FsSpace& w, const FsAsked& asked, const FsRow& r, float low, int vocab) {
-  const float high = r.top;
-  float cut = -INFINITY;
-  if (asked.top_k > 0 && asked.top_k <= fs_full_maxima(vocab) / 2) {
-    const float least = fmaxf(low, high - r.reach);        // (what lies further below weighs nothing)
-    // Few maxima while k is small beside their number (k = 40 of 152: some 50 tokens are no smaller; 150 of them: 700).
-    cut = 2 * asked.top_k <= w.pieces * FS_PIECE_WAVES ? fs_cut_of_maxima<8>(w.of_waves(), w.pieces * FS_PIECE_WAVES, asked.top_k, least, high)
-                                                       : w.pieces * FS_PIECE_ROWS <= 12 * WAVE
-              ? fs_cut_of_maxima<12>(w.of_rows(), w.pieces * FS_PIECE_ROWS, asked.top_k, least, high)
-              : fs_cut_of_maxima<32>(w.of_rows(), w.pieces * FS_PIECE_ROWS, asked.top_k, least, high);
+// Whether the maxima of groups of `of_logits` say that few tokens are no smaller than `cut`: no more groups than the list has room for, or one of
+// sixteen of those with anything above `least` has nothing.  (Spread evenly over N groups, M tokens leave N e^(-M / N) of them without any: a
+// sixteenth at 2.8 a group, that is, in a row of 151,936 logits, at 420 tokens by the waves' maxima and at 1,650 by those of their rows.)
+template <int MOST>
+__device__ __forceinline__ bool fs_few_above(const float* __restrict__ maxima, int count, int of_logits, float cut, float least) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  float m[MOST];
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) {
+    m[j] = -INFINITY;
+    if (j * WAVE + lane < count) m[j] = maxima[j * WAVE + lane];
   }
-  if (!(asked.top_p < 1.f) && asked.min_p > 0.f) {
+  int above = 0, live = 0;
+#pragma unroll
+  for (int j = 0; j < MOST; ++j)
+    if (j * WAVE < count) {
+      above += __popcll(__ballot(m[j] >= cut));
+      live += __popcll(__ballot(m[j] >= least));
+    }
+  return above * of_logits <= FS_LIST || 16 * (live - above) >= live;
+}
+
+// A logit so that every token that counts is no smaller, and whether the list of those is known to be short.  (A list of more than FS_LIST tokens is one
+// workgroup's, which reads the row again and again: rows of 151,936 flat logits (2.2 N(0, 1)) under min-p of 1e-6 took 359 us, under one of 0.01 at
+// T = 1.5 106 to 468; rows of which only 20,000 neighbours are allowed, under top-k 40, 382 to 539.)
+//   top-k: at least k of the maxima are no smaller; found by halving between the largest and the smallest logit that weighs
+//   anything, and what the halvings leave undecided stays above the cut.  Fewer than k maxima say nothing.
+//   min-p (where top-p cuts nothing): max + T ln(min_p), less what 32 bits may be off by: 4 roundings of each of its parts.
+struct FsCut { float cut; bool is_short; };
+__device__ __forceinline__ FsCut fs_cut(const FsSpace& w, const FsAsked& asked, const FsRow& r, float low, int vocab) {
+  const float high = r.top, least = fmaxf(low, high - r.reach);          // (what lies further below weighs nothing)
+  const int maxima = w.pieces * FS_PIECE_ROWS;
+  FsCut c = {-INFINITY, false};
+  if (fs_few_wanted(asked, vocab)) {
+    // Few maxima while k is small beside their number (k = 40 of 152: some 50 tokens are no smaller; 150 of them: 700).
+    c.cut = 2 * asked.top_k <= w.pieces * FS_PIECE_WAVES ? fs_cut_of_maxima<8>(w.of_waves(), w.pieces * FS_PIECE_WAVES, asked.top_k, least, high)
+            : maxima <= 12 * WAVE                        ? fs_cut_of_maxima<12>(w.of_rows(), maxima, asked.top_k, least, high)
+                                                         : fs_cut_of_maxima<32>(w.of_rows(), maxima, asked.top_k, least, high);
+    c.is_short = c.cut > -INFINITY;
+  }
+  if (fs_floor_alone(asked)) {
     const float down = -asked.temperature * logf(fminf(asked.min_p, 1.f));
     const float floor_cut = high - down - 4.8e-7f * (fabsf(high) + 2.f * down) - 1e-6f * asked.temperature;
-    cut = fmaxf(cut, floor_cut);
+    // (The waves' maxima, a quarter as many, say it of most rows: 256 rows under min-p of 0.05 52.0 us, by the others alone 52.6.)
+    const float from = fmaxf(floor_cut, least);
+    if (!c.is_short) c.is_short = fs_few_above<8>(w.of_waves(), w.pieces * FS_PIECE_WAVES, FS_PIECE / FS_PIECE_WAVES, from, least);
+    if (!c.is_short)
+      c.is_short = maxima <= 12 * WAVE ? fs_few_above<12>(w.of_rows(), maxima, FS_PIECE / FS_PIECE_ROWS, from, least)
+                                       : fs_few_above<32>(w.of_rows(), maxima, FS_PIECE / FS_PIECE_ROWS, from, least);
+    c.cut = fmaxf(c.cut, floor_cut);
   }
-  return cut;
+  return c;
 }
 
 // The tokens of piece `p` that `wanted` names, to the row's list: each thread's, their place among the workgroup's, and the
@@ -1017,11 +1048,11 @@ sample_filtered_extents(FsArgs a) {
     e.high = high;
     e.low = low;
     e.at = at;
-    if (blockIdx.x == 0) { w.head()->n_listed = w.head()->gathered = 0; }
+    if (blockIdx.x == 0) { w.head()->n_listed = w.head()->gathered = w.head()->listed = 0; }
   }
 }
 
-// The list, where it can be made at once; else the bins of SPAN pieces.
+// The list, where it can be made at once and is short; else the bins of SPAN pieces.
 template <typename T, int SPAN>
 __global__ void __launch_bounds__(FS_THREADS)
 sample_filtered_bins(FsArgs a) {
@@ -1031,7 +1062,7 @@ sample_filtered_bins(FsArgs a) {
   const T* row = (const T*)a.logits + (size_t)blockIdx.y * a.stride;
   const int first = blockIdx.x * SPAN;
   float v[FS_EACH], high, low;
-  if (fs_listed_at_once(asked, a.vocab)) {
+  if (fs_may_be_listed(asked, a.vocab)) {
     // (One wave works the cut out: eight halvings among six hundred maxima by every wave of 2,432 workgroups took 14 us of their time.)
     float of_row[SPAN], of_piece[SPAN];
 #pragma unroll
@@ -1044,22 +1075,28 @@ sample_filtered_bins(FsArgs a) {
     if (!fs_is_drawn(asked.temperature, high)) return;
     const FsRow r = fs_row(asked.temperature, high, low);
     if (threadIdx.x < WAVE) {
-      const float found = fs_cut(w, asked, r, low, a.vocab);
-      if (threadIdx.x == 0) s.cut = found;
+      const FsCut found = fs_cut(w, asked, r, low, a.vocab);
+      if (threadIdx.x == 0) {
+        s.cut = found.cut;
+        s.listed = found.is_short;
+        if (blockIdx.x == 0) w.head()->listed = found.is_short;          // (every workgroup of the row finds the same)
+      }
     }
     __syncthreads();
-    const float cut = s.cut;
+    if (s.listed) {
+      const float cut = s.cut;
 #pragma unroll
-    for (int j = 0; j < SPAN; ++j) {
-      const int p = first + j;
-      if (p >= a.pieces || of_piece[j] < cut) continue;    // (the same for the whole workgroup)
-      // Only lanes whose row of sixteen has something at or above the cut read their logits again: of 256 rows of 152,064 under min-p, 13
-      // of 26 us of this pass were the second reading.
-      fs_load<FS_THREADS>(row, p * FS_PIECE, a.vocab, v, of_row[j] >= cut);
-      fs_append(w, p, v, s, [&](float x) { return x >= cut && r.top - x <= r.reach; });
-      if (SPAN > 1) __syncthreads();
+      for (int j = 0; j < SPAN; ++j) {
+        const int p = first + j;
+        if (p >= a.pieces || of_piece[j] < cut) continue;  // (the same for the whole workgroup)
+        // Only lanes whose row of sixteen has something at or above the cut read their logits again: of 256 rows of 152,064 under min-p, 13
+        // of 26 us of this pass were the second reading.
+        fs_load<FS_THREADS>(row, p * FS_PIECE, a.vocab, v, of_row[j] >= cut);
+        fs_append(w, p, v, s, [&](float x) { return x >= cut && r.top - x <= r.reach; });
+        if (SPAN > 1) __syncthreads();
+      }
+      return;
     }
-    return;
   }
   fs_load<FS_THREADS>(row, first * FS_PIECE, a.vocab, v);
   fs_row_extent(w, high, low);
@@ -1150,7 +1187,7 @@ sample_filtered_settle(FsArgs a) {
     if (threadIdx.x == 0) a.out[row_at] = at;
     return;
   }
-  if (fs_listed_at_once(asked, a.vocab)) {
+  if (w.head()->listed) {
     fs_draw_listed<T>(a, w, asked, fs_row(asked.temperature, high, low), row_at, nullptr, 0, w.head()->n_listed, s);
     return;
   }
@@ -1179,7 +1216,7 @@ sample_filtered_gather(FsArgs a) {
   const FsAsked asked = fs_asked(a, blockIdx.y);
   float high, low;
   fs_row_extent(w, high, low);
-  if (fs_listed_at_once(asked, a.vocab) || !fs_is_drawn(asked.temperature, high)) return;
+  if (w.head()->listed || !fs_is_drawn(asked.temperature, high)) return;
   fs_gather<SPAN>(a, w, (const T*)a.logits + (size_t)blockIdx.y * a.stride, fs_row(asked.temperature, high, low), fs_kept_ranges(w), s);
 }
 
@@ -1191,7 +1228,7 @@ sample_filtered_draw(FsArgs a) {
   const FsAsked asked = fs_asked(a, blockIdx.x);
   float high, low;
   fs_row_extent(w, high, low);
-  if (fs_listed_at_once(asked, a.vocab) || !fs_is_drawn(asked.temperature, high)) return;
+  if (w.head()->listed || !fs_is_drawn(asked.temperature, high)) return;
   s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x];
   s.count[threadIdx.x] = w.whole()->count[threadIdx.x];
   const FsRanges ranges = fs_kept_ranges(w);
@@ -1209,7 +1246,7 @@ sample_filtered_finish(FsArgs a) {
   const int row_at = blockIdx.y;
   const FsSpace w = fs_space(a, row_at);
   const FsAsked asked = fs_asked(a, row_at);
-  const bool listed = fs_listed_at_once(asked, a.vocab);
+  const bool listed = w.head()->listed;
   if (listed && blockIdx.x > 0) return;
   float high, low;
   fs_row_extent(w, high, low);
