@@ -621,6 +621,45 @@ def test_a_plan_holds_while_requests_grow(ops, any_work):
         assert torch.equal(later.run(ops, plan, max_position=max(later.positions))[0], narrow.run(ops, plan, max_position=max(later.positions))[0])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_of_a_long_request_among_short_ones(ops, any_work, dtype):
+    # One that shares nothing and has many parts of its own among ones that have one; parts end inside blocks and pages.
+    tables, positions = shared_tables(30, 20, 16, [1 + (5 * r) % 33 for r in range(30)])
+    tables.insert(7, [5000 + i for i in range(301)])
+    positions.insert(7, 300 * 16 + 4)
+    batch = Batch(tables, positions, 14, 2, 64, 16, dtype, 21)
+    for growth in (0, 512, None):
+        plan = ops.plan_shared_prefixes(batch.table.numpy(), positions, 16, 14, 2, 64, dtype, "cuda:0", growth=growth)
+        by_row = plan.own_of_row_dev.reshape(-1, 4).tolist()
+        assert growth is None or (by_row[7][3] > 20 and by_row[6][3] < 10)
+        batch.check(batch.run(ops, plan)[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_requests_may_grow_past_what_was_planned_for(ops, any_work, dtype):
+    # The last part of a row takes whatever comes; a plan for no growth at all and one for the whole table give the same keys.
+    tables, _ = shared_tables(5, 9, 16, [900] * 5)
+    start = [9 * 16 + 3 * r for r in range(5)]
+    for growth in (0, 500, None):
+        first = Batch(tables, start, 14, 2, 64, 16, dtype, 22)
+        plan = ops.plan_shared_prefixes(first.table.numpy(), start, 16, 14, 2, 64, dtype, "cuda:0", growth=growth)
+        for grown in (0, 200, 511, 512, 890):
+            later = Batch(tables, [p + grown for p in start[:-1]] + [9 * 16], 14, 2, 64, 16, dtype, 22)
+            later.check(later.run(ops, plan)[0])
+
+
+def test_a_table_cut_to_the_pages_in_use_and_a_named_end_change_nothing(ops, any_work):
+    tables, _ = shared_tables(7, 12, 16, [16 * 12] * 7)
+    for grown in (1, 16, 100, 190):
+        positions = [12 * 16 + (grown * (r + 1)) // 7 for r in range(7)]
+        batch = Batch(tables, positions, 14, 2, 64, 16, torch.bfloat16, 2)
+        got, plan = batch.run(ops)
+        batch.check(got)
+        assert torch.equal(batch.run(ops, plan, max_position=max(positions))[0], got)
+        batch.table = batch.table[:, :max(positions) // 16 + 1].contiguous()
+        assert batch.table.shape[1] == (13, 14, 19, 24)[(1, 16, 100, 190).index(grown)] and torch.equal(batch.run(ops, plan)[0], got)
+
+
 def test_attention_replayed_on_new_data_and_beside_another_stream(ops, any_work):
     tables, positions = shared_tables(16, 30, 16, [1 + 7 * r for r in range(16)])
     first, second = (Batch(tables, positions, 14, 2, 64, 16, torch.bfloat16, s) for s in (1, 2))

@@ -135,3 +135,56 @@ def test_the_work_list_covers_every_query_and_key_once(seed, work, monkeypatch):
             assert sorted(slots) == list(range(parts[row])) and parts[row] <= plan.shared_parts
             ranges = [slots[s] for s in sorted(slots)]
             assert [b for b, _ in ranges] + [own[row]] == [0] + [e for _, e in ranges] if ranges else own[row] == 0
+
+
+def _own_parts(plan):
+    """Per row its own keys' parts: (begin, slot, parts left), in order."""
+    parts = {}
+    for row, begin, slot, left in plan.own_items.reshape(-1, 4).tolist():
+        if row >= 0:
+            parts.setdefault(row, []).append((begin, slot, left))
+    return parts
+
+
+@pytest.mark.parametrize("fill", [0, 32])
+@pytest.mark.parametrize("growth", [0, 512, None])
+@pytest.mark.parametrize("lengths,shared,n_kv,group", [([100] * 255 + [32000], 8192, 4, 7), ([300] * 63 + [32000], 4096, 2, 7), ([5], 0, 1, 1),
+                                                       ([1, 700, 20, 4000], 640, 2, 40), ([40] * 300, 1024, 4, 4)])
+def test_own_keys_fall_into_parts_by_each_rows_own_length(lengths, shared, n_kv, group, growth, fill):
+    # A long request among many short ones is many parts, and the short ones are no more than they need.
+    rows, used = [], shared // 16
+    for at, length in enumerate(lengths):
+        pages = -(-length // 16)
+        alone = at == len(lengths) - 1
+        rows.append(([] if alone else list(range(shared // 16))) + list(range(used, used + pages)))
+        used += pages
+    positions = [len(r) * 16 - 1 for r in rows]
+    plan = SharedPrefixes(_table(rows), positions, 16, n_kv * group, n_kv, 64, torch.bfloat16, "cpu", fill, growth)
+    own_keys, by_row, parts = int(plan.own_keys_dev), plan.own_of_row_dev.reshape(-1, 4).tolist(), _own_parts(plan)
+    reach = [-(-(max(positions) + 1 if growth is None else p + 1 + growth) // 512) * 512 for p in positions]
+    assert sorted(parts) == list(range(len(rows))) and plan.n_own % max(1, fill) == 0 and len(plan.own_items) == 4 * plan.n_own
+    for row, held in parts.items():
+        begins, slots, left = zip(*held)
+        assert by_row[row][1:] == [begins[0], slots[0], len(held)] and begins[0] == plan.own_begin[row]
+        assert list(begins) == [begins[0] + i * own_keys for i in range(len(held))]
+        assert list(slots) == [by_row[row][2] + i for i in range(len(held))] and slots[-1] < plan.slots
+        assert list(left) == list(range(len(held), 0, -1))
+        assert len(held) * own_keys >= reach[row] - begins[0] > (len(held) - 1) * own_keys or len(held) == 1
+    # About as many parts as there are workgroups to be had, and none that holds the others up.
+    work = sum(reach[r] - b for r, b in enumerate(plan.own_begin.tolist())) * n_kv * -(-group // 16)
+    assert own_keys >= 128 and own_keys % 32 == 0 and own_keys <= max(128, 2 * work // 1024 + 32, -(-max(r - b for r, b in zip(reach, plan.own_begin.tolist())) // 64) + 31)
+    if growth is not None and max(lengths) == 32000:
+        assert own_keys <= 1280 and len(parts[len(rows) - 1]) >= 25
+
+
+def test_parts_are_planned_for_the_growth_that_is_named():
+    rows = [list(range(10)) + [100 + r] for r in range(4)]
+    table, positions = _table(rows), [170] * 4
+    plans = [SharedPrefixes(table, positions, 16, 14, 2, 64, torch.bfloat16, "cpu", 0, more) for more in (0, 341, 342, 3800, None)]
+    assert [len(_own_parts(p)[0]) for p in plans] == [3, 3, 7, 31, 3]
+
+
+def test_a_row_has_no_more_parts_than_a_wave_joins_at_a_time():
+    rows = [list(range(256)) + [10000 + r] for r in range(7)] + [list(range(20000, 22000))]
+    plan = SharedPrefixes(_table(rows), [4100] * 7 + [31999], 16, 14, 2, 64, torch.bfloat16, "cpu", 0, 512)
+    assert [len(p) for _, p in sorted(_own_parts(plan).items())] == [2] * 7 + [64]

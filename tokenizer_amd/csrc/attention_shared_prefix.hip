@@ -47,17 +47,21 @@ struct SharedItem {
   int table_row;                       // a request whose block table names the run's pages
   int kv_head;
 };
-struct SharedOwn { int row, begin, slot, unused; };   // a request's own keys: where they begin, its first partial result of them
+struct SharedOwn {                     // a part of a request's own keys (row -1: an item that only fills the list up)
+  int row, begin, slot;                // where it begins, and which of a query's partial results it is
+  int left;                            // of the request's parts, this one included; the last has all keys that come behind it
+};
 
 struct SharedArgs {
   const void *q, *k_pages, *vt_pages;
   float *part_o, *part_ml;             // [rows, n_q, slots, D], [rows, n_q, slots, 2]
   const SharedItem* items;             // those of few columns first, then those of many
   const int* order;                    // the requests, those of a run side by side
-  const SharedOwn *own, *own_of_row;   // in that order, and by request
+  const SharedOwn *own, *own_of_row;   // all parts, and by request the first
+  const int* own_keys;                 // keys of a part (one number; beside the lists, so that a captured launch can be given others)
   const int *positions, *block_table;
   const float* sinks;
-  int q_stride, table_stride, n_narrow, n_many, n_rows, n_q, n_kv, page_size, n_pages, slots, own_splits, own_keys;
+  int q_stride, table_stride, n_narrow, n_many, n_own, n_rows, n_q, n_kv, page_size, n_pages, slots;
   int page_shift;                      // page_size as a power of two, -1 if it is none
   float scale, softcap;
 };
@@ -773,24 +777,23 @@ __device__ __forceinline__ void sp_few(const SharedArgs& a, int block, float* o0
     if (first_column + col < columns) row = a.order[rows_at + (first_column + col) / group];
   } else {
     const int tiles = (group + SP_FEW_COLUMNS - 1) / SP_FEW_COLUMNS;
-    // (First parts of all requests first: the last ones are empty for the short ones.)
     int at = block - a.n_narrow;
     kvh = at % a.n_kv;
     at /= a.n_kv;
     const int tile = at % tiles;
-    at /= tiles;
-    const int split = at / a.n_rows;
-    const int* of = reinterpret_cast<const int*>(a.own + (at - split * a.n_rows));
+    const int* of = reinterpret_cast<const int*>(a.own + at / tiles);
     table_row = scalar_int(of);
-    begin = scalar_int(of + 1) + split * a.own_keys;
-    slot = scalar_int(of + 2) + split;
+    begin = scalar_int(of + 1);
+    slot = scalar_int(of + 2);
+    const int left = scalar_int(of + 3), own_keys = scalar_int(a.own_keys);
+    if (table_row < 0) return;
     columns = group;
     first_column = tile * SP_FEW_COLUMNS;
     table = a.block_table + (size_t)table_row * a.table_stride;
     end = min(scalar_int(a.positions + table_row), a.table_stride * a.page_size - 1) + 1;
     next = look_up(begin + SP_BLOCK * wave, begin + SP_BLOCK * wave + 16);
     if (begin >= end) return;                              // a short request: its last parts are empty, and not asked for
-    end = min(end, begin + a.own_keys);
+    if (left > 1) end = min(end, begin + own_keys);
     if (begin + SP_BLOCK * wave + 16 >= end) { next.page1 = next.page0; next.slot1 = next.slot0; }
     if (first_column + col < columns) row = table_row;
   }
@@ -954,9 +957,9 @@ shared_prefix_join(SharedArgs a, T* __restrict__ out) {
   if (at >= a.n_rows * a.n_q) return;
   const int row = at / a.n_q, head = at - row * a.n_q;
   const int* mine = reinterpret_cast<const int*>(a.own_of_row + row);
-  const int begin = scalar_int(mine + 1), shared = scalar_int(mine + 2);
+  const int begin = scalar_int(mine + 1), shared = scalar_int(mine + 2), own_parts = scalar_int(mine + 3), own_keys = scalar_int(a.own_keys);
   const int own = min(scalar_int(a.positions + row), a.table_stride * a.page_size - 1) + 1 - begin;
-  const int parts = shared + (own > 0 ? min((own + a.own_keys - 1) / a.own_keys, a.own_splits) : 0);      // (a.slots at most)
+  const int parts = shared + (own > 0 ? min((own - 1) / own_keys + 1, own_parts) : 0);                    // (a.slots at most)
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)at * a.slots;
   const float* part = a.part_o + (size_t)at * a.slots * D;
   const float sink = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;
@@ -1006,7 +1009,7 @@ constexpr bool sp_is_wide() { return sizeof(T) == 2 && (D == 64 || D == 128); }
 template <typename T, int D>
 static int launch_shared(const SharedArgs& a, void* out, hipStream_t stream) {
   const int group = a.n_q / a.n_kv, tiles = (group + SP_FEW_COLUMNS - 1) / SP_FEW_COLUMNS;
-  const unsigned few = (unsigned)a.n_narrow + (unsigned)a.n_rows * tiles * a.own_splits * a.n_kv;
+  const unsigned few = (unsigned)a.n_narrow + (unsigned)a.n_own * tiles * a.n_kv;
   int status = 0;
   if constexpr (sp_is_wide<T, D>()) {
     if (a.n_many == 0) shared_prefix_few<T, D><<<few, SP_WAVES * WAVE, 0, stream>>>(a);
@@ -1029,29 +1032,31 @@ static int launch_shared(const SharedArgs& a, void* out, hipStream_t stream) {
 }
 
 // q: the query heads of every row at its start, rows q_stride elements apart; pages as in the other attention kernels; items int32
-// [n_narrow + n_many, 8] (`SharedItem`; sixteen columns each, then 128 or 32); order int32 [n_rows]: the rows, those of a run of shared keys side by side; own, own_of_row int32 [n_rows, 4]
-// (`SharedOwn`): where a request's own keys begin and how many partial results its shared keys leave, in that order and by row; positions
-// int32 [n_rows]; block_table int32 [n_rows, table_stride].  part_o float [n_rows, n_q, slots, head_dim], part_ml float
-// [n_rows, n_q, slots, 2].  -2: a head size without an instance.
+// [n_narrow + n_many, 8] (`SharedItem`; sixteen columns each, then 128 or 32); order int32 [n_rows]: the rows, those of a run of shared keys
+// side by side; own int32 [n_own, 4] (`SharedOwn`): the parts of all rows' own keys; own_of_row int32 [n_rows, 4]: the rows' first parts, whose
+// `slot` is how many partial results their shared keys leave; own_keys int32 [1]: keys of a part; positions int32 [n_rows]; block_table int32
+// [n_rows, table_stride].  part_o float [n_rows, n_q, slots, head_dim], part_ml float [n_rows, n_q, slots, 2].  -2: a head size without an
+// instance.
 extern "C" int ta_shared_prefix_attention(const void* q, int q_stride, void* out, const void* k_pages, const void* vt_pages,
-                                          const void* items, int n_narrow, int n_many, const void* order, const void* own,
-                                          const void* own_of_row, const void* positions, const void* block_table,
-                                          int table_stride, const void* sinks, void* part_o, void* part_ml, int slots,
-                                          int own_splits, int own_keys, int n_rows, int n_q, int n_kv, int head_dim,
-                                          int page_size, int n_pages, float scale, float softcap, int dtype, hipStream_t stream) {
+                                          const void* items, int n_narrow, int n_many, const void* order, const void* own, int n_own,
+                                          const void* own_of_row, const void* own_keys, const void* positions, const void* block_table,
+                                          int table_stride, const void* sinks, void* part_o, void* part_ml, int slots, int n_rows, int n_q,
+                                          int n_kv, int head_dim, int page_size, int n_pages, float scale, float softcap, int dtype,
+                                          hipStream_t stream) {
   if (n_rows <= 0) return 0;
-  if (!q || !out || !k_pages || !vt_pages || !order || !own || !own_of_row || !positions || !block_table || !part_o || !part_ml)
+  if (!q || !out || !k_pages || !vt_pages || !order || !own || !own_of_row || !own_keys || !positions || !block_table || !part_o || !part_ml)
     return -1;
-  if (n_narrow < 0 || n_many < 0 || (n_narrow + n_many && !items) || n_kv < 1 || n_kv > 65535 || n_q < n_kv || n_q % n_kv || page_size < 16 || page_size % 16 || n_pages < 1 ||
-      slots < 1 || own_splits < 1 || own_keys < SP_BLOCK || own_keys % SP_BLOCK || table_stride < 1) return -1;
+  if (n_narrow < 0 || n_many < 0 || (n_narrow + n_many && !items) || n_own < n_rows || n_kv < 1 || n_kv > 65535 || n_q < n_kv || n_q % n_kv ||
+      page_size < 16 || page_size % 16 || n_pages < 1 || slots < 1 || table_stride < 1) return -1;
   SharedArgs a = {};
   a.q = q; a.k_pages = k_pages; a.vt_pages = vt_pages; a.part_o = (float*)part_o; a.part_ml = (float*)part_ml;
   a.items = (const SharedItem*)items; a.order = (const int*)order; a.own = (const SharedOwn*)own;
-  a.own_of_row = (const SharedOwn*)own_of_row; a.positions = (const int*)positions; a.block_table = (const int*)block_table;
-  a.sinks = (const float*)sinks; a.q_stride = q_stride; a.table_stride = table_stride; a.n_narrow = n_narrow; a.n_many = n_many; a.n_rows = n_rows;
-  a.n_q = n_q; a.n_kv = n_kv; a.page_size = page_size; a.n_pages = n_pages; a.slots = slots; a.own_splits = own_splits;
+  a.own_of_row = (const SharedOwn*)own_of_row; a.own_keys = (const int*)own_keys; a.positions = (const int*)positions;
+  a.block_table = (const int*)block_table; a.sinks = (const float*)sinks; a.q_stride = q_stride; a.table_stride = table_stride;
+  a.n_narrow = n_narrow; a.n_many = n_many; a.n_own = n_own; a.n_rows = n_rows; a.n_q = n_q; a.n_kv = n_kv; a.page_size = page_size;
+  a.n_pages = n_pages; a.slots = slots;
   a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size);
-  a.own_keys = own_keys; a.scale = scale; a.softcap = softcap;
+  a.scale = scale; a.softcap = softcap;
 #define SHARED_CASE(D) \
   case D: return dtype == DT_F32 ? launch_shared<float, D>(a, out, stream) : launch_shared<bf16_t, D>(a, out, stream);
   switch (head_dim) {

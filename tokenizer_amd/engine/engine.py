@@ -285,7 +285,8 @@ class Engine:
                                                 writes=entry.cache_of is None))
         self.shared_attention = shared_attention
         self._family: set = set()    # requests that were forked or are forks
-        self._sharing: tuple | None = None        # (epoch, requests), their plans
+        self._sharing: tuple | None = None        # (epoch, requests, bucket of context), their plans
+        self._sharing_due = 0        # the step from which on they may be past that bucket
         self._shared_shapes = self._shapes_that_share()
         self.steps = 0
         self._landing: dict[int, tuple] = {}     # pinned rows and events of `decode_greedy` / `decode_sampled`, by batch size
@@ -475,11 +476,14 @@ class Engine:
             return ("single",) + tuple(len(e.want) for e in entries)
         return ("filled",) + filled_counts([len(e.tokens) for e in entries], [len(e.want) for e in entries])
 
-    def _graph_key(self, entries: list[StepEntry]) -> tuple:
+    def _bucket_of(self, entries: list[StepEntry]) -> tuple[int, int]:
+        """The context that a step's launches are planned for, and the longest that it has.  (With any page size: an eager step plans
+        for its context rounded up in the same way, so both cut their sums alike.)"""
         longest = max(self.cache.seq_len(e.rid) + len(e.tokens) for e in entries)
-        # (The bucket is what the kernels' launch shapes are planned for, with any page size: an eager step plans
-        # for its context rounded up in the same way, so both cut their sums alike.)
-        bucket = -(-longest // self.GRAPH_BUCKET) * self.GRAPH_BUCKET
+        return -(-longest // self.GRAPH_BUCKET) * self.GRAPH_BUCKET, longest
+
+    def _graph_key(self, entries: list[StepEntry]) -> tuple:
+        bucket, _ = self._bucket_of(entries)
         plans = self.sharing(entries)
         if plans:
             return (self._shape_of(entries), bucket, tuple((shape, plans[shape].signature) for shape in sorted(plans)))
@@ -551,16 +555,22 @@ class Engine:
 
     def sharing(self, entries: list[StepEntry]) -> dict:
         """The plans of what the requests of a step of single tokens share, by the shape of the attention that takes them; empty where
-        nothing is shared.  Worked out when the requests of a step change, and kept while they stay."""
+        nothing is shared.  Worked out when the requests of a step change or come to another bucket of context (a
+        plan is made for so many tokens more), and kept while they stay."""
         if self.shared_attention is False or not self._shared_shapes or len(entries) < 2:
             return NOTHING_SHARED
         if self.shared_attention is None and (len(self._family) < 2 or sum(e.rid in self._family for e in entries) < 2):
             return NOTHING_SHARED
         if any(len(e.tokens) != 1 for e in entries):
             return NOTHING_SHARED
-        key = (self.cache.epoch, tuple(e.rid for e in entries))
-        if self._sharing is not None and self._sharing[0] == key:
-            return self._sharing[1]
+        key, held = (self.cache.epoch, tuple(e.rid for e in entries)), self._sharing
+        same = held is not None and held[0][:2] == key
+        if same and self.steps < self._sharing_due:
+            return held[1]
+        bucket, longest = self._bucket_of(entries)
+        self._sharing_due = self.steps + bucket - longest + 1     # (a step of single tokens brings each request one further)
+        if same and held[0][2] == bucket:
+            return held[1]
         positions = [self.cache.seq_len(e.rid) for e in entries]
         plans = {}
         for group, n_q, n_kv, head_dim in self._shared_shapes:
@@ -568,11 +578,11 @@ class Engine:
             width = max([1] + [len(t) for t in tables])
             table = np.array([t + [-1] * (width - len(t)) for t in tables], dtype=np.int32)
             plan = self.model.runtime.ops.plan_shared_prefixes(table, positions, self.cache.page_size, n_q, n_kv, head_dim, self.model.dtype,
-                                                               self.model.device, fill=self.SHARED_FILL)
+                                                               self.model.device, fill=self.SHARED_FILL, growth=self.GRAPH_BUCKET)
             if plan.runs:
                 plans[(group, n_q, n_kv, head_dim)] = plan
         plans = plans or NOTHING_SHARED
-        self._sharing = (key, plans)
+        self._sharing = ((*key, bucket), plans)
         return plans
 
     # ------------------------------------------------------------------ requests
@@ -692,5 +702,7 @@ class Engine:
             logits = logits[:wanted]        # the rows behind them belong to what the step was filled up with
         for entry in entries:
             self.cache.advance(entry.rid, self.cache.seq_len(entry.rid) + len(entry.tokens))
+            if len(entry.tokens) > 1:
+                self._sharing_due = 0                  # (requests that are planned for may have come further than one token)
         self.steps += 1
         return logits

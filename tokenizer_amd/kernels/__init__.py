@@ -205,8 +205,9 @@ class Ops:
         self.lib.ta_library_gemm_bf16.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int] * 5 + [
             ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p]
         pointer, number, real = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
-        self.lib.ta_shared_prefix_attention.argtypes = ([pointer, number] + [pointer] * 4 + [number] * 2 + [pointer] * 5 + [number]
-                                                        + [pointer] * 3 + [number] * 9 + [real] * 2 + [number, pointer])
+        self.lib.ta_shared_prefix_attention.argtypes = ([pointer, number] + [pointer] * 4 + [number] * 2 + [pointer] * 2 + [number]
+                                                        + [pointer] * 4 + [number] + [pointer] * 3 + [number] * 7 + [real] * 2
+                                                        + [number, pointer])
         self.lib.ta_sample_filtered.argtypes = [pointer, ctypes.c_int64] + [pointer] * 7 + [number] * 3 + [pointer]
         self.lib.ta_copy_pages.argtypes = [pointer] * 3 + [number] * 9 + [pointer]
         self._sample_bytes: dict[int, int] = {}    # workspace of a row of so many logits
@@ -1540,12 +1541,14 @@ class Ops:
         return out
 
     def plan_shared_prefixes(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int,
-                             dtype: torch.dtype, device="cuda:0", fill: int = 0) -> SharedPrefixes:
+                             dtype: torch.dtype, device="cuda:0", fill: int = 0, growth: int | None = None) -> SharedPrefixes:
         """What the requests of a batch of single tokens share, laid out for `shared_prefix_attention`.
 
         block_table (on the host) int [B, P]: row i's pages, -1 where there is none; positions (on the host) int [B]: where the rows'
         newest tokens stand.  A plan holds as long as the rows keep their order, their leading pages and do not go back.  `fill`: the list
-        of work is filled up to a multiple of so many items, so that plans that differ a little have one size."""
+        of work is filled up to a multiple of so many items, so that plans that differ a little have one size.  `growth`: by how many
+        tokens the rows are expected to grow (None: all of them to the table's end).  The plan holds past that too, but the work of rows of
+        very different lengths is spread better the less is expected."""
         import numpy as np
         table, positions = np.asarray(block_table), np.asarray(positions)
         _need(table.ndim == 2 and table.shape[1] >= 1 and positions.shape == (table.shape[0],), "one block table row and one position a request")
@@ -1553,7 +1556,8 @@ class Ops:
         _need(page_size >= 16 and page_size % 16 == 0, "pages of a multiple of sixteen tokens")
         _need(head_dim in self.DECODE_HEAD_DIMS, f"head sizes {self.DECODE_HEAD_DIMS}")
         _code(dtype)
-        return SharedPrefixes(table, positions, page_size, n_q, n_kv, head_dim, dtype, device, fill)
+        _need(growth is None or growth >= 0, "rows do not shrink")
+        return SharedPrefixes(table, positions, page_size, n_q, n_kv, head_dim, dtype, device, fill, growth)
 
     def shared_prefix_attention(self, qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                                 positions: torch.Tensor, block_table: torch.Tensor, plan: SharedPrefixes, n_q: int, n_kv: int,
@@ -1565,7 +1569,7 @@ class Ops:
         qkv [B, >= n_q d] (query heads first); out [B, n_q d]; key pages [n_pages, n_kv, page_size, d], value pages [n_pages, n_kv,
         d, page_size]; positions int32 [B]; block_table int32 [B, P].  A row sees the keys of all positions up to its own (a row of
         position -1 none: its result is zero).  `sinks` (float32 [n_q]): exp(sinks[h]) joins the denominator; `softcap` c: a
-        scaled score s becomes c tanh(s / c).  `max_position` (host): the largest position, for the launch's size."""
+        scaled score s becomes c tanh(s / c).  `max_position` (host) lets the wrapper check that the table is wide enough."""
         _here(qkv, out, k_pages, v_pages, positions, block_table, plan.packed, sinks)
         # (Every call of an eager step pays for what is asked here: shapes are taken once and compared whole.)
         shape, dtype, table_shape, k_shape, page_size = qkv.shape, qkv.dtype, block_table.shape, k_pages.shape, plan.page_size
@@ -1595,29 +1599,20 @@ class Ops:
         _need(scale > 0, "the scores' scale is positive")
         width = table_shape[1]
         _need(plan.keys_end <= width * page_size, "block table is too narrow for the shared keys")
-        if max_position is None:
-            max_position = width * page_size - 1
-        _need(max_position < width * page_size, "block table is too narrow for the positions")
+        _need(max_position is None or max_position < width * page_size, "block table is too narrow for the positions")
         if n_rows == 0:
             return out
-        # The requests' own keys, in parts that fill the device (as for single tokens that share nothing).
-        longest = max(1, -(-(max_position + 1) // self.PLAN_KEYS) * self.PLAN_KEYS - plan.smallest_own)
-        head_blocks = -(-(n_q // n_kv) // plan.FEW_COLUMNS)
-        wanted = max(1, self.target_workgroups // (n_rows * n_kv * head_blocks))
-        own_keys = max(self.min_split_keys, -(-longest // wanted))
-        own_keys = -(-own_keys // 32) * 32
-        own_splits = -(-longest // own_keys)
-        slots = plan.shared_parts + own_splits
+        slots = plan.slots
         # Partial results: the weighed values, and behind them the maxima and sums.
         values = n_rows * n_q * slots * head_dim
         partial = torch.empty(values + 2 * n_rows * n_q * slots, dtype=torch.float32, device=qkv.device)
-        items, order, own, own_of_row = plan.places
+        items, order, own, own_of_row, own_keys = plan.places
         packed = plan.packed
         self._check(self.lib.ta_shared_prefix_attention(
             _address(qkv), row_elements, _address(out), _address(k_pages), _address(v_pages), _address(packed, items), plan.n_few, plan.n_many,
-            _address(packed, order), _address(packed, own), _address(packed, own_of_row), _address(positions), _address(block_table), width,
-            _address(sinks), _address(partial), _address(partial, 4 * values), slots, own_splits, own_keys, n_rows, n_q, n_kv, head_dim,
-            page_size, n_pages, scale, softcap or 0.0, _code(dtype), self._stream()), "shared_prefix_attention")
+            _address(packed, order), _address(packed, own), plan.n_own, _address(packed, own_of_row), _address(packed, own_keys),
+            _address(positions), _address(block_table), width, _address(sinks), _address(partial), _address(partial, 4 * values), slots, n_rows,
+            n_q, n_kv, head_dim, page_size, n_pages, scale, softcap or 0.0, _code(dtype), self._stream()), "shared_prefix_attention")
         return out
 
     def talking_attention(self, qkv: torch.Tensor, out: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,

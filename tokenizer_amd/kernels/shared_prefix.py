@@ -89,14 +89,19 @@ class SharedPrefixes:
     # through LDS, a 16th, up to LONG_PART: 2 requests of 32,000 keys of head size 64 in 250 parts 25.8 us, in 63 12.8; 64 of 8,192 in parts
     # of 256 | 512 32.0 | 28.8.
     MIN_PART, MIN_WIDE_PART, LONG_PART = 128, 256, 512
-    OWN_STEP = 128                # `smallest_own` in whole steps: prefixes that differ a little make launches of one shape
+    # The requests' own keys, in parts of one length, about so many of all requests together (as for single tokens that share nothing).  Each
+    # request has as many as its own keys are planned to come to, in steps of OWN_STEP, so a long one among short ones has many, up to what a wave
+    # joins at a time.  (Requests behind 4,096 keys, 256 behind 8,192, with 100 to 300 of their own, and one of 32,000 that shares nothing: 256 of
+    # 28 query heads of size 128, as many parts for each as for the longest 403 us, so 87; 64 of them 149 | 42; 64 of 14 heads of size 64 48 | 20;
+    # 8 of those 22 | 15, in 257 parts 28.)
+    OWN_TARGET, OWN_STEP = 1024, 512
     # Workgroups that the parts aim at: two a compute unit; one where all items are of few columns.  (256 | 512 | 768: 64 requests behind 4,096
     # keys 34.6 | 28.7 | 32.7 us, 256 behind 32,000 187 | 145 | 161; few only, 64 behind 512 11.0 | 13.1 | 13.2, 24 behind 4,096
     # 15.5 | 18.5 | 18.2, 16 15.1 | 14.2 | 18.1, 2 behind 32,000 22.0 | 26.7 | 32.7.)
     TARGET, FEW_TARGET = 512, 256
 
     def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device,
-                 fill: int = 0):
+                 fill: int = 0, growth: int | None = None):
         table = np.asarray(block_table, dtype=np.int32)
         self.n_rows, self.page_size, self.n_q, self.n_kv, self.head_dim, self.dtype = (
             table.shape[0], int(page_size), int(n_q), int(n_kv), int(head_dim), dtype)
@@ -143,12 +148,32 @@ class SharedPrefixes:
         self.shared_parts = int(parts_of.max(initial=0))
         self.own_begin = own_begin                        # int32 [B] on the host
         self.keys_end = max((run.key_end for run in self.runs), default=0)
-        self.smallest_own = int(own_begin.min()) // self.OWN_STEP * self.OWN_STEP if self.n_rows else 0
+        # A request's own keys in parts, the last of which has all that come behind it.
+        ends = np.full(self.n_rows, table.shape[1] * self.page_size) if growth is None else np.asarray(positions, dtype=np.int64) + 1 + growth
+        room = np.maximum(-(-ends // self.OWN_STEP) * self.OWN_STEP - own_begin, 1)
+        longest, all_room = int(room.max(initial=1)), max(1, int(room.sum())) * n_kv * -(-group // self.FEW_COLUMNS)
+        own_keys = max(self.MIN_PART, -(-longest // max(1, min(WAVE, self.OWN_TARGET * longest // all_room))))
+        own_keys = -(-own_keys // 32) * 32
+        own_parts = -(-room // own_keys)
         rows = np.arange(self.n_rows, dtype=np.int32)
-        own = np.stack([rows, own_begin, parts_of, np.zeros_like(rows)], axis=1).astype(np.int32)
+        own_of_row = np.stack([rows, own_begin, parts_of, own_parts], axis=1).astype(np.int32)
+        # (First parts of all requests first: the last ones are empty for the short ones.)
+        own = [own_of_row[self.order]]
+        for part in range(1, int(own_parts.max(initial=1))):
+            with_it = own[0][own[0][:, 3] > part]
+            own.append(with_it + np.array([0, part * own_keys, part, -part], dtype=np.int32))
+        own = np.concatenate(own)
+        self.n_own = self._filled(len(own), fill)
+        own = np.concatenate([own, np.full((self.n_own - len(own), 4), -1, dtype=np.int32)])
+        self.slots = self._filled(int((parts_of + own_parts).max(initial=1)), 2 if fill else 0)
         packed = np.concatenate([np.asarray(items[False] + items[True], dtype=np.int32).reshape(-1), np.asarray(self.order, dtype=np.int32),
-                                 own[self.order].reshape(-1), own.reshape(-1)]).astype(np.int32)
+                                 own.reshape(-1), own_of_row.reshape(-1), np.array([own_keys], dtype=np.int32)]).astype(np.int32)
         self._on_device(torch.from_numpy(packed).to(device))
+
+    @staticmethod
+    def _filled(count: int, fill: int) -> int:
+        """`count` filled up to a multiple of `fill`."""
+        return -(-count // fill) * fill if fill else count
 
     CHIPLETS = 8                  # of the device: each gets every eighth workgroup, and has a cache of its own
 
@@ -171,19 +196,19 @@ class SharedPrefixes:
         order = [queue[i] if i < len(queue) else nothing for i in range(longest) for queue in queues]
         while order and order[-1] is nothing:
             order.pop()
-        return order + [nothing] * (-len(order) % fill if fill else 0)
+        return order + [nothing] * (cls._filled(len(order), fill) - len(order))
 
     def _on_device(self, packed: torch.Tensor) -> None:
         self.packed = packed
-        sizes = [8 * (self.n_few + self.n_many), self.n_rows, 4 * self.n_rows, 4 * self.n_rows]
-        self.items, self.order_dev, self.own_dev, self.own_of_row_dev = torch.split(packed, sizes)
-        self.places = tuple(4 * sum(sizes[:i]) for i in range(4))           # in bytes from the start of `packed`
+        sizes = [8 * (self.n_few + self.n_many), self.n_rows, 4 * self.n_own, 4 * self.n_rows, 1]
+        self.items, self.order_dev, self.own_items, self.own_of_row_dev, self.own_keys_dev = torch.split(packed, sizes)
+        self.own_dev = self.own_items[:4 * self.n_rows]                     # the requests' first parts
+        self.places = tuple(4 * sum(sizes[:i]) for i in range(5))           # in bytes from the start of `packed`
 
     @property
     def signature(self) -> tuple:
         """What a launch depends on beside the tables: plans of one signature may take each other's place in a captured graph."""
-        return (self.n_rows, self.n_few, self.n_many, self.shared_parts, self.smallest_own, self.n_q, self.n_kv, self.head_dim, self.page_size,
-                self.dtype)
+        return (self.n_rows, self.n_few, self.n_many, self.n_own, self.slots, self.n_q, self.n_kv, self.head_dim, self.page_size, self.dtype)
 
     def standing_copy(self) -> "SharedPrefixes":
         """The same plan in memory of its own, which `take` fills with others of its signature (for a captured graph)."""
