@@ -374,3 +374,39 @@ def test_scheduled_requests_draw_under_their_own_filters(model_folders):
     results = scheduler.run()
     for i, (rid, p) in enumerate(zip(ids, asked)):
         assert results[rid].tokens == _alone(folder, random_ids(vocab, 9 + i, i), p).tokens
+
+
+def test_graphs_of_steps_with_plans_are_bounded(model_folders, monkeypatch):
+    # (Stand-ins for the graphs and for the plans: what is kept, what makes room and which steps run eagerly is decided on the host.)
+    from types import SimpleNamespace
+    from tokenizer_amd.engine import engine as of_engine
+    monkeypatch.setattr(of_engine, "StepGraph", lambda engine, entries, bucket: SimpleNamespace(bucket=bucket, last_used=0))
+    engine = _engine(model_folders["A"])
+    engine.use_graphs = True
+    engine.PLAN_GRAPHS, engine.PLAN_IDLE_STEPS = 3, 10
+    for r in range(2):
+        engine.add_request(r)
+    entries = [StepEntry(r, [1], [0]) for r in range(2)]
+    make = 0
+    engine.sharing = lambda entries: {} if make is None else {(0, 2, 2, 16): SimpleNamespace(signature=make)}
+    for make in (1, 2, 3, 2):
+        assert engine._replays(entries) and engine._graph_for(entries) is not None
+        engine.steps += 1
+    assert engine.graphs_captured == 3 and engine.steps_replayed == 4
+    make = 4                                                    # no room, and the oldest has been used three steps ago
+    assert not engine._replays(entries) and engine._graph_for(entries) is None and len(engine.graphs) == 3
+    for make in (None, 1, 2, 3):                                # steps without a plan are captured as ever, those that are kept are replayed
+        assert engine._replays(entries) and engine._graph_for(entries) is not None
+    assert len(engine.graphs) == 4 and engine.graphs_captured == 4
+    engine.steps += 5
+    make = 2
+    assert engine._graph_for(entries) is not None
+    engine.steps += 5
+    make = 4                                                    # one that has idled long enough makes room: not the one used since
+    assert engine._replays(entries) and engine._graph_for(entries) is not None
+    kept = [key[2][0][1] for key in engine.graphs if len(key) > 2]
+    assert len(kept) == 3 and 2 in kept and 4 in kept and any(len(key) == 2 for key in engine.graphs)
+    make = 5
+    assert engine._graph_for(entries) is not None               # (the other idle one)
+    make = 6
+    assert engine._graph_for(entries) is None and len(engine.graphs) == 4

@@ -194,3 +194,29 @@ def test_forks_of_other_designs(module, table, name, dtype, tmp_path):
     for turn in range(6):
         entries = [StepEntry(r, [t], [0]) for r, t in zip("abc", random_ids(vocab, 3, 70 + turn))]
         close(shared.step([dataclasses.replace(e) for e in entries]), apart.step(entries), dtype)
+
+
+@pytest.mark.parametrize("warm", [False, True])
+def test_decode_steps_without_room_for_a_graph(warm, monkeypatch):
+    # Answers of changing number behind prompts of several lengths, with room for one graph with a plan, which a run of steps may lose its way to
+    # in the middle (a bucket of context ends): the tokens are those of an engine with room for all.
+    from tokenizer_amd.engine import Engine
+    out = []
+    for kept in (1, 64):
+        monkeypatch.setattr(Engine, "PLAN_GRAPHS", kept)
+        engine = engine_of("float32", shared_attention=True)
+        seen = []
+        for turn, length in enumerate((500, 490, 900, 1015)):
+            forked(engine, random_ids(1000, length, turn), 5)
+            ids = [11 + r for r in range(5)]
+            draw = lambda k: ([0.9] * 5, [0.9] * 5, [((3 * r + 5 * k + turn) % 16) / 16 for r in range(5)])
+            stop = lambda k, ids: k < 20 or turn < 3
+            run = engine.decode_sampled(list(range(5)), ids, 30, draw, stop) if warm else engine.decode_greedy(list(range(5)), ids, 30, stop)
+            assert len(run) == 30 if turn < 3 else 21 <= len(run) <= 22
+            seen.append(run[:21] if turn == 3 else run)
+            for r in range(5):
+                engine.end_request(r)
+            assert sum(len(key) > 2 for key in engine.graphs) <= kept
+        engine.cache.check_invariants()
+        out.append(seen)
+    assert out[0] == out[1]

@@ -146,7 +146,7 @@ def _own_parts(plan):
     return parts
 
 
-@pytest.mark.parametrize("fill", [0, 32])
+@pytest.mark.parametrize("fill", [False, True])
 @pytest.mark.parametrize("growth", [0, 512, None])
 @pytest.mark.parametrize("lengths,shared,n_kv,group", [([100] * 255 + [32000], 8192, 4, 7), ([300] * 63 + [32000], 4096, 2, 7), ([5], 0, 1, 1),
                                                        ([1, 700, 20, 4000], 640, 2, 40), ([40] * 300, 1024, 4, 4)])
@@ -162,7 +162,7 @@ def test_own_keys_fall_into_parts_by_each_rows_own_length(lengths, shared, n_kv,
     plan = SharedPrefixes(_table(rows), positions, 16, n_kv * group, n_kv, 64, torch.bfloat16, "cpu", fill, growth)
     own_keys, by_row, parts = int(plan.own_keys_dev), plan.own_of_row_dev.reshape(-1, 4).tolist(), _own_parts(plan)
     reach = [-(-(max(positions) + 1 if growth is None else p + 1 + growth) // 512) * 512 for p in positions]
-    assert sorted(parts) == list(range(len(rows))) and plan.n_own % max(1, fill) == 0 and len(plan.own_items) == 4 * plan.n_own
+    assert sorted(parts) == list(range(len(rows))) and plan.n_own % (64 if fill else 1) == 0 and len(plan.own_items) == 4 * plan.n_own
     for row, held in parts.items():
         begins, slots, left = zip(*held)
         assert by_row[row][1:] == [begins[0], slots[0], len(held)] and begins[0] == plan.own_begin[row]
@@ -188,3 +188,25 @@ def test_a_row_has_no_more_parts_than_a_wave_joins_at_a_time():
     rows = [list(range(256)) + [10000 + r] for r in range(7)] + [list(range(20000, 22000))]
     plan = SharedPrefixes(_table(rows), [4100] * 7 + [31999], 16, 14, 2, 64, torch.bfloat16, "cpu", 0, 512)
     assert [len(p) for _, p in sorted(_own_parts(plan).items())] == [2] * 7 + [64]
+
+
+@pytest.mark.parametrize("n_q,n_kv,d", [(14, 2, 64), (28, 4, 128)])
+def test_plans_of_many_prompts_have_few_makes(n_q, n_kv, d):
+    # Captured steps are kept by a plan's make.  Eight answers to each of a hundred prompts of any length, ending one by one: there are not many
+    # more makes than there are counts of requests and buckets of 512 tokens of context.
+    rng = random.Random(1)
+    makes, plain = set(), set()
+    for _ in range(100):
+        length, produced, live = rng.randint(64, 8000), 0, 8
+        for end in sorted(rng.randint(1, 400) for _ in range(8)):
+            while produced < end and live > 1:
+                bucket = -(-(length + produced + 1) // 512) * 512
+                shared = length // 16
+                own = -(-(length + produced + 1) // 16) - shared
+                rows = [list(range(shared)) + list(range(1000 * (r + 1), 1000 * (r + 1) + own)) for r in range(live)]
+                plan = SharedPrefixes(_table(rows), [length + produced] * live, 16, n_q, n_kv, d, torch.bfloat16, "cpu", True, 512)
+                makes.add((live, bucket, plan.signature if plan.runs else None))
+                plain.add((live, bucket))
+                produced = min(end, bucket - length)
+            live -= 1
+    assert len(makes) <= 1.75 * len(plain)

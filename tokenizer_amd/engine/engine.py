@@ -237,6 +237,9 @@ class Engine:
     GRAPH_BUCKET = 512      # graphs are captured per shape of the step and per this many tokens of context
     STEP_GRAPHS = 64        # how many graphs of other steps than plain decode steps are kept
     GRAPH_IDLE_STEPS = 2000  # a kept graph makes room for another only after this many steps without a replay
+    PLAN_GRAPHS = 64        # how many graphs of decode steps with plans of shared prefixes are kept
+    PLAN_IDLE_STEPS = 256   # ... and after how many steps without a replay one makes room: a capture costs some three eager steps, and
+    #                         64 shapes that take turns have four steps each by then
     GRAPH_TOKENS = 2048     # steps with more tokens than this are not captured: the device is the slower side
     GRAPH_AFTER = 3         # a shape is captured when it comes up for this many times ...
     SHAPES_REMEMBERED = 64  # ... among this many shapes seen last
@@ -405,19 +408,7 @@ class Engine:
             raise ValueError("one next token per request")
         count = len(rids)
         if not self.use_graphs:
-            picked, current = [], list(tokens)
-            for k in range(n_steps):
-                logits = self.step([StepEntry(rid, [int(t)], [0]) for rid, t in zip(rids, current)])
-                current = self.argmax(logits)
-                if draw is not None:
-                    temperature, top_p, uniform, *filters = draw(k)
-                    temperature, top_p, uniform, greedy = self._warm_numbers(temperature, top_p, uniform)
-                    drawn = self.sample(logits, list(range(count)), temperature, top_p, uniform, *filters)
-                    current = [pick if g else token for g, pick, token in zip(greedy, current, drawn)]
-                picked.append(list(current))
-                if on_step is not None and on_step(k, picked[-1]) is False:
-                    break
-            return picked
+            return self._decode_by_steps(rids, tokens, [], n_steps, on_step, draw)
         # (Two pinned rows for the ids on their way to the host and an event for each, kept from run to run: pinning
         # memory costs as much as several steps of a small model.)
         if count not in self._landing:
@@ -434,6 +425,14 @@ class Engine:
             self.validate(entries)
             self.reserve(entries)
             graph = self._graph_for(entries)
+            if graph is None:                          # no room for a graph: the steps that are left run one by one
+                self._graph_result = None
+                if k > 0:
+                    arrived[(k - 1) % 2].synchronize()
+                    picked.append(landing[(k - 1) % 2].tolist())
+                    if on_step is not None and on_step(k - 1, picked[-1]) is False:
+                        return picked
+                return self._decode_by_steps(rids, tokens, picked, n_steps, on_step, draw)
             graph.run(self, entries, tokens_on_device=previous)
             for entry in entries:
                 self.cache.advance(entry.rid, self.cache.seq_len(entry.rid) + 1)
@@ -465,6 +464,22 @@ class Engine:
         self._graph_result = None
         return picked
 
+    def _decode_by_steps(self, rids: list, tokens: list[int], picked: list[list[int]], n_steps: int, on_step, draw) -> list[list[int]]:
+        """The rest of a run of decode steps, behind those that have `picked` their ids, through `step`."""
+        current = list(picked[-1] if picked else tokens)
+        for k in range(len(picked), n_steps):
+            logits = self.step([StepEntry(rid, [int(t)], [0]) for rid, t in zip(rids, current)])
+            current = self.argmax(logits)
+            if draw is not None:
+                temperature, top_p, uniform, *filters = draw(k)
+                temperature, top_p, uniform, greedy = self._warm_numbers(temperature, top_p, uniform)
+                drawn = self.sample(logits, list(range(len(rids))), temperature, top_p, uniform, *filters)
+                current = [pick if g else token for g, pick, token in zip(greedy, current, drawn)]
+            picked.append(list(current))
+            if on_step is not None and on_step(k, picked[-1]) is False:
+                break
+        return picked
+
     @staticmethod
     def _shape_of(entries: list[StepEntry]):
         """What fixes the layout of a step's tables and the sizes of its launches: the number of entries for a
@@ -489,10 +504,19 @@ class Engine:
             return (self._shape_of(entries), bucket, tuple((shape, plans[shape].signature) for shape in sorted(plans)))
         return (self._shape_of(entries), bucket)
 
-    def _graph_for(self, entries: list[StepEntry]) -> "StepGraph":
+    @staticmethod
+    def _is_planned(key: tuple) -> bool:
+        """Whether a key is that of a plain decode step whose requests share something: there are many more of these than counts of requests and
+        buckets of context."""
+        return isinstance(key[0], int) and len(key) > 2
+
+    def _graph_for(self, entries: list[StepEntry]) -> "StepGraph | None":
+        """The graph of this step, captured if there is none; None where there is no room for another."""
         key = self._graph_key(entries)
         graph = self.graphs.get(key)
         if graph is None:
+            if self._is_planned(key) and not self._room_for_a_graph(planned=True):
+                return None
             graph = StepGraph(self, entries, key[1])       # its first eager run and the capture write the same
             self.graphs[key] = graph                         # keys and values the replay writes again
             self.graphs_captured += 1
@@ -500,30 +524,34 @@ class Engine:
         graph.last_used = self.steps
         return graph
 
-    def _room_for_a_graph(self) -> bool:
-        """Graphs of other steps than plain decode steps are kept up to `STEP_GRAPHS`; beyond that one makes room
-        only if it has not been replayed for `GRAPH_IDLE_STEPS` steps (else a cycle of more shapes than graphs
-        would capture every one of them again and again, which costs far more than running them eagerly)."""
-        others = [key for key in self.graphs if not isinstance(key[0], int)]
-        if len(others) < self.STEP_GRAPHS:
+    def _room_for_a_graph(self, planned: bool = False) -> bool:
+        """Graphs of other steps than plain decode steps are kept up to `STEP_GRAPHS`, those of decode steps with plans up to
+        `PLAN_GRAPHS`; beyond that one makes room only if it has not been replayed for `GRAPH_IDLE_STEPS` (`PLAN_IDLE_STEPS`) steps
+        (else a cycle of more shapes than graphs would capture every one of them again and again, which costs far more than
+        running them eagerly)."""
+        most, idle = (self.PLAN_GRAPHS, self.PLAN_IDLE_STEPS) if planned else (self.STEP_GRAPHS, self.GRAPH_IDLE_STEPS)
+        others = [key for key in self.graphs if (self._is_planned(key) if planned else not isinstance(key[0], int))]
+        if len(others) < most:
             return True
         oldest = min(others, key=lambda key: self.graphs[key].last_used)
-        if self.steps - self.graphs[oldest].last_used < self.GRAPH_IDLE_STEPS:
+        if self.steps - self.graphs[oldest].last_used < idle:
             return False
         del self.graphs[oldest]
         return True
 
     def _replays(self, entries: list[StepEntry]) -> bool:
-        """Whether this step replays a captured graph.  Plain decode steps always do.  Other steps (portions of
-        prompts, mixed batches) do once their shape has come up `GRAPH_AFTER` times among the last
+        """Whether this step replays a captured graph.  Plain decode steps always do (with plans of what their requests share, where
+        there is room for their graph).  Other steps (portions of prompts, mixed batches) do once their shape has come up `GRAPH_AFTER` times among the last
         `SHAPES_REMEMBERED` shapes: for short steps the host's launches, not the device, set the pace, and some
         shapes recur at once (a prompt cut into equal portions, a full token budget of equal prompts), while
         most mixes of a busy server never come again and are not worth a capture."""
         if not self.use_graphs:
             return False
         key = self._graph_key(entries)
-        if isinstance(key[0], int) or key in self.graphs:
+        if key in self.graphs:
             return True
+        if isinstance(key[0], int):
+            return not self._is_planned(key) or self._room_for_a_graph(planned=True)
         if sum(len(e.tokens) for e in entries) > self.GRAPH_TOKENS:
             return False
         seen = self._shapes_seen.pop(key, 0) + 1              # back in at the young end
@@ -539,8 +567,6 @@ class Engine:
         return logits
 
     # -------------------------------------------------------------------- sharing
-    SHARED_FILL = 32        # a plan's list of work is filled up to a multiple of this, so that plans can share a captured graph
-
     def _shapes_that_share(self) -> list[tuple]:
         """(cache group, query heads, kv heads, head size) of the attention that can use a plan of shared prefixes."""
         ops, shapes = self.model.runtime.ops, set()
@@ -578,7 +604,7 @@ class Engine:
             width = max([1] + [len(t) for t in tables])
             table = np.array([t + [-1] * (width - len(t)) for t in tables], dtype=np.int32)
             plan = self.model.runtime.ops.plan_shared_prefixes(table, positions, self.cache.page_size, n_q, n_kv, head_dim, self.model.dtype,
-                                                               self.model.device, fill=self.SHARED_FILL, growth=self.GRAPH_BUCKET)
+                                                               self.model.device, fill=True, growth=self.GRAPH_BUCKET)
             if plan.runs:
                 plans[(group, n_q, n_kv, head_dim)] = plan
         plans = plans or NOTHING_SHARED

@@ -1541,12 +1541,12 @@ class Ops:
         return out
 
     def plan_shared_prefixes(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int,
-                             dtype: torch.dtype, device="cuda:0", fill: int = 0, growth: int | None = None) -> SharedPrefixes:
+                             dtype: torch.dtype, device="cuda:0", fill: bool = False, growth: int | None = None) -> SharedPrefixes:
         """What the requests of a batch of single tokens share, laid out for `shared_prefix_attention`.
 
         block_table (on the host) int [B, P]: row i's pages, -1 where there is none; positions (on the host) int [B]: where the rows'
-        newest tokens stand.  A plan holds as long as the rows keep their order, their leading pages and do not go back.  `fill`: the list
-        of work is filled up to a multiple of so many items, so that plans that differ a little have one size.  `growth`: by how many
+        newest tokens stand.  A plan holds as long as the rows keep their order, their leading pages and do not go back.  `fill`: the lists
+        of work are filled up to a few sizes, so that plans that differ a little can share a captured graph.  `growth`: by how many
         tokens the rows are expected to grow (None: all of them to the table's end).  The plan holds past that too, but the work of rows of
         very different lengths is spread better the less is expected."""
         import numpy as np
