@@ -381,7 +381,7 @@ def test_graphs_of_steps_with_plans_are_bounded(model_folders, monkeypatch):
     from types import SimpleNamespace
     from tokenizer_amd.engine import engine as of_engine
     monkeypatch.setattr(of_engine, "StepGraph", lambda engine, entries, bucket: SimpleNamespace(bucket=bucket, last_used=0))
-    engine = _engine(model_folders["A"])
+    engine = _engine(model_folders["A"], shared_attention=True)
     engine.use_graphs = True
     engine.PLAN_GRAPHS, engine.PLAN_IDLE_STEPS = 3, 10
     for r in range(2):

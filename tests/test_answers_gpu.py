@@ -220,3 +220,49 @@ def test_decode_steps_without_room_for_a_graph(warm, monkeypatch):
         engine.cache.check_invariants()
         out.append(seen)
     assert out[0] == out[1]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_forks_that_share_little_take_the_faster_way(dtype):
+    # Small batches of forks go as requests that share nothing do, bit for bit; a batch that shares much does not, unless it is told to.
+    from tokenizer_amd.engine import StepEntry
+    for n, length, pays in ((6, 64, False), (6, 1100, False), (24, 3000 if dtype == "float32" else 3900, True)):
+        more = dict(num_pages=1000)
+        engines = [engine_of(dtype, **more), engine_of(dtype, shared_attention=True, **more), engine_of(dtype, shared_attention=False, **more)]
+        for e in engines:
+            forked(e, random_ids(1000, length, 1), n)
+        for turn in range(3):
+            entries = [StepEntry(r, [int(t)], [0]) for r, t in enumerate(random_ids(1000, n, 50 + turn))]
+            default, always, never = (e.step([dataclasses.replace(x) for x in entries]).clone() for e in engines)
+            assert bool(engines[0].sharing_used(entries)) == pays and engines[1].sharing_used(entries) and not engines[2].sharing_used(entries)
+            assert torch.equal(default, always if pays else never)
+            close(always, never, dtype)
+
+
+@pytest.fixture
+def every_plan(monkeypatch):
+    from tokenizer_amd.kernels.shared_prefix import SharedPrefixes
+    monkeypatch.setattr(SharedPrefixes, "PAYS_FROM", 0)
+    monkeypatch.setattr(SharedPrefixes, "WHOLE_KEYS", 0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("length", [64, 1100])
+def test_steps_of_forks_where_every_plan_is_taken(every_plan, dtype, length):
+    test_steps_of_forks_are_those_of_requests_alone(dtype, length)
+
+
+def test_plans_that_are_all_taken_change_with_the_requests(every_plan):
+    test_plans_change_with_the_requests()
+
+
+@pytest.mark.parametrize("params", [dict(temperature=1.0, top_k=20), dict(temperature=0.8, top_p=0.9, min_p=0.01), dict(temperature=0.0)],
+                         ids=["top-k", "min-p", "greedy"])
+def test_answers_where_every_plan_is_taken(every_plan, params):
+    test_answers_are_those_of_single_requests(params)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("module,table,name", [("napadra_configs", "NAPADRA", "P"), ("gafonex_configs", "GAFONEX", "A"), ("zeridra_configs", "ZERIDRA", "A")])
+def test_forks_of_other_designs_where_every_plan_is_taken(every_plan, module, table, name, dtype, tmp_path):
+    test_forks_of_other_designs(module, table, name, dtype, tmp_path)

@@ -210,3 +210,14 @@ def test_plans_of_many_prompts_have_few_makes(n_q, n_kv, d):
                 produced = min(end, bucket - length)
             live -= 1
     assert len(makes) <= 1.75 * len(plain)
+
+
+@pytest.mark.parametrize("rows,keys,n_q,n_kv,d,dtype,pays", [
+    (2, 256, 14, 2, 64, torch.bfloat16, False), (2, 4096, 14, 2, 64, torch.bfloat16, False), (8, 1024, 14, 2, 64, torch.bfloat16, False),
+    (16, 4096, 14, 2, 64, torch.bfloat16, True), (64, 2048, 14, 2, 64, torch.bfloat16, True), (128, 512, 14, 2, 64, torch.bfloat16, False),
+    (4, 4096, 28, 4, 128, torch.bfloat16, True), (64, 512, 28, 4, 128, torch.bfloat16, False), (64, 1024, 28, 4, 128, torch.bfloat16, True),
+    (4, 1024, 14, 2, 64, torch.float32, False), (64, 512, 14, 2, 64, torch.float32, True)])
+def test_plans_say_whether_they_are_faster_than_none(rows, keys, n_q, n_kv, d, dtype, pays):
+    table = _table([list(range(keys // 16)) + [10000 + 3 * r + i for i in range(3)] for r in range(rows)])
+    assert SharedPrefixes(table, [keys + 40] * rows, 16, n_q, n_kv, d, dtype, "cpu").pays == pays
+    assert not SharedPrefixes(np.arange(rows * 3, dtype=np.int32).reshape(rows, 3), [40] * rows, 16, n_q, n_kv, d, dtype, "cpu").pays

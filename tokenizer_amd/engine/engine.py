@@ -87,7 +87,7 @@ class StepGraph:
         self.ctx = build_context(entries, engine.cache, device, table_width=self.width, into=(self.host, self.dev), fill=True)
         self.ctx.max_position = bucket - 1          # what the kernels' launch sizes are planned for
         # What the requests share is filled in again too, where it has changed (plans of one signature: they are in the graph's key).
-        self.sharing_now = engine.sharing(entries)
+        self.sharing_now = engine.sharing_used(entries)
         self.ctx.sharing = {shape: plan.standing_copy() for shape, plan in self.sharing_now.items()}
         ops = engine.model.runtime.ops
         before = getattr(ops, "capturing", False)
@@ -194,7 +194,7 @@ class StepGraph:
             self.uploads += 1
             if tokens_on_device is not None:
                 self.dev[:count].copy_(tokens_on_device[:count], non_blocking=True)
-        plans = engine.sharing(entries)
+        plans = engine.sharing_used(entries)
         if plans is not self.sharing_now:
             for shape, plan in plans.items():
                 self.ctx.sharing[shape].take(plan)
@@ -258,7 +258,8 @@ class Engine:
                  max_num_batched_tokens: int = 2048, shared_attention: bool | None = None):
         """`shared_attention`: whether decode steps go through keys that several of their requests share once for all of them
         (attention that sees every key; sums fall apart differently then, so logits differ in their last bits).  None: where
-        requests are forks of one (`fork_request`); True: wherever leading pages are shared, by the prefix cache too; False: never.
+        requests are forks of one (`fork_request`) and share so much that it is faster; True: wherever leading pages are shared, by the
+        prefix cache too; False: never.
 
         `num_blocks` and `max_batch_size` are the reference's names (qwen-server/src/lib.rs:33-56) for
         `num_pages` and `max_requests`; `max_num_batched_tokens` is the token budget of `run()`.  Without
@@ -290,6 +291,7 @@ class Engine:
         self._family: set = set()    # requests that were forked or are forks
         self._sharing: tuple | None = None        # (epoch, requests, bucket of context), their plans
         self._sharing_due = 0        # the step from which on they may be past that bucket
+        self._paying: tuple = (NOTHING_SHARED, NOTHING_SHARED)    # plans, and those of them that are faster than none
         self._shared_shapes = self._shapes_that_share()
         self.steps = 0
         self._landing: dict[int, tuple] = {}     # pinned rows and events of `decode_greedy` / `decode_sampled`, by batch size
@@ -499,7 +501,7 @@ class Engine:
 
     def _graph_key(self, entries: list[StepEntry]) -> tuple:
         bucket, _ = self._bucket_of(entries)
-        plans = self.sharing(entries)
+        plans = self.sharing_used(entries)
         if plans:
             return (self._shape_of(entries), bucket, tuple((shape, plans[shape].signature) for shape in sorted(plans)))
         return (self._shape_of(entries), bucket)
@@ -610,6 +612,15 @@ class Engine:
         plans = plans or NOTHING_SHARED
         self._sharing = ((*key, bucket), plans)
         return plans
+
+    def sharing_used(self, entries: list[StepEntry]) -> dict:
+        """Those of the step's plans that its attention goes by: all where `shared_attention` asks for it, else those that pay."""
+        plans = self.sharing(entries)
+        if self.shared_attention or not plans:
+            return plans
+        if self._paying[0] is not plans:
+            self._paying = (plans, {shape: plan for shape, plan in plans.items() if plan.pays} or NOTHING_SHARED)
+        return self._paying[1]
 
     # ------------------------------------------------------------------ requests
     def fork_request(self, rid, new_rids) -> None:
@@ -722,7 +733,7 @@ class Engine:
             logits = self._graph_step(entries)
         else:
             ctx = build_context(entries, self.cache, self.model.device, fill=True)
-            ctx.sharing = self.sharing(entries)
+            ctx.sharing = self.sharing_used(entries)
             logits = self.model.decoder.forward(ctx, self.layer_caches)
         if logits.shape[0] != wanted:
             logits = logits[:wanted]        # the rows behind them belong to what the step was filled up with

@@ -100,6 +100,16 @@ class SharedPrefixes:
     # 15.5 | 18.5 | 18.2, 16 15.1 | 14.2 | 18.1, 2 behind 32,000 22.0 | 26.7 | 32.7.)
     TARGET, FEW_TARGET = 512, 256
 
+    # Whether going through shared keys once is faster than each request's going through them by itself (`pays`): it spares the reading of so many
+    # bytes of keys and values, and costs a launch that joins the parts where the other way often has none; in bfloat16 that one has none for
+    # contexts of up to WHOLE_KEYS and from WHOLE_ROWS rows x kv heads on.  (Each alone | shared, us in captured steps, 40 keys of their own: 14 query
+    # heads of size 64, 2 kv heads, bfloat16, 2 requests of 256 keys 5.1 | 7.1, of 4,096 7.5 | 10.1; 8 of 4,096 (14.7 MB) 9.7 | 10.3, 16 of
+    # 4,096 (31) 10.5 | 10.1; 64 of 512 (16.5) 8.8 | 8.3, of 4,096 18.0 | 12.7; 128 of 512 6.8 | 9.2, of 1,024 12.9 | 10.5.  28 heads of 128,
+    # 4 kv heads, 8 of 1,024 (14.7) 9.6 | 10.0, 4 of 4,096 (25) 14.7 | 12.1, 64 of 4,096 57 | 20.  In 32 bits, 14 heads of 64, 4 of 2,048 (6.3)
+    # 9.8 | 10.6, 8 of 2,048 (14.7) 11.4 | 10.6, 64 of 2,048 26.1 | 15.7.  Over 732 such pairs of three more shapes, and with 400 keys of their own, this
+    # rule is 0.8 % off the faster one on average, always sharing 12.8 %.  At worst, 32 of 256 keys of size 128 in 32 bits, 15.4 for 11.1.)
+    PAYS_FROM, WHOLE_KEYS, WHOLE_ROWS = 16_000_000, 1024, 128
+
     def __init__(self, block_table, positions, page_size: int, n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype, device,
                  fill: bool = False, growth: int | None = None):
         table = np.asarray(block_table, dtype=np.int32)
@@ -109,6 +119,10 @@ class SharedPrefixes:
         self.order, self.runs, own_begin = find_shared_runs(table, positions, page_size, self.MIN_KEYS)
         place = {row: at for at, row in enumerate(self.order)}
         group = n_q // n_kv
+        spared = sum((len(run.rows) - 1) * (run.key_end - run.key_begin) for run in self.runs) * 2 * n_kv * head_dim * dtype.itemsize
+        whole = (dtype == torch.bfloat16 and max(positions, default=0) < self.WHOLE_KEYS
+                 and self.n_rows * n_kv * -(-group // self.FEW_COLUMNS) >= self.WHOLE_ROWS)
+        self.pays = bool(self.runs) and spared >= self.PAYS_FROM and not whole
         # A run's columns in tiles of many, where there is work for them, and what is left, if that is little, in tiles of few.
         wide = dtype == torch.bfloat16 and head_dim in self.WIDE_HEADS
         size, little = (self.WIDE_COLUMNS, self.WIDE_LITTLE) if wide else (self.MANY_COLUMNS, self.MANY_LITTLE)
