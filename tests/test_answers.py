@@ -410,3 +410,34 @@ def test_graphs_of_steps_with_plans_are_bounded(model_folders, monkeypatch):
     assert engine._graph_for(entries) is not None               # (the other idle one)
     make = 6
     assert engine._graph_for(entries) is None and len(engine.graphs) == 4
+
+
+@pytest.mark.parametrize("name", ["A", "B"])
+@pytest.mark.parametrize("num_pages", [5, 6, 7, 9, 12])
+@pytest.mark.parametrize("params", [GenerateParams(max_tokens=40, temperature=1.2, top_k=20, seed=3), GenerateParams(max_tokens=37, temperature=3.0, seed=1, eos=list(range(0, 64, 9))),
+                                    GenerateParams.greedy(35)], ids=["top-k", "some end early", "greedy"])
+def test_answers_wait_where_the_pool_runs_out(model_folders, name, num_pages, params):
+    # Five answers hold up to sixteen pages together, one of them four: the newest wait until the others have ended, and lose nothing.
+    import dataclasses
+    folder = model_folders[name]
+    prompt = random_ids(_engine(folder).model.vocab_size, 16, 8)
+    engine = _engine(folder, num_pages=num_pages)
+    forked = []
+    inner = engine.fork_request
+    engine.fork_request = lambda rid, new: (forked.append(len(new)), inner(rid, new))[1]
+    answers = generate_answers(engine, prompt, params, 5)
+    for i, answer in enumerate(answers):
+        want = _alone(folder, prompt, dataclasses.replace(params, seed=params.seed + i))
+        assert (answer.tokens, answer.text, answer.reason, answer.completion_tokens) == (want.tokens, want.text, want.reason, want.completion_tokens)
+    assert params.eos or num_pages > 9 or len(forked) > 1
+    assert len(engine.cache.requests) == 0
+    engine.cache.check_invariants()
+    assert all(g.allocator.free_count() == num_pages for g in engine.cache.groups)
+
+
+def test_one_answer_that_the_pool_cannot_hold_is_out_of_pages(model_folders):
+    engine = _engine(model_folders["A"], num_pages=3)
+    with pytest.raises(OutOfPages):
+        generate_answers(engine, random_ids(engine.model.vocab_size, 16, 8), GenerateParams(max_tokens=60, temperature=1.0), 3)
+    assert len(engine.cache.requests) == 0
+    engine.cache.check_invariants()

@@ -5,6 +5,7 @@ from __future__ import annotations
 import dataclasses
 import time
 
+from ..cache import OutOfPages
 from .batch import StepEntry
 from .generate import (Control, GenerateParams, Generated, SampleCursor, Sampled, StopReason, _go_on, _no_bytes,
                        filters_of)
@@ -107,7 +108,9 @@ def generate_answers(engine, prompt, params: GenerateParams, n: int, token_bytes
     """`n` answers to one prompt, decoded together: the prompt is run once, its request forked (the answers share its pages of the
     cache, which every decode step goes through once for all of them), and answer i is drawn with the seed `params.seed` + i.
     `engine`: an `Engine` with room for `n` requests, or a bare model; `prompt`, `token_bytes`, `tokenizer` as for `generate`.
-    The times of an answer are those of all."""
+    The times of an answer are those of all.  Where the pool runs out of pages while they decode, the newest answers' requests go, and come
+    back, the prompt and what they had drawn run again, when the others have ended; `OutOfPages` where there is no room for the
+    forks to begin with, or for a single answer."""
     if n < 1:
         raise ValueError("at least one answer")
     if isinstance(prompt, str):
@@ -159,15 +162,27 @@ def generate_answers(engine, prompt, params: GenerateParams, n: int, token_bytes
         going_on = sorted(tokens)
         if going_on:
             # (The prompt's own request is the first answer that goes on.)
-            names = {i: rids[0] if at == 0 else rids[i] if i else rids[going_on[0]] for at, i in enumerate(going_on)}
+            names = {i: rids[i] if at else rids[0] for at, i in enumerate(going_on)}
             others = [names[i] for i in going_on[1:]]
             if others:
                 engine.fork_request(rids[0], others)
                 live += others
-        while tokens:
+        waiting: list[int] = []                           # answers whose requests had to go, the oldest first
+        while tokens or waiting:
+            if not tokens:
+                back = _come_back(engine, prompt, [(names[i], cursors[i].tokens) for i in waiting], live)
+                tokens.update((i, cursors[i].tokens[-1]) for i in waiting[:back])
+                waiting = waiting[back:]
             answers = sorted(tokens)
             steps = min(min(params.max_tokens - cursors[i].produced for i in answers), ANSWER_BURST)
-            handled = 0
+            steps = engine.steps_with_pages([names[i] for i in answers], steps)
+            if steps == 0 and len(answers) > 1:
+                waiting.insert(0, answers[-1])
+                engine.end_request(names[answers[-1]])
+                live.remove(names[answers[-1]])
+                tokens.pop(answers[-1])
+                continue
+            steps, handled = max(1, steps), 0             # (no page for a single answer: its step says so)
 
             def on_step(_k, ids):
                 nonlocal handled
@@ -193,6 +208,41 @@ def generate_answers(engine, prompt, params: GenerateParams, n: int, token_bytes
             engine.end_request(rid)
     decode = time.perf_counter() - started
     return [Generated(d.tokens, d.text, d.chunks, d.reason, d.completion_tokens, prefill, decode) for d in done]
+
+
+def _come_back(engine, prompt, answers, live) -> int:
+    """Makes requests for answers, (name, tokens drawn) each, that hold the prompt and all but the last of those tokens: the prompt is run
+    once, for the first of them, and as many others are its forks as there are pages for.  Returns how many answers are back."""
+    names = []
+
+    def fits() -> bool:
+        missing = [0] * len(engine.cache.groups)
+        for name, drawn in answers[:len(names)]:
+            for group, pages in enumerate(engine.cache.pages_missing(name, len(prompt) + len(drawn))):
+                missing[group] += pages
+        return all(pages <= group.allocator.available() for pages, group in zip(missing, engine.cache.groups))
+
+    for name, _ in answers:
+        if not names:
+            engine.add_request(name)
+            live.append(name)
+            engine.step([StepEntry(name, list(prompt), [])])
+        else:
+            try:
+                engine.fork_request(names[0], [name])
+            except OutOfPages:
+                break
+            live.append(name)
+        names.append(name)
+        if len(names) > 1 and not fits():
+            names.pop()
+            engine.end_request(name)
+            live.remove(name)
+            break
+    entries = [StepEntry(name, list(drawn[:-1]), []) for name, drawn in answers[:len(names)] if len(drawn) > 1]
+    if entries:
+        engine.step(entries)
+    return len(names)
 
 
 ANSWER_BURST = 16       # decode steps of answers that run back to back before finished ones leave

@@ -718,6 +718,19 @@ class Engine:
                 raise OutOfPages(f"no pages left for request {entry.rid!r} to reach {new_len} tokens "
                                  f"({self.cache.num_pages} pages of {self.cache.page_size})")
 
+    def steps_with_pages(self, rids: list, most: int) -> int:
+        """How many next tokens, up to `most`, the pool has pages for in all of these requests together (in halves of `most`)."""
+        steps = most
+        while steps > 0:
+            missing = [0] * len(self.cache.groups)
+            for rid in rids:
+                for group, pages in enumerate(self.cache.pages_missing(rid, self.cache.seq_len(rid) + steps)):
+                    missing[group] += pages
+            if all(pages <= group.allocator.available() for pages, group in zip(missing, self.cache.groups)):
+                break
+            steps //= 2
+        return steps
+
     def step(self, entries: list[StepEntry], reserve: bool = True) -> torch.Tensor:
         """Run the entries' tokens as one batch; float32 logits [wanted, vocab].  The step itself works on pages
         that are there: `reserve=True` (callers without a scheduler: replay, `generate`, tests) first asks the
