@@ -441,3 +441,31 @@ def test_one_answer_that_the_pool_cannot_hold_is_out_of_pages(model_folders):
         generate_answers(engine, random_ids(engine.model.vocab_size, 16, 8), GenerateParams(max_tokens=60, temperature=1.0), 3)
     assert len(engine.cache.requests) == 0
     engine.cache.check_invariants()
+
+
+def test_forks_that_cannot_all_be_made_leave_everything_as_it_was(model_folders):
+    # Not the requests alone: the prefixes that the pool keeps are still there too, and so are names that cannot be a request's.
+    engine = _engine(model_folders["A"], num_pages=10, prefix_cache=True)
+    vocab = engine.model.vocab_size
+    kept = random_ids(vocab, 49, 1)
+    engine.add_request("old")
+    engine.step([StepEntry("old", kept)])
+    engine.cache.publish("old", kept)
+    engine.end_request("old")
+    engine.add_request("a")
+    engine.step([StepEntry("a", random_ids(vocab, 70, 2))])
+    free, epoch = [g.allocator.available() for g in engine.cache.groups], engine.cache.epoch
+    for bad, error in (([f"b{i}" for i in range(6)], OutOfPages), (["b", "c", "b"], KeyError), (["b", "a"], KeyError), (["b", []], TypeError),
+                       (["b", "c", "d", "e", "f", "g", "h", "i"], OutOfPages)):
+        with pytest.raises(error):
+            engine.fork_request("a", bad)
+        assert list(engine.cache.requests) == ["a"] and engine.cache.epoch == epoch
+        assert [g.allocator.available() for g in engine.cache.groups] == free
+        engine.cache.check_invariants()
+    with pytest.raises(KeyError):
+        engine.fork_request("none", ["b"])
+    engine.add_request("again")
+    assert engine.cache.attach_shared_prefix("again", kept) == 48
+    engine.end_request("again")
+    engine.fork_request("a", [f"b{i}" for i in range(5)])         # as many as there are pages for (the kept ones make room)
+    assert len(engine.cache.requests) == 6

@@ -267,6 +267,11 @@ class CacheManager:
         self._lib.ta_cache_publish(self._core, self._handle_of(rid), pointer, len(keep))
 
     # --------------------------------------------------------------------- forks
+    def can_fork(self, rid, count: int) -> bool:
+        """Whether there are slots, and pages for the one that is not full, for so many forks of a request."""
+        last = 1 if self.seq_len(rid) % self.page_size else 0
+        return self.free_slot_count() >= count and all(group.allocator.available() >= count * last for group in self.groups)
+
     def fork(self, rid, new_rid) -> tuple[list[tuple[int, int, int]], tuple[int, int]]:
         """`new_rid` becomes a live request that holds what `rid` holds: they share the full pages, and the page that is not full
         (one in every group) is the new request's own.  Returns the pages whose contents are to be copied, as (group, from, to), and

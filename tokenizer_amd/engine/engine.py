@@ -627,17 +627,17 @@ class Engine:
         """Make every one of `new_rids` a live request that holds what `rid` holds: the same tokens, to be continued on their own.  Full
         pages are shared; the last one, where it is not full, is copied for each, and so is what layers keep in the request's slot.
         `OutOfPages` with nothing changed if a slot or a page is missing."""
-        new_rids, made, copies, slots = list(new_rids), [], [], []
-        try:
-            for new_rid in new_rids:
-                pages, pair = self.cache.fork(rid, new_rid)
-                made.append(new_rid)
-                copies += pages
-                slots.append(pair)
-        except (OutOfPages, KeyError):
-            for new_rid in made:
-                self.cache.release(new_rid)
-            raise
+        # (All is asked before the first fork is made: one taken back would have cost the pool prefixes that it keeps.)
+        new_rids, copies, slots = list(new_rids), [], []
+        taken = [r for r in new_rids if self.cache.has_request(r)]
+        if taken or len(set(new_rids)) < len(new_rids):
+            raise KeyError(f"request {taken[0]!r} is already live" if taken else "a fork is named twice")
+        if not self.cache.can_fork(rid, len(new_rids)):
+            raise OutOfPages(f"no slots or no pages left for {len(new_rids)} forks of request {rid!r}")
+        for new_rid in new_rids:
+            pages, pair = self.cache.fork(rid, new_rid)
+            copies += pages
+            slots.append(pair)
         self.pools.copy_pages(copies, self.model.runtime.ops)
         for src, dst in slots:
             self.pools.copy_states(src, dst)
