@@ -266,3 +266,24 @@ def test_answers_where_every_plan_is_taken(every_plan, params):
 @pytest.mark.parametrize("module,table,name", [("napadra_configs", "NAPADRA", "P"), ("gafonex_configs", "GAFONEX", "A"), ("zeridra_configs", "ZERIDRA", "A")])
 def test_forks_of_other_designs_where_every_plan_is_taken(every_plan, module, table, name, dtype, tmp_path):
     test_forks_of_other_designs(module, table, name, dtype, tmp_path)
+
+
+def test_pages_move_under_held_plans_and_captured_steps():
+    # A request that lies low ends, and the pages of the others, shared ones among them, move into its place between steps.
+    from tokenizer_amd.engine import StepEntry
+    engines = [engine_of("float32", shared_attention=True), engine_of("float32", shared_attention=True, use_graphs=False), engine_of("float32", shared_attention=False)]
+    for e in engines:
+        e.add_request(50)
+        e.step([StepEntry(50, random_ids(1000, 300, 5))])
+        forked(e, random_ids(1000, 210, 6), 7)
+    for turn in range(12):
+        if turn == 4:
+            for e in engines:
+                before = [e.cache.table(r, 0) for r in range(7)]
+                e.end_request(50)
+                assert e.compact_cache() >= 13                  # the thirteen shared pages at least
+                assert [e.cache.table(r, 0) for r in range(7)] != before and e.compact_cache() == 0
+        entries = [StepEntry(r, [int(t)], [0]) for r, t in enumerate(random_ids(1000, 7, 130 + turn))]
+        shared, eager, apart = (e.step([dataclasses.replace(x) for x in entries]).clone() for e in engines)
+        assert engines[0].sharing(entries) and torch.equal(shared, eager)
+        close(shared, apart, "float32")
