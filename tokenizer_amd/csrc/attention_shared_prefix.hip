@@ -202,36 +202,29 @@ struct Frag<float, D> {
   }
 };
 
-// A step of the softmax: `s` holds BLOCKS blocks of 32 scores a column (a lane half's sixteen each), of which the first `there` keys count;
+// A step of the softmax: `s` holds 32 scores a column (a lane half's sixteen each), of which the first `there` keys count;
 // they become weights.  m: the largest score so far, in units of 1 / log2(e) (a weight is then one instruction of the exponent's),
 // l: this lane's sum of weights, o: the weighed values, all brought to the new maximum where it has grown for any of the wave's columns.
 //   The maximum is a reference alone: a weight may be up to 2^SP_SLACK as long as no rescaling has been due (rescaling at every new maximum
 //   of any of 32 columns came up in nearly every block: 64 of 220 vector instructions of a block of 64 keys at head size 128).
 #define SP_SLACK 8.f
-template <typename T, int BLOCKS, int ROWS>
-__device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)[BLOCKS], int there, int half, float& m, float& l,
-                                           sp_floatx16 (&o)[ROWS]) {
+template <typename T, int ROWS>
+__device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16& s, int there, int half, float& m, float& l, sp_floatx16 (&o)[ROWS]) {
   float scale = a.scale * LOG2E;
   if (a.softcap > 0.f) {
     const float inner = 2.f * LOG2E * a.scale / a.softcap;
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[b][i] = sp_capped<T>(s[b][i], inner, a.softcap);
+    for (int i = 0; i < 16; ++i) s[i] = sp_capped<T>(s[i], inner, a.softcap);
     scale = LOG2E;
   }
-  if (there < BLOCKS * SP_BLOCK) {
+  if (there < SP_BLOCK) {
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (SP_BLOCK * b + 16 * (i >> 3) + 8 * half + (i & 7) >= there) s[b][i] = -INFINITY;
+    for (int i = 0; i < 16; ++i)
+      if (16 * (i >> 3) + 8 * half + (i & 7) >= there) s[i] = -INFINITY;
   }
-  float high = s[0][0];
+  float high = s[0];
 #pragma unroll
-  for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) high = fmaxf(high, s[b][i]);
+  for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
   high = wave_max_across<32>(high) * scale;                // (the scale is positive)
   if (__any(high > m + SP_SLACK)) {
     const float m_new = high > m + SP_SLACK ? high : m;       // (each column for itself: what stands beside it changes nothing)
@@ -246,12 +239,10 @@ __device__ __forceinline__ void sp_softmax(const SharedArgs& a, sp_floatx16 (&s)
   const float from = m == -INFINITY ? 0.f : m;             // (no key yet: weights of exp(-inf))
   float sum = 0.f;
 #pragma unroll
-  for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], scale, -from));
-      sum += s[b][i];
-    }
+  for (int i = 0; i < 16; ++i) {
+    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], scale, -from));
+    sum += s[i];
+  }
   l += sum;
 }
 
@@ -506,14 +497,14 @@ __device__ __forceinline__ void sp_wide(const SharedArgs& a, char* keys0, char* 
 }
 
 // ------------------------------------------------------------------------------------------------
-// One workgroup: some columns (COLS blocks of 32) of one kv head and a run of keys, which its waves share out block by block.
-template <typename T, int D, int COLS>
+// One workgroup: 32 columns of one kv head and a run of keys, which its waves share out block by block.
+template <typename T, int D>
 __global__ void __launch_bounds__(SP_WAVES * WAVE)
 shared_prefix_kernel(SharedArgs a) {
   typedef Frag<T, D> F;
   constexpr int ROWS = F::ROWS;
-  __shared__ float o_s[SP_WAVES / 2][COLS][ROWS * 32][33];
-  __shared__ float m_s[SP_WAVES][COLS * 32], l_s[SP_WAVES][COLS * 32];
+  __shared__ float o_s[SP_WAVES / 2][ROWS * 32][33];
+  __shared__ float m_s[SP_WAVES][32], l_s[SP_WAVES][32];
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int col = lane & 31, half = lane >> 5;
   const int group = a.n_q / a.n_kv;
@@ -522,27 +513,17 @@ shared_prefix_kernel(SharedArgs a) {
   const int begin = scalar_int(item + 3), end = scalar_int(item + 4), slot = scalar_int(item + 5);
   const int kvh = scalar_int(item + 7);
   if (columns <= 0) return;                                // an item that only fills the list up
-  // This lane's columns: request (row of the batch) and query head of each.
-  int row_of[COLS], head_of[COLS];
-  typename F::Query q[COLS];
-#pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    const int column = first_column + 32 * c + col;
-    const bool there = column < columns;
-    row_of[c] = there ? a.order[rows_at + column / group] : -1;
-    head_of[c] = kvh * group + column % group;
-    F::load_query(q[c], (const T*)a.q + (size_t)max(row_of[c], 0) * a.q_stride + (size_t)head_of[c] * D, there, half);
-  }
+  // This lane's column: request (row of the batch) and query head.
+  const int column = first_column + col;
+  const int row = column < columns ? a.order[rows_at + column / group] : -1;
+  const int head = kvh * group + column % group;
+  typename F::Query q;
+  F::load_query(q, (const T*)a.q + (size_t)max(row, 0) * a.q_stride + (size_t)head * D, row >= 0, half);
   const int* table = a.block_table + (size_t)scalar_int(item + 6) * a.table_stride;
-  sp_floatx16 o[COLS][ROWS];
-  float m[COLS], l[COLS];
+  sp_floatx16 o[ROWS];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    m[c] = -INFINITY;
-    l[c] = 0.f;
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) o[c][r] = (sp_floatx16){};
-  }
+  for (int r = 0; r < ROWS; ++r) o[r] = (sp_floatx16){};
   const size_t page_elems = (size_t)a.page_size * D;
   const T *k_pages = (const T*)a.k_pages, *vt_pages = (const T*)a.vt_pages;
   // Which key of a block this lane's row of the first product is.
@@ -562,71 +543,50 @@ shared_prefix_kernel(SharedArgs a) {
     f.load_values(vt_pages + at0 + slot0, vt_pages + at1 + slot1, a.page_size, col, half);
     const int there = end - kb;                            // keys of the block that count
     if (there < SP_BLOCK) f.cut_values(there, half);
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-      sp_floatx16 s[1] = {f.scores(q[c])};
-      sp_softmax<T, 1, ROWS>(a, s, there, half, m[c], l[c], o[c]);
-      f.add_values(s[0], o[c]);
-    }
+    sp_floatx16 s = f.scores(q);
+    sp_softmax<T, ROWS>(a, s, there, half, m, l, o);
+    f.add_values(s, o);
   }
   // The waves' results brought together: two halves of the waves, then one wave takes what the other left.
-#pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    l[c] = wave_add_across<32>(l[c]);
-    if (half == 0) { m_s[wave][32 * c + col] = m[c]; l_s[wave][32 * c + col] = l[c]; }
-  }
+  l = wave_add_across<32>(l);
+  if (half == 0) { m_s[wave][col] = m; l_s[wave][col] = l; }
   __syncthreads();
-  float all_m[COLS], all_l[COLS];
+  float all_m = -INFINITY, all_l = 0.f;
+  for (int w = 0; w < SP_WAVES; ++w) all_m = fmaxf(all_m, m_s[w][col]);
+  for (int w = 0; w < SP_WAVES; ++w) all_l += all_m == -INFINITY ? 0.f : l_s[w][col] * __builtin_amdgcn_exp2f(m_s[w][col] - all_m);
+  const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - all_m);
 #pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    all_m[c] = -INFINITY;
-    all_l[c] = 0.f;
-    for (int w = 0; w < SP_WAVES; ++w) all_m[c] = fmaxf(all_m[c], m_s[w][32 * c + col]);
-    for (int w = 0; w < SP_WAVES; ++w)
-      all_l[c] += all_m[c] == -INFINITY ? 0.f : l_s[w][32 * c + col] * __builtin_amdgcn_exp2f(m_s[w][32 * c + col] - all_m[c]);
-    const float mine = m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[c] - all_m[c]);
+  for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[c][r][i] *= mine;
-  }
+    for (int i = 0; i < 16; ++i) o[r][i] *= mine;
 #pragma unroll
   for (int step = SP_WAVES / 2; step >= 1; step >>= 1) {
     if (wave >= step && wave < 2 * step) {
 #pragma unroll
-      for (int c = 0; c < COLS; ++c)
+      for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o_s[wave - step][c][32 * r + 8 * (i >> 2) + 4 * half + (i & 3)][col] = o[c][r][i];
+        for (int i = 0; i < 16; ++i) o_s[wave - step][32 * r + 8 * (i >> 2) + 4 * half + (i & 3)][col] = o[r][i];
     }
     __syncthreads();
     if (wave < step) {
 #pragma unroll
-      for (int c = 0; c < COLS; ++c)
+      for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[c][r][i] += o_s[wave][c][32 * r + 8 * (i >> 2) + 4 * half + (i & 3)][col];
+        for (int i = 0; i < 16; ++i) o[r][i] += o_s[wave][32 * r + 8 * (i >> 2) + 4 * half + (i & 3)][col];
     }
     __syncthreads();
   }
-  if (wave != 0) return;
+  if (wave != 0 || row < 0) return;
+  const size_t at = ((size_t)row * a.n_q + head) * a.slots + slot;
+  if (half == 0) { a.part_ml[2 * at] = all_m; a.part_ml[2 * at + 1] = all_l; }
 #pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    if (row_of[c] < 0) continue;
-    const size_t at = ((size_t)row_of[c] * a.n_q + head_of[c]) * a.slots + slot;
-    if (half == 0) { a.part_ml[2 * at] = all_m[c]; a.part_ml[2 * at + 1] = all_l[c]; }
+  for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = 32 * r + 8 * j + 4 * half;
-        if (D % 32 == 0 || d < D)
-          *reinterpret_cast<sp_floatx4*>(a.part_o + at * D + d) =
-              (sp_floatx4){o[c][r][4 * j], o[c][r][4 * j + 1], o[c][r][4 * j + 2], o[c][r][4 * j + 3]};
-      }
-  }
+    for (int j = 0; j < 4; ++j) {
+      const int d = 32 * r + 8 * j + 4 * half;
+      if (D % 32 == 0 || d < D)
+        *reinterpret_cast<sp_floatx4*>(a.part_o + at * D + d) = (sp_floatx4){o[r][4 * j], o[r][4 * j + 1], o[r][4 * j + 2], o[r][4 * j + 3]};
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1018,7 +978,7 @@ static int launch_shared(const SharedArgs& a, void* out, hipStream_t stream) {
     status = LAUNCH_STATUS();
   } else {
     if (a.n_many > 0) {
-      shared_prefix_kernel<T, D, 1><<<a.n_many, SP_WAVES * WAVE, 0, stream>>>(a);
+      shared_prefix_kernel<T, D><<<a.n_many, SP_WAVES * WAVE, 0, stream>>>(a);
       status = LAUNCH_STATUS();
       if (status) return status;
     }
