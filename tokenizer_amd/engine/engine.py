@@ -599,14 +599,12 @@ class Engine:
         self._sharing_due = self.steps + bucket - longest + 1     # (a step of single tokens brings each request one further)
         if same and held[0][2] == bucket:
             return held[1]
-        positions = [self.cache.seq_len(e.rid) for e in entries]
+        positions, rids = [self.cache.seq_len(e.rid) for e in entries], [e.rid for e in entries]
         plans = {}
         for group, n_q, n_kv, head_dim in self._shared_shapes:
-            tables = [self.cache.table(e.rid, group) for e in entries]
-            width = max([1] + [len(t) for t in tables])
-            table = np.array([t + [-1] * (width - len(t)) for t in tables], dtype=np.int32)
-            plan = self.model.runtime.ops.plan_shared_prefixes(table, positions, self.cache.page_size, n_q, n_kv, head_dim, self.model.dtype,
-                                                               self.model.device, fill=True, growth=self.GRAPH_BUCKET)
+            plan = self.model.runtime.ops.plan_shared_prefixes(self.cache.tables(rids, group), positions, self.cache.page_size, n_q, n_kv,
+                                                               head_dim, self.model.dtype, self.model.device, fill=True,
+                                                               growth=self.GRAPH_BUCKET)
             if plan.runs:
                 plans[(group, n_q, n_kv, head_dim)] = plan
         plans = plans or NOTHING_SHARED
