@@ -282,6 +282,26 @@ def test_draws_of_few_and_many_long_rows(ops, rows):
         check_draws(ops, logits, uniform=rng.uniform(0, 1, rows), **given)
 
 
+@pytest.mark.parametrize("rows,spread", [(1, 2.2), (2, 0.5), (5, 3.0)])
+def test_the_workgroup_that_comes_last_finds_every_token(ops, rows, spread):
+    # Few rows: the workgroups of a row's pieces leave their tokens, and the last one to come draws.  Hundreds of draws of other logits each time, a
+    # list of up to some thousands from all pieces, in memory that the draw before has left full of its own.
+    first, second = hills(rows, 151936, torch.float32, rows, spread), hills(rows, 151936, torch.float32, 100 + rows, spread)
+    uniform = np.random.default_rng(rows).uniform(0, 1, rows)
+    given = dict(top_p=0.9, uniform=uniform)
+    want = [check_draws(ops, x, **given) for x in (first, second)]
+    numbers, held = settings(rows, **given), first.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.sample_filtered(held, **numbers)
+    seen = torch.empty((300, rows), dtype=torch.int32).cuda()
+    for turn in range(300):
+        held.copy_((first, second)[turn % 2])
+        graph.replay()
+        seen[turn] = out
+    assert seen[0::2].tolist() == [want[0]] * 150 and seen[1::2].tolist() == [want[1]] * 150
+
+
 @pytest.mark.parametrize("rows,vocab,dtype", [(216, 151936, torch.bfloat16), (830, 40001, torch.float32)])
 def test_draws_of_very_many_long_rows(ops, rows, vocab, dtype):
     # (A workgroup sees to several pieces of a row then.)  Each row's draw is what it is among eight, and of some by the definition.

@@ -1263,8 +1263,11 @@ sample_filtered_finish(FsArgs a) {
   u64 over;
   const FsRanges ranges = fs_settle(w, asked, over, s);
   fs_gather<1>(a, w, (const T*)a.logits + (size_t)row_at * a.stride, r, ranges, s);
+  // Every wave waits for its own tokens to have come to the chiplet's cache: a barrier does not wait for stores to global memory (its fences are
+  // the workgroup's, whose waves see each other's through the compute unit's cache), and one wave's fence waits for that wave's stores.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (threadIdx.x == 0) {                                  // (one thread's fences, between barriers, stand for the workgroup's)
+  if (threadIdx.x == 0) {                                  // (what is in that cache one thread's fences bring out, and in, for all)
     __threadfence();                                       // the tokens are there for all that see the count
     came = atomicAdd(&w.head()->gathered, 1);
     __threadfence();                                       // and so is what the others left before they counted themselves in
