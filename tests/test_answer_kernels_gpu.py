@@ -211,6 +211,19 @@ def test_draws_where_a_floor_keeps_few_or_thousands(ops, rows, vocab):
         check_draws(ops, logits, uniform=rng.uniform(0, 1, rows), **given)
 
 
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("vocab", [9000, 60000, 151936])
+def test_draws_where_fewer_tokens_weigh_anything_than_top_k_asks_for(ops, rows, vocab):
+    # A cold row, or one with a token far above the rest: a few dozen tokens, here and there or side by side, are all there is to list.
+    logits = hills(rows, vocab, torch.float32, rows + 1, 2.2)
+    logits[::3, 100:160] += 15.0
+    logits[1::3, 5] += 18.0
+    rng = np.random.default_rng(rows)
+    for given in (dict(top_k=100), dict(top_k=15, top_p=0.9), dict(top_k=200, min_p=1e-4)):
+        for temperature in (0.05, 0.2, 0.4, 1.0):
+            check_draws(ops, logits, uniform=rng.uniform(0, 1, rows), temperature=temperature, **given)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [196609, 256000, 1 << 19])
 def test_draws_from_the_largest_vocabularies(ops, vocab, dtype):

@@ -941,11 +941,10 @@ __device__ __forceinline__ float fs_cut_of_maxima(const float* __restrict__ maxi
   return least;
 }
 
-// Whether the maxima of groups of `of_logits` say that few tokens are no smaller than `cut`: no more groups than the list has room for, or one of
-// sixteen of those with anything above `least` has nothing.  (Spread evenly over N groups, M tokens leave N e^(-M / N) of them without any: a
-// sixteenth at 2.8 a group, that is, in a row of 151,936 logits, at 420 tokens by the waves' maxima and at 1,650 by those of their rows.)
+// Of how many groups of logits the maximum is no smaller than `cut`, and than `least`.
+struct FsAbove { int cut, least; };
 template <int MOST>
-__device__ __forceinline__ bool fs_few_above(const float* __restrict__ maxima, int count, int of_logits, float cut, float least) {
+__device__ __forceinline__ FsAbove fs_above(const float* __restrict__ maxima, int count, float cut, float least) {
   const int lane = threadIdx.x & (WAVE - 1);
   float m[MOST];
 #pragma unroll
@@ -953,21 +952,36 @@ __device__ __forceinline__ bool fs_few_above(const float* __restrict__ maxima, i
     m[j] = -INFINITY;
     if (j * WAVE + lane < count) m[j] = maxima[j * WAVE + lane];
   }
-  int above = 0, live = 0;
+  FsAbove above = {0, 0};
 #pragma unroll
   for (int j = 0; j < MOST; ++j)
     if (j * WAVE < count) {
-      above += __popcll(__ballot(m[j] >= cut));
-      live += __popcll(__ballot(m[j] >= least));
+      above.cut += __popcll(__ballot(m[j] >= cut));
+      above.least += __popcll(__ballot(m[j] >= least));
     }
-  return above * of_logits <= FS_LIST || 16 * (live - above) >= live;
+  return above;
+}
+
+// Whether the maxima say that few tokens are no smaller than `cut` (`least`: what lies below weighs nothing): there are no more groups with such a
+// token than the list has room for; or one in sixteen of the groups with anything to weigh has none; or the groups with one are hardly more
+// than the waves' of four groups.  (Spread evenly over N groups, M tokens leave N e^(-M / N) without any: a sixteenth at 2.8 a group, that is, in a
+// row of 151,936 logits, at 420 tokens by the waves' maxima and at 1,650 by those of their rows; and there are one and a half times as many
+// groups with a token as waves with one at 200 tokens, where a stretch of neighbours has four times as many.)  The waves' maxima, a quarter as
+// many, say it of most rows: 256 rows under min-p of 0.05 52.0 us, by the others alone 52.6.
+__device__ __forceinline__ bool fs_is_short(const FsSpace& w, float cut, float least) {
+  const int n_waves = w.pieces * FS_PIECE_WAVES, n_rows = w.pieces * FS_PIECE_ROWS;
+  const FsAbove waves = fs_above<8>(w.of_waves(), n_waves, cut, least);
+  if (waves.cut * (FS_PIECE / FS_PIECE_WAVES) <= FS_LIST || 16 * (waves.least - waves.cut) >= waves.least) return true;
+  const FsAbove rows = n_rows <= 12 * WAVE ? fs_above<12>(w.of_rows(), n_rows, cut, least) : fs_above<32>(w.of_rows(), n_rows, cut, least);
+  return rows.cut * (FS_PIECE / FS_PIECE_ROWS) <= FS_LIST || 16 * (rows.least - rows.cut) >= rows.least || 2 * rows.cut <= 3 * waves.cut;
 }
 
 // A logit so that every token that counts is no smaller, and whether the list of those is known to be short.  (A list of more than FS_LIST tokens is one
 // workgroup's, which reads the row again and again: rows of 151,936 flat logits (2.2 N(0, 1)) under min-p of 1e-6 took 359 us, under one of 0.01 at
 // T = 1.5 106 to 468; rows of which only 20,000 neighbours are allowed, under top-k 40, 382 to 539.)
 //   top-k: at least k of the maxima are no smaller; found by halving between the largest and the smallest logit that weighs
-//   anything, and what the halvings leave undecided stays above the cut.  Fewer than k maxima say nothing.
+//   anything, and what the halvings leave undecided stays above the cut.  Fewer than k maxima say nothing: the list is then whatever weighs
+//   anything.
 //   min-p (where top-p cuts nothing): max + T ln(min_p), less what 32 bits may be off by: 4 roundings of each of its parts.
 struct FsCut { float cut; bool is_short; };
 __device__ __forceinline__ FsCut fs_cut(const FsSpace& w, const FsAsked& asked, const FsRow& r, float low, int vocab) {
@@ -979,17 +993,12 @@ __device__ __forceinline__ FsCut fs_cut(const FsSpace& w, const FsAsked& asked, 
     c.cut = 2 * asked.top_k <= w.pieces * FS_PIECE_WAVES ? fs_cut_of_maxima<8>(w.of_waves(), w.pieces * FS_PIECE_WAVES, asked.top_k, least, high)
             : maxima <= 12 * WAVE                        ? fs_cut_of_maxima<12>(w.of_rows(), maxima, asked.top_k, least, high)
                                                          : fs_cut_of_maxima<32>(w.of_rows(), maxima, asked.top_k, least, high);
-    c.is_short = c.cut > -INFINITY;
+    c.is_short = c.cut > -INFINITY || fs_is_short(w, least, least);
   }
   if (fs_floor_alone(asked)) {
     const float down = -asked.temperature * logf(fminf(asked.min_p, 1.f));
     const float floor_cut = high - down - 4.8e-7f * (fabsf(high) + 2.f * down) - 1e-6f * asked.temperature;
-    // (The waves' maxima, a quarter as many, say it of most rows: 256 rows under min-p of 0.05 52.0 us, by the others alone 52.6.)
-    const float from = fmaxf(floor_cut, least);
-    if (!c.is_short) c.is_short = fs_few_above<8>(w.of_waves(), w.pieces * FS_PIECE_WAVES, FS_PIECE / FS_PIECE_WAVES, from, least);
-    if (!c.is_short)
-      c.is_short = maxima <= 12 * WAVE ? fs_few_above<12>(w.of_rows(), maxima, FS_PIECE / FS_PIECE_ROWS, from, least)
-                                       : fs_few_above<32>(w.of_rows(), maxima, FS_PIECE / FS_PIECE_ROWS, from, least);
+    if (!c.is_short) c.is_short = fs_is_short(w, fmaxf(floor_cut, least), least);
     c.cut = fmaxf(c.cut, floor_cut);
   }
   return c;
@@ -1180,6 +1189,7 @@ sample_filtered_settle(FsArgs a) {
   const int row_at = blockIdx.x;
   const FsSpace w = fs_space(a, row_at);
   const FsAsked asked = fs_asked(a, row_at);
+  const int listed = scalar_int(&w.head()->listed);
   float high, low;
   fs_row_extent(w, high, low);
   if (!fs_is_drawn(asked.temperature, high)) {
@@ -1187,7 +1197,7 @@ sample_filtered_settle(FsArgs a) {
     if (threadIdx.x == 0) a.out[row_at] = at;
     return;
   }
-  if (w.head()->listed) {
+  if (listed) {
     fs_draw_listed<T>(a, w, asked, fs_row(asked.temperature, high, low), row_at, nullptr, 0, w.head()->n_listed, s);
     return;
   }
@@ -1214,9 +1224,10 @@ sample_filtered_gather(FsArgs a) {
   __shared__ FsSmall s;
   const FsSpace w = fs_space(a, blockIdx.y);
   const FsAsked asked = fs_asked(a, blockIdx.y);
+  if (scalar_int(&w.head()->listed)) return;
   float high, low;
   fs_row_extent(w, high, low);
-  if (w.head()->listed || !fs_is_drawn(asked.temperature, high)) return;
+  if (!fs_is_drawn(asked.temperature, high)) return;
   fs_gather<SPAN>(a, w, (const T*)a.logits + (size_t)blockIdx.y * a.stride, fs_row(asked.temperature, high, low), fs_kept_ranges(w), s);
 }
 
@@ -1226,9 +1237,10 @@ sample_filtered_draw(FsArgs a) {
   __shared__ FsShared s;
   const FsSpace w = fs_space(a, blockIdx.x);
   const FsAsked asked = fs_asked(a, blockIdx.x);
+  if (scalar_int(&w.head()->listed)) return;
   float high, low;
   fs_row_extent(w, high, low);
-  if (w.head()->listed || !fs_is_drawn(asked.temperature, high)) return;
+  if (!fs_is_drawn(asked.temperature, high)) return;
   s.mass[threadIdx.x] = w.whole()->mass[threadIdx.x];
   s.count[threadIdx.x] = w.whole()->count[threadIdx.x];
   const FsRanges ranges = fs_kept_ranges(w);
@@ -1246,7 +1258,7 @@ sample_filtered_finish(FsArgs a) {
   const int row_at = blockIdx.y;
   const FsSpace w = fs_space(a, row_at);
   const FsAsked asked = fs_asked(a, row_at);
-  const bool listed = w.head()->listed;
+  const bool listed = scalar_int(&w.head()->listed);
   if (listed && blockIdx.x > 0) return;
   float high, low;
   fs_row_extent(w, high, low);
