@@ -9,8 +9,9 @@
 //
 // Weights are whole numbers, w_i * 2^44 rounded to nearest (the exponential in 64 bits).  Sums of whole numbers do not depend on their
 // order, so a draw is the same however a row is cut over workgroups, and up to 2^19 tokens' sum stays within 63 bits.  A weight is off
-// by 2^-45 of the row's largest at most: 32-bit weights would move the border between two tokens of a flat row of 150,000 by a good
-// part of a token.  Tokens that weigh nothing then (31.2 T below the maximum) are never drawn.
+// by its rounding, 2^-45 of the row's largest, and by what the exponential was off before it, some 2^-46 of itself: 32-bit weights would
+// move the border between two tokens of a flat row of 150,000 by a good part of a token.  Tokens that weigh nothing then (31.2 T below the
+// maximum) are never drawn.
 //
 // No row is sorted whole: the tokens among which the answers lie, some hundreds, are gathered and ordered in LDS.
 //   * Where the first k tokens are all that counts, or those that min-p keeps, a logit is known below which nothing does
