@@ -287,3 +287,20 @@ def test_pages_move_under_held_plans_and_captured_steps():
         shared, eager, apart = (e.step([dataclasses.replace(x) for x in entries]).clone() for e in engines)
         assert engines[0].sharing(entries) and torch.equal(shared, eager)
         close(shared, apart, "float32")
+
+
+@pytest.mark.parametrize("params", [dict(temperature=0.0), dict(temperature=1.0, top_k=20)], ids=["greedy", "top-k"])
+@pytest.mark.parametrize("num_pages", [12, 15, 24])
+def test_answers_that_wait_for_pages(params, num_pages):
+    # Six answers to 90 tokens, of 40 each, hold up to 23 pages: the newest wait, the prompt and what they had drawn run again behind the others.
+    from tokenizer_amd.engine import GenerateParams, generate, generate_answers
+    prompt = random_ids(1000, 90, 8)
+    asked = GenerateParams(max_tokens=40, seed=7, **params)
+    engine = engine_of("float32", num_pages=num_pages, shared_attention=True)
+    for turn in range(2):                                   # (the second time captured steps are there)
+        answers = generate_answers(engine, prompt, asked, 6)
+        for i, answer in enumerate(answers):
+            want = generate(engine_of("float32"), prompt, dataclasses.replace(asked, seed=7 + i))
+            assert answer.tokens == want.tokens and answer.reason == want.reason
+        assert len(engine.cache.requests) == 0
+        engine.cache.check_invariants()
